@@ -413,6 +413,118 @@ PNFT_API int pnft_gelu_bwd_colsum(const void* dh, int64_t sdh, const void* a, in
  * (torch.autocast around experiments/exp4_wikitext2_lm.py:712-729). */
 PNFT_API int pnft_cast_bf16(const int64_t* table, int count, int64_t max_n, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Operators of a decoder's training step that keep little: the gated
+ * feed-forward product, the head's cross entropy without its logits, and
+ * activations kept in 8 bits. Operands are bfloat16 or float16 (`dtype`), sums
+ * are fp32. Operand rows that a matrix product reads are 16-byte aligned
+ * (16-byte base, row strides multiples of 8 elements; widths are free:
+ * pnft_copy_rows16 brings other rows into such a buffer). sm_100 devices only.
+ * status: as the flash entry points (bounded pipeline waits).
+ * ------------------------------------------------------------------------- */
+
+#define PNFT_ACT_SILU 0
+#define PNFT_ACT_GELU 1 /* the exact (erf) form */
+
+/* Gated feed-forward product h[M x F] = act(x Wg^T + bg) * (x Wu^T + bu), x [M x D],
+ * Wg and Wu [F x D], one kernel. bg / bu [F] of type b_dtype (each may be NULL).
+ * g, u (both or neither, row stride ldp): the pre-activations, kept for
+ * pnft_gated_bwd_point. h, g, u are written in `dtype`.
+ * Beside: the MLP of the Pre-LN blocks (experiments/exp4_wikitext2_lm.py:183-200). */
+PNFT_API int pnft_gated_fwd(const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
+                   const void* bg, const void* bu, int b_dtype, void* h, int64_t ldh, void* g, void* u,
+                   int64_t ldp, int64_t M, int64_t D, int64_t F, int act, int dtype, int32_t* status,
+                   void* stream);
+
+/* dg = dh * u * act'(g), du = dh * act(g) with g, u computed again from x (the
+ * backward of pnft_gated_fwd that kept only its input). */
+PNFT_API int pnft_gated_bwd_recompute(const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
+                             int64_t ldwu, const void* bg, const void* bu, int b_dtype, const void* dh,
+                             int64_t lddh, void* dg, void* du, int64_t ldd, int64_t M, int64_t D, int64_t F,
+                             int act, int dtype, int32_t* status, void* stream);
+
+/* The same from kept g, u (dh given), and the biases' gradients dbg / dbu
+ * (b_dtype, may be NULL): the column sums of dg / du in a fixed order. With dh
+ * NULL, g and u stand for dg and du and only the sums are taken. workspace:
+ * pnft_gated_bias_workspace_size(M, F) bytes when a sum is asked for. */
+PNFT_API int pnft_gated_bwd_point(const void* dh, int64_t lddh, const void* g, const void* u, int64_t ldp, void* dg,
+                         void* du, int64_t ldd, void* dbg, void* dbu, int b_dtype, void* workspace,
+                         size_t workspace_bytes, int64_t M, int64_t F, int act, int dtype, void* stream);
+
+PNFT_API size_t pnft_gated_bias_workspace_size(int64_t M, int64_t F);
+
+/* dx[M x D] (dx_dtype) = dg Wg + du Wu, one kernel over both (plus a sum of the
+ * splits of F when there are few rows). workspace: pnft_gated_dx_workspace_size
+ * bytes, 16-byte aligned. */
+PNFT_API int pnft_gated_dx(const void* dg, const void* du, int64_t ldd, const void* wg, int64_t ldwg, const void* wu,
+                  int64_t ldwu, void* dx, int64_t lddx, int dx_dtype, void* workspace, size_t workspace_bytes,
+                  int64_t M, int64_t D, int64_t F, int dtype, int32_t* status, void* stream);
+
+PNFT_API size_t pnft_gated_dx_workspace_size(int64_t M, int64_t D, int64_t F);
+
+/* Weight gradient of one Linear layer, or of two that share their input:
+ * C = dY^T X over K rows, dY [K x M], X [K x N]. Rows r < min(rows, row_split) of
+ * the product go to c0, rows row_split + r (r < rows) to c1 (NULL when
+ * row_split >= M), both with row stride ldc, of type c_dtype. Splits of K are
+ * added in a fixed order. workspace: pnft_weight_grad_workspace_size(K, M, N)
+ * bytes, 16-byte aligned. */
+PNFT_API int pnft_weight_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* c0, void* c1,
+                     int64_t ldc, int64_t row_split, int64_t rows, int c_dtype, void* workspace,
+                     size_t workspace_bytes, int64_t K, int64_t M, int64_t N, int dtype, int32_t* status,
+                     void* stream);
+
+PNFT_API size_t pnft_weight_grad_workspace_size(int64_t K, int64_t M, int64_t N);
+
+/* dst[r, c] = src[r, c] for 16-bit elements, any row strides (elements). */
+PNFT_API int pnft_copy_rows16(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols,
+                     void* stream);
+
+/* Softmax cross entropy of the logits h W^T (h [M x D], W [V x D]) against
+ * targets [M] in pieces of the vocabulary; the logits are never stored.
+ * row_loss [M] (may be NULL): every row's loss, 0 where the target is
+ * ignore_index. loss (may be NULL): their sum, or with `mean` the mean over the
+ * other rows (0/0 when there is none). A target outside [0, V) that is not
+ * ignore_index gives NaN and sets the status word to PNFT_DEV_BAD_INDEX. Rows to
+ * ignore are left out of all work; what they hold reaches no result.
+ * Kept for the backward: hc (rows of h that count, [ceil(M / 128) * 128 x ldc])
+ * and saved (pnft_stream_xent_saved_size(M) bytes, 16-byte aligned). workspace:
+ * pnft_stream_xent_fwd_workspace_size(M, V) bytes. M >= 1.
+ * Beside: pnft_lm_xent, which wants the logits (experiments/exp4_wikitext2_lm.py:714-719). */
+PNFT_API int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* targets,
+                         int64_t ignore_index, void* hc, int64_t ldc, void* saved, float* row_loss,
+                         float* loss, int mean, void* workspace, size_t workspace_bytes, int64_t M, int64_t V,
+                         int64_t D, int dtype, int32_t* status, void* stream);
+
+PNFT_API size_t pnft_stream_xent_saved_size(int64_t M);
+PNFT_API size_t pnft_stream_xent_fwd_workspace_size(int64_t M, int64_t V);
+
+/* Gradient of pnft_stream_xent_fwd: dh [M x D] and / or dw [V x D] (either may be
+ * NULL). dloss: the loss's own gradient on the device, one value (`mean` as in the
+ * forward) or, with per_row, one per row of h with stride dloss_stride. The
+ * logits' gradient exists for one piece of the vocabulary at a time. workspace:
+ * pnft_stream_xent_bwd_workspace_size(M, V, D) bytes, 16-byte aligned. */
+PNFT_API int pnft_stream_xent_bwd(const void* hc, int64_t ldc, const void* w, int64_t ldw, const void* saved,
+                         const float* dloss, int64_t dloss_stride, int per_row, int mean, void* dh,
+                         int64_t lddh, int dh_dtype, void* dw, int64_t lddw, int dw_dtype, void* workspace,
+                         size_t workspace_bytes, int64_t M, int64_t V, int64_t D, int dtype, int32_t* status,
+                         void* stream);
+
+PNFT_API size_t pnft_stream_xent_bwd_workspace_size(int64_t M, int64_t V, int64_t D);
+
+/* Rows of x (any PNFT_DTYPE_*) in 8 bits: per row and block of 128 columns the
+ * least exponent e (in [-110, 120]; float16 [-15, 8]) with max |x| <= 448 * 2^e,
+ * and q = e4m3(x * 2^-e), rounded to nearest even. In the largest exponent
+ * magnitudes end at 240 (256 * 2^e is past the type). NaN and infinities become
+ * NaN and take no part in the maximum. q: rows of ldq bytes (a multiple of 8, 8-byte
+ * aligned base); e: rows of lde bytes, ceil(D / 128) used. */
+PNFT_API int pnft_act8_pack(const void* x, int64_t ldx, void* q, int64_t ldq, int8_t* e, int64_t lde, int64_t M,
+                   int64_t D, int dtype, void* stream);
+
+/* y = q * 2^e in `dtype` (exact for the type that was packed, and for bfloat16
+ * and float32 whatever was packed). */
+PNFT_API int pnft_act8_unpack(const void* q, int64_t ldq, const int8_t* e, int64_t lde, void* y, int64_t ldy, int64_t M,
+                     int64_t D, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -4,6 +4,15 @@ reference's Python API (mcfax-arch/paper_01_anti_decoy_pnfirtau, ``src/``).
 Exports the reference's eager names (src/__init__.py) plus the fused-op
 entry points of src/triton_pnfirtau.py.
 """
+from .lm_lean_ops import (
+    Act8,
+    act8_pack,
+    act8_unpack,
+    act8_weight_grad,
+    gated_linear,
+    gated_mlp,
+    streamed_cross_entropy,
+)
 from .lm_ops import LayerNorm, head_cross_entropy, layer_norm
 from .pnfirtau_attention import (
     PnFirConfig,
@@ -58,4 +67,11 @@ __all__ = [
     "LayerNorm",
     "layer_norm",
     "head_cross_entropy",
+    "gated_linear",
+    "gated_mlp",
+    "streamed_cross_entropy",
+    "Act8",
+    "act8_pack",
+    "act8_unpack",
+    "act8_weight_grad",
 ]

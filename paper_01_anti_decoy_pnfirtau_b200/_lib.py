@@ -19,6 +19,7 @@ SILENCE_PEAK, SILENCE_MASS_RELU, SILENCE_MASS_POW = 0, 1, 2
 FLASH_FORCE_GENERIC, FLASH_DETERMINISTIC, FLASH_PREFER_SM100 = 0x1, 0x2, 0x4
 FLASH_TEST_STALL = 0x100  # test-only: the tcgen05 kernels take their timeout path
 FIR_FUSED_TAPS = 7  # PNFT_FIR_FUSED_TAPS
+ACT_SILU, ACT_GELU = 0, 1
 GELU_TABLE_FLOATS = 10240  # PNFT_GELU_TABLE_FLOATS
 
 _I64x4 = c_int64 * 4
@@ -110,6 +111,49 @@ SIGNATURES: dict[str, tuple] = {
     "pnft_cast_bf16": (c_int, [_P, c_int, c_int64, _P]),
     "pnft_gelu_bwd_colsum": (
         c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_size_t, c_int64, c_int64, c_int, _P, _P]),
+    "pnft_gated_fwd": (
+        c_int,
+        [_P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64,
+         c_int, c_int, _P, _P],
+    ),
+    "pnft_gated_bwd_recompute": (
+        c_int,
+        [_P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64,
+         c_int, c_int, _P, _P],
+    ),
+    "pnft_gated_bwd_point": (
+        c_int,
+        [_P, c_int64, _P, _P, c_int64, _P, _P, c_int64, _P, _P, c_int, _P, c_size_t, c_int64, c_int64, c_int, c_int, _P],
+    ),
+    "pnft_gated_bias_workspace_size": (c_size_t, [c_int64, c_int64]),
+    "pnft_gated_dx": (
+        c_int,
+        [_P, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, c_int, _P, c_size_t, c_int64, c_int64, c_int64, c_int,
+         _P, _P],
+    ),
+    "pnft_gated_dx_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
+    "pnft_weight_grad": (
+        c_int,
+        [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int, _P, c_size_t, c_int64, c_int64, c_int64,
+         c_int, _P, _P],
+    ),
+    "pnft_weight_grad_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
+    "pnft_copy_rows16": (c_int, [_P, c_int64, _P, c_int64, c_int64, c_int64, _P]),
+    "pnft_stream_xent_fwd": (
+        c_int,
+        [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P, _P, c_int, _P, c_size_t, c_int64, c_int64, c_int64,
+         c_int, _P, _P],
+    ),
+    "pnft_stream_xent_saved_size": (c_size_t, [c_int64]),
+    "pnft_stream_xent_fwd_workspace_size": (c_size_t, [c_int64, c_int64]),
+    "pnft_stream_xent_bwd": (
+        c_int,
+        [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int, c_int, _P, c_int64, c_int, _P, c_int64, c_int, _P, c_size_t,
+         c_int64, c_int64, c_int64, c_int, _P, _P],
+    ),
+    "pnft_stream_xent_bwd_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
+    "pnft_act8_pack": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64, c_int, _P]),
+    "pnft_act8_unpack": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64, c_int, _P]),
 }
 
 _lock = threading.Lock()

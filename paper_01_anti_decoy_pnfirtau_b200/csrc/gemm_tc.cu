@@ -1,0 +1,160 @@
+// Host side and split sums of the tcgen05 GEMM core (gemm_tc.cuh), and the weight
+// gradient dW = dY^T X built on it.
+#include "gemm_tc.cuh"
+
+namespace pnft {
+namespace tc {
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
+    n = 148;
+  return n;
+}
+
+int plan_splits(int tiles, int kb) {
+  const int want = std::max(1, sm_count() / std::max(1, tiles));
+  return std::max(1, std::min(want, kb / 8));
+}
+
+namespace {
+
+// Four columns per thread; partial rows are 16-byte aligned (ldp a multiple of 4).
+__global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict__ part, int64_t ldp,
+                                                         int64_t split_stride, int splits, StoreEpi::Params o,
+                                                         int rows_total) {
+  const int n4 = (o.cols + 3) / 4;
+  const float alpha = o.alpha ? *o.alpha : 1.f;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)rows_total * n4; i += (int64_t)gridDim.x * 256) {
+    int row = (int)(i / n4);
+    const int c = (int)(i - (int64_t)row * n4) * 4;
+    const float* src = part + (int64_t)row * ldp + c;
+    const int side = row >= o.row_split;
+    if (side) row -= o.row_split;
+    if (row >= o.rows) continue;
+    float4 a = *reinterpret_cast<const float4*>(src);
+#pragma unroll 4
+    for (int s = 1; s < splits; ++s) {
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(src + s * split_stride));
+      a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+    }
+    float v[4] = {a.x * alpha, a.y * alpha, a.z * alpha, a.w * alpha};
+    const int n = min(4, o.cols - c);
+    const int64_t at = (int64_t)row * o.ldc + c;
+    if (o.dtype == PNFT_DTYPE_F32) {
+      float* dst = static_cast<float*>(side ? o.c[1] : o.c[0]) + at;
+      for (int k = 0; k < n; ++k) dst[k] = o.accumulate ? dst[k] + v[k] : v[k];
+    } else {
+      const bool bf16 = o.dtype == PNFT_DTYPE_BF16;
+      uint16_t* dst = static_cast<uint16_t*>(side ? o.c[1] : o.c[0]) + at;
+      if (n == 4 && o.vec) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(v[0], v[1], bf16), pack2(v[2], v[3], bf16));
+      } else {
+        for (int k = 0; k < n; ++k) store16(dst + k, v[k], bf16);
+      }
+    }
+  }
+}
+
+// dst[r] = src[r], rows of `bytes`; the widths and strides are free, so the copy
+// takes 4-byte words when both rows allow it and 2-byte elements otherwise.
+template <typename W>
+__global__ void __launch_bounds__(256) copy_rows_kernel(const char* __restrict__ src, int64_t ss, char* __restrict__ dst,
+                                                        int64_t ds, int64_t rows, int64_t words) {
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256)
+      reinterpret_cast<W*>(dst + r * ds)[i] = reinterpret_cast<const W*>(src + r * ss)[i];
+}
+}  // namespace
+
+int sum_splits(const float* part, int64_t ldp, int64_t split_stride, int splits, const StoreEpi::Params& out,
+               int rows_total, cudaStream_t st) {
+  const int64_t items = (int64_t)rows_total * ((out.cols + 3) / 4);
+  const int64_t blocks = std::min<int64_t>((items + 255) / 256, (int64_t)sm_count() * 8);
+  sum_splits_kernel<<<(unsigned)blocks, 256, 0, st>>>(part, ldp, split_stride, splits, out, rows_total);
+  return check_launch("split sum", 1);
+}
+
+}  // namespace tc
+}  // namespace pnft
+
+using namespace pnft;
+using namespace pnft::tc;
+
+static int wgrad_splits(int64_t K, int64_t M, int64_t N) {
+  return plan_splits((int)(((M + BM - 1) / BM) * ((N + BN - 1) / BN)), (int)((K + BK - 1) / BK));
+}
+
+extern "C" size_t pnft_weight_grad_workspace_size(int64_t K, int64_t M, int64_t N) {
+  if (K <= 0 || M <= 0 || N <= 0) return 0;
+  const int s = wgrad_splits(K, M, N);
+  return s > 1 ? sizeof(float) * (size_t)s * (size_t)M * (size_t)((N + 3) / 4 * 4) : 0;
+}
+
+extern "C" int pnft_weight_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* c0, void* c1, int64_t ldc,
+                                int64_t row_split, int64_t rows, int c_dtype, void* workspace, size_t workspace_bytes,
+                                int64_t K, int64_t M, int64_t N, int dtype, int32_t* status, void* stream) {
+  if (K < 0 || M <= 0 || N <= 0 || M > (1 << 24) || N > (1 << 24) || K >= ((int64_t)1 << 31) - BK)
+    return fail(PNFT_EINVAL, "weight_grad: bad shape K=%lld M=%lld N=%lld", (long long)K, (long long)M, (long long)N);
+  if (!type16(dtype)) return fail(PNFT_EUNSUPPORTED, "weight_grad: bfloat16 or float16 operands expected");
+  if (c_dtype < PNFT_DTYPE_F32 || c_dtype > PNFT_DTYPE_F16) return fail(PNFT_EINVAL, "weight_grad: unknown output type %d", c_dtype);
+  if (!c0 || (row_split < M && !c1)) return fail(PNFT_EINVAL, "weight_grad: null output");
+  if (row_split >= M) row_split = 0x7fffffff, rows = std::min(rows, M);  // one output
+  if (rows <= 0 || row_split < rows || (row_split < M && row_split + rows > M) || ldc < N) return fail(PNFT_EINVAL, "weight_grad: bad output layout");
+  const int osize = c_dtype == PNFT_DTYPE_F32 ? 4 : 2;
+  cudaStream_t st = as_stream(stream);
+  if (K == 0) {
+    for (int part = 0; part < (row_split < M ? 2 : 1); ++part) {
+      char* c = static_cast<char*>(part ? c1 : c0);
+      const int64_t n = std::min<int64_t>(rows, part ? M - row_split : M);
+      if (cudaMemset2DAsync(c, (size_t)(ldc * osize), 0, (size_t)(N * osize), (size_t)n, st) != cudaSuccess)
+        return check_launch("weight_grad memset", 0);
+    }
+    return PNFT_OK;
+  }
+  if (!tma_rows_ok(dy, lddy, M) || !tma_rows_ok(x, ldx, N))
+    return fail(PNFT_EUNSUPPORTED, "weight_grad: operand rows must be 16-byte aligned (strides multiples of 8)");
+  if (!device_is_sm100()) return fail(PNFT_EUNSUPPORTED, "weight_grad: needs an sm_100 device");
+  Args a;
+  memset(&a, 0, sizeof(a));
+  int rc = map_mnmajor(&a.ta[0], dy, M, K, lddy);
+  if (!rc) rc = map_mnmajor(&a.tb[0], x, N, K, ldx);
+  if (rc) return rc;
+  const int splits = wgrad_splits(K, M, N);
+  a.s = plain_sched(M, N, (K + BK - 1) / BK, splits);
+  a.idesc = idesc(dtype, true, true);
+  a.status = status;
+  StoreEpi::Params out{{c0, c1}, ldc, (int)row_split, (int)rows, (int)N, nullptr, c_dtype, 0, 0,
+                       rows16(c0, ldc, osize) && rows16(c1, ldc, osize)};
+  if (splits == 1) return launch<true, true, false, StoreEpi>("weight_grad", a, out, st);
+  const size_t need = pnft_weight_grad_workspace_size(K, M, N);
+  if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(PNFT_EINVAL, "weight_grad: workspace of %zu bytes < required %zu (16-byte aligned)", workspace_bytes, need);
+  const int64_t ldp = (N + 3) / 4 * 4;
+  StoreEpi::Params part{{workspace, nullptr}, ldp, 0x7fffffff, (int)M, (int)N, nullptr, PNFT_DTYPE_F32, 0, M * ldp, 1};
+  rc = launch<true, true, false, StoreEpi>("weight_grad", a, part, st);
+  if (rc) return rc;
+  return sum_splits(static_cast<const float*>(workspace), ldp, M * ldp, splits, out, (int)M, st);
+}
+
+extern "C" int pnft_copy_rows16(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols,
+                                void* stream) {
+  if (rows < 0 || cols < 0 || lds < 0 || ldd < cols) return fail(PNFT_EINVAL, "copy_rows16: bad layout");
+  if (rows == 0 || cols == 0) return PNFT_OK;
+  if (!src || !dst) return fail(PNFT_EINVAL, "copy_rows16: null pointer");
+  const uintptr_t any = reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) | (uintptr_t)(lds * 2) |
+                        (uintptr_t)(ldd * 2) | (uintptr_t)(cols * 2);
+  const int64_t w = any % 16 == 0 ? 16 : any % 4 == 0 ? 4 : 2, words = cols * 2 / w;
+  const dim3 grid((unsigned)std::min<int64_t>((words + 255) / 256, 64), (unsigned)std::min<int64_t>(rows, 8192));
+  const char* s = static_cast<const char*>(src);
+  char* d = static_cast<char*>(dst);
+  cudaStream_t st = as_stream(stream);
+  if (w == 16)
+    copy_rows_kernel<uint4><<<grid, 256, 0, st>>>(s, lds * 2, d, ldd * 2, rows, words);
+  else if (w == 4)
+    copy_rows_kernel<uint32_t><<<grid, 256, 0, st>>>(s, lds * 2, d, ldd * 2, rows, words);
+  else
+    copy_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(s, lds * 2, d, ldd * 2, rows, words);
+  return check_launch("copy_rows16", 1);
+}

@@ -1,0 +1,629 @@
+// Softmax cross entropy of a language-model head in pieces of the vocabulary, without
+// keeping the logits, and its gradient:
+//
+//   z_iv = h_i . W_v,  loss_i = log sum_v exp(z_iv) - z_{i,t_i}
+//   dz_iv = s_i (exp(z_iv - lse_i) - [v = t_i]),  dh = dz W,  dW = dz^T h
+//
+// Forward: one pass of the GEMM over strips of the vocabulary; the epilogue keeps each
+// row's running maximum and sum in registers, so nothing of size rows x vocabulary
+// exists. Backward: for one piece of the vocabulary at a time the logits are computed
+// again from the kept logarithm of the sum, their gradient goes to a buffer of that
+// piece, and two GEMMs turn it into a share of dh and the piece's rows of dW.
+//
+// Rows whose target is ignore_index cost nothing: the first kernel moves the rows that
+// count to the front of a buffer (and their number to device memory), and every later
+// kernel sizes its work by that number. So nothing in a masked row, NaN and infinities
+// included, reaches a result.
+#include "gemm_tc.cuh"
+
+namespace pnft {
+namespace {
+
+using namespace tc;
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLow = -1e30f;  // running maximum before any logit: finite, so that low - low is 0
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Device state of one call, in the caller's buffers (rows are compacted rows).
+struct State {
+  int32_t* counts;   // [0] rows that count, [1] blocks of the reduction that are done
+  int32_t* pos;      // [M] compacted row of a row, or -1
+  int32_t* idx;      // [Mp] row of a compacted row
+  int32_t* tgt;      // [Mp] its target
+  float* lse2;       // [Mp] log2 of the sum of exponentials
+};
+
+// ------------------------------------------------------------------ compaction
+constexpr int CT = 256;
+struct CompactArgs {
+  const int64_t* t;
+  int64_t ignore;
+  const uint16_t* h;
+  int64_t ldh;
+  uint16_t* hc;
+  int64_t ldc;
+  State s;
+  float* zt;        // [Mp] target logits (NaN where the target is no column)
+  float* row_loss;  // [M] or NULL: ignored rows get 0
+  int64_t M;
+  int V, D, rows, vec;
+  int64_t Mp;
+  int32_t* status;
+};
+
+__device__ __forceinline__ int block_total(int v, int* red) {
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int t = 0;
+  for (int k = 0; k < CT / 32; ++k) t += red[k];
+  return t;
+}
+
+__device__ __forceinline__ void copy_row(uint16_t* dst, const uint16_t* src, int D, bool vec, int lane) {
+  if (vec) {
+    for (int i = lane; i < D / 8; i += 32) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+    for (int i = D / 8 * 8 + lane; i < D; i += 32) dst[i] = src[i];
+  } else {
+    for (int i = lane; i < D; i += 32) dst[i] = src[i];
+  }
+}
+
+// Block b owns rows [b * rows, ...): it counts the rows that count before them (every
+// block reads all earlier targets: at most 1024 blocks, a few bytes per row), places its
+// own in order and copies them.
+__global__ void __launch_bounds__(CT) xent_compact_kernel(CompactArgs p) {
+  __shared__ int red[CT / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t r0 = (int64_t)blockIdx.x * p.rows, r1 = std::min<int64_t>(p.M, r0 + p.rows);
+  int n = 0;
+  for (int64_t r = threadIdx.x; r < r0; r += CT) n += p.t[r] != p.ignore;
+  int base = block_total(n, red);
+  for (int64_t c0 = r0; c0 < r1; c0 += CT) {
+    const int64_t r = c0 + threadIdx.x;
+    const int64_t t = r < r1 ? p.t[r] : 0;
+    const bool counts = r < r1 && t != p.ignore;
+    const unsigned vote = __ballot_sync(0xffffffffu, counts);
+    __syncthreads();
+    if (lane == 0) red[warp] = __popc(vote);
+    __syncthreads();
+    int at = base, total = 0;
+    for (int k = 0; k < CT / 32; ++k) {
+      if (k < warp) at += red[k];
+      total += red[k];
+    }
+    at += __popc(vote & ((1u << lane) - 1));
+    if (r < r1) p.s.pos[r] = counts ? at : -1;
+    if (counts) {
+      p.s.idx[at] = (int)r;
+      const bool good = t >= 0 && t < p.V;
+      p.s.tgt[at] = good ? (int)t : -1;
+      if (!good) {
+        p.zt[at] = __int_as_float(0x7fc00000);
+        report_status(p.status, PNFT_DEV_BAD_INDEX);
+      }
+    } else if (r < r1 && p.row_loss) {
+      p.row_loss[r] = 0.f;
+    }
+    base += total;
+  }
+  __syncthreads();
+  for (int64_t r = r0 + warp; r < r1; r += CT / 32) {
+    const int at = p.s.pos[r];
+    if (at >= 0) copy_row(p.hc + at * p.ldc, p.h + r * p.ldh, p.D, p.vec, lane);
+  }
+  if (r1 == p.M) {  // the last block knows the number of rows; zeros up to the tile's end
+    if (threadIdx.x == 0) p.s.counts[0] = base, p.s.counts[1] = 0;
+    const int64_t end = std::min<int64_t>(p.Mp, ((int64_t)base + 127) / 128 * 128);
+    for (int64_t r = base + warp; r < end; r += CT / 32)
+      for (int i = lane; i < p.D; i += 32) p.hc[r * p.ldc + i] = 0;
+  }
+}
+
+// ------------------------------------------------------------------ forward epilogue
+// Per row and half of the columns: running maximum (times log2 e) and sum of
+// 2^(z log2 e - max), both fp32, over the tiles of a strip.
+struct LseEpi {
+  struct Params {
+    float *part_m, *part_s;  // [strips * 2][Mp]
+    float* zt;
+    const int32_t* tgt;
+    const int32_t* live;
+    int64_t Mp;
+    int V, strip_tiles;
+  };
+  const Params& p;
+  EpiWarp w;
+  float m, s;
+  int tgt;
+  __device__ LseEpi(const Params& p_, const EpiWarp& w_) : p(p_), w(w_) {}
+  __device__ void item_begin(const Item& it) {
+    m = kLow, s = 0.f;
+    const int row = it.mt * BM + w.row();
+    tgt = row < *p.live ? p.tgt[row] : -1;
+  }
+  __device__ void item_end(const Item& it) {
+    const int row = it.mt * BM + w.row();
+    if (row >= *p.live) return;
+    const int64_t at = (int64_t)(it.nt0 / p.strip_tiles * 2 + w.half) * p.Mp + row;
+    p.part_m[at] = m;
+    p.part_s[at] = s;
+  }
+  template <class Release>
+  __device__ void tile(const Item& it, int nt, uint32_t acc, bool zero, Release release) {
+#pragma unroll 1
+    for (int c = w.half * (BN / 2); c < (w.half + 1) * (BN / 2); c += 32) {
+      float z[32];
+      acc_load32(acc + c, zero, z);
+      if (c + 32 == (w.half + 1) * (BN / 2)) release();
+      const int col = nt * BN + c, n = p.V - col;
+      if (n < 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i >= n) z[i] = -INFINITY;
+      }
+      const int tc = tgt - col;
+      if ((unsigned)tc < 32u) {
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v = i == tc ? z[i] : v;
+        p.zt[it.mt * BM + w.row()] = v;
+      }
+      float a = max3(z[0], z[1], z[2]), b = max3(z[3], z[4], z[5]);
+#pragma unroll
+      for (int i = 6; i < 30; i += 4) a = max3(a, z[i], z[i + 1]), b = max3(b, z[i + 2], z[i + 3]);
+      a = max3(a, z[30], z[31]);
+      const float nm = max3(m, a * kLog2e, b * kLog2e);
+      float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        s0 += ex2(fmaf(z[i], kLog2e, -nm));
+        s1 += ex2(fmaf(z[i + 1], kLog2e, -nm));
+        s2 += ex2(fmaf(z[i + 2], kLog2e, -nm));
+        s3 += ex2(fmaf(z[i + 3], kLog2e, -nm));
+      }
+      s = fmaf(s, ex2(m - nm), (s0 + s1) + (s2 + s3));
+      m = nm;
+    }
+  }
+};
+
+// Joins the strips' maxima and sums: lse2, the row's loss, and (last block) the loss of
+// all rows, summed block by block in a fixed order in 64 bits.
+struct ReduceArgs {
+  const float *part_m, *part_s, *zt;
+  State s;
+  float* row_loss;  // [M], or NULL
+  float* loss;      // scalar, or NULL
+  double* block_sum;
+  int64_t Mp;
+  int parts, mean;
+};
+__global__ void __launch_bounds__(256) xent_reduce_kernel(ReduceArgs p) {
+  __shared__ double red[256];
+  __shared__ int last;
+  const int n = p.s.counts[0];
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  double mine = 0.0;
+  if (i < n) {
+    float m = kLow;
+    for (int k = 0; k < p.parts; ++k) m = fmaxf(m, p.part_m[k * p.Mp + i]);
+    float s = 0.f;
+    for (int k = 0; k < p.parts; ++k) s += p.part_s[k * p.Mp + i] * ex2(p.part_m[k * p.Mp + i] - m);
+    const float l = log2f(s);
+    p.s.lse2[i] = m + l;
+    const float loss = kLn2 * (fmaf(-p.zt[i], kLog2e, m) + l);
+    if (p.row_loss) p.row_loss[p.s.idx[i]] = loss;
+    mine = loss;
+  }
+  if (!p.loss) return;
+  red[threadIdx.x] = mine;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    p.block_sum[blockIdx.x] = red[0];
+    __threadfence();
+    last = atomicAdd(&p.s.counts[1], 1) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double t = 0.0;
+  for (int b = threadIdx.x; b < (int)gridDim.x; b += 256) t += __ldcg(p.block_sum + b);
+  __syncthreads();
+  red[threadIdx.x] = t;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *p.loss = (float)(p.mean ? red[0] / (double)n : red[0]);
+}
+
+// ------------------------------------------------------------------ backward
+// The rows' factors: row i's gradient is multiplied by alpha * rs[i]. rs reaches from
+// -top to top with top 1 for bf16; 2^14 for fp16, so that the small probabilities of a
+// large vocabulary stay inside fp16's range whatever the loss's own factor is.
+struct ScaleArgs {
+  State s;
+  const float* dloss;  // scalar, or [M] with stride `stride`
+  int64_t stride;
+  float *rs, *alpha;
+  int per_row, mean;
+  float top;
+};
+__global__ void __launch_bounds__(1024) xent_scale_kernel(ScaleArgs p) {
+  __shared__ float red[32];
+  const int n = p.s.counts[0];
+  if (!p.per_row) {
+    for (int i = threadIdx.x; i < n; i += 1024) p.rs[i] = p.top;
+    if (threadIdx.x == 0) *p.alpha = n == 0 ? 0.f : *p.dloss / (p.mean ? (float)n : 1.f) / p.top;
+    return;
+  }
+  float m = 0.f;
+  for (int i = threadIdx.x; i < n; i += 1024) m = fmaxf(m, fabsf(p.dloss[p.s.idx[i] * p.stride]));
+  m = group_max<32>(m);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = group_max<32>(red[threadIdx.x & 31]);
+  if (!(m > 0.f)) m = 1.f;  // all zero (or NaN alone, which the factors carry)
+  for (int i = threadIdx.x; i < n; i += 1024) p.rs[i] = p.dloss[p.s.idx[i] * p.stride] / m * p.top;
+  if (threadIdx.x == 0) *p.alpha = m / p.top;
+}
+
+// dz of one piece, 16 bits, zeros in rows past the last one that counts and in columns
+// past the vocabulary (the two GEMMs run over whole 64-deep blocks of both).
+struct DzEpi {
+  struct Params {
+    uint16_t* dz;
+    int64_t ld;
+    const float *lse2, *rs;
+    const int32_t *tgt, *live;
+    int64_t Mp;
+    int v0, V, bf16;
+  };
+  const Params& p;
+  EpiWarp w;
+  float lse, rs;
+  int tgt, row;
+  __device__ DzEpi(const Params& p_, const EpiWarp& w_) : p(p_), w(w_) {}
+  __device__ void item_begin(const Item& it) {
+    row = it.mt * BM + w.row();
+    const bool live = row < *p.live;
+    lse = live ? p.lse2[row] : 0.f;
+    rs = live ? p.rs[row] : 0.f;
+    tgt = live ? p.tgt[row] - p.v0 : -1;
+  }
+  __device__ void item_end(const Item&) {}
+  template <class Release>
+  __device__ void tile(const Item& it, int nt, uint32_t acc, bool zero, Release release) {
+    const bool live = row < *p.live;
+#pragma unroll 1
+    for (int c = w.half * (BN / 2); c < (w.half + 1) * (BN / 2); c += 32) {
+      float z[32];
+      acc_load32(acc + c, zero, z);
+      if (c + 32 == (w.half + 1) * (BN / 2)) release();
+      const int col = nt * BN + c, n = p.V - p.v0 - col;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        float v = ex2(fmaf(z[i], kLog2e, -lse)) * rs;
+        if (i == tgt - col) v -= rs;
+        z[i] = live && i < n ? v : 0.f;
+      }
+      if (row < p.Mp) store_row16<32>(p.dz + (int64_t)row * p.ld + col, z, 32, true, p.bf16);
+    }
+  }
+};
+
+// dh[r] = alpha * acc[compacted row of r], 0 for rows that do not count.
+__global__ void __launch_bounds__(256) xent_dh_kernel(const float* __restrict__ acc, int64_t lda, const int32_t* __restrict__ pos,
+                                                      const float* __restrict__ alpha, void* dh, int64_t lddh, int dtype,
+                                                      int64_t M, int D) {
+  const float a = *alpha;
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < M; r += (int64_t)gridDim.x * 8) {
+    const int at = pos[r];
+    for (int c = 4 * lane; c < D; c += 128) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (at >= 0) {
+        v = *reinterpret_cast<const float4*>(acc + at * lda + c);
+        v.x *= a, v.y *= a, v.z *= a, v.w *= a;
+      }
+      const float f[4] = {v.x, v.y, v.z, v.w};
+      for (int k = 0; k < 4 && c + k < D; ++k) {
+        if (dtype == PNFT_DTYPE_F32)
+          static_cast<float*>(dh)[r * lddh + c + k] = f[k];
+        else
+          store16(static_cast<uint16_t*>(dh) + r * lddh + c + k, f[k], dtype == PNFT_DTYPE_BF16);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ plans
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Column tiles per strip: the fewest rounds of tiles over the SMs, counting a third of a
+// tile for each strip's start and end.
+int strip_tiles(int64_t tiles_m, int tiles_n) {
+  const int sms = sm_count();
+  int best = 1;
+  double cost = 1e300;
+  for (int strips = 1; strips <= std::min(tiles_n, 2 * sms); ++strips) {
+    const int per = (tiles_n + strips - 1) / strips;
+    const int64_t items = tiles_m * ((tiles_n + per - 1) / per);
+    const double c = (double)((items + sms - 1) / sms) * (per + 1.0 / 3);
+    if (c < cost) cost = c, best = per;
+  }
+  return best;
+}
+
+struct SavedLayout {
+  size_t counts, pos, idx, tgt, lse2, total;
+};
+SavedLayout saved_layout(int64_t M) {
+  const int64_t Mp = up(std::max<int64_t>(M, 1), BM);
+  SavedLayout l;
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t r = at;
+    at += (n + 255) / 256 * 256;
+    return r;
+  };
+  l.counts = take(8);
+  l.pos = take(4 * Mp);
+  l.idx = take(4 * Mp);
+  l.tgt = take(4 * Mp);
+  l.lse2 = take(4 * Mp);
+  l.total = at;
+  return l;
+}
+State state_of(void* saved, int64_t M) {
+  const SavedLayout l = saved_layout(M);
+  char* b = static_cast<char*>(saved);
+  return State{reinterpret_cast<int32_t*>(b + l.counts), reinterpret_cast<int32_t*>(b + l.pos),
+               reinterpret_cast<int32_t*>(b + l.idx), reinterpret_cast<int32_t*>(b + l.tgt),
+               reinterpret_cast<float*>(b + l.lse2)};
+}
+
+struct FwdLayout {
+  int per, strips;
+  size_t zt, part_m, part_s, sums, total;
+};
+FwdLayout fwd_layout(int64_t M, int64_t V) {
+  const int64_t Mp = up(M, BM);
+  FwdLayout l;
+  const int tiles_n = (int)((V + BN - 1) / BN);
+  l.per = strip_tiles(Mp / BM, tiles_n);
+  l.strips = (tiles_n + l.per - 1) / l.per;
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t r = at;
+    at += (n + 255) / 256 * 256;
+    return r;
+  };
+  l.zt = take(4 * Mp);
+  l.part_m = take(4 * Mp * 2 * l.strips);
+  l.part_s = take(4 * Mp * 2 * l.strips);
+  l.sums = take(8 * ((M + 255) / 256));
+  l.total = at;
+  return l;
+}
+
+// A piece's gradient buffer is about 64 MB, so that the two GEMMs find it in L2.
+int64_t piece_width(int64_t M, int64_t V) {
+  const int64_t Mp = up(M, BM);
+  const int64_t w = std::max<int64_t>(1024, ((int64_t)64 << 20) / (2 * Mp) / BN * BN);
+  return std::min(w, up(V, BN));
+}
+struct BwdLayout {
+  int64_t P;
+  int dh_splits, dw_splits;
+  size_t rs, alpha, dz, acc, part, total;
+};
+BwdLayout bwd_layout(int64_t M, int64_t V, int64_t D) {
+  const int64_t Mp = up(M, BM), D4 = up(D, 4);
+  BwdLayout l;
+  l.P = piece_width(M, V);
+  const int td = (int)((D + BN - 1) / BN);
+  l.dh_splits = plan_splits((int)(Mp / BM) * td, (int)(l.P / BK));
+  l.dw_splits = plan_splits((int)((l.P + BM - 1) / BM) * td, (int)((Mp + BK - 1) / BK));
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t r = at;
+    at += (n + 255) / 256 * 256;
+    return r;
+  };
+  l.rs = take(4 * Mp);
+  l.alpha = take(4);
+  l.dz = take(2 * (size_t)Mp * l.P);
+  l.acc = take(4 * (size_t)Mp * D4);
+  const size_t a = l.dh_splits > 1 ? 4 * (size_t)l.dh_splits * Mp * D4 : 0;
+  const size_t b = l.dw_splits > 1 ? 4 * (size_t)l.dw_splits * l.P * D4 : 0;
+  l.part = take(std::max(a, b));
+  l.total = at;
+  return l;
+}
+
+int xent_check(const char* what, int64_t M, int64_t D, int64_t V, int dtype) {
+  if (M < 0 || D <= 0 || V <= 0 || M >= ((int64_t)1 << 31) - 256 || D > (1 << 24) || V >= ((int64_t)1 << 31) - 2 * BN)
+    return fail(PNFT_EINVAL, "%s: bad shape M=%lld D=%lld V=%lld", what, (long long)M, (long long)D, (long long)V);
+  if (!type16(dtype)) return fail(PNFT_EUNSUPPORTED, "%s: bfloat16 or float16 expected", what);
+  return PNFT_OK;
+}
+
+}  // namespace
+}  // namespace pnft
+
+using namespace pnft;
+using namespace pnft::tc;
+
+extern "C" size_t pnft_stream_xent_saved_size(int64_t M) { return M < 0 ? 0 : saved_layout(M).total; }
+
+extern "C" size_t pnft_stream_xent_fwd_workspace_size(int64_t M, int64_t V) {
+  return M <= 0 || V <= 0 ? 0 : fwd_layout(M, V).total;
+}
+
+extern "C" size_t pnft_stream_xent_bwd_workspace_size(int64_t M, int64_t V, int64_t D) {
+  return M <= 0 || V <= 0 || D <= 0 ? 0 : bwd_layout(M, V, D).total;
+}
+
+extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* targets,
+                                    int64_t ignore_index, void* hc, int64_t ldc, void* saved, float* row_loss,
+                                    float* loss, int mean, void* workspace, size_t workspace_bytes, int64_t M, int64_t V,
+                                    int64_t D, int dtype, int32_t* status, void* stream) {
+  if (int rc = xent_check("stream_xent_fwd", M, D, V, dtype)) return rc;
+  if (!saved || (!row_loss && !loss)) return fail(PNFT_EINVAL, "stream_xent_fwd: null output");
+  if (M == 0) return fail(PNFT_EINVAL, "stream_xent_fwd: no rows");
+  if (!h || !w || !targets || !hc) return fail(PNFT_EINVAL, "stream_xent_fwd: null pointer");
+  if (ldh < D) return fail(PNFT_EINVAL, "stream_xent_fwd: row stride below the width");
+  if (!tma_rows_ok(hc, ldc, D) || !tma_rows_ok(w, ldw, D))
+    return fail(PNFT_EUNSUPPORTED, "stream_xent_fwd: weight and buffer rows must be 16-byte aligned (strides multiples of 8)");
+  if (reinterpret_cast<uintptr_t>(saved) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(PNFT_EINVAL, "stream_xent_fwd: buffers must be 16-byte aligned");
+  const FwdLayout l = fwd_layout(M, V);
+  if (!workspace || workspace_bytes < l.total)
+    return fail(PNFT_EINVAL, "stream_xent_fwd: workspace of %zu bytes < required %zu", workspace_bytes, l.total);
+  if (!device_is_sm100()) return fail(PNFT_EUNSUPPORTED, "stream_xent_fwd: needs an sm_100 device");
+  const int64_t Mp = up(M, BM);
+  char* ws = static_cast<char*>(workspace);
+  cudaStream_t st = as_stream(stream);
+  CompactArgs c;
+  memset(&c, 0, sizeof(c));
+  c.t = targets, c.ignore = ignore_index;
+  c.h = static_cast<const uint16_t*>(h), c.ldh = ldh;
+  c.hc = static_cast<uint16_t*>(hc), c.ldc = ldc;
+  c.s = state_of(saved, M);
+  c.zt = reinterpret_cast<float*>(ws + l.zt);
+  c.row_loss = row_loss;
+  c.M = M, c.V = (int)V, c.D = (int)D, c.Mp = Mp;
+  c.rows = (int)std::max<int64_t>(32, (M + 1023) / 1024);
+  c.vec = rows16(h, ldh, 2);
+  c.status = status;
+  xent_compact_kernel<<<(unsigned)((M + c.rows - 1) / c.rows), CT, 0, st>>>(c);
+  int rc = check_launch("stream_xent compaction", 1);
+  if (rc) return rc;
+
+  Args a;
+  memset(&a, 0, sizeof(a));
+  rc = map_kmajor(&a.ta[0], hc, D, Mp, ldc);
+  if (!rc) rc = map_kmajor(&a.tb[0], w, D, V, ldw);
+  if (rc) return rc;
+  a.s = plain_sched(M, V, (D + BK - 1) / BK, 1);
+  a.s.strips = l.strips;
+  a.s.tiles_per_strip = l.per;
+  a.s.group_m = a.s.tiles_m;
+  a.s.live = c.s.counts;
+  a.s.live_m = 1;
+  a.idesc = idesc(dtype, false, false);
+  a.status = status;
+  LseEpi::Params ep{reinterpret_cast<float*>(ws + l.part_m), reinterpret_cast<float*>(ws + l.part_s), c.zt, c.s.tgt,
+                    c.s.counts, Mp, (int)V, l.per};
+  rc = launch<false, false, false, LseEpi>("stream_xent forward", a, ep, st);
+  if (rc) return rc;
+  ReduceArgs r{ep.part_m, ep.part_s, c.zt, c.s, row_loss, loss, reinterpret_cast<double*>(ws + l.sums), Mp, 2 * l.strips, mean};
+  xent_reduce_kernel<<<(unsigned)((M + 255) / 256), 256, 0, st>>>(r);
+  return check_launch("stream_xent reduction", 1);
+}
+
+extern "C" int pnft_stream_xent_bwd(const void* hc, int64_t ldc, const void* w, int64_t ldw, const void* saved,
+                                    const float* dloss, int64_t dloss_stride, int per_row, int mean, void* dh,
+                                    int64_t lddh, int dh_dtype, void* dw, int64_t lddw, int dw_dtype, void* workspace,
+                                    size_t workspace_bytes, int64_t M, int64_t V, int64_t D, int dtype, int32_t* status,
+                                    void* stream) {
+  if (int rc = xent_check("stream_xent_bwd", M, D, V, dtype)) return rc;
+  if (M == 0) return fail(PNFT_EINVAL, "stream_xent_bwd: no rows");
+  if (!hc || !w || !saved || !dloss || (!dh && !dw)) return fail(PNFT_EINVAL, "stream_xent_bwd: null pointer");
+  if (!tma_rows_ok(hc, ldc, D) || !tma_rows_ok(w, ldw, D))
+    return fail(PNFT_EUNSUPPORTED, "stream_xent_bwd: weight and buffer rows must be 16-byte aligned (strides multiples of 8)");
+  if ((dh && lddh < D) || (dw && lddw < D)) return fail(PNFT_EINVAL, "stream_xent_bwd: row stride below the width");
+  for (int t : {dh_dtype, dw_dtype})
+    if (t < PNFT_DTYPE_F32 || t > PNFT_DTYPE_F16) return fail(PNFT_EINVAL, "stream_xent_bwd: unknown output type %d", t);
+  const BwdLayout l = bwd_layout(M, V, D);
+  if (!workspace || workspace_bytes < l.total || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(PNFT_EINVAL, "stream_xent_bwd: workspace of %zu bytes < required %zu (16-byte aligned)", workspace_bytes, l.total);
+  if (!device_is_sm100()) return fail(PNFT_EUNSUPPORTED, "stream_xent_bwd: needs an sm_100 device");
+  const int64_t Mp = up(M, BM), D4 = up(D, 4);
+  char* ws = static_cast<char*>(workspace);
+  cudaStream_t st = as_stream(stream);
+  const State s = state_of(const_cast<void*>(saved), M);
+  float* rs = reinterpret_cast<float*>(ws + l.rs);
+  float* alpha = reinterpret_cast<float*>(ws + l.alpha);
+  uint16_t* dz = reinterpret_cast<uint16_t*>(ws + l.dz);
+  float* acc = reinterpret_cast<float*>(ws + l.acc);
+  float* part = reinterpret_cast<float*>(ws + l.part);
+  const bool bf16 = dtype == PNFT_DTYPE_BF16;
+  xent_scale_kernel<<<1, 1024, 0, st>>>(ScaleArgs{s, dloss, dloss_stride, rs, alpha, per_row, mean, bf16 ? 1.f : 16384.f});
+  int rc = check_launch("stream_xent scale", 1);
+  for (int64_t v0 = 0; !rc && v0 < V; v0 += l.P) {
+    const int64_t n = std::min(l.P, V - v0);
+    const uint16_t* wp = static_cast<const uint16_t*>(w) + v0 * ldw;
+    Args a;
+    memset(&a, 0, sizeof(a));
+    a.status = status;
+    // dz of the piece
+    rc = map_kmajor(&a.ta[0], hc, D, Mp, ldc);
+    if (!rc) rc = map_kmajor(&a.tb[0], wp, D, n, ldw);
+    if (rc) break;
+    a.s = plain_sched(M, n, (D + BK - 1) / BK, 1);
+    a.s.live = s.counts;
+    a.s.live_m = 1;
+    a.idesc = idesc(dtype, false, false);
+    DzEpi::Params ep{dz, l.P, s.lse2, rs, s.tgt, s.counts, Mp, (int)v0, (int)V, bf16};
+    rc = launch<false, false, false, DzEpi>("stream_xent dz", a, ep, st);
+    if (rc) break;
+    if (dh) {  // dh (+)= dz W
+      rc = map_kmajor(&a.ta[0], dz, n, Mp, l.P);
+      if (!rc) rc = map_mnmajor(&a.tb[0], wp, D, n, ldw);
+      if (rc) break;
+      const int kb = (int)((n + BK - 1) / BK), splits = std::min(l.dh_splits, std::max(1, kb / 8));
+      a.s = plain_sched(M, D, kb, splits);
+      a.s.live = s.counts;
+      a.s.live_m = 1;
+      a.idesc = idesc(dtype, false, true);
+      StoreEpi::Params out{{acc, nullptr}, D4, 0x7fffffff, (int)M, (int)D, nullptr, PNFT_DTYPE_F32, v0 > 0, 0, 1};
+      if (splits > 1) {
+        StoreEpi::Params o = out;
+        o.c[0] = part, o.accumulate = 0, o.split_stride = Mp * D4;
+        rc = launch<false, true, false, StoreEpi>("stream_xent dh", a, o, st);
+        if (!rc) rc = sum_splits(part, D4, Mp * D4, splits, out, (int)M, st);
+      } else {
+        rc = launch<false, true, false, StoreEpi>("stream_xent dh", a, out, st);
+      }
+      if (rc) break;
+    }
+    if (dw) {  // the piece's rows of dW = dz^T h
+      rc = map_mnmajor(&a.ta[0], dz, n, Mp, l.P);
+      if (!rc) rc = map_mnmajor(&a.tb[0], hc, D, Mp, ldc);
+      if (rc) break;
+      a.s = plain_sched(n, D, (Mp + BK - 1) / BK, l.dw_splits);
+      a.s.live = s.counts;
+      a.s.live_k = 1;
+      a.idesc = idesc(dtype, true, true);
+      const int size = dw_dtype == PNFT_DTYPE_F32 ? 4 : 2;
+      void* dst = static_cast<char*>(dw) + v0 * lddw * size;
+      StoreEpi::Params out{{dst, nullptr}, lddw, 0x7fffffff, (int)n, (int)D, alpha, dw_dtype, 0, 0, rows16(dst, lddw, size)};
+      if (l.dw_splits > 1) {
+        StoreEpi::Params o{{part, nullptr}, D4, 0x7fffffff, (int)n, (int)D, nullptr, PNFT_DTYPE_F32, 0, l.P * D4, 1};
+        rc = launch<true, true, false, StoreEpi>("stream_xent dW", a, o, st);
+        if (!rc) rc = sum_splits(part, D4, l.P * D4, l.dw_splits, out, (int)n, st);
+      } else {
+        rc = launch<true, true, false, StoreEpi>("stream_xent dW", a, out, st);
+      }
+    }
+  }
+  if (rc || !dh) return rc;
+  xent_dh_kernel<<<(unsigned)std::min<int64_t>((M + 7) / 8, (int64_t)sm_count() * 16), 256, 0, st>>>(
+      acc, D4, s.pos, alpha, dh, lddh, dh_dtype, M, (int)D);
+  return check_launch("stream_xent dh rows", 1);
+}

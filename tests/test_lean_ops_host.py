@@ -1,0 +1,117 @@
+"""Argument checks of the lean training-step operators that need no GPU: the C entry
+points refuse bad shapes, types, layouts and workspaces before any device work, and the
+Python calls refuse CPU tensors."""
+import pytest
+import torch
+
+import paper_01_anti_decoy_pnfirtau_b200 as P
+from paper_01_anti_decoy_pnfirtau_b200 import _lib
+
+BF16, FP32 = _lib.DTYPE_BF16, _lib.DTYPE_F32
+A = 1 << 20  # an address that is never read: every call below is refused first
+
+
+def refused(rc, code, word):
+    assert rc == code and word in _lib.last_error(), (rc, _lib.last_error())
+
+
+def gated(M=4, D=64, F=128, act=0, dtype=BF16, ldx=64, ldh=128, x=A, h=A, g=None, u=None):
+    return _lib.lib().pnft_gated_fwd(x, ldx, A, 64, A, 64, None, None, FP32, h, ldh, g, u, 128, M, D, F, act, dtype, None, None)
+
+
+def test_gated_fwd_refuses():
+    refused(gated(M=-1), _lib.EINVAL, "shape")
+    refused(gated(D=0), _lib.EINVAL, "shape")
+    refused(gated(F=0), _lib.EINVAL, "shape")
+    refused(gated(act=2), _lib.EINVAL, "activation")
+    refused(gated(dtype=FP32), _lib.EUNSUPPORTED, "float16")
+    refused(gated(h=None), _lib.EINVAL, "null")
+    refused(gated(g=A), _lib.EINVAL, "null")
+    refused(gated(ldh=127), _lib.EINVAL, "stride")
+    refused(gated(ldx=65), _lib.EUNSUPPORTED, "aligned")
+    refused(gated(x=A + 2), _lib.EUNSUPPORTED, "aligned")
+    refused(gated(ldx=56), _lib.EUNSUPPORTED, "aligned")
+    assert gated(M=0, x=None) == _lib.OK
+
+
+def test_gated_backward_refuses():
+    L = _lib.lib()
+    args = lambda dh=A, ldd=128: (A, 64, A, 64, A, 64, None, None, FP32, dh, 128, A, A, ldd, 4, 64, 128, 0, BF16, None, None)  # noqa: E731
+    refused(L.pnft_gated_bwd_recompute(*args(dh=None)), _lib.EINVAL, "null")
+    refused(L.pnft_gated_bwd_recompute(*args(ldd=100)), _lib.EINVAL, "stride")
+    point = lambda dh, dbg, ws, n: L.pnft_gated_bwd_point(dh, 128, A, A, 128, A, A, 128, dbg, None, FP32, ws, n, 4, 128, 0, BF16, None)  # noqa: E731
+    refused(point(None, None, None, 0), _lib.EINVAL, "null")
+    refused(point(A, A, A, 16), _lib.EINVAL, "workspace")
+    dx = lambda ldd, ws, n, M=4: L.pnft_gated_dx(A, A, ldd, A, 64, A, 64, A, 64, BF16, ws, n, M, 64, 8192, BF16, None, None)  # noqa: E731
+    refused(dx(8191, A, 1 << 30), _lib.EUNSUPPORTED, "aligned")
+    assert L.pnft_gated_dx_workspace_size(0, 64, 128) == 0
+
+
+def wgrad(K=64, M=16, N=32, c1=None, row_split=16, rows=16, ldc=32, dtype=BF16, c_dtype=FP32, lddy=16):
+    return _lib.lib().pnft_weight_grad(A, lddy, A, 32, A, c1, ldc, row_split, rows, c_dtype, None, 0, K, M, N, dtype, None, None)
+
+
+def test_weight_grad_refuses():
+    refused(wgrad(K=-1), _lib.EINVAL, "shape")
+    refused(wgrad(dtype=FP32), _lib.EUNSUPPORTED, "float16")
+    refused(wgrad(c_dtype=9), _lib.EINVAL, "type")
+    refused(wgrad(row_split=8, rows=8), _lib.EINVAL, "null")
+    refused(wgrad(row_split=8, rows=9, c1=A), _lib.EINVAL, "layout")  # more rows than the split leaves
+    refused(wgrad(row_split=10, rows=8, c1=A), _lib.EINVAL, "layout")  # past the product's end
+    refused(wgrad(ldc=31), _lib.EINVAL, "layout")
+    refused(wgrad(lddy=17), _lib.EUNSUPPORTED, "aligned")
+
+
+def test_stream_xent_refuses():
+    L = _lib.lib()
+    n = L.pnft_stream_xent_fwd_workspace_size(10, 1000)
+    fwd = lambda M=10, V=1000, dtype=BF16, ws=A, nb=n, ldc=64, saved=A, loss=A: L.pnft_stream_xent_fwd(  # noqa: E731
+        A, 64, A, 64, A, -100, A, ldc, saved, None, loss, 1, ws, nb, M, V, 64, dtype, None, None)
+    refused(fwd(M=0), _lib.EINVAL, "rows")
+    refused(fwd(V=0), _lib.EINVAL, "shape")
+    refused(fwd(dtype=FP32), _lib.EUNSUPPORTED, "float16")
+    refused(fwd(loss=None), _lib.EINVAL, "null")
+    refused(fwd(saved=None), _lib.EINVAL, "null")
+    refused(fwd(ldc=60), _lib.EUNSUPPORTED, "aligned")
+    refused(fwd(ws=None), _lib.EINVAL, "workspace")
+    refused(fwd(nb=n - 1), _lib.EINVAL, "workspace")
+    m = L.pnft_stream_xent_bwd_workspace_size(10, 1000, 64)
+    bwd = lambda dh=A, dw=A, nb=m, lddh=64, t=BF16: L.pnft_stream_xent_bwd(  # noqa: E731
+        A, 64, A, 64, A, A, 1, 0, 1, dh, lddh, t, dw, 64, t, A, nb, 10, 1000, 64, BF16, None, None)
+    refused(bwd(dh=None, dw=None), _lib.EINVAL, "null")
+    refused(bwd(nb=m - 1), _lib.EINVAL, "workspace")
+    refused(bwd(lddh=63), _lib.EINVAL, "stride")
+    refused(bwd(t=5), _lib.EINVAL, "type")
+
+
+def test_stream_xent_memory_stays_small():
+    """The backward's buffers for the repository's language model (32 x 511 rows, vocabulary
+    33278, width 256) and a long batch: a fraction of the logits' 2 bytes per row and word."""
+    L = _lib.lib()
+    for M, V, D in ((16352, 33278, 256), (131072, 33278, 256), (4096, 128000, 2048)):
+        kept = L.pnft_stream_xent_saved_size(M) + 2 * M * D
+        work = max(L.pnft_stream_xent_fwd_workspace_size(M, V), L.pnft_stream_xent_bwd_workspace_size(M, V, D))
+        assert kept < 0.06 * 2 * M * V and work < 0.6 * 2 * M * V, (M, V, D, kept, work)
+
+
+def test_act8_and_copies_refuse():
+    L = _lib.lib()
+    pack = lambda M=4, D=100, ldx=100, ldq=104, lde=1, dtype=BF16, x=A: L.pnft_act8_pack(x, ldx, A, ldq, A, lde, M, D, dtype, None)  # noqa: E731
+    refused(pack(D=0), _lib.EINVAL, "shape")
+    refused(pack(dtype=3), _lib.EINVAL, "dtype")
+    refused(pack(x=None), _lib.EINVAL, "null")
+    refused(pack(ldx=99), _lib.EINVAL, "stride")
+    refused(pack(ldq=100), _lib.EINVAL, "stride")
+    refused(pack(lde=0), _lib.EINVAL, "stride")
+    assert pack(M=0, x=None) == _lib.OK
+    refused(L.pnft_copy_rows16(A, 8, A, 4, 2, 8, None), _lib.EINVAL, "layout")
+
+
+def test_python_calls_refuse_cpu_tensors_and_bad_arguments():
+    x, w = torch.randn(4, 64).bfloat16(), torch.randn(128, 64).bfloat16()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        P.gated_linear(x, w, w)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        P.streamed_cross_entropy(x, w, torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        P.act8_pack(x)
