@@ -427,45 +427,35 @@ PNFT_API int pnft_cast_bf16(const int64_t* table, int count, int64_t max_n, void
 #define PNFT_ACT_GELU 1 /* the exact (erf) form */
 
 /* Gated feed-forward product h[M x F] = act(x Wg^T + bg) * (x Wu^T + bu), x [M x D],
- * Wg and Wu [F x D], one kernel. bg / bu [F] of type b_dtype (each may be NULL).
- * g, u (both or neither, row stride ldp): the pre-activations, kept for
- * pnft_gated_bwd_point. h, g, u are written in `dtype`.
+ * Wg and Wu [F x D], one kernel. bg / bu [F] of type b_dtype (each may be NULL). h is
+ * written in `dtype`. pre (may be NULL): the pre-activations x Wg^T + bg and x Wu^T + bu
+ * kept for pnft_gated_bwd with 24 bits each, as three matrices [M x ldp] of 16-bit
+ * words one after the other (ldp a multiple of 8, 16-byte aligned).
  * Beside: the MLP of the Pre-LN blocks (experiments/exp4_wikitext2_lm.py:183-200). */
 PNFT_API int pnft_gated_fwd(const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
-                   const void* bg, const void* bu, int b_dtype, void* h, int64_t ldh, void* g, void* u,
-                   int64_t ldp, int64_t M, int64_t D, int64_t F, int act, int dtype, int32_t* status,
-                   void* stream);
+                   const void* bg, const void* bu, int b_dtype, void* h, int64_t ldh, void* pre, int64_t ldp,
+                   int64_t M, int64_t D, int64_t F, int act, int dtype, int32_t* status, void* stream);
 
-/* dg = dh * u * act'(g), du = dh * act(g) with g, u computed again from x (the
- * backward of pnft_gated_fwd that kept only its input). */
-PNFT_API int pnft_gated_bwd_recompute(const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
-                             int64_t ldwu, const void* bg, const void* bu, int b_dtype, const void* dh,
-                             int64_t lddh, void* dg, void* du, int64_t ldd, int64_t M, int64_t D, int64_t F,
-                             int act, int dtype, int32_t* status, void* stream);
+/* Backward of pnft_gated_fwd: dx [M x D] (dx_dtype), dwg / dwu [F x D] (dw_dtype, row
+ * stride lddw), dbg / dbu [F] (b_dtype); each may be NULL. With g, u the pre-activations
+ * (from `pre`, or computed again from x when pre is NULL):
+ *   dg = dh * u * act'(g), du = dh * act(g)              (rounded to `dtype`)
+ *   dx = dg Wg + du Wu, dwg = dg^T x, dwu = du^T x, dbg / dbu = column sums
+ * dh [M x F]: 16-byte aligned rows, or any rows when F is no multiple of 8 or `pre` is
+ * given. Sums run in a fixed order. workspace: pnft_gated_bwd_workspace_size bytes,
+ * 16-byte aligned. */
+PNFT_API int pnft_gated_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
+                   const void* bg, const void* bu, int b_dtype, const void* pre, int64_t ldp, const void* dh,
+                   int64_t lddh, void* dx, int64_t lddx, int dx_dtype, void* dwg, void* dwu, int64_t lddw,
+                   int dw_dtype, void* dbg, void* dbu, void* workspace, size_t workspace_bytes, int64_t M,
+                   int64_t D, int64_t F, int act, int dtype, int32_t* status, void* stream);
 
-/* The same from kept g, u (dh given), and the biases' gradients dbg / dbu
- * (b_dtype, may be NULL): the column sums of dg / du in a fixed order. With dh
- * NULL, g and u stand for dg and du and only the sums are taken. workspace:
- * pnft_gated_bias_workspace_size(M, F) bytes when a sum is asked for. */
-PNFT_API int pnft_gated_bwd_point(const void* dh, int64_t lddh, const void* g, const void* u, int64_t ldp, void* dg,
-                         void* du, int64_t ldd, void* dbg, void* dbu, int b_dtype, void* workspace,
-                         size_t workspace_bytes, int64_t M, int64_t F, int act, int dtype, void* stream);
-
-PNFT_API size_t pnft_gated_bias_workspace_size(int64_t M, int64_t F);
-
-/* dx[M x D] (dx_dtype) = dg Wg + du Wu, one kernel over both (plus a sum of the
- * splits of F when there are few rows). workspace: pnft_gated_dx_workspace_size
- * bytes, 16-byte aligned. */
-PNFT_API int pnft_gated_dx(const void* dg, const void* du, int64_t ldd, const void* wg, int64_t ldwg, const void* wu,
-                  int64_t ldwu, void* dx, int64_t lddx, int dx_dtype, void* workspace, size_t workspace_bytes,
-                  int64_t M, int64_t D, int64_t F, int dtype, int32_t* status, void* stream);
-
-PNFT_API size_t pnft_gated_dx_workspace_size(int64_t M, int64_t D, int64_t F);
+PNFT_API size_t pnft_gated_bwd_workspace_size(int64_t M, int64_t D, int64_t F);
 
 /* Weight gradient of one Linear layer, or of two that share their input:
  * C = dY^T X over K rows, dY [K x M], X [K x N]. Rows r < min(rows, row_split) of
  * the product go to c0, rows row_split + r (r < rows) to c1 (NULL when
- * row_split >= M), both with row stride ldc, of type c_dtype. Splits of K are
+ * row_split >= M; else row_split is a multiple of 128), both with row stride ldc, of type c_dtype. Splits of K are
  * added in a fixed order. workspace: pnft_weight_grad_workspace_size(K, M, N)
  * bytes, 16-byte aligned. */
 PNFT_API int pnft_weight_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* c0, void* c1,

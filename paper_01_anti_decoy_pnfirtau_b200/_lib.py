@@ -113,25 +113,15 @@ SIGNATURES: dict[str, tuple] = {
         c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_size_t, c_int64, c_int64, c_int, _P, _P]),
     "pnft_gated_fwd": (
         c_int,
-        [_P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64,
-         c_int, c_int, _P, _P],
+        [_P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int, _P, c_int64, _P, c_int64, c_int64, c_int64, c_int64, c_int,
+         c_int, _P, _P],
     ),
-    "pnft_gated_bwd_recompute": (
+    "pnft_gated_bwd": (
         c_int,
-        [_P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64,
-         c_int, c_int, _P, _P],
+        [_P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int, _P, c_int64, _P, c_int64, _P, c_int64, c_int, _P, _P,
+         c_int64, c_int, _P, _P, _P, c_size_t, c_int64, c_int64, c_int64, c_int, c_int, _P, _P],
     ),
-    "pnft_gated_bwd_point": (
-        c_int,
-        [_P, c_int64, _P, _P, c_int64, _P, _P, c_int64, _P, _P, c_int, _P, c_size_t, c_int64, c_int64, c_int, c_int, _P],
-    ),
-    "pnft_gated_bias_workspace_size": (c_size_t, [c_int64, c_int64]),
-    "pnft_gated_dx": (
-        c_int,
-        [_P, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, c_int, _P, c_size_t, c_int64, c_int64, c_int64, c_int,
-         _P, _P],
-    ),
-    "pnft_gated_dx_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
+    "pnft_gated_bwd_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
     "pnft_weight_grad": (
         c_int,
         [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int, _P, c_size_t, c_int64, c_int64, c_int64,

@@ -4,10 +4,15 @@
 //   dg = dh * u * act'(g),  du = dh * act(g),  dx = dg Wg + du Wu
 //
 // (the weight gradients dg^T x, du^T x are pnft_weight_grad's). Both projections are
-// one GEMM: a 128 x 256 accumulator holds 128 columns of g and the same 128 of u, fed
+// one GEMM: a 256-column accumulator holds 128 columns of g and the same 128 of u, fed
 // from the two weights' tiles with the x tile read once, so the epilogue has both
 // values of an element in one thread and g, u never meet in memory unless a backward
 // wants them.
+//
+// The backward has g, u again in one of two ways: computed from x by the same GEMM, whose
+// epilogue then reads dh and writes dg, du; or kept by the forward with 24 bits each (the
+// upper 16 bits of fp32 in two planes, the next 8 of both in a third: kept in 16 bits,
+// their rounding would add as much error to the gradients as the operands' own).
 #include "gemm_tc.cuh"
 
 namespace pnft {
@@ -20,9 +25,9 @@ constexpr float kSqrtHalf = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143
 // act(g); deriv: also act'(g). The exponentials and the quotient are the fast ones
 // (a few units of 2^-23): the results are rounded to 16 bits. GELU's normal
 // distribution goes through erfc, which keeps its relative accuracy for g << 0.
-template <bool DERIV>
-__device__ __forceinline__ float act_value(float g, int act, float* deriv) {
-  if (act == PNFT_ACT_SILU) {
+template <bool DERIV, int ACT>
+__device__ __forceinline__ float act_value(float g, float* deriv) {
+  if (ACT == PNFT_ACT_SILU) {
     const float s = __fdividef(1.f, 1.f + __expf(-g));
     if (DERIV) *deriv = s * (1.f + g * (1.f - s));
     return g * s;
@@ -37,97 +42,201 @@ __device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
   return load16(static_cast<const uint16_t*>(p) + i, dtype == PNFT_DTYPE_BF16);
 }
 
-// Forward (dh NULL): h, and g, u when asked for. Backward recomputation (dh given):
-// dg, du of the recomputed g, u.
+// 32 values of a bias vector from column `col`, `n` of them inside.
+__device__ __forceinline__ void add_bias(float (&v)[32], const void* bias, int dtype, int col, int n) {
+  if (n >= 32 && reinterpret_cast<uintptr_t>(bias) % 16 == 0) {
+    if (dtype == PNFT_DTYPE_F32) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(bias) + col + i);
+        v[i] += f.x, v[i + 1] += f.y, v[i + 2] += f.z, v[i + 3] += f.w;
+      }
+    } else {
+      float b[32];
+      load_row16<32>(static_cast<const uint16_t*>(bias) + col, b, 32, true, dtype == PNFT_DTYPE_BF16);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] += b[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) v[i] += load_any(bias, col + i, dtype);
+  }
+}
+
+// FWD: h. KEEP: h and the three planes of g, u. BWD: dg, du from dh and the recomputed g, u.
+enum { FWD, KEEP, BWD };
+template <int MODE, int ACT>
 struct GatedEpi {
+  static constexpr int OUTS = MODE == FWD ? 2 : MODE == KEEP ? 3 : 2;  // boxes for results
+  static constexpr int BOXES = OUTS + (MODE == BWD);                  // and one for dh
   struct Params {
     const void *bg, *bu;
-    int b_dtype;
-    uint16_t* h;
-    int64_t ldh;
-    uint16_t *g, *u;  // forward: the pre-activations to keep (may be NULL); backward: dg, du
-    int64_t ldp;
-    const uint16_t* dh;
-    int64_t lddh;
-    int M, F, act, bf16;
-    int vec_h, vec_p, vec_dh;
+    int b_dtype, bf16;
+    Out h;            // FWD, KEEP: h; BWD: dg
+    Out k;            // KEEP: the planes; BWD: du
+    CUtensorMap dh;   // BWD
   };
   const Params& p;
-  EpiWarp w;
-  __device__ GatedEpi(const Params& p_, const EpiWarp& w_) : p(p_), w(w_) {}
-  __device__ void item_begin(const Item&) {}
-  __device__ void item_end(const Item&) {}
+  EpiWarp w, out;
+  const Abort& ab;
+  Boxes<OUTS> boxes;
+  int phase, issued;
+  __device__ GatedEpi(const Params& p_, const EpiWarp& w_, const Abort& ab_)
+      : p(p_), w(w_), out{w_.quad, w_.half, w_.lane, w_.smem + (MODE == BWD ? BOX_BYTES : 0), w_.bar}, ab(ab_), boxes(out),
+        phase(0), issued(0) {}
+  __device__ int col0(const Steps& q) const { return q.nt * (BN / 2) + w.half * (BN / 4); }
+  __device__ void load_dh(const Steps& q) {
+    if (w.lane == 0) {
+      mbar_arrive_expect_tx(w.bar, BOX_BYTES);
+      tma_load_3d(w.smem, &p.dh, w.bar, col0(q), q.it.row0 + 32 * w.quad, 0);
+    }
+    ++issued;
+  }
+  __device__ void prepare(const Steps& q) {
+    if (MODE == BWD && issued == 0) load_dh(q);
+  }
+  __device__ void done() {
+    if (MODE == BWD && issued > phase) drain_wait(w.bar, phase & 1);  // an abandoned tile's dh
+    boxes.finish();
+  }
+  __device__ __forceinline__ void write(const Out& o, uint32_t b, int row, int col, int z) {
+    if (o.tma)
+      boxes.store(b, &o.map, col, row, z);
+    else
+      boxes.template store_plain<2>(b, static_cast<uint16_t*>(o.base) + (int64_t)row * o.ld + col, o.ld, o.rows - row,
+                                    o.cols - col);
+  }
   template <class Release>
-  __device__ void tile(const Item& it, int nt, uint32_t acc, bool zero, Release release) {
-    const int row = it.mt * BM + w.row();
-    const bool live = row < p.M;
-    const bool bf16 = p.bf16;
-    constexpr int W = BN / 4;  // columns of g (and of u) of this warp's half
-#pragma unroll 1
-    for (int c = w.half * W; c < (w.half + 1) * W; c += 32) {
+  __device__ __forceinline__ void tile(const Steps& q, uint32_t acc, Release release) {
+    constexpr int W = BN / 4;  // columns of g (and of u) of this warp
+    const int row = q.it.row0 + 32 * w.quad, col = col0(q);
+    const bool live = row < p.h.rows && col < p.h.cols, bf16 = p.bf16;
+    if (MODE == BWD) {
+      if (!warp_wait(w.bar, phase & 1, ab)) return;
+      ++phase;
+    }
+    uint32_t b[OUTS];
+    uint4 low[MODE == KEEP ? W / 8 : 1];
+    if (live) {
+      if (MODE == FWD)
+        b[0] = boxes.take();
+      else
+        boxes.take_all(b);
+    }
+#pragma unroll
+    for (int c = 0; c < W; c += 32) {
       uint32_t rg[32], ru[32];
-      tmem_load32x2(acc + c, rg, acc + BN / 2 + c, ru);
-      if (c + 32 == (w.half + 1) * W) release();
-      const int col = nt * (BN / 2) + c, n = p.F - col;
-      if (!live || n <= 0) continue;
+      tmem_load32x2(acc + w.half * W + c, rg, acc + BN / 2 + w.half * W + c, ru);
+      if (c + 32 == W) release();
       float g[32], u[32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        g[i] = zero ? 0.f : __uint_as_float(rg[i]);
-        u[i] = zero ? 0.f : __uint_as_float(ru[i]);
-      }
-      if (p.bg) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < n) g[i] += load_any(p.bg, col + i, p.b_dtype);
-      }
-      if (p.bu) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < n) u[i] += load_any(p.bu, col + i, p.b_dtype);
-      }
-      if (p.dh) {
+      for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(rg[i]), u[i] = __uint_as_float(ru[i]);
+      const int n = p.h.cols - col - c;
+      if (p.bg) add_bias(g, p.bg, p.b_dtype, col + c, n);
+      if (p.bu) add_bias(u, p.bu, p.b_dtype, col + c, n);
+      if (MODE == BWD) {
         float d[32];
-        load_row16<32>(p.dh + (int64_t)row * p.lddh + col, d, n, p.vec_dh, bf16);
+        boxes.get16(w.smem, c / 32, d, bf16);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           float da;
-          const float a = act_value<true>(g[i], p.act, &da);
+          const float a = act_value<true, ACT>(g[i], &da);
           g[i] = d[i] * u[i] * da;
           u[i] = d[i] * a;
         }
-      }
-      if (p.g) {
-        store_row16<32>(p.g + (int64_t)row * p.ldp + col, g, n, p.vec_p, bf16);
-        store_row16<32>(p.u + (int64_t)row * p.ldp + col, u, n, p.vec_p, bf16);
-      }
-      if (p.h) {
+        if (c + 32 == W) {  // dh's box has been read: the next tile's may come
+          __syncwarp();
+          Steps next = q;
+          next.next();
+          if (next.valid()) load_dh(next);
+        }
+        if (!live) continue;
+        boxes.put16(b[0], c / 32, g, bf16);
+        boxes.put16(b[OUTS - 1], c / 32, u, bf16);
+      } else {
+        if (!live) continue;
+        if (MODE == KEEP) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) g[i] = act_value<false>(g[i], p.act, nullptr) * u[i];
-        store_row16<32>(p.h + (int64_t)row * p.ldh + col, g, n, p.vec_h, bf16);
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t x[4], y[4], z[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t g0 = __float_as_uint(g[i + 2 * k]), g1 = __float_as_uint(g[i + 2 * k + 1]);
+              const uint32_t u0 = __float_as_uint(u[i + 2 * k]), u1 = __float_as_uint(u[i + 2 * k + 1]);
+              x[k] = __byte_perm(g0, g1, 0x7632);  // the upper halves of g
+              y[k] = __byte_perm(u0, u1, 0x7632);  // and of u
+              z[k] = __byte_perm(__byte_perm(g0, u0, 0x0051), __byte_perm(g1, u1, 0x0051), 0x5410);  // the bytes below
+            }
+            boxes.put(b[OUTS - 2], (c + i) / 8, x[0], x[1], x[2], x[3]);
+            boxes.put(b[OUTS - 1], (c + i) / 8, y[0], y[1], y[2], y[3]);
+            low[(c + i) / 8] = make_uint4(z[0], z[1], z[2], z[3]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) g[i] = act_value<false, ACT>(g[i], nullptr) * u[i];
+        boxes.put16(b[0], c / 32, g, bf16);
+      }
+    }
+    if (!live) return;
+    write(p.h, b[0], row, col, 0);
+    if (MODE == BWD) write(p.k, b[OUTS - 1], row, col, 0);
+    if (MODE == KEEP) {
+      write(p.k, b[OUTS - 2], row, col, 0);
+      write(p.k, b[OUTS - 1], row, col, 1);
+      if (p.h.tma) {
+        const uint32_t z = boxes.take();  // h's box again, once its store has read it
+#pragma unroll
+        for (int i = 0; i < W / 8; ++i) boxes.put(z, i, low[i].x, low[i].y, low[i].z, low[i].w);
+        boxes.store(z, &p.k.map, col, row, 2);
+      } else {
+#pragma unroll
+        for (int i = 0; i < W / 8; ++i) boxes.put(b[0], i, low[i].x, low[i].y, low[i].z, low[i].w);
+        boxes.store(b[0], &p.k.map, col, row, 2);
       }
     }
   }
 };
 
 // ------------------------------------------------------------------ pointwise backward
-// dg, du from dh and the kept g, u (16-bit rows), with the column sums of dg and du as
-// stored for the biases' gradients; without dh only the sums of given dg, du. A block
-// takes 8 columns per lane (256 in all) of a run of rows, a warp a row at a time.
-constexpr int PT = 256, PCOLS = 256;
+// dg, du from dh and the kept g, u (their three planes), with the column sums of dg and du
+// as stored for the biases' gradients; without dh only the sums of given dg, du. A block
+// takes 8 columns per lane (256 in all) of a run of rows, a warp two rows at a time.
+constexpr int PT = 256, PCOLS = 256, PBLOCKS = 2;  // blocks per SM
 struct PointArgs {
   const uint16_t* dh;
   int64_t lddh;
-  const uint16_t *g, *u;
+  const uint16_t *g, *u, *low;
   int64_t ldp;
   uint16_t *dg, *du;
   int64_t ldd;
   float* part;  // [gridDim.y][2][F] (NULL: no sums)
-  int M, F, act, bf16, rows, vec;
+  int M, F, bf16, rows, vec;
 };
 
-template <bool POINT>
-__global__ void __launch_bounds__(PT) gated_point_kernel(PointArgs p) {
+// 8 values of 24 bits from their upper 16 and a byte of the third plane.
+__device__ __forceinline__ void join24(const uint16_t* hi, const uint16_t* low, int n, bool up, float (&v)[8]) {
+  uint32_t h[4], l[4];
+  if (n >= 8) {
+    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(hi)), b = *reinterpret_cast<const uint4*>(low);
+    h[0] = a.x, h[1] = a.y, h[2] = a.z, h[3] = a.w, l[0] = b.x, l[1] = b.y, l[2] = b.z, l[3] = b.w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      h[k] = (2 * k < n ? hi[2 * k] : 0u) | (2 * k + 1 < n ? (uint32_t)hi[2 * k + 1] << 16 : 0u);
+      l[k] = (2 * k < n ? low[2 * k] : 0u) | (2 * k + 1 < n ? (uint32_t)low[2 * k + 1] << 16 : 0u);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    // bytes 3, 2: the upper half; byte 1: the low plane's byte (g's, or u's after it); byte 0: cleared
+    v[2 * k] = __uint_as_float(__byte_perm(h[k], l[k], up ? 0x1050 : 0x1040) & 0xffffff00u);
+    v[2 * k + 1] = __uint_as_float(__byte_perm(h[k], l[k], up ? 0x3270 : 0x3260) & 0xffffff00u);
+  }
+}
+
+template <bool POINT, int ACT>
+__global__ void __launch_bounds__(PT, PBLOCKS) gated_point_kernel(PointArgs p) {
   __shared__ float red[PT / 32][2][PCOLS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col = blockIdx.x * PCOLS + 8 * lane, n = p.F - col;
@@ -137,22 +246,26 @@ __global__ void __launch_bounds__(PT) gated_point_kernel(PointArgs p) {
   for (int k = 0; k < 8; ++k) sg[k] = su[k] = 0.f;
   const int64_t r0 = (int64_t)blockIdx.y * p.rows, r1 = std::min<int64_t>(p.M, r0 + p.rows);
   if (n > 0) {
+#pragma unroll 2
     for (int64_t r = r0 + warp; r < r1; r += PT / 32) {
       float g[8], u[8];
-      load_row16<8>(p.g + r * p.ldp + col, g, n, p.vec, bf16);
-      load_row16<8>(p.u + r * p.ldp + col, u, n, p.vec, bf16);
       if (POINT) {
         float d[8];
         load_row16<8>(p.dh + r * p.lddh + col, d, n, p.vec, bf16);
+        join24(p.g + r * p.ldp + col, p.low + r * p.ldp + col, n, false, g);
+        join24(p.u + r * p.ldp + col, p.low + r * p.ldp + col, n, true, u);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           float da;
-          const float a = act_value<true>(g[k], p.act, &da);
+          const float a = act_value<true, ACT>(g[k], &da);
           g[k] = d[k] * u[k] * da;
           u[k] = d[k] * a;
         }
-        store_row16<8>(p.dg + r * p.ldd + col, g, n, p.vec, bf16);
-        store_row16<8>(p.du + r * p.ldd + col, u, n, p.vec, bf16);
+        store_row16<8>(p.dg + r * p.ldd + col, g, n, true, bf16);
+        store_row16<8>(p.du + r * p.ldd + col, u, n, true, bf16);
+      } else {
+        load_row16<8>(p.g + r * p.ldp + col, g, n, p.vec, bf16);
+        load_row16<8>(p.u + r * p.ldp + col, u, n, p.vec, bf16);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) sg[k] += g[k], su[k] += u[k];
@@ -187,10 +300,10 @@ __global__ void __launch_bounds__(256) gated_bias_sum_kernel(const float* __rest
     store16(static_cast<uint16_t*>(dst) + c, t, dtype == PNFT_DTYPE_BF16);
 }
 
-// Rows per block of the pointwise kernel: about four blocks per SM.
+// Rows per block of the pointwise kernel: one wave of PBLOCKS per SM.
 int point_rows(int64_t M, int64_t F) {
   const int64_t cols = (F + PCOLS - 1) / PCOLS;
-  const int64_t want = std::max<int64_t>(1, 4 * sm_count() / cols);
+  const int64_t want = std::max<int64_t>(1, PBLOCKS * sm_count() / cols);
   const int64_t rows = std::max<int64_t>(16, (M + want - 1) / want);
   return (int)std::min<int64_t>(std::max<int64_t>(rows, (M + 65534) / 65535), 1 << 30);
 }
@@ -203,11 +316,21 @@ int gated_check(const char* what, int64_t M, int64_t D, int64_t F, int act, int 
   return PNFT_OK;
 }
 
-int gated_gemm(const char* what, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
-               int64_t M, int64_t D, int64_t F, int dtype, const GatedEpi::Params& ep, int32_t* status, cudaStream_t st) {
-  if (!tma_rows_ok(x, ldx, D) || !tma_rows_ok(wg, ldwg, D) || !tma_rows_ok(wu, ldwu, D))
-    return fail(PNFT_EUNSUPPORTED, "%s: x and weight rows must be 16-byte aligned (strides multiples of 8)", what);
-  if (!device_is_sm100()) return fail(PNFT_EUNSUPPORTED, "%s: needs an sm_100 device", what);
+template <int MODE, int ACT>
+int gated_launch(const char* what, const Args& a, const void* bg, const void* bu, int b_dtype, int dtype, const Out& h,
+                 const Out& k, const CUtensorMap* dh, cudaStream_t st) {
+  typename GatedEpi<MODE, ACT>::Params ep;
+  memset(&ep, 0, sizeof(ep));
+  ep.bg = bg, ep.bu = bu, ep.b_dtype = b_dtype, ep.bf16 = dtype == PNFT_DTYPE_BF16;
+  ep.h = h, ep.k = k;
+  if (dh) ep.dh = *dh;
+  return launch<false, false, true, GatedEpi<MODE, ACT>>(what, a, ep, st);
+}
+
+int gated_gemm(const char* what, int mode, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
+               int64_t ldwu, const void* bg, const void* bu, int b_dtype, const Out& h, const Out& k, const CUtensorMap* dh,
+               int64_t M, int64_t D, int64_t F, int act, int dtype, int32_t* status, cudaStream_t st) {
+  if (b_dtype < PNFT_DTYPE_F32 || b_dtype > PNFT_DTYPE_F16) return fail(PNFT_EINVAL, "%s: unknown bias type %d", what, b_dtype);
   Args a;
   memset(&a, 0, sizeof(a));
   int rc = map_kmajor(&a.ta[0], x, D, M, ldx);
@@ -217,7 +340,23 @@ int gated_gemm(const char* what, const void* x, int64_t ldx, const void* wg, int
   a.s = plain_sched(M, 2 * ((F + BN / 2 - 1) / (BN / 2) * (BN / 2)), (D + BK - 1) / BK, 1);
   a.idesc = idesc(dtype, false, false);
   a.status = status;
-  return launch<false, false, true, GatedEpi>(what, a, ep, st);
+  auto go = [&](auto m, auto c) {
+    return gated_launch<decltype(m)::value, decltype(c)::value>(what, a, bg, bu, b_dtype, dtype, h, k, dh, st);
+  };
+  auto with_act = [&](auto m) {
+    return act == PNFT_ACT_SILU ? go(m, std::integral_constant<int, PNFT_ACT_SILU>()) : go(m, std::integral_constant<int, PNFT_ACT_GELU>());
+  };
+  if (mode == FWD) return with_act(std::integral_constant<int, FWD>());
+  if (mode == KEEP) return with_act(std::integral_constant<int, KEEP>());
+  return with_act(std::integral_constant<int, BWD>());
+}
+
+int gated_operands(const char* what, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
+                   int64_t D) {
+  if (!tma_rows_ok(x, ldx, D) || !tma_rows_ok(wg, ldwg, D) || !tma_rows_ok(wu, ldwu, D))
+    return fail(PNFT_EUNSUPPORTED, "%s: x and weight rows must be 16-byte aligned (strides multiples of 8)", what);
+  if (!device_is_sm100()) return fail(PNFT_EUNSUPPORTED, "%s: needs an sm_100 device", what);
+  return PNFT_OK;
 }
 
 }  // namespace
@@ -227,96 +366,81 @@ using namespace pnft;
 using namespace pnft::tc;
 
 extern "C" int pnft_gated_fwd(const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
-                              const void* bg, const void* bu, int b_dtype, void* h, int64_t ldh, void* g, void* u,
-                              int64_t ldp, int64_t M, int64_t D, int64_t F, int act, int dtype, int32_t* status,
-                              void* stream) {
+                              const void* bg, const void* bu, int b_dtype, void* h, int64_t ldh, void* pre, int64_t ldp,
+                              int64_t M, int64_t D, int64_t F, int act, int dtype, int32_t* status, void* stream) {
   if (int rc = gated_check("gated_fwd", M, D, F, act, dtype)) return rc;
   if (M == 0) return PNFT_OK;
-  if (!h || (!g) != (!u)) return fail(PNFT_EINVAL, "gated_fwd: null output");
-  if (ldh < F || (g && ldp < F)) return fail(PNFT_EINVAL, "gated_fwd: row strides below the width");
-  GatedEpi::Params ep{bg, bu, b_dtype, static_cast<uint16_t*>(h), ldh, static_cast<uint16_t*>(g),
-                      static_cast<uint16_t*>(u), ldp, nullptr, 0, (int)M, (int)F, act, dtype == PNFT_DTYPE_BF16,
-                      rows16(h, ldh, 2), rows16(g, ldp, 2) && rows16(u, ldp, 2), 0};
-  return gated_gemm("gated_fwd", x, ldx, wg, ldwg, wu, ldwu, M, D, F, dtype, ep, status, as_stream(stream));
+  if (!h) return fail(PNFT_EINVAL, "gated_fwd: null output");
+  if (ldh < F || (pre && ldp < F)) return fail(PNFT_EINVAL, "gated_fwd: row strides below the width");
+  if (pre && !rows16(pre, ldp, 2)) return fail(PNFT_EINVAL, "gated_fwd: the kept rows must be 16-byte aligned");
+  if (int rc = gated_operands("gated_fwd", x, ldx, wg, ldwg, wu, ldwu, D)) return rc;
+  Out o, k;
+  int rc = make_out(&o, h, dtype, F, M, ldh);
+  if (!rc) rc = make_out(&k, pre, dtype, F, M, ldp, 3, M * ldp);
+  if (rc) return rc;
+  return gated_gemm("gated_fwd", pre ? KEEP : FWD, x, ldx, wg, ldwg, wu, ldwu, bg, bu, b_dtype, o, k, nullptr, M, D, F, act,
+                    dtype, status, as_stream(stream));
 }
 
-extern "C" int pnft_gated_bwd_recompute(const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
-                                        int64_t ldwu, const void* bg, const void* bu, int b_dtype, const void* dh,
-                                        int64_t lddh, void* dg, void* du, int64_t ldd, int64_t M, int64_t D, int64_t F,
-                                        int act, int dtype, int32_t* status, void* stream) {
-  if (int rc = gated_check("gated_bwd_recompute", M, D, F, act, dtype)) return rc;
-  if (M == 0) return PNFT_OK;
-  if (!dh || !dg || !du) return fail(PNFT_EINVAL, "gated_bwd_recompute: null pointer");
-  if (lddh < F || ldd < F) return fail(PNFT_EINVAL, "gated_bwd_recompute: row strides below the width");
-  GatedEpi::Params ep{bg, bu, b_dtype, nullptr, 0, static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du), ldd,
-                      static_cast<const uint16_t*>(dh), lddh, (int)M, (int)F, act, dtype == PNFT_DTYPE_BF16, 0,
-                      rows16(dg, ldd, 2) && rows16(du, ldd, 2), rows16(dh, lddh, 2)};
-  return gated_gemm("gated_bwd_recompute", x, ldx, wg, ldwg, wu, ldwu, M, D, F, dtype, ep, status, as_stream(stream));
+namespace {
+
+// Buffers of a backward call: dg, du side by side (each padded to whole row tiles of the
+// weight-gradient product), dh with aligned rows where the caller's are not, the biases'
+// partial sums, and the partial sums of the two products (one after the other).
+struct BwdLayout {
+  int64_t Fp;
+  size_t d, dh, bias, part, total;
+};
+BwdLayout bwd_layout(int64_t M, int64_t D, int64_t F) {
+  BwdLayout l;
+  l.Fp = (F + BM - 1) / BM * BM;
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t r = at;
+    at += (n + 255) / 256 * 256;
+    return r;
+  };
+  l.d = take(2 * (size_t)M * 2 * l.Fp);
+  l.dh = take(F % 8 ? 2 * (size_t)M * l.Fp : 0);
+  l.bias = take(sizeof(float) * 2 * (size_t)F * (size_t)((M + point_rows(M, F) - 1) / point_rows(M, F)));
+  const int s = plan_splits(tiles_of(M, D), 2 * ((F + BK - 1) / BK));
+  const size_t dx = s > 1 ? sizeof(float) * (size_t)s * (size_t)M * (size_t)((D + 3) / 4 * 4) : 0;
+  l.part = take(std::max(dx, pnft_weight_grad_workspace_size(M, 2 * l.Fp, D)));
+  l.total = at;
+  return l;
 }
 
-extern "C" size_t pnft_gated_bias_workspace_size(int64_t M, int64_t F) {
-  if (M <= 0 || F <= 0) return 0;
-  const int64_t rows = point_rows(M, F);
-  return sizeof(float) * 2 * (size_t)F * (size_t)((M + rows - 1) / rows);
-}
-
-extern "C" int pnft_gated_bwd_point(const void* dh, int64_t lddh, const void* g, const void* u, int64_t ldp, void* dg,
-                                    void* du, int64_t ldd, void* dbg, void* dbu, int b_dtype, void* workspace,
-                                    size_t workspace_bytes, int64_t M, int64_t F, int act, int dtype, void* stream) {
-  if (int rc = gated_check("gated_bwd_point", M, 1, F, act, dtype)) return rc;
+int point(const uint16_t* dh, int64_t lddh, const void* pre, int64_t ldp, uint16_t* dg, uint16_t* du, int64_t ldd, void* dbg,
+          void* dbu, int b_dtype, float* part, int64_t M, int64_t F, int act, int dtype, cudaStream_t st) {
   const bool sums = dbg || dbu;
-  cudaStream_t st = as_stream(stream);
-  if (M == 0) {
-    const size_t n = (size_t)F * (b_dtype == PNFT_DTYPE_F32 ? 4 : 2);
-    if ((dbg && cudaMemsetAsync(dbg, 0, n, st) != cudaSuccess) || (dbu && cudaMemsetAsync(dbu, 0, n, st) != cudaSuccess))
-      return check_launch("gated_bwd_point memset", 0);
-    return PNFT_OK;
-  }
-  if (!g || !u || (dh && (!dg || !du)) || (!dh && !sums)) return fail(PNFT_EINVAL, "gated_bwd_point: null pointer");
-  if (ldp < F || (dh && (lddh < F || ldd < F))) return fail(PNFT_EINVAL, "gated_bwd_point: row strides below the width");
-  const size_t need = sums ? pnft_gated_bias_workspace_size(M, F) : 0;
-  if (sums && (!workspace || workspace_bytes < need))
-    return fail(PNFT_EINVAL, "gated_bwd_point: workspace of %zu bytes < required %zu", workspace_bytes, need);
   PointArgs p;
   memset(&p, 0, sizeof(p));
-  p.dh = static_cast<const uint16_t*>(dh), p.lddh = lddh;
-  p.g = static_cast<const uint16_t*>(g), p.u = static_cast<const uint16_t*>(u), p.ldp = ldp;
-  p.dg = static_cast<uint16_t*>(dg), p.du = static_cast<uint16_t*>(du), p.ldd = ldd;
-  p.part = sums ? static_cast<float*>(workspace) : nullptr;
-  p.M = (int)M, p.F = (int)F, p.act = act, p.bf16 = dtype == PNFT_DTYPE_BF16;
+  if (dh) {
+    p.dh = dh, p.lddh = lddh;
+    p.g = static_cast<const uint16_t*>(pre), p.u = p.g + M * ldp, p.low = p.u + M * ldp, p.ldp = ldp;
+    p.vec = rows16(dh, lddh, 2);
+  } else {
+    p.g = dg, p.u = du, p.ldp = ldd, p.vec = 1;
+  }
+  p.dg = dg, p.du = du, p.ldd = ldd;
+  p.part = sums ? part : nullptr;
+  p.M = (int)M, p.F = (int)F, p.bf16 = dtype == PNFT_DTYPE_BF16;
   p.rows = point_rows(M, F);
-  p.vec = rows16(g, ldp, 2) && rows16(u, ldp, 2) && (!dh || (rows16(dh, lddh, 2) && rows16(dg, ldd, 2) && rows16(du, ldd, 2)));
   const dim3 grid((unsigned)((F + PCOLS - 1) / PCOLS), (unsigned)((M + p.rows - 1) / p.rows));
-  if (dh)
-    gated_point_kernel<true><<<grid, PT, 0, st>>>(p);
+  if (!dh)
+    gated_point_kernel<false, 0><<<grid, PT, 0, st>>>(p);
+  else if (act == PNFT_ACT_SILU)
+    gated_point_kernel<true, PNFT_ACT_SILU><<<grid, PT, 0, st>>>(p);
   else
-    gated_point_kernel<false><<<grid, PT, 0, st>>>(p);
+    gated_point_kernel<true, PNFT_ACT_GELU><<<grid, PT, 0, st>>>(p);
   if (sums)
     gated_bias_sum_kernel<<<(unsigned)((2 * F + 255) / 256), 256, 0, st>>>(p.part, (int)grid.y, (int)F, dbg, dbu, b_dtype);
-  return check_launch("gated_bwd_point", sums ? 2 : 1);
+  return check_launch("gated_bwd pointwise", sums ? 2 : 1);
 }
 
-static int dx_splits(int64_t M, int64_t D, int64_t F) {
-  return plan_splits((int)(((M + BM - 1) / BM) * ((D + BN - 1) / BN)), (int)(2 * ((F + BK - 1) / BK)));
-}
-
-extern "C" size_t pnft_gated_dx_workspace_size(int64_t M, int64_t D, int64_t F) {
-  if (M <= 0 || D <= 0 || F <= 0) return 0;
-  const int s = dx_splits(M, D, F);
-  return s > 1 ? sizeof(float) * (size_t)s * (size_t)M * (size_t)((D + 3) / 4 * 4) : 0;
-}
-
-extern "C" int pnft_gated_dx(const void* dg, const void* du, int64_t ldd, const void* wg, int64_t ldwg, const void* wu,
-                             int64_t ldwu, void* dx, int64_t lddx, int dx_dtype, void* workspace, size_t workspace_bytes,
-                             int64_t M, int64_t D, int64_t F, int dtype, int32_t* status, void* stream) {
-  if (int rc = gated_check("gated_dx", M, D, F, PNFT_ACT_SILU, dtype)) return rc;
-  if (M == 0) return PNFT_OK;
-  if (!dx || lddx < D) return fail(PNFT_EINVAL, "gated_dx: null output or row stride below the width");
-  if (dx_dtype < PNFT_DTYPE_F32 || dx_dtype > PNFT_DTYPE_F16) return fail(PNFT_EINVAL, "gated_dx: unknown output type %d", dx_dtype);
-  if (!tma_rows_ok(dg, ldd, F) || !tma_rows_ok(du, ldd, F) || !tma_rows_ok(wg, ldwg, D) || !tma_rows_ok(wu, ldwu, D))
-    return fail(PNFT_EUNSUPPORTED, "gated_dx: operand rows must be 16-byte aligned (strides multiples of 8)");
-  if (!device_is_sm100()) return fail(PNFT_EUNSUPPORTED, "gated_dx: needs an sm_100 device");
-  cudaStream_t st = as_stream(stream);
+int gated_dx(const uint16_t* dg, const uint16_t* du, int64_t ldd, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
+             void* dx, int64_t lddx, int dx_dtype, void* part, int64_t M, int64_t D, int64_t F, int dtype, int32_t* status,
+             cudaStream_t st) {
   Args a;
   memset(&a, 0, sizeof(a));
   int rc = map_kmajor(&a.ta[0], dg, F, M, ldd);
@@ -324,20 +448,90 @@ extern "C" int pnft_gated_dx(const void* dg, const void* du, int64_t ldd, const 
   if (!rc) rc = map_mnmajor(&a.tb[0], wg, D, F, ldwg);
   if (!rc) rc = map_mnmajor(&a.tb[1], wu, D, F, ldwu);
   if (rc) return rc;
-  const int kb = (int)((F + BK - 1) / BK), splits = dx_splits(M, D, F);
+  const int kb = (int)((F + BK - 1) / BK), splits = plan_splits(tiles_of(M, D), 2 * kb);
   a.s = plain_sched(M, D, 2 * kb, splits);
   a.s.seg_kb = kb;
   a.idesc = idesc(dtype, false, true);
   a.status = status;
-  const int osize = dx_dtype == PNFT_DTYPE_F32 ? 4 : 2;
-  StoreEpi::Params out{{dx, nullptr}, lddx, 0x7fffffff, (int)M, (int)D, nullptr, dx_dtype, 0, 0, rows16(dx, lddx, osize)};
-  if (splits == 1) return launch<false, true, false, StoreEpi>("gated_dx", a, out, st);
-  const size_t need = pnft_gated_dx_workspace_size(M, D, F);
-  if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
-    return fail(PNFT_EINVAL, "gated_dx: workspace of %zu bytes < required %zu (16-byte aligned)", workspace_bytes, need);
+  StoreEpi<false>::Params out;
+  memset(&out, 0, sizeof(out));
+  out.row_split = 0x7fffffff;
+  out.dtype = dx_dtype;
+  if (splits == 1) {
+    rc = make_out(&out.c[0], dx, dx_dtype, D, M, lddx);
+    return rc ? rc : launch_store<false, true>("gated_bwd dx", a, out, st);
+  }
   const int64_t ldp = (D + 3) / 4 * 4;
-  StoreEpi::Params part{{workspace, nullptr}, ldp, 0x7fffffff, (int)M, (int)D, nullptr, PNFT_DTYPE_F32, 0, M * ldp, 1};
-  rc = launch<false, true, false, StoreEpi>("gated_dx", a, part, st);
+  out.dtype = PNFT_DTYPE_F32;
+  rc = make_out(&out.c[0], part, PNFT_DTYPE_F32, D, M, ldp, splits, M * ldp);
+  if (!rc) rc = launch_store<false, true>("gated_bwd dx", a, out, st);
   if (rc) return rc;
-  return sum_splits(static_cast<const float*>(workspace), ldp, M * ldp, splits, out, (int)M, st);
+  const SumArgs sum{{dx, nullptr}, lddx, 0x7fffffff, (int)M, (int)D, nullptr, dx_dtype, 0, rows16(dx, lddx, dtype_size(dx_dtype))};
+  return sum_splits(static_cast<const float*>(part), ldp, M * ldp, splits, sum, (int)M, st);
+}
+
+}  // namespace
+
+extern "C" size_t pnft_gated_bwd_workspace_size(int64_t M, int64_t D, int64_t F) {
+  return M <= 0 || D <= 0 || F <= 0 ? 0 : bwd_layout(M, D, F).total;
+}
+
+extern "C" int pnft_gated_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
+                              const void* bg, const void* bu, int b_dtype, const void* pre, int64_t ldp, const void* dh,
+                              int64_t lddh, void* dx, int64_t lddx, int dx_dtype, void* dwg, void* dwu, int64_t lddw,
+                              int dw_dtype, void* dbg, void* dbu, void* workspace, size_t workspace_bytes, int64_t M,
+                              int64_t D, int64_t F, int act, int dtype, int32_t* status, void* stream) {
+  if (int rc = gated_check("gated_bwd", M, D, F, act, dtype)) return rc;
+  for (int t : {b_dtype, dx_dtype, dw_dtype})
+    if (t < PNFT_DTYPE_F32 || t > PNFT_DTYPE_F16) return fail(PNFT_EINVAL, "gated_bwd: unknown type %d", t);
+  if ((dx && lddx < D) || ((dwg || dwu) && lddw < D)) return fail(PNFT_EINVAL, "gated_bwd: row strides below the width");
+  cudaStream_t st = as_stream(stream);
+  if (M == 0) {
+    for (void* d : {dwg, dwu})
+      if (d && cudaMemset2DAsync(d, (size_t)lddw * dtype_size(dw_dtype), 0, (size_t)D * dtype_size(dw_dtype), (size_t)F, st) !=
+                   cudaSuccess)
+        return check_launch("gated_bwd memset", 0);
+    for (void* d : {dbg, dbu})
+      if (d && cudaMemsetAsync(d, 0, (size_t)F * dtype_size(b_dtype), st) != cudaSuccess) return check_launch("gated_bwd memset", 0);
+    return PNFT_OK;
+  }
+  if (!dh) return fail(PNFT_EINVAL, "gated_bwd: null pointer");
+  if (lddh < F || (pre && ldp < F)) return fail(PNFT_EINVAL, "gated_bwd: row strides below the width");
+  if (pre && !rows16(pre, ldp, 2)) return fail(PNFT_EINVAL, "gated_bwd: the kept rows must be 16-byte aligned");
+  const BwdLayout l = bwd_layout(M, D, F);
+  if (!workspace || workspace_bytes < l.total || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(PNFT_EINVAL, "gated_bwd: workspace of %zu bytes < required %zu (16-byte aligned)", workspace_bytes, l.total);
+  if (F % 8 == 0 && !pre && !rows16(dh, lddh, 2))
+    return fail(PNFT_EUNSUPPORTED, "gated_bwd: dh rows must be 16-byte aligned (or F not a multiple of 8)");
+  if (int rc = gated_operands("gated_bwd", x, ldx, wg, ldwg, wu, ldwu, D)) return rc;
+  char* ws = static_cast<char*>(workspace);
+  uint16_t* dg = reinterpret_cast<uint16_t*>(ws + l.d);
+  uint16_t* du = dg + l.Fp;
+  const int64_t ldd = 2 * l.Fp;
+  float* bias = reinterpret_cast<float*>(ws + l.bias);
+  int rc = PNFT_OK;
+  if (pre) {
+    rc = point(static_cast<const uint16_t*>(dh), lddh, pre, ldp, dg, du, ldd, dbg, dbu, b_dtype, bias, M, F, act, dtype, st);
+  } else {
+    const void* d = dh;
+    int64_t ldh = lddh;
+    if (!rows16(dh, lddh, 2)) {  // TMA reads dh: bring its rows to 16 bytes
+      d = ws + l.dh, ldh = l.Fp;
+      rc = pnft_copy_rows16(dh, lddh, ws + l.dh, l.Fp, M, F, stream);
+    }
+    Out g, u;
+    CUtensorMap map;
+    if (!rc) rc = make_out(&g, dg, dtype, F, M, ldd);
+    if (!rc) rc = make_out(&u, du, dtype, F, M, ldd);
+    if (!rc) rc = tma_map_out(&map, d, 2, F, M, ldh, 1, 0, 32);
+    if (!rc)
+      rc = gated_gemm("gated_bwd", BWD, x, ldx, wg, ldwg, wu, ldwu, bg, bu, b_dtype, g, u, &map, M, D, F, act, dtype, status, st);
+    if (!rc && (dbg || dbu))
+      rc = point(nullptr, 0, nullptr, 0, dg, du, ldd, dbg, dbu, b_dtype, bias, M, F, act, dtype, st);
+  }
+  if (!rc && dx) rc = gated_dx(dg, du, ldd, wg, ldwg, wu, ldwu, dx, lddx, dx_dtype, ws + l.part, M, D, F, dtype, status, st);
+  if (!rc && (dwg || dwu))
+    rc = weight_grad("gated_bwd dW", dg, ldd, x, ldx, dwg, dwu, lddw, l.Fp, F, dw_dtype, ws + l.part, M, 2 * l.Fp, D, dtype,
+                     status, st);
+  return rc;
 }

@@ -13,16 +13,16 @@ int sm_count() {
   return n;
 }
 
-int plan_splits(int tiles, int kb) {
-  const int want = std::max(1, sm_count() / std::max(1, tiles));
-  return std::max(1, std::min(want, kb / 8));
+int plan_splits(int64_t tiles, int64_t kb) {
+  const int64_t want = std::max<int64_t>(1, sm_count() / 2 / std::max<int64_t>(1, tiles));
+  return (int)std::max<int64_t>(1, std::min(want, kb / 8));
 }
 
 namespace {
 
 // Four columns per thread; partial rows are 16-byte aligned (ldp a multiple of 4).
 __global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict__ part, int64_t ldp,
-                                                         int64_t split_stride, int splits, StoreEpi::Params o,
+                                                         int64_t split_stride, int splits, SumArgs o,
                                                          int rows_total) {
   const int n4 = (o.cols + 3) / 4;
   const float alpha = o.alpha ? *o.alpha : 1.f;
@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict
     const float* src = part + (int64_t)row * ldp + c;
     const int side = row >= o.row_split;
     if (side) row -= o.row_split;
-    if (row >= o.rows) continue;
+    if (row >= o.rows || !(side ? o.c[1] : o.c[0])) continue;
     float4 a = *reinterpret_cast<const float4*>(src);
 #pragma unroll 4
     for (int s = 1; s < splits; ++s) {
@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict
     const int64_t at = (int64_t)row * o.ldc + c;
     if (o.dtype == PNFT_DTYPE_F32) {
       float* dst = static_cast<float*>(side ? o.c[1] : o.c[0]) + at;
-      for (int k = 0; k < n; ++k) dst[k] = o.accumulate ? dst[k] + v[k] : v[k];
+      for (int k = 0; k < n; ++k) dst[k] = o.add ? dst[k] + v[k] : v[k];
     } else {
       const bool bf16 = o.dtype == PNFT_DTYPE_BF16;
       uint16_t* dst = static_cast<uint16_t*>(side ? o.c[1] : o.c[0]) + at;
@@ -57,18 +57,29 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict
   }
 }
 
-// dst[r] = src[r], rows of `bytes`; the widths and strides are free, so the copy
-// takes 4-byte words when both rows allow it and 2-byte elements otherwise.
+// dst[r] = src[r] for rows of any alignment: a warp per row, eight words in flight per lane.
 template <typename W>
 __global__ void __launch_bounds__(256) copy_rows_kernel(const char* __restrict__ src, int64_t ss, char* __restrict__ dst,
                                                         int64_t ds, int64_t rows, int64_t words) {
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256)
-      reinterpret_cast<W*>(dst + r * ds)[i] = reinterpret_cast<const W*>(src + r * ss)[i];
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
+    const W* from = reinterpret_cast<const W*>(src + r * ss);
+    W* to = reinterpret_cast<W*>(dst + r * ds);
+    for (int64_t i = lane; i < words; i += 256) {
+      W v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i + 32 * k < words) v[k] = from[i + 32 * k];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i + 32 * k < words) to[i + 32 * k] = v[k];
+    }
+  }
 }
+
 }  // namespace
 
-int sum_splits(const float* part, int64_t ldp, int64_t split_stride, int splits, const StoreEpi::Params& out,
+int sum_splits(const float* part, int64_t ldp, int64_t split_stride, int splits, const SumArgs& out,
                int rows_total, cudaStream_t st) {
   const int64_t items = (int64_t)rows_total * ((out.cols + 3) / 4);
   const int64_t blocks = std::min<int64_t>((items + 255) / 256, (int64_t)sm_count() * 8);
@@ -82,9 +93,46 @@ int sum_splits(const float* part, int64_t ldp, int64_t split_stride, int splits,
 using namespace pnft;
 using namespace pnft::tc;
 
-static int wgrad_splits(int64_t K, int64_t M, int64_t N) {
-  return plan_splits((int)(((M + BM - 1) / BM) * ((N + BN - 1) / BN)), (int)((K + BK - 1) / BK));
+static int wgrad_splits(int64_t K, int64_t M, int64_t N) { return plan_splits(tiles_of(M, N), (K + BK - 1) / BK); }
+
+namespace pnft {
+namespace tc {
+
+int weight_grad(const char* what, const void* dy, int64_t lddy, const void* x, int64_t ldx, void* c0, void* c1, int64_t ldc,
+                int64_t row_split, int64_t rows, int c_dtype, void* workspace, int64_t K, int64_t M, int64_t N, int dtype,
+                int32_t* status, cudaStream_t st) {
+  Args a;
+  memset(&a, 0, sizeof(a));
+  int rc = map_mnmajor(&a.ta[0], dy, M, K, lddy);
+  if (!rc) rc = map_mnmajor(&a.tb[0], x, N, K, ldx);
+  if (rc) return rc;
+  const int splits = wgrad_splits(K, M, N);
+  a.s = plain_sched(M, N, (K + BK - 1) / BK, splits);
+  a.idesc = idesc(dtype, true, true);
+  a.status = status;
+  StoreEpi<false>::Params out;
+  memset(&out, 0, sizeof(out));
+  out.row_split = (int)row_split;
+  out.dtype = c_dtype;
+  if (splits == 1) {
+    rc = make_out(&out.c[0], c0, c_dtype, N, rows, ldc);
+    if (!rc && row_split < M) rc = make_out(&out.c[1], c1, c_dtype, N, rows, ldc);
+    return rc ? rc : launch_store<true, true>(what, a, out, st);
+  }
+  const int64_t ldp = (N + 3) / 4 * 4;
+  out.row_split = 0x7fffffff;
+  out.dtype = PNFT_DTYPE_F32;
+  rc = make_out(&out.c[0], workspace, PNFT_DTYPE_F32, N, M, ldp, splits, M * ldp);
+  if (!rc) rc = launch_store<true, true>(what, a, out, st);
+  if (rc) return rc;
+  const SumArgs sum{{c0, c1}, ldc, (int)row_split, (int)rows, (int)N, nullptr, c_dtype, 0,
+                    rows16(c0, ldc, dtype_size(c_dtype)) && rows16(c1, ldc, dtype_size(c_dtype))};
+  return sum_splits(static_cast<const float*>(workspace), ldp, M * ldp, splits, sum, (int)M, st);
 }
+
+}  // namespace tc
+}  // namespace pnft
+
 
 extern "C" size_t pnft_weight_grad_workspace_size(int64_t K, int64_t M, int64_t N) {
   if (K <= 0 || M <= 0 || N <= 0) return 0;
@@ -101,6 +149,7 @@ extern "C" int pnft_weight_grad(const void* dy, int64_t lddy, const void* x, int
   if (c_dtype < PNFT_DTYPE_F32 || c_dtype > PNFT_DTYPE_F16) return fail(PNFT_EINVAL, "weight_grad: unknown output type %d", c_dtype);
   if (!c0 || (row_split < M && !c1)) return fail(PNFT_EINVAL, "weight_grad: null output");
   if (row_split >= M) row_split = 0x7fffffff, rows = std::min(rows, M);  // one output
+  if (row_split < M && row_split % BM) return fail(PNFT_EINVAL, "weight_grad: row_split must be a multiple of %d", BM);
   if (rows <= 0 || row_split < rows || (row_split < M && row_split + rows > M) || ldc < N) return fail(PNFT_EINVAL, "weight_grad: bad output layout");
   const int osize = c_dtype == PNFT_DTYPE_F32 ? 4 : 2;
   cudaStream_t st = as_stream(stream);
@@ -116,26 +165,11 @@ extern "C" int pnft_weight_grad(const void* dy, int64_t lddy, const void* x, int
   if (!tma_rows_ok(dy, lddy, M) || !tma_rows_ok(x, ldx, N))
     return fail(PNFT_EUNSUPPORTED, "weight_grad: operand rows must be 16-byte aligned (strides multiples of 8)");
   if (!device_is_sm100()) return fail(PNFT_EUNSUPPORTED, "weight_grad: needs an sm_100 device");
-  Args a;
-  memset(&a, 0, sizeof(a));
-  int rc = map_mnmajor(&a.ta[0], dy, M, K, lddy);
-  if (!rc) rc = map_mnmajor(&a.tb[0], x, N, K, ldx);
-  if (rc) return rc;
-  const int splits = wgrad_splits(K, M, N);
-  a.s = plain_sched(M, N, (K + BK - 1) / BK, splits);
-  a.idesc = idesc(dtype, true, true);
-  a.status = status;
-  StoreEpi::Params out{{c0, c1}, ldc, (int)row_split, (int)rows, (int)N, nullptr, c_dtype, 0, 0,
-                       rows16(c0, ldc, osize) && rows16(c1, ldc, osize)};
-  if (splits == 1) return launch<true, true, false, StoreEpi>("weight_grad", a, out, st);
   const size_t need = pnft_weight_grad_workspace_size(K, M, N);
-  if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(PNFT_EINVAL, "weight_grad: workspace of %zu bytes < required %zu (16-byte aligned)", workspace_bytes, need);
-  const int64_t ldp = (N + 3) / 4 * 4;
-  StoreEpi::Params part{{workspace, nullptr}, ldp, 0x7fffffff, (int)M, (int)N, nullptr, PNFT_DTYPE_F32, 0, M * ldp, 1};
-  rc = launch<true, true, false, StoreEpi>("weight_grad", a, part, st);
-  if (rc) return rc;
-  return sum_splits(static_cast<const float*>(workspace), ldp, M * ldp, splits, out, (int)M, st);
+  return weight_grad("weight_grad", dy, lddy, x, ldx, c0, c1, ldc, row_split, rows, c_dtype, workspace, K, M, N, dtype,
+                     status, st);
 }
 
 extern "C" int pnft_copy_rows16(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols,
@@ -146,7 +180,7 @@ extern "C" int pnft_copy_rows16(const void* src, int64_t lds, void* dst, int64_t
   const uintptr_t any = reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) | (uintptr_t)(lds * 2) |
                         (uintptr_t)(ldd * 2) | (uintptr_t)(cols * 2);
   const int64_t w = any % 16 == 0 ? 16 : any % 4 == 0 ? 4 : 2, words = cols * 2 / w;
-  const dim3 grid((unsigned)std::min<int64_t>((words + 255) / 256, 64), (unsigned)std::min<int64_t>(rows, 8192));
+  const unsigned grid = (unsigned)std::min<int64_t>((rows + 7) / 8, (int64_t)sm_count() * 8);
   const char* s = static_cast<const char*>(src);
   char* d = static_cast<char*>(dst);
   cudaStream_t st = as_stream(stream);

@@ -3,14 +3,17 @@
 //
 //   acc[m, n] = sum_k A[m, k] B[n, k]     (bf16 or fp16 operands, fp32 in TMEM)
 //
-// One CTA per SM walks work items; an item is a 128 x 256 output tile (or, for
-// epilogues that carry state along a row, a strip of such tiles), optionally one
-// of several splits of K. Warp 0 loads 64-deep stages of A and B by TMA into a
-// ring, one lane of warp 1 issues the MMAs (M = 128, N = 256, K = 16) into one of
-// two TMEM accumulators, warps 2-9 run the epilogue of the other, so the epilogue
-// of a tile overlaps the next tile's MMAs. Either operand may be K-major (rows of
-// K) or MN-major (K rows of M or N), so no caller transposes anything. Rows,
-// columns and K past the end are zero-filled by TMA.
+// Two CTAs of a cluster (one per SM) share a 256 x 256 output tile: each holds 128 rows
+// of A and 128 rows of B in shared memory, and the even CTA issues the MMAs of both
+// (cta_group::2, M = 256, N = 256, K = 16), so an operand byte brought into an SM feeds
+// twice the products of a one-CTA tile. Each CTA has its 128 rows of the accumulator in
+// its own TMEM, twice (2 x 256 columns). The pair walks work items; an item is one tile
+// (or, for epilogues that carry state along a row, a strip of tiles), optionally one of
+// several splits of K. Warp 0 loads 64-deep stages of A and B by TMA into a ring, one
+// lane of the even CTA's warp 1 issues the MMAs, and warps 2-9 run the epilogue of the
+// other accumulator, so a tile's epilogue overlaps the next tile's MMAs. Either operand
+// may be K-major (rows of K) or MN-major (K rows of M or N), so no caller transposes
+// anything. Rows, columns and K past the end are zero-filled by TMA.
 #pragma once
 
 #include <string.h>
@@ -25,25 +28,99 @@ namespace tc {
 
 using namespace sm100;
 
-constexpr int BM = 128, BN = 256, BK = 64;
-constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
-constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int STAGES = 4;
-constexpr int GROUP_BYTES = 64 * BK * 2;  // MN-major: 64 columns x 64 K rows
-constexpr int SMEM = STAGES * STAGE_BYTES + 1024;
+constexpr int BM = 128;       // rows per CTA (TMEM lanes)
+constexpr int PM = 2 * BM;    // rows per pair
+constexpr int BN = 256, BK = 64;
+constexpr int HALF_BYTES = BM * BK * 2;    // a CTA's A rows, or its half of B, of one stage
+constexpr int STAGE_BYTES = 2 * HALF_BYTES;
+constexpr int GROUP_BYTES = 64 * BK * 2;   // MN-major: 64 columns x 64 K rows
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 32 * (2 + EPI_WARPS);
+constexpr int STAGE_MAX = 226 * 1024;      // shared memory for the ring and the epilogue's buffers
+constexpr int BOX_BYTES = 4096;            // an epilogue box: 32 rows of 128 bytes, 128-byte swizzled
+
+// ------------------------------------------------------------------ PTX of the pair
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Address of the same shared-memory location in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Load into this CTA's shared memory, completing on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish_pair() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kSw128DescHi)
+      : "memory");
+}
+// Arrive on `bar` in both CTAs once every MMA issued so far completes.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
 
 // Which tiles there are and in which order: items of one split are taken group_m
-// row tiles at a time, the row tile running fastest, so the CTAs in flight share
+// row tiles at a time, the row tile running fastest, so the pairs in flight share
 // both operands in L2.
 struct Sched {
-  int tiles_m;          // row tiles (upper bound when live is given)
+  int tiles_m;          // 256-row tiles (upper bound when live is given)
   int strips;           // items along N
   int tiles_n;          // column tiles
   int tiles_per_strip;  // column tiles per item
   int kb;               // 64-deep K blocks (upper bound when live_k)
   int splits;           // splits of K
+  int chunk;            // K blocks that one accumulator takes before the epilogue collects it
   int group_m;
   int seg_kb;           // K blocks of the first pair of maps; the rest use the second
   const int32_t* live;  // device: rows that count (NULL: all)
@@ -59,6 +136,7 @@ struct Args {
 
 struct Item {
   int mt, nt0, ntn, split, kb0, kbn;
+  int row0;  // first row of this CTA
 };
 
 struct Walk {
@@ -67,12 +145,12 @@ struct Walk {
     tiles_m = s.tiles_m, kb = s.kb;
     if (s.live) {
       const int n = *s.live;
-      if (s.live_m) tiles_m = (n + BM - 1) / BM;
+      if (s.live_m) tiles_m = (n + PM - 1) / PM;
       if (s.live_k) kb = (n + BK - 1) / BK;
     }
     items = tiles_m * s.strips * s.splits;
   }
-  __device__ Item at(const Sched& s, int i) const {
+  __device__ Item at(const Sched& s, int i, int rank) const {
     Item it;
     const int per_split = tiles_m * s.strips;
     it.split = i / per_split;
@@ -81,6 +159,7 @@ struct Walk {
     r -= g * per;
     const int gm = min(s.group_m, tiles_m - g * s.group_m);
     it.mt = g * s.group_m + r % gm;
+    it.row0 = it.mt * PM + rank * BM;
     const int strip = r / gm;
     it.nt0 = strip * s.tiles_per_strip;
     it.ntn = min(s.tiles_per_strip, s.tiles_n - it.nt0);
@@ -91,55 +170,102 @@ struct Walk {
   }
 };
 
-// What an epilogue warp knows: its TMEM lane quadrant, its half of the columns.
-struct EpiWarp {
-  int quad, half, lane;
-  __device__ int row() const { return 32 * quad + lane; }
-  __device__ uint32_t lanes() const { return (uint32_t)(32 * quad) << 16; }
+// The accumulators in the order in which they are filled: item by item, tile by tile,
+// and within a tile one per `chunk` K blocks (at least one, empty where K is).
+struct Steps {
+  const Walk& walk;
+  const Sched& s;
+  int i, stride, rank, nt, kb;
+  Item it;
+  __device__ Steps(const Walk& w, const Sched& s_, int pair, int pairs, int rank_)
+      : walk(w), s(s_), i(pair), stride(pairs), rank(rank_) {
+    load();
+  }
+  __device__ void load() {
+    if (i < walk.items) it = walk.at(s, i, rank), nt = it.nt0, kb = it.kb0;
+  }
+  __device__ bool valid() const { return i < walk.items; }
+  __device__ int kb_end() const { return min(kb + s.chunk, it.kb0 + it.kbn); }
+  __device__ bool tile_first() const { return kb == it.kb0; }
+  __device__ bool tile_last() const { return kb + s.chunk >= it.kb0 + it.kbn; }
+  __device__ bool item_first() const { return nt == it.nt0 && tile_first(); }
+  __device__ bool item_last() const { return nt == it.nt0 + it.ntn - 1 && tile_last(); }
+  __device__ void next() {
+    if (!tile_last()) {
+      kb += s.chunk;
+      return;
+    }
+    kb = it.kb0;
+    if (++nt == it.nt0 + it.ntn) {
+      i += stride;
+      load();
+    }
+  }
 };
 
-// Epi: item_begin(item), tile(item, nt, acc, zero, release), item_end(item).
-// `acc` is the accumulator's TMEM address with the warp's lanes; `zero` says that
-// no K block contributed (the accumulator is then undefined and stands for 0);
-// release() hands the accumulator back once its last column is in registers.
-// DUAL_B: columns 0-127 of a tile come from tb[0] and 128-255 from tb[1], both at
-// row 128 * nt.
+// What an epilogue warp has: its TMEM lane quadrant, its half of the columns, its boxes
+// in shared memory and a barrier for loads into them.
+struct EpiWarp {
+  int quad, half, lane;
+  uint32_t smem, bar;
+  __device__ int row() const { return 32 * quad + lane; }
+};
+
+// Epi: BOXES (4 KB buffers per warp); tile(steps, acc, release) for every accumulator
+// (acc: its TMEM address with the warp's lanes; release() hands it back once its last
+// column is in registers), done() at the end.
+// DUAL_B: columns 0-127 of a tile come from tb[0] and 128-255 from tb[1], both at row
+// 128 * nt.
+template <class Epi>
+constexpr int stages() {
+  return (STAGE_MAX - EPI_WARPS * Epi::BOXES * BOX_BYTES) / STAGE_BYTES;
+}
+template <class Epi>
+constexpr int smem_bytes() {
+  return stages<Epi>() * STAGE_BYTES + EPI_WARPS * Epi::BOXES * BOX_BYTES + 1024;
+}
+
 template <bool A_MN, bool B_MN, bool DUAL_B, class Epi>
-__global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant__ Args p,
-                                                          const __grid_constant__ typename Epi::Params ep) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    gemm_kernel(const __grid_constant__ Args p, const __grid_constant__ typename Epi::Params ep) {
+  constexpr int STAGES = stages<Epi>();
   extern __shared__ __align__(1024) uint8_t raw[];
   const uint32_t sb = (smem_u32(raw) + 1023u) & ~1023u;
-  __shared__ __align__(8) uint64_t bars[2 * STAGES + 5];  // full, empty, acc full x2, acc empty x2, done
+  __shared__ __align__(8) uint64_t bars[2 * STAGES + 5 + EPI_WARPS];  // full, empty, acc full x2, acc empty x2, done, warps
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const uint32_t b0 = smem_u32(bars);
   auto full = [&](int s) { return b0 + 8u * s; };
   auto empty = [&](int s) { return b0 + 8u * (STAGES + s); };
   auto acc_full = [&](int s) { return b0 + 8u * (2 * STAGES + s); };
   auto acc_empty = [&](int s) { return b0 + 8u * (2 * STAGES + 2 + s); };
   const uint32_t done = b0 + 8u * (2 * STAGES + 4);
+  auto warp_bar = [&](int w) { return b0 + 8u * (2 * STAGES + 5 + w); };
   const Abort ab{&abort_flag, p.status};
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(full(s), 1);
-      mbar_init(empty(s), 1);
+      mbar_init(full(s), 1);   // the even CTA's: its producer's arrival, and the bytes of both CTAs
+      mbar_init(empty(s), 1);  // the MMAs that read the stage, told to both CTAs
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(acc_full(s), 1);
-      mbar_init(acc_empty(s), EPI_WARPS);
+      mbar_init(acc_empty(s), 2 * EPI_WARPS);  // the even CTA's: the epilogue warps of both
     }
     mbar_init(done, 1);
+    for (int w = 0; w < EPI_WARPS; ++w) mbar_init(warp_bar(w), 1);
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(&tmem_slot), 2 * BN);
-    tmem_relinquish();
+    tmem_alloc_pair(smem_u32(&tmem_slot), 2 * BN);
+    tmem_relinquish_pair();
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // the other CTA's barriers are ready for this one's arrivals
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
   const Walk walk(p.s);
@@ -149,111 +275,99 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
     if (lane == 0) {
       int st = 0, ph = 1, issued = 0;
       bool ok = true;
-      for (int i = blockIdx.x; ok && i < walk.items; i += gridDim.x) {
-        const Item it = walk.at(p.s, i);
-        for (int nt = it.nt0; ok && nt < it.nt0 + it.ntn; ++nt) {
-          for (int kb = it.kb0; kb < it.kb0 + it.kbn; ++kb) {
-            if (!mbar_wait(empty(st), ph, ab)) {
-              ok = false;
-              break;
-            }
-            mbar_arrive_expect_tx(full(st), STAGE_BYTES);
-            const int seg = kb >= p.s.seg_kb;
-            const int k = (kb - (seg ? p.s.seg_kb : 0)) * BK;
-            const uint32_t sa = sb + (uint32_t)st * STAGE_BYTES, sB = sa + A_BYTES;
-            if (A_MN) {
-#pragma unroll
-              for (int g = 0; g < BM / 64; ++g)
-                tma_load_2d(sa + g * GROUP_BYTES, &p.ta[seg], full(st), it.mt * BM + 64 * g, k);
-            } else {
-              tma_load_2d(sa, &p.ta[seg], full(st), k, it.mt * BM);
-            }
-            if (B_MN) {
-#pragma unroll
-              for (int g = 0; g < BN / 64; ++g)
-                tma_load_2d(sB + g * GROUP_BYTES, &p.tb[seg], full(st), nt * BN + 64 * g, k);
-            } else if (DUAL_B) {
-              tma_load_2d(sB, &p.tb[0], full(st), k, nt * (BN / 2));
-              tma_load_2d(sB + B_BYTES / 2, &p.tb[1], full(st), k, nt * (BN / 2));
-            } else {
-              tma_load_2d(sB, &p.tb[seg], full(st), k, nt * BN);
-              tma_load_2d(sB + B_BYTES / 2, &p.tb[seg], full(st), k, nt * BN + BN / 2);
-            }
-            ++issued;
-            if (++st == STAGES) st = 0, ph ^= 1;
+      for (Steps q(walk, p.s, pair, pairs, rank); ok && q.valid(); q.next()) {
+        for (int kb = q.kb; kb < q.kb_end(); ++kb) {
+          if (!mbar_wait(empty(st), ph, ab)) {
+            ok = false;
+            break;
           }
+          if (rank == 0) mbar_arrive_expect_tx(full(st), 2 * STAGE_BYTES);
+          const uint32_t bar = map_rank(full(st), 0);
+          const int seg = kb >= p.s.seg_kb;
+          const int k = (kb - (seg ? p.s.seg_kb : 0)) * BK;
+          const uint32_t sa = sb + (uint32_t)st * STAGE_BYTES, sB = sa + HALF_BYTES;
+          if (A_MN) {
+#pragma unroll
+            for (int g = 0; g < BM / 64; ++g) tma_load_pair(sa + g * GROUP_BYTES, &p.ta[seg], bar, q.it.row0 + 64 * g, k);
+          } else {
+            tma_load_pair(sa, &p.ta[seg], bar, k, q.it.row0);
+          }
+          if (B_MN) {
+#pragma unroll
+            for (int g = 0; g < BM / 64; ++g)
+              tma_load_pair(sB + g * GROUP_BYTES, &p.tb[seg], bar, q.nt * BN + rank * (BN / 2) + 64 * g, k);
+          } else if (DUAL_B) {
+            tma_load_pair(sB, &p.tb[rank], bar, k, q.nt * (BN / 2));
+          } else {
+            tma_load_pair(sB, &p.tb[seg], bar, k, q.nt * BN + rank * (BN / 2));
+          }
+          ++issued;
+          if (++st == STAGES) st = 0, ph ^= 1;
         }
       }
-      // never leave a copy in flight into this CTA's shared memory
-      for (int n = 0; n < min(issued, STAGES); ++n) {
-        const int last = issued - 1 - n;
-        drain_wait(full(last % STAGES), (last / STAGES) & 1);
+      // Never leave a copy in flight into shared memory: the even CTA's barriers count the
+      // copies of both, and the odd CTA stays until the even one comes to the final barrier.
+      if (rank == 0) {
+        for (int n = 0; n < min(issued, STAGES); ++n) {
+          const int last = issued - 1 - n;
+          drain_wait(full(last % STAGES), (last / STAGES) & 1);
+        }
       }
     }
   } else if (warp == 1) {
-    // -------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    // -------------------------------------------------------------- MMA issuer (even CTA)
+    if (rank == 0 && lane == 0) {
       int st = 0, ph = 0, t = 0;
       bool ok = true;
-      for (int i = blockIdx.x; ok && i < walk.items; i += gridDim.x) {
-        const Item it = walk.at(p.s, i);
-        for (int j = 0; ok && j < it.ntn; ++j, ++t) {
-          if (!mbar_wait(acc_empty(t & 1), ((t >> 1) & 1) ^ 1, ab)) {
+      for (Steps q(walk, p.s, pair, pairs, rank); ok && q.valid(); q.next(), ++t) {
+        if (!mbar_wait(acc_empty(t & 1), ((t >> 1) & 1) ^ 1, ab)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(t & 1) * BN;
+        for (int kb = q.kb; kb < q.kb_end(); ++kb) {
+          if (!mbar_wait(full(st), ph, ab)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t d = tmem + (uint32_t)(t & 1) * BN;
-          for (int kb = 0; kb < it.kbn; ++kb) {
-            if (!mbar_wait(full(st), ph, ab)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const uint32_t sa = sb + (uint32_t)st * STAGE_BYTES;
-            const uint32_t da = sw128_desc(sa, A_MN ? GROUP_BYTES : 0), db = sw128_desc(sa + A_BYTES, B_MN ? GROUP_BYTES : 0);
+          const uint32_t sa = sb + (uint32_t)st * STAGE_BYTES;
+          const uint32_t da = sw128_desc(sa, A_MN ? GROUP_BYTES : 0), db = sw128_desc(sa + HALF_BYTES, B_MN ? GROUP_BYTES : 0);
 #pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk)  // 16 K: 32 bytes of a K-major row, 16 rows (2048 bytes) MN-major
-              mma_ss(d, da + kk * (A_MN ? 128 : 2), db + kk * (B_MN ? 128 : 2), p.idesc, (kb | kk) != 0);
-            mma_commit(empty(st));
-            if (++st == STAGES) st = 0, ph ^= 1;
-          }
-          if (ok) mma_commit(acc_full(t & 1));
+          for (int kk = 0; kk < BK / 16; ++kk)  // 16 K: 32 bytes of a K-major row, 16 rows (2048 bytes) MN-major
+            mma_pair(d, da + kk * (A_MN ? 128 : 2), db + kk * (B_MN ? 128 : 2), p.idesc, kb > q.kb || kk > 0);
+          commit_pair(empty(st));
+          if (++st == STAGES) st = 0, ph ^= 1;
         }
+        if (ok) commit_pair(acc_full(t & 1));
       }
-      mma_commit(done);
-      drain_wait(done, 0);  // no MMA may still be writing TMEM at teardown
+      commit_pair(done);
+      drain_wait(done, 0);  // no MMA may still be writing TMEM, or reading either CTA's tiles, at teardown
     }
   } else {
     // -------------------------------------------------------------- epilogue
-    const EpiWarp w{warp & 3, (warp - 2) >> 2, lane};
-    Epi epi(ep, w);
+    const EpiWarp w{warp & 3, (warp - 2) >> 2, lane,
+                    sb + (uint32_t)(STAGES * STAGE_BYTES + (warp - 2) * Epi::BOXES * BOX_BYTES), warp_bar(warp - 2)};
+    Epi epi(ep, w, ab);
     int t = 0;
-    bool ok = true;
-    for (int i = blockIdx.x; ok && i < walk.items; i += gridDim.x) {
-      const Item it = walk.at(p.s, i);
-      epi.item_begin(it);
-      for (int j = 0; j < it.ntn; ++j, ++t) {
-        if (!warp_wait(acc_full(t & 1), (t >> 1) & 1, ab)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        epi.tile(it, it.nt0 + j, tmem + (uint32_t)(t & 1) * BN + w.lanes(), it.kbn == 0, [&]() {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty(t & 1));
-        });
-      }
-      if (ok) epi.item_end(it);
+    for (Steps q(walk, p.s, pair, pairs, rank); q.valid(); q.next(), ++t) {
+      epi.prepare(q);
+      if (!warp_wait(acc_full(t & 1), (t >> 1) & 1, ab)) break;
+      tc_fence_after();
+      const uint32_t release = map_rank(acc_empty(t & 1), 0);
+      epi.tile(q, tmem + (uint32_t)(t & 1) * BN + ((uint32_t)(32 * w.quad) << 16), [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(release);
+      });
     }
+    epi.done();
   }
   // ---------------------------------------------------------------- teardown
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other may still signal it or read its tiles
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * BN);
+    tmem_dealloc_pair(tmem, 2 * BN);
   }
 }
 
@@ -326,68 +440,214 @@ __device__ __forceinline__ void store_row32(float* dst, const float (&v)[N], int
   }
 }
 
-__device__ __forceinline__ void acc_load32(uint32_t addr, bool zero, float (&v)[32]) {
+// 32 columns of an accumulator; `empty`: no K block contributed (it stands for 0).
+__device__ __forceinline__ void acc_load32(uint32_t addr, bool empty, float (&v)[32]) {
   uint32_t r[32];
   tmem_load32(addr, r);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = zero ? 0.f : __uint_as_float(r[i]);
+  for (int i = 0; i < 32; ++i) v[i] = empty ? 0.f : __uint_as_float(r[i]);
 }
 
+// ------------------------------------------------------------------ boxes
+// A box is 32 rows of 128 bytes in shared memory, 128-byte swizzled (16-byte chunk c of row
+// r at chunk c ^ (r & 7)): a lane writes or reads its own row without bank conflicts, and
+// TMA moves the box, clipped to the matrix. Boxes of a warp are used in turn; a box is free
+// again once the store out of it has read it.
+template <int N>
+struct Boxes {
+  EpiWarp w;
+  int at;
+  __device__ explicit Boxes(const EpiWarp& w_) : w(w_), at(0) {}
+  __device__ __forceinline__ uint32_t box(int i) const { return w.smem + (uint32_t)i * BOX_BYTES; }
+  // the next box, free to write (stores of the N - 1 others may be in flight)
+  __device__ __forceinline__ uint32_t take() {
+    if (w.lane == 0) bulk_wait_read<N - 1>();
+    __syncwarp();
+    const uint32_t b = box(at);
+    at = at + 1 == N ? 0 : at + 1;
+    return b;
+  }
+  // all N boxes, free to write
+  __device__ __forceinline__ void take_all(uint32_t (&b)[N]) {
+    if (w.lane == 0) bulk_wait_read<0>();
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < N; ++i) b[i] = box(i);
+    at = 0;
+  }
+  __device__ __forceinline__ void put(uint32_t b, int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t u) const {
+    const uint32_t a = b + 128u * w.lane + 16u * (chunk ^ (w.lane & 7));
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(u) : "memory");
+  }
+  __device__ __forceinline__ uint4 get(uint32_t b, int chunk) const {
+    const uint32_t a = b + 128u * w.lane + 16u * (chunk ^ (w.lane & 7));
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+  }
+  // 32 columns as 16-bit values: half `h` of the box
+  __device__ __forceinline__ void put16(uint32_t b, int h, const float (&v)[32], bool bf16) const {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+      put(b, 4 * h + i / 8, pack2(v[i], v[i + 1], bf16), pack2(v[i + 2], v[i + 3], bf16), pack2(v[i + 4], v[i + 5], bf16),
+          pack2(v[i + 6], v[i + 7], bf16));
+  }
+  __device__ __forceinline__ void get16(uint32_t b, int h, float (&v)[32], bool bf16) const {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+      const uint4 u = get(b, 4 * h + i / 8);
+      const uint32_t q[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack2(q[k], bf16);
+        v[i + 2 * k] = f.x, v[i + 2 * k + 1] = f.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void put32(uint32_t b, const float (&v)[32]) const {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+      put(b, i / 4, __float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]));
+  }
+  // box -> matrix at column x, row y, slice z
+  __device__ __forceinline__ void store(uint32_t b, const CUtensorMap* map, int x, int y, int z, bool add = false) const {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (w.lane == 0) {
+      if (add)
+        tma_add_3d(map, b, x, y, z);
+      else
+        tma_store_3d(map, b, x, y, z);
+      bulk_commit();
+    }
+  }
+  // The same for rows that TMA cannot address (not 16-byte aligned): `rows` rows of `cols`
+  // elements of SIZE bytes, whole warps along a row.
+  template <int SIZE>
+  __device__ __forceinline__ void store_plain(uint32_t b, void* dst, int64_t ld, int rows, int cols) const {
+    __syncwarp();
+    constexpr int PER = 128 / SIZE;  // elements per row of a box
+    for (int r = 0; r < min(rows, 32); ++r) {
+#pragma unroll
+      for (int k = 0; k < PER / 32; ++k) {
+        const int c = 32 * k + w.lane, byte = c * SIZE;
+        const uint32_t a = b + 128u * r + 16u * ((byte >> 4) ^ (r & 7)) + (byte & 15);
+        if (c >= cols) continue;
+        if (SIZE == 2) {
+          uint16_t v;
+          asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+          static_cast<uint16_t*>(dst)[r * ld + c] = v;
+        } else {
+          uint32_t v;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+          static_cast<uint32_t*>(dst)[r * ld + c] = v;
+        }
+      }
+    }
+    __syncwarp();
+  }
+  // Every store has been performed (before the CTA may leave).
+  __device__ void finish() const {
+    if (w.lane == 0) bulk_wait_all();
+  }
+};
+
+// A matrix that an epilogue writes: by TMA where its rows are 16-byte aligned.
+struct Out {
+  CUtensorMap map;  // {columns, rows, slices}, boxes of 128 bytes x 32 rows
+  void* base;
+  int64_t ld;
+  int rows, cols;
+  int tma;
+};
+
 // ------------------------------------------------------------------ plain epilogue
-// C = alpha * acc into rows of fp32 / bf16 / fp16 (rows row_split.. go to c[1]), or
-// the fp32 partial of a split, or added to an fp32 C.
+// C = alpha * acc as fp32, bf16 or fp16: the rows of two matrices one after the other
+// (row_split, a multiple of 128, rows apart), or the fp32 partials of the splits (slices),
+// or added to an fp32 C. PROMOTE: an item's accumulators (chunks of K) are collected in
+// fp32 registers: the tensor core's own sum over K loses about 2^-24 per 16 products,
+// which an fp32 C would show.
+template <bool PROMOTE>
 struct StoreEpi {
+  static constexpr int BOXES = 2;
   struct Params {
-    void* c[2];
-    int64_t ldc;
-    int row_split;         // rows of c[0]'s part in the product (a multiple of nothing: any)
-    int rows, cols;        // rows of each part that exist, columns
-    const float* alpha;    // device scalar (NULL: 1)
-    int dtype;             // of C
-    int accumulate;        // C (fp32) += acc
-    int64_t split_stride;  // elements between the splits' partials (0: no splits)
-    int vec;               // C's rows are 16-byte aligned
+    Out c[2];
+    int row_split;
+    const float* alpha;  // device scalar (NULL: 1)
+    int dtype;           // of C
+    int add;             // C (fp32) += acc
   };
   const Params& p;
   EpiWarp w;
+  Boxes<BOXES> boxes;
   float alpha;
-  __device__ StoreEpi(const Params& p_, const EpiWarp& w_) : p(p_), w(w_) { alpha = p.alpha ? *p.alpha : 1.f; }
-  __device__ void item_begin(const Item&) {}
-  __device__ void item_end(const Item&) {}
-  template <class Release>
-  __device__ void tile(const Item& it, int nt, uint32_t acc, bool zero, Release release) {
-    int row = it.mt * BM + w.row();
+  float sum[PROMOTE ? BN / 2 : 1];
+  __device__ StoreEpi(const Params& p_, const EpiWarp& w_, const Abort&) : p(p_), w(w_), boxes(w) {
+    alpha = p.alpha ? *p.alpha : 1.f;
+#pragma unroll
+    for (float& v : sum) v = 0.f;
+  }
+  __device__ void prepare(const Steps&) {}
+  __device__ void done() { boxes.finish(); }
+  __device__ __forceinline__ void out32(const Steps& q, int c, float (&v)[32], uint32_t& box) {
+    int row = q.it.row0 + 32 * w.quad;
     const int part = row >= p.row_split;
     if (part) row -= p.row_split;
-    const bool live = row < p.rows;
-    const int64_t at = (int64_t)it.split * p.split_stride + (int64_t)row * p.ldc;
+    const Out& o = p.c[part];
+    const int col = q.nt * BN + c, rows = o.rows - row;
+    if (rows <= 0) return;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] *= alpha;
+    if (PROMOTE || p.dtype == PNFT_DTYPE_F32) {
+      if (o.cols - col <= 0) return;
+      const uint32_t b = boxes.take();
+      boxes.put32(b, v);
+      if (o.tma)
+        boxes.store(b, &o.map, col, row, q.it.split, p.add);
+      else
+        boxes.template store_plain<4>(b, static_cast<float*>(o.base) + (int64_t)row * o.ld + col, o.ld, rows, o.cols - col);
+    } else {
+      const int h = (c >> 5) & 1;  // a box takes 64 columns: two calls
+      if (o.cols - (col - 32 * h) <= 0) return;
+      if (h == 0) box = boxes.take();
+      boxes.put16(box, h, v, p.dtype == PNFT_DTYPE_BF16);
+      if (h == 0) return;
+      if (o.tma)
+        boxes.store(box, &o.map, col - 32, row, 0);
+      else
+        boxes.template store_plain<2>(box, static_cast<uint16_t*>(o.base) + (int64_t)row * o.ld + col - 32, o.ld, rows,
+                                      o.cols - col + 32);
+    }
+  }
+  template <class Release>
+  __device__ __forceinline__ void tile(const Steps& q, uint32_t acc, Release release) {
+    const int c0 = w.half * (BN / 2);
+    const bool empty = q.it.kbn == 0;
+    uint32_t box = 0;
+    if (PROMOTE) {
+#pragma unroll
+      for (int c = 0; c < BN / 2; c += 16) {  // 16 at a time: the sums take 128 registers
+        uint32_t r[16];
+        tmem_load16(acc + c0 + c, r);
+        if (c + 16 == BN / 2) release();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[c + i] += empty ? 0.f : __uint_as_float(r[i]);
+      }
+      if (!q.tile_last()) return;
+#pragma unroll
+      for (int c = 0; c < BN / 2; c += 32) {
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = sum[c + i], sum[c + i] = 0.f;
+        out32(q, c0 + c, v, box);
+      }
+    } else {
 #pragma unroll 1
-    for (int c = w.half * (BN / 2); c < (w.half + 1) * (BN / 2); c += 32) {
-      float v[32];
-      acc_load32(acc + c, zero, v);
-      if (c + 32 == (w.half + 1) * (BN / 2)) release();
-      const int col = nt * BN + c, n = p.cols - col;
-      if (!live || n <= 0) continue;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] *= alpha;
-      if (p.dtype == PNFT_DTYPE_F32) {
-        float* dst = static_cast<float*>(p.c[part]) + at + col;
-        if (p.accumulate) {
-          if (p.vec && n >= 32) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(dst + i);
-              v[i] += f.x, v[i + 1] += f.y, v[i + 2] += f.z, v[i + 3] += f.w;
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < n) v[i] += dst[i];
-          }
-        }
-        store_row32<32>(dst, v, n, p.vec);
-      } else {
-        store_row16<32>(static_cast<uint16_t*>(p.c[part]) + at + col, v, n, p.vec, p.dtype == PNFT_DTYPE_BF16);
+      for (int c = 0; c < BN / 2; c += 32) {
+        float v[32];
+        acc_load32(acc + c0 + c, empty, v);
+        if (c + 32 == BN / 2) release();
+        out32(q, c0 + c, v, box);
       }
     }
   }
@@ -395,37 +655,64 @@ struct StoreEpi {
 
 // ------------------------------------------------------------------ host side
 int sm_count();
-// Splits of K for an output of `tiles` tiles: about one work item per SM, at least
-// 8 K blocks (512 of K) each, since shorter ones cost more in partial sums than
+// Splits of K for an output of `tiles` tiles: about one work item per pair of SMs, at
+// least 8 K blocks (512 of K) each, since shorter ones cost more in partial sums than
 // they gain.
-int plan_splits(int tiles, int kb);
+int plan_splits(int64_t tiles, int64_t kb);
+inline int64_t tiles_of(int64_t m, int64_t n) { return ((m + PM - 1) / PM) * ((n + BN - 1) / BN); }
+
 // Sums the splits' fp32 partials [splits][rows_total][ldp] in split order (bitwise
 // reproducible), times alpha, into C (two parts as StoreEpi) or onto an fp32 C.
-int sum_splits(const float* part, int64_t ldp, int64_t split_stride, int splits, const StoreEpi::Params& out,
-               int rows_total, cudaStream_t st);
+struct SumArgs {
+  void* c[2];
+  int64_t ldc;
+  int row_split, rows, cols;
+  const float* alpha;
+  int dtype, add, vec;
+};
+// The weight-gradient product behind pnft_weight_grad, its arguments checked.
+int weight_grad(const char* what, const void* dy, int64_t lddy, const void* x, int64_t ldx, void* c0, void* c1, int64_t ldc,
+                int64_t row_split, int64_t rows, int c_dtype, void* workspace, int64_t K, int64_t M, int64_t N, int dtype,
+                int32_t* status, cudaStream_t st);
+int sum_splits(const float* part, int64_t ldp, int64_t split_stride, int splits, const SumArgs& out, int rows_total,
+               cudaStream_t st);
+
+inline bool rows16(const void* p, int64_t ld, int size) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0;
+}
+inline int dtype_size(int dtype) { return dtype == PNFT_DTYPE_F32 ? 4 : 2; }
+
+inline int make_out(Out* o, void* base, int dtype, int64_t cols, int64_t rows, int64_t ld, int64_t slices = 1,
+                    int64_t slice_stride = 0) {
+  memset(o, 0, sizeof(*o));
+  o->base = base, o->ld = ld, o->rows = (int)rows, o->cols = (int)cols;
+  if (!base) return PNFT_OK;
+  o->tma = rows16(base, ld, dtype_size(dtype)) && ld < ((int64_t)1 << 37);
+  return o->tma ? tma_map_out(&o->map, base, dtype_size(dtype), cols, rows, ld, slices, slice_stride, 32) : PNFT_OK;
+}
 
 // K-major operand: `rows` rows of K elements; MN-major operand: K rows of `cols`
 // elements. Both take the row stride in elements (a multiple of 8, 16-byte base).
 inline int map_kmajor(CUtensorMap* m, const void* base, int64_t k, int64_t rows, int64_t ld) {
-  return tma_map_rows(m, base, k, rows, ld, 128);
+  return tma_map_rows(m, base, k, rows, ld, BM);
 }
 inline int map_mnmajor(CUtensorMap* m, const void* base, int64_t cols, int64_t k, int64_t ld) {
   return tma_map_rows(m, base, cols, k, ld, BK);
 }
 
 inline uint32_t idesc(int dtype, bool a_mn, bool b_mn) {
-  return idesc_f16(BM, BN, dtype == PNFT_DTYPE_BF16 ? 1 : 0, a_mn, b_mn);
+  return idesc_f16(PM, BN, dtype == PNFT_DTYPE_BF16 ? 1 : 0, a_mn, b_mn);
 }
 
 inline Sched plain_sched(int64_t m, int64_t n, int64_t kb, int splits) {
   Sched s;
   memset(&s, 0, sizeof(s));
-  s.tiles_m = (int)((m + BM - 1) / BM);
+  s.tiles_m = (int)((m + PM - 1) / PM);
   s.tiles_n = s.strips = (int)((n + BN - 1) / BN);
   s.tiles_per_strip = 1;
-  s.kb = s.seg_kb = (int)kb;
+  s.kb = s.seg_kb = s.chunk = (int)std::max<int64_t>(kb, 1);
   s.splits = splits;
-  s.group_m = 16;
+  s.group_m = 8;
   return s;
 }
 
@@ -435,15 +722,27 @@ int launch(const char* what, const Args& a, const typename Epi::Params& ep, cuda
   if (items <= 0) return PNFT_OK;
   if (items > (1 << 30)) return fail(PNFT_EUNSUPPORTED, "%s: too many tiles", what);
   auto* k = gemm_kernel<A_MN, B_MN, DUAL_B, Epi>;
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess)
+  constexpr int smem = smem_bytes<Epi>();
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return check_launch(what, 0);
-  k<<<(unsigned)std::min<int64_t>(items, sm_count()), THREADS, SMEM, st>>>(a, ep);
+  k<<<(unsigned)(2 * std::min<int64_t>(items, sm_count() / 2)), THREADS, smem, st>>>(a, ep);
   return check_launch(what, 1);
 }
 
-inline bool rows16(const void* p, int64_t ld, int size) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0;
+// C = A B^T with the plain epilogue; K in chunks of 2048 for an fp32 C (see StoreEpi).
+constexpr int PROMOTE_KB = 32;
+template <bool A_MN, bool B_MN>
+int launch_store(const char* what, Args a, const StoreEpi<false>::Params& ep, cudaStream_t st) {
+  if (ep.dtype == PNFT_DTYPE_F32 && a.s.kb > PROMOTE_KB * a.s.splits) {
+    a.s.chunk = PROMOTE_KB;
+    typename StoreEpi<true>::Params e;
+    static_assert(sizeof(e) == sizeof(ep), "same parameters");
+    memcpy(&e, &ep, sizeof(e));
+    return launch<A_MN, B_MN, false, StoreEpi<true>>(what, a, e, st);
+  }
+  return launch<A_MN, B_MN, false, StoreEpi<false>>(what, a, ep, st);
 }
+
 // An operand that TMA can read: 16-byte base, row stride a multiple of 8 elements
 // and inside the map's limit.
 inline bool tma_rows_ok(const void* p, int64_t ld, int64_t cols) {

@@ -69,6 +69,7 @@ __device__ __forceinline__ int block_total(int v, int* red) {
 
 __device__ __forceinline__ void copy_row(uint16_t* dst, const uint16_t* src, int D, bool vec, int lane) {
   if (vec) {
+#pragma unroll 8
     for (int i = lane; i < D / 8; i += 32) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
     for (int i = D / 8 * 8 + lane; i < D; i += 32) dst[i] = src[i];
   } else {
@@ -84,6 +85,7 @@ __global__ void __launch_bounds__(CT) xent_compact_kernel(CompactArgs p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t r0 = (int64_t)blockIdx.x * p.rows, r1 = std::min<int64_t>(p.M, r0 + p.rows);
   int n = 0;
+#pragma unroll 4
   for (int64_t r = threadIdx.x; r < r0; r += CT) n += p.t[r] != p.ignore;
   int base = block_total(n, red);
   for (int64_t c0 = r0; c0 < r1; c0 += CT) {
@@ -131,6 +133,7 @@ __global__ void __launch_bounds__(CT) xent_compact_kernel(CompactArgs p) {
 // Per row and half of the columns: running maximum (times log2 e) and sum of
 // 2^(z log2 e - max), both fp32, over the tiles of a strip.
 struct LseEpi {
+  static constexpr int BOXES = 0;
   struct Params {
     float *part_m, *part_s;  // [strips * 2][Mp]
     float* zt;
@@ -142,28 +145,24 @@ struct LseEpi {
   const Params& p;
   EpiWarp w;
   float m, s;
-  int tgt;
-  __device__ LseEpi(const Params& p_, const EpiWarp& w_) : p(p_), w(w_) {}
-  __device__ void item_begin(const Item& it) {
+  int tgt, live;
+  __device__ LseEpi(const Params& p_, const EpiWarp& w_, const Abort&) : p(p_), w(w_) { live = *p.live; }
+  __device__ void prepare(const Steps& q) {
+    if (!q.item_first()) return;
     m = kLow, s = 0.f;
-    const int row = it.mt * BM + w.row();
-    tgt = row < *p.live ? p.tgt[row] : -1;
+    const int row = q.it.row0 + w.row();
+    tgt = row < live ? p.tgt[row] : -1;
   }
-  __device__ void item_end(const Item& it) {
-    const int row = it.mt * BM + w.row();
-    if (row >= *p.live) return;
-    const int64_t at = (int64_t)(it.nt0 / p.strip_tiles * 2 + w.half) * p.Mp + row;
-    p.part_m[at] = m;
-    p.part_s[at] = s;
-  }
+  __device__ void done() {}
   template <class Release>
-  __device__ void tile(const Item& it, int nt, uint32_t acc, bool zero, Release release) {
+  __device__ __forceinline__ void tile(const Steps& q, uint32_t acc, Release release) {
+    const int row = q.it.row0 + w.row();
 #pragma unroll 1
     for (int c = w.half * (BN / 2); c < (w.half + 1) * (BN / 2); c += 32) {
       float z[32];
-      acc_load32(acc + c, zero, z);
+      acc_load32(acc + c, false, z);
       if (c + 32 == (w.half + 1) * (BN / 2)) release();
-      const int col = nt * BN + c, n = p.V - col;
+      const int col = q.nt * BN + c, n = p.V - col;
       if (n < 32) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
@@ -174,7 +173,7 @@ struct LseEpi {
         float v = 0.f;
 #pragma unroll
         for (int i = 0; i < 32; ++i) v = i == tc ? z[i] : v;
-        p.zt[it.mt * BM + w.row()] = v;
+        p.zt[row] = v;
       }
       float a = max3(z[0], z[1], z[2]), b = max3(z[3], z[4], z[5]);
 #pragma unroll
@@ -192,6 +191,11 @@ struct LseEpi {
       s = fmaf(s, ex2(m - nm), (s0 + s1) + (s2 + s3));
       m = nm;
     }
+    if (q.item_last() && row < live) {
+      const int64_t at = (int64_t)(q.it.nt0 / p.strip_tiles * 2 + w.half) * p.Mp + row;
+      p.part_m[at] = m;
+      p.part_s[at] = s;
+    }
   }
 };
 
@@ -206,17 +210,43 @@ struct ReduceArgs {
   int64_t Mp;
   int parts, mean;
 };
+// A block takes ROWS rows, 256 / ROWS threads each: many threads per row when there are
+// few rows, which then have many strips.
+template <int ROWS>
 __global__ void __launch_bounds__(256) xent_reduce_kernel(ReduceArgs p) {
   __shared__ double red[256];
+  __shared__ float top[256], sum[256];
   __shared__ int last;
+  constexpr int LANES = 256 / ROWS;
   const int n = p.s.counts[0];
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  double mine = 0.0;
+  const int r = threadIdx.x % ROWS, lane = threadIdx.x / ROWS;
+  const int64_t i = (int64_t)blockIdx.x * ROWS + r;
+  float m = kLow;
   if (i < n) {
-    float m = kLow;
-    for (int k = 0; k < p.parts; ++k) m = fmaxf(m, p.part_m[k * p.Mp + i]);
-    float s = 0.f;
-    for (int k = 0; k < p.parts; ++k) s += p.part_s[k * p.Mp + i] * ex2(p.part_m[k * p.Mp + i] - m);
+#pragma unroll 4
+    for (int k = lane; k < p.parts; k += LANES) m = fmaxf(m, p.part_m[k * p.Mp + i]);
+  }
+  top[threadIdx.x] = m;
+  __syncthreads();
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    if (lane < o) top[threadIdx.x] = fmaxf(top[threadIdx.x], top[threadIdx.x + o * ROWS]);
+    __syncthreads();
+  }
+  m = top[r];
+  float s = 0.f;
+  if (i < n) {
+#pragma unroll 4
+    for (int k = lane; k < p.parts; k += LANES) s += p.part_s[k * p.Mp + i] * ex2(p.part_m[k * p.Mp + i] - m);
+  }
+  sum[threadIdx.x] = s;
+  __syncthreads();
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    if (lane < o) sum[threadIdx.x] += sum[threadIdx.x + o * ROWS];
+    __syncthreads();
+  }
+  double mine = 0.0;
+  if (i < n && lane == 0) {
+    s = sum[r];
     const float l = log2f(s);
     p.s.lse2[i] = m + l;
     const float loss = kLn2 * (fmaf(-p.zt[i], kLog2e, m) + l);
@@ -284,43 +314,53 @@ __global__ void __launch_bounds__(1024) xent_scale_kernel(ScaleArgs p) {
 // dz of one piece, 16 bits, zeros in rows past the last one that counts and in columns
 // past the vocabulary (the two GEMMs run over whole 64-deep blocks of both).
 struct DzEpi {
+  static constexpr int BOXES = 2;
   struct Params {
-    uint16_t* dz;
-    int64_t ld;
+    Out dz;
     const float *lse2, *rs;
     const int32_t *tgt, *live;
-    int64_t Mp;
     int v0, V, bf16;
   };
   const Params& p;
   EpiWarp w;
+  Boxes<BOXES> boxes;
   float lse, rs;
-  int tgt, row;
-  __device__ DzEpi(const Params& p_, const EpiWarp& w_) : p(p_), w(w_) {}
-  __device__ void item_begin(const Item& it) {
-    row = it.mt * BM + w.row();
-    const bool live = row < *p.live;
-    lse = live ? p.lse2[row] : 0.f;
-    rs = live ? p.rs[row] : 0.f;
-    tgt = live ? p.tgt[row] - p.v0 : -1;
+  int tgt, live;
+  __device__ DzEpi(const Params& p_, const EpiWarp& w_, const Abort&) : p(p_), w(w_), boxes(w) { live = *p.live; }
+  __device__ void prepare(const Steps& q) {
+    if (!q.item_first()) return;
+    const int row = q.it.row0 + w.row();
+    lse = row < live ? p.lse2[row] : 0.f;
+    rs = row < live ? p.rs[row] : 0.f;
+    tgt = row < live ? p.tgt[row] - p.v0 : -1;
   }
-  __device__ void item_end(const Item&) {}
+  __device__ void done() { boxes.finish(); }
   template <class Release>
-  __device__ void tile(const Item& it, int nt, uint32_t acc, bool zero, Release release) {
-    const bool live = row < *p.live;
+  __device__ __forceinline__ void tile(const Steps& q, uint32_t acc, Release release) {
+    const int row = q.it.row0 + w.row();
+    uint32_t b = 0;
 #pragma unroll 1
     for (int c = w.half * (BN / 2); c < (w.half + 1) * (BN / 2); c += 32) {
       float z[32];
-      acc_load32(acc + c, zero, z);
+      acc_load32(acc + c, false, z);
       if (c + 32 == (w.half + 1) * (BN / 2)) release();
-      const int col = nt * BN + c, n = p.V - p.v0 - col;
+      const int col = q.nt * BN + c, n = row < live ? p.V - p.v0 - col : 0, tc = tgt - col;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        float v = ex2(fmaf(z[i], kLog2e, -lse)) * rs;
-        if (i == tgt - col) v -= rs;
-        z[i] = live && i < n ? v : 0.f;
+      for (int i = 0; i < 32; ++i) z[i] = ex2(fmaf(z[i], kLog2e, -lse)) * rs;
+      if ((unsigned)tc < 32u) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i == tc) z[i] -= rs;
       }
-      if (row < p.Mp) store_row16<32>(p.dz + (int64_t)row * p.ld + col, z, 32, true, p.bf16);
+      if (n < 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i >= n) z[i] = 0.f;
+      }
+      const int h = (c >> 5) & 1;
+      if (h == 0) b = boxes.take();
+      boxes.put16(b, h, z, p.bf16);
+      if (h == 1 && q.it.row0 < p.dz.rows) boxes.store(b, &p.dz.map, col - 32, q.it.row0 + 32 * w.quad, 0);
     }
   }
 };
@@ -353,10 +393,10 @@ __global__ void __launch_bounds__(256) xent_dh_kernel(const float* __restrict__ 
 // ------------------------------------------------------------------ plans
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Column tiles per strip: the fewest rounds of tiles over the SMs, counting a third of a
+// Column tiles per strip: the fewest rounds of tiles over the pairs of SMs, counting a third of a
 // tile for each strip's start and end.
 int strip_tiles(int64_t tiles_m, int tiles_n) {
-  const int sms = sm_count();
+  const int sms = sm_count() / 2;  // pairs
   int best = 1;
   double cost = 1e300;
   for (int strips = 1; strips <= std::min(tiles_n, 2 * sms); ++strips) {
@@ -404,7 +444,7 @@ FwdLayout fwd_layout(int64_t M, int64_t V) {
   const int64_t Mp = up(M, BM);
   FwdLayout l;
   const int tiles_n = (int)((V + BN - 1) / BN);
-  l.per = strip_tiles(Mp / BM, tiles_n);
+  l.per = strip_tiles((M + PM - 1) / PM, tiles_n);
   l.strips = (tiles_n + l.per - 1) / l.per;
   size_t at = 0;
   auto take = [&](size_t n) {
@@ -415,7 +455,7 @@ FwdLayout fwd_layout(int64_t M, int64_t V) {
   l.zt = take(4 * Mp);
   l.part_m = take(4 * Mp * 2 * l.strips);
   l.part_s = take(4 * Mp * 2 * l.strips);
-  l.sums = take(8 * ((M + 255) / 256));
+  l.sums = take(8 * std::max<int64_t>(64, (M + 31) / 32));
   l.total = at;
   return l;
 }
@@ -435,9 +475,8 @@ BwdLayout bwd_layout(int64_t M, int64_t V, int64_t D) {
   const int64_t Mp = up(M, BM), D4 = up(D, 4);
   BwdLayout l;
   l.P = piece_width(M, V);
-  const int td = (int)((D + BN - 1) / BN);
-  l.dh_splits = plan_splits((int)(Mp / BM) * td, (int)(l.P / BK));
-  l.dw_splits = plan_splits((int)((l.P + BM - 1) / BM) * td, (int)((Mp + BK - 1) / BK));
+  l.dh_splits = plan_splits(tiles_of(M, D), l.P / BK);
+  l.dw_splits = plan_splits(tiles_of(l.P, D), Mp / BK);
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t r = at;
@@ -507,7 +546,7 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
   c.zt = reinterpret_cast<float*>(ws + l.zt);
   c.row_loss = row_loss;
   c.M = M, c.V = (int)V, c.D = (int)D, c.Mp = Mp;
-  c.rows = (int)std::max<int64_t>(32, (M + 1023) / 1024);
+  c.rows = (int)std::max<int64_t>(8, (M + 1023) / 1024);
   c.vec = rows16(h, ldh, 2);
   c.status = status;
   xent_compact_kernel<<<(unsigned)((M + c.rows - 1) / c.rows), CT, 0, st>>>(c);
@@ -532,7 +571,10 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
   rc = launch<false, false, false, LseEpi>("stream_xent forward", a, ep, st);
   if (rc) return rc;
   ReduceArgs r{ep.part_m, ep.part_s, c.zt, c.s, row_loss, loss, reinterpret_cast<double*>(ws + l.sums), Mp, 2 * l.strips, mean};
-  xent_reduce_kernel<<<(unsigned)((M + 255) / 256), 256, 0, st>>>(r);
+  if (M > 64)
+    xent_reduce_kernel<32><<<(unsigned)((M + 31) / 32), 256, 0, st>>>(r);
+  else
+    xent_reduce_kernel<1><<<(unsigned)M, 256, 0, st>>>(r);
   return check_launch("stream_xent reduction", 1);
 }
 
@@ -579,7 +621,12 @@ extern "C" int pnft_stream_xent_bwd(const void* hc, int64_t ldc, const void* w, 
     a.s.live = s.counts;
     a.s.live_m = 1;
     a.idesc = idesc(dtype, false, false);
-    DzEpi::Params ep{dz, l.P, s.lse2, rs, s.tgt, s.counts, Mp, (int)v0, (int)V, bf16};
+    DzEpi::Params ep;
+    memset(&ep, 0, sizeof(ep));
+    rc = make_out(&ep.dz, dz, dtype, l.P, Mp, l.P);
+    if (rc) break;
+    ep.lse2 = s.lse2, ep.rs = rs, ep.tgt = s.tgt, ep.live = s.counts;
+    ep.v0 = (int)v0, ep.V = (int)V, ep.bf16 = bf16;
     rc = launch<false, false, false, DzEpi>("stream_xent dz", a, ep, st);
     if (rc) break;
     if (dh) {  // dh (+)= dz W
@@ -591,14 +638,19 @@ extern "C" int pnft_stream_xent_bwd(const void* hc, int64_t ldc, const void* w, 
       a.s.live = s.counts;
       a.s.live_m = 1;
       a.idesc = idesc(dtype, false, true);
-      StoreEpi::Params out{{acc, nullptr}, D4, 0x7fffffff, (int)M, (int)D, nullptr, PNFT_DTYPE_F32, v0 > 0, 0, 1};
+      StoreEpi<false>::Params out;
+      memset(&out, 0, sizeof(out));
+      out.row_split = 0x7fffffff;
+      out.dtype = PNFT_DTYPE_F32;
       if (splits > 1) {
-        StoreEpi::Params o = out;
-        o.c[0] = part, o.accumulate = 0, o.split_stride = Mp * D4;
-        rc = launch<false, true, false, StoreEpi>("stream_xent dh", a, o, st);
-        if (!rc) rc = sum_splits(part, D4, Mp * D4, splits, out, (int)M, st);
+        rc = make_out(&out.c[0], part, PNFT_DTYPE_F32, D, M, D4, splits, Mp * D4);
+        if (!rc) rc = launch_store<false, true>("stream_xent dh", a, out, st);
+        const SumArgs sum{{acc, nullptr}, D4, 0x7fffffff, (int)M, (int)D, nullptr, PNFT_DTYPE_F32, v0 > 0, 1};
+        if (!rc) rc = sum_splits(part, D4, Mp * D4, splits, sum, (int)M, st);
       } else {
-        rc = launch<false, true, false, StoreEpi>("stream_xent dh", a, out, st);
+        rc = make_out(&out.c[0], acc, PNFT_DTYPE_F32, D, M, D4);
+        out.add = v0 > 0;
+        if (!rc) rc = launch_store<false, true>("stream_xent dh", a, out, st);
       }
       if (rc) break;
     }
@@ -610,15 +662,22 @@ extern "C" int pnft_stream_xent_bwd(const void* hc, int64_t ldc, const void* w, 
       a.s.live = s.counts;
       a.s.live_k = 1;
       a.idesc = idesc(dtype, true, true);
-      const int size = dw_dtype == PNFT_DTYPE_F32 ? 4 : 2;
+      const int size = dtype_size(dw_dtype);
       void* dst = static_cast<char*>(dw) + v0 * lddw * size;
-      StoreEpi::Params out{{dst, nullptr}, lddw, 0x7fffffff, (int)n, (int)D, alpha, dw_dtype, 0, 0, rows16(dst, lddw, size)};
+      StoreEpi<false>::Params out;
+      memset(&out, 0, sizeof(out));
+      out.row_split = 0x7fffffff;
       if (l.dw_splits > 1) {
-        StoreEpi::Params o{{part, nullptr}, D4, 0x7fffffff, (int)n, (int)D, nullptr, PNFT_DTYPE_F32, 0, l.P * D4, 1};
-        rc = launch<true, true, false, StoreEpi>("stream_xent dW", a, o, st);
-        if (!rc) rc = sum_splits(part, D4, l.P * D4, l.dw_splits, out, (int)n, st);
+        out.dtype = PNFT_DTYPE_F32;
+        rc = make_out(&out.c[0], part, PNFT_DTYPE_F32, D, n, D4, l.dw_splits, l.P * D4);
+        if (!rc) rc = launch_store<true, true>("stream_xent dW", a, out, st);
+        const SumArgs sum{{dst, nullptr}, lddw, 0x7fffffff, (int)n, (int)D, alpha, dw_dtype, 0, rows16(dst, lddw, size)};
+        if (!rc) rc = sum_splits(part, D4, l.P * D4, l.dw_splits, sum, (int)n, st);
       } else {
-        rc = launch<true, true, false, StoreEpi>("stream_xent dW", a, out, st);
+        out.dtype = dw_dtype;
+        out.alpha = alpha;
+        rc = make_out(&out.c[0], dst, dw_dtype, D, n, lddw);
+        if (!rc) rc = launch_store<true, true>("stream_xent dW", a, out, st);
       }
     }
   }

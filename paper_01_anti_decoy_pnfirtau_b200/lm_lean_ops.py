@@ -23,6 +23,7 @@ only; a CPU tensor raises. Results are bitwise reproducible on a given GPU.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from dataclasses import dataclass
 
@@ -30,7 +31,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .pnfirtau_ops import _DTYPES, _check_pending, _ptr, _require_cuda, _status_ptr, _stream
+from .pnfirtau_ops import _DTYPES, _check_pending, _ptr, _require_cuda, _status_ptr
 
 _ACTS = {"silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
 _TYPES16 = (torch.bfloat16, torch.float16)
@@ -41,6 +42,18 @@ def _compute_dtype(x: torch.Tensor, what: str) -> torch.dtype:
     if dt not in _TYPES16:
         raise RuntimeError(f"{what}: bfloat16 or float16 expected (or CUDA autocast to one of them), got {dt}")
     return dt
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """Makes ``dev`` the current device, as the library's launches need (free when it is)."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
@@ -110,7 +123,7 @@ def act8_pack(x: torch.Tensor) -> Act8:
     M, nb = x2.shape[0], (D + 127) // 128
     q = torch.empty((M, (D + 15) // 16 * 16), dtype=torch.uint8, device=dev)
     e = torch.empty((M, nb), dtype=torch.int8, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.check(_lib.lib().pnft_act8_pack(x2.data_ptr(), max(x2.stride(0), D), q.data_ptr(), q.shape[1], e.data_ptr(), nb, M, D,
                                              _DTYPES[x.dtype], _stream(dev)), "pnft_act8_pack")
     return Act8(q, e, x.shape, x.dtype)
@@ -128,7 +141,7 @@ def _act8_rows(p: Act8, dt: torch.dtype) -> torch.Tensor:
 def act8_unpack(p: Act8) -> torch.Tensor:
     """The tensor that ``p`` stands for, in the shape and dtype that were packed (exact:
     the dtype holds every packed value)."""
-    with torch.cuda.device(p.q.device):
+    with _on(p.q.device):
         return _act8_rows(p, p.dtype).reshape(p.shape)
 
 
@@ -137,6 +150,8 @@ def act8_weight_grad(dy: torch.Tensor, p: Act8, out_dtype: torch.dtype = torch.f
     from its output's gradient ``dy`` (``[..., N]``, bfloat16 or float16, as many rows as
     ``x``) and its input kept in 8 bits; fp32 sums."""
     dev = _require_cuda("act8_weight_grad", dy, p.q)
+    if out_dtype not in _DTYPES:
+        raise RuntimeError(f"act8_weight_grad: float32, bfloat16 or float16 result expected, got {out_dtype}")
     if dy.dtype not in _TYPES16:
         raise RuntimeError(f"act8_weight_grad: bfloat16 or float16 gradient expected, got {dy.dtype}")
     if dy.dtype == torch.float16 and p.dtype != torch.float16:
@@ -146,119 +161,98 @@ def act8_weight_grad(dy: torch.Tensor, p: Act8, out_dtype: torch.dtype = torch.f
     dy2 = dy.detach().reshape(-1, dy.shape[-1])
     if dy2.shape[0] != p.q.shape[0]:
         raise RuntimeError(f"act8_weight_grad: {dy2.shape[0]} rows of gradient but {p.q.shape[0]} of activation")
-    with torch.cuda.device(dev):
-        return _weight_grads(_rows16(dy2, dy.dtype), _act8_rows(p, dy.dtype), (out_dtype,))[0]
+    with _on(dev):
+        return _weight_grad(_rows16(dy2, dy.dtype), _act8_rows(p, dy.dtype), out_dtype)
 
 
-def _weight_grads(dy: torch.Tensor, x: torch.Tensor, dtypes, split: int | None = None, rows: int | None = None):
-    """``dy^T x`` (both from ``_rows16``) as one matrix, or as two of ``rows`` rows each
-    that start at rows 0 and ``split`` of the product."""
+def _weight_grad(dy: torch.Tensor, x: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
+    """``dy^T x`` of two ``_rows16`` matrices."""
     K, M = dy.shape
     N, dev = x.shape[1], dy.device
-    two = split is not None
-    split, rows = split or M, rows or M
-    dt = dtypes[0]
-    code = _DTYPES[dt]
-    outs = [torch.empty((rows, N), dtype=dt, device=dev) for _ in range(2 if two else 1)]
+    out = torch.empty((M, N), dtype=out_dtype, device=dev)
     L = _lib.lib()
     nbytes = L.pnft_weight_grad_workspace_size(K, M, N)
     ws = _workspace(nbytes, dev)
-    _lib.check(L.pnft_weight_grad(dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), outs[0].data_ptr(),
-                                  outs[1].data_ptr() if two else None, N, split, rows, code, ws.data_ptr(), nbytes, K, M,
-                                  N, _DTYPES[dy.dtype], _status_ptr(dev), _stream(dev)), "pnft_weight_grad")
-    return outs
+    rc = L.pnft_weight_grad(dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), out.data_ptr(), None, N, M, M, _DTYPES[out_dtype],
+                            ws.data_ptr(), nbytes, K, M, N, _DTYPES[dy.dtype], _status_ptr(dev), _stream(dev))
+    _lib.check(rc, "pnft_weight_grad")
+    return out
 
 
 # ---------------------------------------------------------------- gated product
+# From this input width on the forward keeps the pre-activations (6 bytes per element of each,
+# written once and read once) and the backward reads them; below it computes them again, which
+# costs 4 M D F operations but no memory. <measured below>
+_KEEP_FROM = 640
+
+
+def _gated_forward(x, wg, wu, bg, bu, act: int, dt: torch.dtype, keep: bool):
+    """(h, x's rows, the weights' rows, the kept pre-activations or None)."""
+    dev = x.device
+    _check_pending(dev)
+    F_, D = wg.shape
+    with _on(dev):
+        x2 = _rows16(x.reshape(-1, D), dt)
+        wgc, wuc = _rows16(wg, dt), _rows16(wu, dt)
+        M = x2.shape[0]
+        h = torch.empty((M, F_), dtype=dt, device=dev)
+        pre = torch.empty((3, M, _pad8(F_)), dtype=torch.int16, device=dev) if keep else None
+        b = bg if bg is not None else bu
+        rc = _lib.lib().pnft_gated_fwd(
+            x2.data_ptr(), _ld(x2), wgc.data_ptr(), _ld(wgc), wuc.data_ptr(), _ld(wuc), _ptr(bg), _ptr(bu),
+            _lib.DTYPE_F32 if b is None else _DTYPES[b.dtype], h.data_ptr(), F_, _ptr(pre), _pad8(F_), M, D, F_, act,
+            _DTYPES[dt], _status_ptr(dev), _stream(dev))
+        _lib.check(rc, "pnft_gated_fwd")
+    return h.view(*x.shape[:-1], F_), x2, wgc, wuc, pre
+
+
 class _GatedLinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, wg, wu, bg, bu, act: int, dt: torch.dtype, keep: str | None, pre=None):
-        dev = x.device
-        _check_pending(dev)
-        D, F_ = wg.shape[1], wg.shape[0]
-        with torch.cuda.device(dev):
-            x2 = _rows16(x.reshape(-1, D), dt)
-            wgc, wuc = (_rows16(w, dt) for w in (pre if pre is not None else (wg, wu)))
-            M, L, st = x2.shape[0], _lib.lib(), _stream(dev)
-            biases = _biases(bg, bu)
-            h = torch.empty((M, F_), dtype=dt, device=dev)
-            g = u = None
-            if keep == "pre":
-                Fp = _pad8(F_)
-                g, u = torch.empty((2, M, Fp), dtype=dt, device=dev)
-            _lib.check(L.pnft_gated_fwd(x2.data_ptr(), _ld(x2), wgc.data_ptr(), _ld(wgc), wuc.data_ptr(), _ld(wuc),
-                                        *biases, h.data_ptr(), F_, _ptr(g), _ptr(u), 0 if g is None else g.stride(0), M, D,
-                                        F_, act, _DTYPES[dt], _status_ptr(dev), st), "pnft_gated_fwd")
-        if keep is not None:
-            ctx.act8 = None
-            if keep == "act8":
-                p = act8_pack(x2)
-                ctx.act8 = (p.shape, p.dtype)
-                ctx.save_for_backward(p.q, p.exponents, None, None, wgc, wuc, bg, bu)
-            else:
-                ctx.save_for_backward(x2, None, g, u, wgc, wuc, bg, bu)
-            ctx.act, ctx.dt, ctx.x_shape, ctx.x_dtype = act, dt, x.shape, x.dtype
-            ctx.w_dtypes = (wg.dtype, wu.dtype)
-        return h.view(*x.shape[:-1], F_)
+    def forward(ctx, x, wg, wu, bg, bu, act: int, dt: torch.dtype, in8: bool, copies):
+        wgc, wuc = copies if copies is not None else (wg, wu)
+        h, x2, wgc, wuc, pre = _gated_forward(x, wgc, wuc, bg, bu, act, dt, not in8 and wg.shape[1] >= _KEEP_FROM)
+        p = act8_pack(x2) if in8 else None
+        if in8:
+            ctx.save_for_backward(p.q, p.exponents, wgc, wuc, bg, bu)
+        else:
+            ctx.save_for_backward(x2, pre, wgc, wuc, bg, bu)
+        ctx.p8 = (p.shape, p.dtype) if in8 else None
+        ctx.act, ctx.dt, ctx.x_shape, ctx.x_dtype, ctx.w_dtype = act, dt, x.shape, x.dtype, wg.dtype
+        return h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        a, b, g, u, wg, wu, bg, bu = ctx.saved_tensors
+        a, b, wg, wu, bg, bu = ctx.saved_tensors
         dt, dev = ctx.dt, wg.device
         F_, D = wg.shape
+        need = ctx.needs_input_grad
         L = _lib.lib()
-        with torch.cuda.device(dev):
-            st = _stream(dev)
-            dh2 = _rows16(dh.reshape(-1, F_), dt)
-            M = dh2.shape[0]
-            Fp = _pad8(F_)
-            x2 = a if ctx.act8 is None else _act8_rows(Act8(a, b, *ctx.act8), dt)
-            need = ctx.needs_input_grad
-            d = torch.empty((M, 2 * Fp), dtype=dt, device=dev)  # dg, du side by side: one weight-gradient product
-            dg, du = d[:, :F_], d[:, Fp:Fp + F_]
-            dbg = torch.empty(F_, dtype=bg.dtype, device=dev) if bg is not None and need[3] else None
-            dbu = torch.empty(F_, dtype=bu.dtype, device=dev) if bu is not None and need[4] else None
-            code, b_code = _DTYPES[dt], _b_code(bg, bu)
-            sums = dbg is not None or dbu is not None
-            nbytes = L.pnft_gated_bias_workspace_size(M, F_) if sums else 0
-            ws = _workspace(nbytes, dev) if sums else None
-            if ctx.act8 is None:
-                _lib.check(L.pnft_gated_bwd_point(dh2.data_ptr(), _ld(dh2), g.data_ptr(), u.data_ptr(), g.stride(0),
-                                                  dg.data_ptr(), du.data_ptr(), 2 * Fp, _ptr(dbg), _ptr(dbu), b_code, _ptr(ws),
-                                                  nbytes, M, F_, ctx.act, code, st), "pnft_gated_bwd_point")
-            else:
-                _lib.check(L.pnft_gated_bwd_recompute(x2.data_ptr(), _ld(x2), wg.data_ptr(), _ld(wg), wu.data_ptr(), _ld(wu),
-                                                      *_biases(bg, bu), dh2.data_ptr(), _ld(dh2), dg.data_ptr(),
-                                                      du.data_ptr(), 2 * Fp, M, D, F_, ctx.act, code, _status_ptr(dev), st),
-                           "pnft_gated_bwd_recompute")
-                if sums:
-                    _lib.check(L.pnft_gated_bwd_point(None, 0, dg.data_ptr(), du.data_ptr(), 2 * Fp, None, None, 0, _ptr(dbg),
-                                                      _ptr(dbu), b_code, _ptr(ws), nbytes, M, F_, ctx.act, code, st),
-                               "pnft_gated_bwd_point")
-            dx = None
-            if need[0]:
-                dx = torch.empty((M, D), dtype=ctx.x_dtype, device=dev)
-                nb = L.pnft_gated_dx_workspace_size(M, D, F_)
-                ws2 = _workspace(nb, dev)
-                _lib.check(L.pnft_gated_dx(dg.data_ptr(), du.data_ptr(), 2 * Fp, wg.data_ptr(), _ld(wg), wu.data_ptr(), _ld(wu),
-                                           dx.data_ptr(), D, _DTYPES[ctx.x_dtype], ws2.data_ptr(), nb, M, D, F_, code,
-                                           _status_ptr(dev), st), "pnft_gated_dx")
-                dx = dx.view(ctx.x_shape)
-            dwg = dwu = None
-            if need[1] or need[2]:
-                dwg, dwu = _weight_grads(d, x2, ctx.w_dtypes, split=Fp, rows=F_)
-                dwg, dwu = (t if n else None for t, n in ((dwg, need[1]), (dwu, need[2])))
+        with _on(dev):
+            x2, pre = (a, b) if ctx.p8 is None else (_act8_rows(Act8(a, b, *ctx.p8), dt), None)
+            M = x2.shape[0]
+            dh2 = dh.reshape(-1, F_)
+            if dh2.dtype != dt:
+                dh2 = dh2.to(dt)
+            if F_ % 8 == 0:
+                dh2 = _rows16(dh2, dt)
+            elif dh2.stride(1) != 1 or dh2.stride(0) < F_:
+                dh2 = dh2.contiguous()
+            grad = lambda n, shape, t: torch.empty(shape, dtype=t, device=dev) if n else None  # noqa: E731
+            dx = grad(need[0], ctx.x_shape, ctx.x_dtype)
+            dwg, dwu = grad(need[1], (F_, D), ctx.w_dtype), grad(need[2], (F_, D), ctx.w_dtype)
+            bias = bg if bg is not None else bu
+            b_dtype = torch.float32 if bias is None else bias.dtype
+            dbg, dbu = grad(bg is not None and need[3], F_, b_dtype), grad(bu is not None and need[4], F_, b_dtype)
+            nbytes = L.pnft_gated_bwd_workspace_size(M, D, F_)
+            ws = _workspace(nbytes, dev)
+            rc = L.pnft_gated_bwd(
+                x2.data_ptr(), _ld(x2), wg.data_ptr(), _ld(wg), wu.data_ptr(), _ld(wu), _ptr(bg), _ptr(bu), _DTYPES[b_dtype],
+                _ptr(pre), _pad8(F_), dh2.data_ptr(), max(_ld(dh2) if F_ % 8 == 0 else dh2.stride(0), F_), _ptr(dx), D,
+                _DTYPES[ctx.x_dtype], _ptr(dwg), _ptr(dwu), D, _DTYPES[ctx.w_dtype], _ptr(dbg), _ptr(dbu), ws.data_ptr(),
+                nbytes, M, D, F_, ctx.act, _DTYPES[dt], _status_ptr(dev), _stream(dev))
+            _lib.check(rc, "pnft_gated_bwd")
         return dx, dwg, dwu, dbg, dbu, None, None, None, None
-
-
-def _b_code(bg, bu) -> int:
-    b = bg if bg is not None else bu
-    return _lib.DTYPE_F32 if b is None else _DTYPES[b.dtype]
-
-
-def _biases(bg, bu):
-    return _ptr(bg), _ptr(bu), _b_code(bg, bu)
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: torch.Tensor | None = None,
@@ -293,44 +287,52 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
         raise RuntimeError("gated_linear: the two projections' parameters must have the same dtype")
     dt = _compute_dtype(x, "gated_linear")
     b_gate, b_up = (None if b is None else b.contiguous() for b in (b_gate, b_up))
-    keep = None
+    copies = casts.lookup(w_gate, w_up) if casts is not None and dt == torch.bfloat16 else None
     if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        keep = "act8" if checkpoint_8bit else "pre"
-    pre = casts.lookup(w_gate, w_up) if casts is not None and dt == torch.bfloat16 else None
-    return _GatedLinearFn.apply(x, w_gate, w_up, b_gate, b_up, _ACTS[activation], dt, keep, pre)
+        return _GatedLinearFn.apply(x, w_gate, w_up, b_gate, b_up, _ACTS[activation], dt, checkpoint_8bit, copies)
+    wg, wu = copies if copies is not None else (w_gate, w_up)
+    return _gated_forward(x, wg, wu, b_gate, b_up, _ACTS[activation], dt, False)[0]
 
 
 # ---------------------------------------------------------------- streamed cross entropy
+def _xent_forward(h, weight, targets, ignore_index: int, reduction: str, dt: torch.dtype):
+    """(loss, the rows that count, the kept state, the weight's rows)."""
+    dev = h.device
+    _check_pending(dev)
+    V, D = weight.shape
+    L = _lib.lib()
+    with _on(dev):
+        h2 = h.reshape(-1, D)
+        if h2.dtype != dt:
+            h2 = h2.to(dt)
+        if h2.stride(1) != 1 and D > 1 or h2.stride(0) < D:
+            h2 = h2.contiguous()
+        w = _rows16(weight, dt)
+        t = targets.reshape(-1)
+        if t.dtype != torch.int64 or not t.is_contiguous():
+            t = t.to(torch.int64).contiguous()
+        M, Dp = h2.shape[0], _pad8(D)
+        hc = torch.empty(((M + 127) // 128 * 128, Dp), dtype=dt, device=dev)
+        saved = _workspace(L.pnft_stream_xent_saved_size(M), dev)
+        rows = torch.empty(M, dtype=torch.float32, device=dev) if reduction == "none" else None
+        loss = torch.empty((), dtype=torch.float32, device=dev) if rows is None else None
+        nbytes = L.pnft_stream_xent_fwd_workspace_size(M, V)
+        ws = _workspace(nbytes, dev)
+        rc = L.pnft_stream_xent_fwd(h2.data_ptr(), h2.stride(0), w.data_ptr(), _ld(w), t.data_ptr(), ignore_index,
+                                    hc.data_ptr(), Dp, saved.data_ptr(), _ptr(rows), _ptr(loss), reduction == "mean",
+                                    ws.data_ptr(), nbytes, M, V, D, _DTYPES[dt], _status_ptr(dev), _stream(dev))
+        _lib.check(rc, "pnft_stream_xent_fwd")
+    return (loss if rows is None else rows.view(targets.shape)), hc, saved, w
+
+
 class _StreamXentFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, h, weight, targets, ignore_index: int, reduction: str, dt: torch.dtype, need: bool, pre=None):
-        dev = h.device
-        _check_pending(dev)
-        V, D = weight.shape
-        L = _lib.lib()
-        with torch.cuda.device(dev):
-            st = _stream(dev)
-            h2 = h.reshape(-1, D)
-            h2 = h2 if h2.dtype == dt else h2.to(dt)
-            h2 = h2 if D == 1 or h2.stride(1) == 1 else h2.contiguous()
-            w = _rows16(weight if pre is None else pre, dt)
-            t = targets.reshape(-1).to(torch.int64).contiguous()
-            M = h2.shape[0]
-            Mp, Dp = (M + 127) // 128 * 128, _pad8(D)
-            hc = torch.empty((Mp, Dp), dtype=dt, device=dev)
-            saved = _workspace(L.pnft_stream_xent_saved_size(M), dev)
-            rows = torch.empty(M, dtype=torch.float32, device=dev) if reduction == "none" else None
-            loss = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
-            nbytes = L.pnft_stream_xent_fwd_workspace_size(M, V)
-            ws = _workspace(nbytes, dev)
-            _lib.check(L.pnft_stream_xent_fwd(h2.data_ptr(), max(h2.stride(0), D), w.data_ptr(), _ld(w), t.data_ptr(),
-                                              ignore_index, hc.data_ptr(), Dp, saved.data_ptr(), _ptr(rows), _ptr(loss),
-                                              reduction == "mean", ws.data_ptr(), nbytes, M, V, D, _DTYPES[dt],
-                                              _status_ptr(dev), st), "pnft_stream_xent_fwd")
-        if need:
-            ctx.save_for_backward(hc, saved, w)
-            ctx.M, ctx.dt, ctx.reduction, ctx.h_shape, ctx.h_dtype, ctx.w_dtype = M, dt, reduction, h.shape, h.dtype, weight.dtype
-        return loss if rows is None else rows.view(targets.shape)
+    def forward(ctx, h, weight, targets, ignore_index: int, reduction: str, dt: torch.dtype, copy):
+        loss, hc, saved, w = _xent_forward(h, weight if copy is None else copy, targets, ignore_index, reduction, dt)
+        ctx.save_for_backward(hc, saved, w)
+        ctx.M, ctx.dt, ctx.reduction = targets.numel(), dt, reduction
+        ctx.h_shape, ctx.h_dtype, ctx.w_dtype = h.shape, h.dtype, weight.dtype
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -339,7 +341,7 @@ class _StreamXentFn(torch.autograd.Function):
         V, D = w.shape
         M, dev = ctx.M, w.device
         L = _lib.lib()
-        with torch.cuda.device(dev):
+        with _on(dev):
             dl = dloss.reshape(-1).float()
             need_h, need_w = ctx.needs_input_grad[:2]
             dh = torch.empty((M, D), dtype=ctx.h_dtype, device=dev) if need_h else None
@@ -351,7 +353,7 @@ class _StreamXentFn(torch.autograd.Function):
                                               _ptr(dh), D, _DTYPES[ctx.h_dtype], _ptr(dw), D, _DTYPES[ctx.w_dtype],
                                               ws.data_ptr(), nbytes, M, V, D, _DTYPES[ctx.dt], _status_ptr(dev), _stream(dev)),
                        "pnft_stream_xent_bwd")
-        return None if dh is None else dh.view(ctx.h_shape), dw, None, None, None, None, None, None
+        return None if dh is None else dh.view(ctx.h_shape), dw, None, None, None, None, None
 
 
 def streamed_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, *,
@@ -387,8 +389,11 @@ def streamed_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch
         if reduction == "none":
             return h.float().sum(-1)
         return zero * 0.0 if reduction == "sum" else zero * math.nan
-    pre = casts.lookup(weight)[0] if casts is not None and dt == torch.bfloat16 and casts.lookup(weight) else None
-    return _StreamXentFn.apply(h, weight, targets, int(ignore_index), reduction, dt, need, pre)
+    copy = casts.lookup(weight) if casts is not None and dt == torch.bfloat16 else None
+    copy = None if copy is None else copy[0]
+    if need:
+        return _StreamXentFn.apply(h, weight, targets, int(ignore_index), reduction, dt, copy)
+    return _xent_forward(h, weight if copy is None else copy, targets, int(ignore_index), reduction, dt)[0]
 
 
 # ---------------------------------------------------------------- the block

@@ -89,10 +89,11 @@ class _StatusWord:
             self.host = None
             self.dev = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
             self.ptr = self.dev.data_ptr()
+        self._word = None if self.host is None else ctypes.c_int32.from_address(self.host.data_ptr())
 
     def peek(self) -> int:
         """The code seen so far without synchronising (0 when only device memory holds it)."""
-        return int(self.host[0]) if self.host is not None else _lib.DEV_OK
+        return self._word.value if self._word is not None else _lib.DEV_OK
 
     def read(self) -> int:
         return int(self.host[0]) if self.host is not None else int(self.dev.item())

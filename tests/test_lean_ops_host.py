@@ -15,8 +15,9 @@ def refused(rc, code, word):
     assert rc == code and word in _lib.last_error(), (rc, _lib.last_error())
 
 
-def gated(M=4, D=64, F=128, act=0, dtype=BF16, ldx=64, ldh=128, x=A, h=A, g=None, u=None):
-    return _lib.lib().pnft_gated_fwd(x, ldx, A, 64, A, 64, None, None, FP32, h, ldh, g, u, 128, M, D, F, act, dtype, None, None)
+def gated(M=4, D=64, F=128, act=0, dtype=BF16, ldx=64, ldh=128, x=A, h=A, pre=None, ldp=128, b_dtype=FP32):
+    return _lib.lib().pnft_gated_fwd(x, ldx, A, 64, A, 64, None, None, b_dtype, h, ldh, pre, ldp, M, D, F, act, dtype, None,
+                                     None)
 
 
 def test_gated_fwd_refuses():
@@ -26,7 +27,8 @@ def test_gated_fwd_refuses():
     refused(gated(act=2), _lib.EINVAL, "activation")
     refused(gated(dtype=FP32), _lib.EUNSUPPORTED, "float16")
     refused(gated(h=None), _lib.EINVAL, "null")
-    refused(gated(g=A), _lib.EINVAL, "null")
+    refused(gated(pre=A, ldp=100), _lib.EINVAL, "stride")
+    refused(gated(pre=A + 8), _lib.EINVAL, "aligned")
     refused(gated(ldh=127), _lib.EINVAL, "stride")
     refused(gated(ldx=65), _lib.EUNSUPPORTED, "aligned")
     refused(gated(x=A + 2), _lib.EUNSUPPORTED, "aligned")
@@ -36,15 +38,25 @@ def test_gated_fwd_refuses():
 
 def test_gated_backward_refuses():
     L = _lib.lib()
-    args = lambda dh=A, ldd=128: (A, 64, A, 64, A, 64, None, None, FP32, dh, 128, A, A, ldd, 4, 64, 128, 0, BF16, None, None)  # noqa: E731
-    refused(L.pnft_gated_bwd_recompute(*args(dh=None)), _lib.EINVAL, "null")
-    refused(L.pnft_gated_bwd_recompute(*args(ldd=100)), _lib.EINVAL, "stride")
-    point = lambda dh, dbg, ws, n: L.pnft_gated_bwd_point(dh, 128, A, A, 128, A, A, 128, dbg, None, FP32, ws, n, 4, 128, 0, BF16, None)  # noqa: E731
-    refused(point(None, None, None, 0), _lib.EINVAL, "null")
-    refused(point(A, A, A, 16), _lib.EINVAL, "workspace")
-    dx = lambda ldd, ws, n, M=4: L.pnft_gated_dx(A, A, ldd, A, 64, A, 64, A, 64, BF16, ws, n, M, 64, 8192, BF16, None, None)  # noqa: E731
-    refused(dx(8191, A, 1 << 30), _lib.EUNSUPPORTED, "aligned")
-    assert L.pnft_gated_dx_workspace_size(0, 64, 128) == 0
+    n = L.pnft_gated_bwd_workspace_size(4, 64, 128)
+    assert n > 0 and L.pnft_gated_bwd_workspace_size(0, 64, 128) == 0
+
+    def bwd(dh=A, lddh=128, pre=None, ldp=128, lddx=64, lddw=64, b=FP32, t=BF16, ws=A, nb=n, ldx=64, F=128):
+        return L.pnft_gated_bwd(A, ldx, A, 64, A, 64, None, None, b, pre, ldp, dh, lddh, A, lddx, t, A, A, lddw, t, A, A, ws,
+                                nb, 4, 64, F, 0, BF16, None, None)
+
+    refused(bwd(dh=None), _lib.EINVAL, "null")
+    refused(bwd(lddh=127), _lib.EINVAL, "stride")
+    refused(bwd(lddx=63), _lib.EINVAL, "stride")
+    refused(bwd(lddw=63), _lib.EINVAL, "stride")
+    refused(bwd(pre=A + 2), _lib.EINVAL, "aligned")
+    refused(bwd(lddh=129), _lib.EUNSUPPORTED, "aligned")
+    refused(bwd(dh=A + 2), _lib.EUNSUPPORTED, "aligned")
+    refused(bwd(b=7), _lib.EINVAL, "type")
+    refused(bwd(t=-1), _lib.EINVAL, "type")
+    refused(bwd(ws=None), _lib.EINVAL, "workspace")
+    refused(bwd(nb=n - 1), _lib.EINVAL, "workspace")
+    refused(bwd(ldx=65), _lib.EUNSUPPORTED, "aligned")
 
 
 def wgrad(K=64, M=16, N=32, c1=None, row_split=16, rows=16, ldc=32, dtype=BF16, c_dtype=FP32, lddy=16):
@@ -56,8 +68,10 @@ def test_weight_grad_refuses():
     refused(wgrad(dtype=FP32), _lib.EUNSUPPORTED, "float16")
     refused(wgrad(c_dtype=9), _lib.EINVAL, "type")
     refused(wgrad(row_split=8, rows=8), _lib.EINVAL, "null")
-    refused(wgrad(row_split=8, rows=9, c1=A), _lib.EINVAL, "layout")  # more rows than the split leaves
-    refused(wgrad(row_split=10, rows=8, c1=A), _lib.EINVAL, "layout")  # past the product's end
+    refused(wgrad(row_split=8, rows=8, c1=A), _lib.EINVAL, "multiple of 128")
+    two = dict(M=256, lddy=256, row_split=128, c1=A)
+    refused(wgrad(rows=129, **two), _lib.EINVAL, "layout")  # more rows than the split leaves
+    refused(wgrad(rows=120, **{**two, "M": 240}), _lib.EINVAL, "layout")  # past the product's end
     refused(wgrad(ldc=31), _lib.EINVAL, "layout")
     refused(wgrad(lddy=17), _lib.EUNSUPPORTED, "aligned")
 
