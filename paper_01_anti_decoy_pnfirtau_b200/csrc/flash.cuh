@@ -145,9 +145,9 @@ bool tma_ok_bhnd(const void* ptr, const int64_t* s);
 // 128-byte swizzled, out-of-range elements read as zero.
 int tma_map_rows(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t row_stride, int box_rows);
 // 3-D map {cols, rows, slices} of 2-byte (any 16-bit type) or fp32 elements, strides
-// in elements: boxes of 128 bytes x box_rows rows, 128-byte swizzled.
+// in elements: boxes of row_bytes (64 or 128, swizzled over as many) x box_rows rows.
 int tma_map_out(CUtensorMap* m, const void* base, int size, int64_t cols, int64_t rows, int64_t ld, int64_t slices,
-                int64_t slice_stride, int box_rows);
+                int64_t slice_stride, int box_rows, int row_bytes = 128);
 bool device_is_sm100();
 
 }  // namespace pnft

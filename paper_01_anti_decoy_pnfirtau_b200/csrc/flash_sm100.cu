@@ -606,18 +606,18 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// Encodes a map of 128-byte-swizzled boxes. The driver wants a current context, which a
+// Encodes a map of swizzled boxes. The driver wants a current context, which a
 // thread that has made no runtime call yet (autograd's, on its first backward) lacks:
 // setting the current device once makes its primary context current.
 static int encode(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
-                  const cuuint64_t* strides, const cuuint32_t* box) {
+                  const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return fail(PNFT_ECUDA, "cuTensorMapEncodeTiled unavailable from the driver");
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = CUDA_SUCCESS;
   for (int attempt = 0; attempt < 2; ++attempt) {
     r = enc(m, type, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+            swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     int dev = 0;
     if (r != CUDA_ERROR_INVALID_CONTEXT || cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) break;
   }
@@ -640,11 +640,12 @@ int tma_map_rows(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, i
 }
 
 int tma_map_out(CUtensorMap* m, const void* base, int size, int64_t cols, int64_t rows, int64_t ld, int64_t slices,
-                int64_t slice_stride, int box_rows) {
+                int64_t slice_stride, int box_rows, int row_bytes) {
   const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)slices};
   const cuuint64_t strides[2] = {(cuuint64_t)(ld * size), (cuuint64_t)((slices > 1 ? slice_stride : ld) * size)};
-  const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
-  return encode(m, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box);
+  const cuuint32_t box[3] = {(cuuint32_t)(row_bytes / size), (cuuint32_t)box_rows, 1};
+  return encode(m, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box,
+                row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 bool tma_ok_bhnd(const void* ptr, const int64_t* s) {

@@ -20,7 +20,18 @@ namespace {
 
 using namespace tc;
 
-constexpr float kSqrtHalf = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143268f;
+constexpr float kSqrtHalf = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143268f, kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float fast_ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
 // act(g); deriv: also act'(g). The exponentials and the quotient are the fast ones
 // (a few units of 2^-23): the results are rounded to 16 bits. GELU's normal
@@ -28,12 +39,12 @@ constexpr float kSqrtHalf = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143
 template <bool DERIV, int ACT>
 __device__ __forceinline__ float act_value(float g, float* deriv) {
   if (ACT == PNFT_ACT_SILU) {
-    const float s = __fdividef(1.f, 1.f + __expf(-g));
+    const float s = fast_rcp(1.f + fast_ex2(-kLog2e * g));
     if (DERIV) *deriv = s * (1.f + g * (1.f - s));
     return g * s;
   }
   const float cdf = 0.5f * erfcf(-kSqrtHalf * g);
-  if (DERIV) *deriv = cdf + g * (kInvSqrt2Pi * __expf(-0.5f * g * g));
+  if (DERIV) *deriv = cdf + g * (kInvSqrt2Pi * fast_ex2(-0.5f * kLog2e * g * g));
   return g * cdf;
 }
 
@@ -42,34 +53,37 @@ __device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
   return load16(static_cast<const uint16_t*>(p) + i, dtype == PNFT_DTYPE_BF16);
 }
 
-// 32 values of a bias vector from column `col`, `n` of them inside.
-__device__ __forceinline__ void add_bias(float (&v)[32], const void* bias, int dtype, int col, int n) {
-  if (n >= 32 && reinterpret_cast<uintptr_t>(bias) % 16 == 0) {
+// W values of a bias vector from column `col` (a multiple of 16), `n` of them inside.
+template <int W>
+__device__ __forceinline__ void add_bias(float (&v)[W], const void* bias, int dtype, int col, int n) {
+  if (n >= W && reinterpret_cast<uintptr_t>(bias) % 16 == 0) {
     if (dtype == PNFT_DTYPE_F32) {
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) {
+      for (int i = 0; i < W; i += 4) {
         const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(bias) + col + i);
         v[i] += f.x, v[i + 1] += f.y, v[i + 2] += f.z, v[i + 3] += f.w;
       }
     } else {
-      float b[32];
-      load_row16<32>(static_cast<const uint16_t*>(bias) + col, b, 32, true, dtype == PNFT_DTYPE_BF16);
+      float b[W];
+      load_row16<W>(static_cast<const uint16_t*>(bias) + col, b, W, true, dtype == PNFT_DTYPE_BF16);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] += b[i];
+      for (int i = 0; i < W; ++i) v[i] += b[i];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < W; ++i)
       if (i < n) v[i] += load_any(bias, col + i, dtype);
   }
 }
 
 // FWD: h. KEEP: h and the three planes of g, u. BWD: dg, du from dh and the recomputed g, u.
+// A warp has 32 columns of g and of u of a tile, and takes them 16 at a time (96 registers).
 enum { FWD, KEEP, BWD };
 template <int MODE, int ACT>
 struct GatedEpi {
-  static constexpr int OUTS = MODE == FWD ? 2 : MODE == KEEP ? 3 : 2;  // boxes for results
-  static constexpr int BOXES = OUTS + (MODE == BWD);                  // and one for dh
+  static constexpr int WARPS = 16, W = 32, ROW_BYTES = 2 * W;
+  static constexpr int OUTS = MODE == KEEP ? 3 : 2;                                       // boxes for results
+  static constexpr int BOXES = OUTS + (MODE == BWD), BOX_BYTES = 32 * ROW_BYTES;          // and one for dh
   struct Params {
     const void *bg, *bu;
     int b_dtype, bf16;
@@ -78,14 +92,14 @@ struct GatedEpi {
     CUtensorMap dh;   // BWD
   };
   const Params& p;
-  EpiWarp w, out;
+  EpiWarp w;
   const Abort& ab;
-  Boxes<OUTS> boxes;
+  Boxes<OUTS, ROW_BYTES> boxes;
   int phase, issued;
   __device__ GatedEpi(const Params& p_, const EpiWarp& w_, const Abort& ab_)
-      : p(p_), w(w_), out{w_.quad, w_.half, w_.lane, w_.smem + (MODE == BWD ? BOX_BYTES : 0), w_.bar}, ab(ab_), boxes(out),
+      : p(p_), w(w_), ab(ab_), boxes(EpiWarp{w_.quad, w_.slice, w_.lane, w_.smem + (MODE == BWD ? BOX_BYTES : 0), w_.bar}),
         phase(0), issued(0) {}
-  __device__ int col0(const Steps& q) const { return q.nt * (BN / 2) + w.half * (BN / 4); }
+  __device__ int col0(const Steps& q) const { return q.nt * (BN / 2) + w.slice * W; }
   __device__ void load_dh(const Steps& q) {
     if (w.lane == 0) {
       mbar_arrive_expect_tx(w.bar, BOX_BYTES);
@@ -109,7 +123,6 @@ struct GatedEpi {
   }
   template <class Release>
   __device__ __forceinline__ void tile(const Steps& q, uint32_t acc, Release release) {
-    constexpr int W = BN / 4;  // columns of g (and of u) of this warp
     const int row = q.it.row0 + 32 * w.quad, col = col0(q);
     const bool live = row < p.h.rows && col < p.h.cols, bf16 = p.bf16;
     if (MODE == BWD) {
@@ -125,40 +138,42 @@ struct GatedEpi {
         boxes.take_all(b);
     }
 #pragma unroll
-    for (int c = 0; c < W; c += 32) {
-      uint32_t rg[32], ru[32];
-      tmem_load32x2(acc + w.half * W + c, rg, acc + BN / 2 + w.half * W + c, ru);
-      if (c + 32 == W) release();
-      float g[32], u[32];
+    for (int c = 0; c < W; c += 16) {
+      float g[16], u[16];
+      {
+        uint32_t rg[16], ru[16];
+        tmem_load16x2(acc + w.slice * W + c, rg, acc + BN / 2 + w.slice * W + c, ru);
+        if (c + 16 == W) release();
 #pragma unroll
-      for (int i = 0; i < 32; ++i) g[i] = __uint_as_float(rg[i]), u[i] = __uint_as_float(ru[i]);
+        for (int i = 0; i < 16; ++i) g[i] = __uint_as_float(rg[i]), u[i] = __uint_as_float(ru[i]);
+      }
       const int n = p.h.cols - col - c;
-      if (p.bg) add_bias(g, p.bg, p.b_dtype, col + c, n);
-      if (p.bu) add_bias(u, p.bu, p.b_dtype, col + c, n);
+      if (p.bg) add_bias<16>(g, p.bg, p.b_dtype, col + c, n);
+      if (p.bu) add_bias<16>(u, p.bu, p.b_dtype, col + c, n);
       if (MODE == BWD) {
-        float d[32];
-        boxes.get16(w.smem, c / 32, d, bf16);
+        float d[16];
+        boxes.get16(w.smem, c, d, bf16);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
+        for (int i = 0; i < 16; ++i) {
           float da;
           const float a = act_value<true, ACT>(g[i], &da);
           g[i] = d[i] * u[i] * da;
           u[i] = d[i] * a;
         }
-        if (c + 32 == W) {  // dh's box has been read: the next tile's may come
+        if (c + 16 == W) {  // dh's box has been read: the next tile's may come
           __syncwarp();
           Steps next = q;
           next.next();
           if (next.valid()) load_dh(next);
         }
         if (!live) continue;
-        boxes.put16(b[0], c / 32, g, bf16);
-        boxes.put16(b[OUTS - 1], c / 32, u, bf16);
+        boxes.put16(b[0], c, g, bf16);
+        boxes.put16(b[OUTS - 1], c, u, bf16);
       } else {
         if (!live) continue;
         if (MODE == KEEP) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
+          for (int i = 0; i < 16; i += 8) {
             uint32_t x[4], y[4], z[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -174,8 +189,8 @@ struct GatedEpi {
           }
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) g[i] = act_value<false, ACT>(g[i], nullptr) * u[i];
-        boxes.put16(b[0], c / 32, g, bf16);
+        for (int i = 0; i < 16; ++i) g[i] = act_value<false, ACT>(g[i], nullptr) * u[i];
+        boxes.put16(b[0], c, g, bf16);
       }
     }
     if (!live) return;
@@ -184,16 +199,10 @@ struct GatedEpi {
     if (MODE == KEEP) {
       write(p.k, b[OUTS - 2], row, col, 0);
       write(p.k, b[OUTS - 1], row, col, 1);
-      if (p.h.tma) {
-        const uint32_t z = boxes.take();  // h's box again, once its store has read it
+      const uint32_t z = p.h.tma ? boxes.take() : b[0];  // h's box again, once its store has read it
 #pragma unroll
-        for (int i = 0; i < W / 8; ++i) boxes.put(z, i, low[i].x, low[i].y, low[i].z, low[i].w);
-        boxes.store(z, &p.k.map, col, row, 2);
-      } else {
-#pragma unroll
-        for (int i = 0; i < W / 8; ++i) boxes.put(b[0], i, low[i].x, low[i].y, low[i].z, low[i].w);
-        boxes.store(b[0], &p.k.map, col, row, 2);
-      }
+      for (int i = 0; i < W / 8; ++i) boxes.put(z, i, low[i].x, low[i].y, low[i].z, low[i].w);
+      boxes.store(z, &p.k.map, col, row, 2);
     }
   }
 };
@@ -375,8 +384,8 @@ extern "C" int pnft_gated_fwd(const void* x, int64_t ldx, const void* wg, int64_
   if (pre && !rows16(pre, ldp, 2)) return fail(PNFT_EINVAL, "gated_fwd: the kept rows must be 16-byte aligned");
   if (int rc = gated_operands("gated_fwd", x, ldx, wg, ldwg, wu, ldwu, D)) return rc;
   Out o, k;
-  int rc = make_out(&o, h, dtype, F, M, ldh);
-  if (!rc) rc = make_out(&k, pre, dtype, F, M, ldp, 3, M * ldp);
+  int rc = make_out(&o, h, dtype, F, M, ldh, 1, 0, 64);
+  if (!rc) rc = make_out(&k, pre, dtype, F, M, ldp, 3, M * ldp, 64);
   if (rc) return rc;
   return gated_gemm("gated_fwd", pre ? KEEP : FWD, x, ldx, wg, ldwg, wu, ldwu, bg, bu, b_dtype, o, k, nullptr, M, D, F, act,
                     dtype, status, as_stream(stream));
@@ -521,9 +530,9 @@ extern "C" int pnft_gated_bwd(const void* x, int64_t ldx, const void* wg, int64_
     }
     Out g, u;
     CUtensorMap map;
-    if (!rc) rc = make_out(&g, dg, dtype, F, M, ldd);
-    if (!rc) rc = make_out(&u, du, dtype, F, M, ldd);
-    if (!rc) rc = tma_map_out(&map, d, 2, F, M, ldh, 1, 0, 32);
+    if (!rc) rc = make_out(&g, dg, dtype, F, M, ldd, 1, 0, 64);
+    if (!rc) rc = make_out(&u, du, dtype, F, M, ldd, 1, 0, 64);
+    if (!rc) rc = tma_map_out(&map, d, 2, F, M, ldh, 1, 0, 32, 64);
     if (!rc)
       rc = gated_gemm("gated_bwd", BWD, x, ldx, wg, ldwg, wu, ldwu, bg, bu, b_dtype, g, u, &map, M, D, F, act, dtype, status, st);
     if (!rc && (dbg || dbu))

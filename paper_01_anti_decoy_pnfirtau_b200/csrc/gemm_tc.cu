@@ -5,11 +5,20 @@
 namespace pnft {
 namespace tc {
 
+int current_device() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? dev : 0;
+}
+
 int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-    n = 148;
+  static std::atomic<int> counts[64];
+  const int dev = current_device();
+  std::atomic<int>& c = counts[dev & 63];
+  int n = c.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    c.store(n, std::memory_order_relaxed);
+  }
   return n;
 }
 

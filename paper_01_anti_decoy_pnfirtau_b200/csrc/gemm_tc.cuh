@@ -10,7 +10,7 @@
 // its own TMEM, twice (2 x 256 columns). The pair walks work items; an item is one tile
 // (or, for epilogues that carry state along a row, a strip of tiles), optionally one of
 // several splits of K. Warp 0 loads 64-deep stages of A and B by TMA into a ring, one
-// lane of the even CTA's warp 1 issues the MMAs, and warps 2-9 run the epilogue of the
+// lane of the even CTA's warp 1 issues the MMAs, and 8 or 16 more run the epilogue of the
 // other accumulator, so a tile's epilogue overlaps the next tile's MMAs. Either operand
 // may be K-major (rows of K) or MN-major (K rows of M or N), so no caller transposes
 // anything. Rows, columns and K past the end are zero-filled by TMA.
@@ -19,6 +19,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "flash.cuh"
 #include "sm100_ptx.cuh"
@@ -34,10 +35,7 @@ constexpr int BN = 256, BK = 64;
 constexpr int HALF_BYTES = BM * BK * 2;    // a CTA's A rows, or its half of B, of one stage
 constexpr int STAGE_BYTES = 2 * HALF_BYTES;
 constexpr int GROUP_BYTES = 64 * BK * 2;   // MN-major: 64 columns x 64 K rows
-constexpr int EPI_WARPS = 8;
-constexpr int THREADS = 32 * (2 + EPI_WARPS);
 constexpr int STAGE_MAX = 226 * 1024;      // shared memory for the ring and the epilogue's buffers
-constexpr int BOX_BYTES = 4096;            // an epilogue box: 32 rows of 128 bytes, 128-byte swizzled
 
 // ------------------------------------------------------------------ PTX of the pair
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -203,32 +201,34 @@ struct Steps {
   }
 };
 
-// What an epilogue warp has: its TMEM lane quadrant, its half of the columns, its boxes
-// in shared memory and a barrier for loads into them.
+// What an epilogue warp has: its TMEM lane quadrant, its slice of the columns (of 2 or 4),
+// its boxes in shared memory and a barrier for loads into them.
 struct EpiWarp {
-  int quad, half, lane;
+  int quad, slice, lane;
   uint32_t smem, bar;
   __device__ int row() const { return 32 * quad + lane; }
 };
 
-// Epi: BOXES (4 KB buffers per warp); tile(steps, acc, release) for every accumulator
+// Epi: WARPS (8, or 16 where the arithmetic per element is what takes the time: a warp's
+// chain of TMEM load, exponentials and stores has long latencies, and 16 warps of at most 96
+// registers hide them twice as well), BOXES of BOX_BYTES per warp; tile(steps, acc, release) for every accumulator
 // (acc: its TMEM address with the warp's lanes; release() hands it back once its last
 // column is in registers), done() at the end.
 // DUAL_B: columns 0-127 of a tile come from tb[0] and 128-255 from tb[1], both at row
 // 128 * nt.
 template <class Epi>
 constexpr int stages() {
-  return (STAGE_MAX - EPI_WARPS * Epi::BOXES * BOX_BYTES) / STAGE_BYTES;
+  return (STAGE_MAX - Epi::WARPS * Epi::BOXES * Epi::BOX_BYTES) / STAGE_BYTES;
 }
 template <class Epi>
 constexpr int smem_bytes() {
-  return stages<Epi>() * STAGE_BYTES + EPI_WARPS * Epi::BOXES * BOX_BYTES + 1024;
+  return stages<Epi>() * STAGE_BYTES + Epi::WARPS * Epi::BOXES * Epi::BOX_BYTES + 1024;
 }
 
 template <bool A_MN, bool B_MN, bool DUAL_B, class Epi>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS), 1)
     gemm_kernel(const __grid_constant__ Args p, const __grid_constant__ typename Epi::Params ep) {
-  constexpr int STAGES = stages<Epi>();
+  constexpr int STAGES = stages<Epi>(), EPI_WARPS = Epi::WARPS;
   extern __shared__ __align__(1024) uint8_t raw[];
   const uint32_t sb = (smem_u32(raw) + 1023u) & ~1023u;
   __shared__ __align__(8) uint64_t bars[2 * STAGES + 5 + EPI_WARPS];  // full, empty, acc full x2, acc empty x2, done, warps
@@ -345,7 +345,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   } else {
     // -------------------------------------------------------------- epilogue
     const EpiWarp w{warp & 3, (warp - 2) >> 2, lane,
-                    sb + (uint32_t)(STAGES * STAGE_BYTES + (warp - 2) * Epi::BOXES * BOX_BYTES), warp_bar(warp - 2)};
+                    sb + (uint32_t)(STAGES * STAGE_BYTES + (warp - 2) * Epi::BOXES * Epi::BOX_BYTES), warp_bar(warp - 2)};
     Epi epi(ep, w, ab);
     int t = 0;
     for (Steps q(walk, p.s, pair, pairs, rank); q.valid(); q.next(), ++t) {
@@ -449,16 +449,19 @@ __device__ __forceinline__ void acc_load32(uint32_t addr, bool empty, float (&v)
 }
 
 // ------------------------------------------------------------------ boxes
-// A box is 32 rows of 128 bytes in shared memory, 128-byte swizzled (16-byte chunk c of row
-// r at chunk c ^ (r & 7)): a lane writes or reads its own row without bank conflicts, and
+// A box is 32 rows of RB = 128 (or 64) bytes in shared memory, swizzled (16-byte chunk c of
+// row r at chunk c ^ (r & 7), or c ^ (r / 2 & 3)): a lane writes or reads its own row without bank conflicts, and
 // TMA moves the box, clipped to the matrix. Boxes of a warp are used in turn; a box is free
 // again once the store out of it has read it.
-template <int N>
+template <int N, int RB = 128>
 struct Boxes {
   EpiWarp w;
   int at;
   __device__ explicit Boxes(const EpiWarp& w_) : w(w_), at(0) {}
-  __device__ __forceinline__ uint32_t box(int i) const { return w.smem + (uint32_t)i * BOX_BYTES; }
+  __device__ __forceinline__ uint32_t box(int i) const { return w.smem + (uint32_t)(i * 32 * RB); }
+  __device__ __forceinline__ static uint32_t chunk_at(uint32_t b, int row, int chunk) {
+    return b + (uint32_t)(RB * row) + 16u * (chunk ^ (RB == 128 ? row & 7 : (row >> 1) & 3));
+  }
   // the next box, free to write (stores of the N - 1 others may be in flight)
   __device__ __forceinline__ uint32_t take() {
     if (w.lane == 0) bulk_wait_read<N - 1>();
@@ -476,26 +479,28 @@ struct Boxes {
     at = 0;
   }
   __device__ __forceinline__ void put(uint32_t b, int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t u) const {
-    const uint32_t a = b + 128u * w.lane + 16u * (chunk ^ (w.lane & 7));
+    const uint32_t a = chunk_at(b, w.lane, chunk);
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(u) : "memory");
   }
   __device__ __forceinline__ uint4 get(uint32_t b, int chunk) const {
-    const uint32_t a = b + 128u * w.lane + 16u * (chunk ^ (w.lane & 7));
+    const uint32_t a = chunk_at(b, w.lane, chunk);
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
     return v;
   }
-  // 32 columns as 16-bit values: half `h` of the box
-  __device__ __forceinline__ void put16(uint32_t b, int h, const float (&v)[32], bool bf16) const {
+  // W columns as 16-bit values from column `c` of the box
+  template <int W>
+  __device__ __forceinline__ void put16(uint32_t b, int c, const float (&v)[W], bool bf16) const {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
-      put(b, 4 * h + i / 8, pack2(v[i], v[i + 1], bf16), pack2(v[i + 2], v[i + 3], bf16), pack2(v[i + 4], v[i + 5], bf16),
+    for (int i = 0; i < W; i += 8)
+      put(b, (c + i) / 8, pack2(v[i], v[i + 1], bf16), pack2(v[i + 2], v[i + 3], bf16), pack2(v[i + 4], v[i + 5], bf16),
           pack2(v[i + 6], v[i + 7], bf16));
   }
-  __device__ __forceinline__ void get16(uint32_t b, int h, float (&v)[32], bool bf16) const {
+  template <int W>
+  __device__ __forceinline__ void get16(uint32_t b, int c, float (&v)[W], bool bf16) const {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      const uint4 u = get(b, 4 * h + i / 8);
+    for (int i = 0; i < W; i += 8) {
+      const uint4 u = get(b, (c + i) / 8);
       const uint32_t q[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -526,12 +531,12 @@ struct Boxes {
   template <int SIZE>
   __device__ __forceinline__ void store_plain(uint32_t b, void* dst, int64_t ld, int rows, int cols) const {
     __syncwarp();
-    constexpr int PER = 128 / SIZE;  // elements per row of a box
+    constexpr int PER = RB / SIZE;  // elements per row of a box
     for (int r = 0; r < min(rows, 32); ++r) {
 #pragma unroll
       for (int k = 0; k < PER / 32; ++k) {
         const int c = 32 * k + w.lane, byte = c * SIZE;
-        const uint32_t a = b + 128u * r + 16u * ((byte >> 4) ^ (r & 7)) + (byte & 15);
+        const uint32_t a = chunk_at(b, r, byte >> 4) + (byte & 15);
         if (c >= cols) continue;
         if (SIZE == 2) {
           uint16_t v;
@@ -554,7 +559,7 @@ struct Boxes {
 
 // A matrix that an epilogue writes: by TMA where its rows are 16-byte aligned.
 struct Out {
-  CUtensorMap map;  // {columns, rows, slices}, boxes of 128 bytes x 32 rows
+  CUtensorMap map;  // {columns, rows, slices}, boxes of 32 rows
   void* base;
   int64_t ld;
   int rows, cols;
@@ -569,7 +574,7 @@ struct Out {
 // which an fp32 C would show.
 template <bool PROMOTE>
 struct StoreEpi {
-  static constexpr int BOXES = 2;
+  static constexpr int WARPS = 8, BOXES = 2, BOX_BYTES = 4096;
   struct Params {
     Out c[2];
     int row_split;
@@ -610,7 +615,7 @@ struct StoreEpi {
       const int h = (c >> 5) & 1;  // a box takes 64 columns: two calls
       if (o.cols - (col - 32 * h) <= 0) return;
       if (h == 0) box = boxes.take();
-      boxes.put16(box, h, v, p.dtype == PNFT_DTYPE_BF16);
+      boxes.put16(box, 32 * h, v, p.dtype == PNFT_DTYPE_BF16);
       if (h == 0) return;
       if (o.tma)
         boxes.store(box, &o.map, col - 32, row, 0);
@@ -621,7 +626,7 @@ struct StoreEpi {
   }
   template <class Release>
   __device__ __forceinline__ void tile(const Steps& q, uint32_t acc, Release release) {
-    const int c0 = w.half * (BN / 2);
+    const int c0 = w.slice * (BN / 2);
     const bool empty = q.it.kbn == 0;
     uint32_t box = 0;
     if (PROMOTE) {
@@ -654,7 +659,8 @@ struct StoreEpi {
 };
 
 // ------------------------------------------------------------------ host side
-int sm_count();
+int current_device();
+int sm_count();  // of the current device
 // Splits of K for an output of `tiles` tiles: about one work item per pair of SMs, at
 // least 8 K blocks (512 of K) each, since shorter ones cost more in partial sums than
 // they gain.
@@ -683,12 +689,12 @@ inline bool rows16(const void* p, int64_t ld, int size) {
 inline int dtype_size(int dtype) { return dtype == PNFT_DTYPE_F32 ? 4 : 2; }
 
 inline int make_out(Out* o, void* base, int dtype, int64_t cols, int64_t rows, int64_t ld, int64_t slices = 1,
-                    int64_t slice_stride = 0) {
+                    int64_t slice_stride = 0, int row_bytes = 128) {
   memset(o, 0, sizeof(*o));
   o->base = base, o->ld = ld, o->rows = (int)rows, o->cols = (int)cols;
   if (!base) return PNFT_OK;
   o->tma = rows16(base, ld, dtype_size(dtype)) && ld < ((int64_t)1 << 37);
-  return o->tma ? tma_map_out(&o->map, base, dtype_size(dtype), cols, rows, ld, slices, slice_stride, 32) : PNFT_OK;
+  return o->tma ? tma_map_out(&o->map, base, dtype_size(dtype), cols, rows, ld, slices, slice_stride, 32, row_bytes) : PNFT_OK;
 }
 
 // K-major operand: `rows` rows of K elements; MN-major operand: K rows of `cols`
@@ -723,9 +729,14 @@ int launch(const char* what, const Args& a, const typename Epi::Params& ep, cuda
   if (items > (1 << 30)) return fail(PNFT_EUNSUPPORTED, "%s: too many tiles", what);
   auto* k = gemm_kernel<A_MN, B_MN, DUAL_B, Epi>;
   constexpr int smem = smem_bytes<Epi>();
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return check_launch(what, 0);
-  k<<<(unsigned)(2 * std::min<int64_t>(items, sm_count() / 2)), THREADS, smem, st>>>(a, ep);
+  static std::atomic<uint64_t> ready{0};  // devices on which the kernel has its shared memory
+  const uint64_t bit = 1ull << (current_device() & 63);
+  if (!(ready.load(std::memory_order_acquire) & bit)) {
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return check_launch(what, 0);
+    ready.fetch_or(bit, std::memory_order_release);
+  }
+  k<<<(unsigned)(2 * std::min<int64_t>(items, sm_count() / 2)), 32 * (2 + Epi::WARPS), smem, st>>>(a, ep);
   return check_launch(what, 1);
 }
 

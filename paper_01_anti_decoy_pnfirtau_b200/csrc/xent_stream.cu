@@ -130,12 +130,12 @@ __global__ void __launch_bounds__(CT) xent_compact_kernel(CompactArgs p) {
 }
 
 // ------------------------------------------------------------------ forward epilogue
-// Per row and half of the columns: running maximum (times log2 e) and sum of
+// Per row and quarter of the columns: running maximum (times log2 e) and sum of
 // 2^(z log2 e - max), both fp32, over the tiles of a strip.
 struct LseEpi {
-  static constexpr int BOXES = 0;
+  static constexpr int WARPS = 16, BOXES = 0, BOX_BYTES = 0;
   struct Params {
-    float *part_m, *part_s;  // [strips * 2][Mp]
+    float *part_m, *part_s;  // [strips * 4][Mp]
     float* zt;
     const int32_t* tgt;
     const int32_t* live;
@@ -158,10 +158,10 @@ struct LseEpi {
   __device__ __forceinline__ void tile(const Steps& q, uint32_t acc, Release release) {
     const int row = q.it.row0 + w.row();
 #pragma unroll 1
-    for (int c = w.half * (BN / 2); c < (w.half + 1) * (BN / 2); c += 32) {
+    for (int c = w.slice * (BN / 4); c < (w.slice + 1) * (BN / 4); c += 32) {
       float z[32];
       acc_load32(acc + c, false, z);
-      if (c + 32 == (w.half + 1) * (BN / 2)) release();
+      if (c + 32 == (w.slice + 1) * (BN / 4)) release();
       const int col = q.nt * BN + c, n = p.V - col;
       if (n < 32) {
 #pragma unroll
@@ -192,7 +192,7 @@ struct LseEpi {
       m = nm;
     }
     if (q.item_last() && row < live) {
-      const int64_t at = (int64_t)(q.it.nt0 / p.strip_tiles * 2 + w.half) * p.Mp + row;
+      const int64_t at = (int64_t)(q.it.nt0 / p.strip_tiles * 4 + w.slice) * p.Mp + row;
       p.part_m[at] = m;
       p.part_s[at] = s;
     }
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(1024) xent_scale_kernel(ScaleArgs p) {
 // dz of one piece, 16 bits, zeros in rows past the last one that counts and in columns
 // past the vocabulary (the two GEMMs run over whole 64-deep blocks of both).
 struct DzEpi {
-  static constexpr int BOXES = 2;
+  static constexpr int WARPS = 16, BOXES = 1, BOX_BYTES = 4096;
   struct Params {
     Out dz;
     const float *lse2, *rs;
@@ -340,10 +340,10 @@ struct DzEpi {
     const int row = q.it.row0 + w.row();
     uint32_t b = 0;
 #pragma unroll 1
-    for (int c = w.half * (BN / 2); c < (w.half + 1) * (BN / 2); c += 32) {
+    for (int c = w.slice * (BN / 4); c < (w.slice + 1) * (BN / 4); c += 32) {
       float z[32];
       acc_load32(acc + c, false, z);
-      if (c + 32 == (w.half + 1) * (BN / 2)) release();
+      if (c + 32 == (w.slice + 1) * (BN / 4)) release();
       const int col = q.nt * BN + c, n = row < live ? p.V - p.v0 - col : 0, tc = tgt - col;
 #pragma unroll
       for (int i = 0; i < 32; ++i) z[i] = ex2(fmaf(z[i], kLog2e, -lse)) * rs;
@@ -359,7 +359,7 @@ struct DzEpi {
       }
       const int h = (c >> 5) & 1;
       if (h == 0) b = boxes.take();
-      boxes.put16(b, h, z, p.bf16);
+      boxes.put16(b, 32 * h, z, p.bf16);
       if (h == 1 && q.it.row0 < p.dz.rows) boxes.store(b, &p.dz.map, col - 32, q.it.row0 + 32 * w.quad, 0);
     }
   }
@@ -453,8 +453,8 @@ FwdLayout fwd_layout(int64_t M, int64_t V) {
     return r;
   };
   l.zt = take(4 * Mp);
-  l.part_m = take(4 * Mp * 2 * l.strips);
-  l.part_s = take(4 * Mp * 2 * l.strips);
+  l.part_m = take(4 * Mp * 4 * l.strips);
+  l.part_s = take(4 * Mp * 4 * l.strips);
   l.sums = take(8 * std::max<int64_t>(64, (M + 31) / 32));
   l.total = at;
   return l;
@@ -570,7 +570,7 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
                     c.s.counts, Mp, (int)V, l.per};
   rc = launch<false, false, false, LseEpi>("stream_xent forward", a, ep, st);
   if (rc) return rc;
-  ReduceArgs r{ep.part_m, ep.part_s, c.zt, c.s, row_loss, loss, reinterpret_cast<double*>(ws + l.sums), Mp, 2 * l.strips, mean};
+  ReduceArgs r{ep.part_m, ep.part_s, c.zt, c.s, row_loss, loss, reinterpret_cast<double*>(ws + l.sums), Mp, 4 * l.strips, mean};
   if (M > 64)
     xent_reduce_kernel<32><<<(unsigned)((M + 31) / 32), 256, 0, st>>>(r);
   else
