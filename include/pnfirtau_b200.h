@@ -427,7 +427,8 @@ PNFT_API int pnft_cast_bf16(const int64_t* table, int count, int64_t max_n, void
 #define PNFT_ACT_GELU 1 /* the exact (erf) form */
 
 /* Gated feed-forward product h[M x F] = act(x Wg^T + bg) * (x Wu^T + bu), x [M x D],
- * Wg and Wu [F x D], one kernel. bg / bu [F] of type b_dtype (each may be NULL). h is
+ * Wg and Wu [F x D], one kernel (calls of up to 64 rows without pre have one of their
+ * own, which takes any row strides >= D). bg / bu [F] of type b_dtype (each may be NULL). h is
  * written in `dtype`. pre (may be NULL): the pre-activations x Wg^T + bg and x Wu^T + bu
  * kept for pnft_gated_bwd with 24 bits each, as three matrices [M x ldp] of 16-bit
  * words one after the other (ldp a multiple of 8, 16-byte aligned).
@@ -476,28 +477,30 @@ PNFT_API int pnft_copy_rows16(const void* src, int64_t lds, void* dst, int64_t l
  * other rows (0/0 when there is none). A target outside [0, V) that is not
  * ignore_index gives NaN and sets the status word to PNFT_DEV_BAD_INDEX. Rows to
  * ignore are left out of all work; what they hold reaches no result.
- * Kept for the backward: hc (rows of h that count, [ceil(M / 128) * 128 x ldc])
- * and saved (pnft_stream_xent_saved_size(M) bytes, 16-byte aligned). workspace:
- * pnft_stream_xent_fwd_workspace_size(M, V) bytes. M >= 1.
+ * saved (pnft_stream_xent_saved_size(M, D) bytes, 16-byte aligned): the rows that
+ * count and their state, kept for the backward; NULL when there will be none (calls of
+ * up to 64 rows then take a kernel of their own). h: any row stride >= D; W: 16-byte
+ * aligned rows, except in those small calls. workspace:
+ * pnft_stream_xent_fwd_workspace_size(M, V, D, saved != NULL) bytes, 16-byte aligned.
+ * M >= 1.
  * Beside: pnft_lm_xent, which wants the logits (experiments/exp4_wikitext2_lm.py:714-719). */
 PNFT_API int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* targets,
-                         int64_t ignore_index, void* hc, int64_t ldc, void* saved, float* row_loss,
-                         float* loss, int mean, void* workspace, size_t workspace_bytes, int64_t M, int64_t V,
-                         int64_t D, int dtype, int32_t* status, void* stream);
+                         int64_t ignore_index, void* saved, float* row_loss, float* loss, int mean,
+                         void* workspace, size_t workspace_bytes, int64_t M, int64_t V, int64_t D, int dtype,
+                         int32_t* status, void* stream);
 
-PNFT_API size_t pnft_stream_xent_saved_size(int64_t M);
-PNFT_API size_t pnft_stream_xent_fwd_workspace_size(int64_t M, int64_t V);
+PNFT_API size_t pnft_stream_xent_saved_size(int64_t M, int64_t D);
+PNFT_API size_t pnft_stream_xent_fwd_workspace_size(int64_t M, int64_t V, int64_t D, int save);
 
 /* Gradient of pnft_stream_xent_fwd: dh [M x D] and / or dw [V x D] (either may be
  * NULL). dloss: the loss's own gradient on the device, one value (`mean` as in the
  * forward) or, with per_row, one per row of h with stride dloss_stride. The
  * logits' gradient exists for one piece of the vocabulary at a time. workspace:
  * pnft_stream_xent_bwd_workspace_size(M, V, D) bytes, 16-byte aligned. */
-PNFT_API int pnft_stream_xent_bwd(const void* hc, int64_t ldc, const void* w, int64_t ldw, const void* saved,
-                         const float* dloss, int64_t dloss_stride, int per_row, int mean, void* dh,
-                         int64_t lddh, int dh_dtype, void* dw, int64_t lddw, int dw_dtype, void* workspace,
-                         size_t workspace_bytes, int64_t M, int64_t V, int64_t D, int dtype, int32_t* status,
-                         void* stream);
+PNFT_API int pnft_stream_xent_bwd(const void* w, int64_t ldw, const void* saved, const float* dloss,
+                         int64_t dloss_stride, int per_row, int mean, void* dh, int64_t lddh, int dh_dtype,
+                         void* dw, int64_t lddw, int dw_dtype, void* workspace, size_t workspace_bytes,
+                         int64_t M, int64_t V, int64_t D, int dtype, int32_t* status, void* stream);
 
 PNFT_API size_t pnft_stream_xent_bwd_workspace_size(int64_t M, int64_t V, int64_t D);
 
@@ -514,6 +517,17 @@ PNFT_API int pnft_act8_pack(const void* x, int64_t ldx, void* q, int64_t ldq, in
  * and float32 whatever was packed). */
 PNFT_API int pnft_act8_unpack(const void* q, int64_t ldq, const int8_t* e, int64_t lde, void* y, int64_t ldy, int64_t M,
                      int64_t D, int dtype, void* stream);
+
+/* Weight gradient from an input kept in 8 bits: dw [N x D] (dw_dtype) = dy^T (q * 2^e),
+ * dy [M x N] of type `dtype` (16-byte aligned rows, or any when N is no multiple of 8).
+ * float16 needs values packed from float16. workspace:
+ * pnft_act8_weight_grad_workspace_size(M, N, D) bytes, 16-byte aligned. */
+PNFT_API int pnft_act8_weight_grad(const void* dy, int64_t lddy, const void* q, int64_t ldq, const int8_t* e,
+                          int64_t lde, void* dw, int64_t lddw, int dw_dtype, void* workspace,
+                          size_t workspace_bytes, int64_t M, int64_t N, int64_t D, int dtype,
+                          int32_t* status, void* stream);
+
+PNFT_API size_t pnft_act8_weight_grad_workspace_size(int64_t M, int64_t N, int64_t D);
 
 #ifdef __cplusplus
 }

@@ -131,17 +131,21 @@ SIGNATURES: dict[str, tuple] = {
     "pnft_copy_rows16": (c_int, [_P, c_int64, _P, c_int64, c_int64, c_int64, _P]),
     "pnft_stream_xent_fwd": (
         c_int,
-        [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P, _P, c_int, _P, c_size_t, c_int64, c_int64, c_int64,
-         c_int, _P, _P],
+        [_P, c_int64, _P, c_int64, _P, c_int64, _P, _P, _P, c_int, _P, c_size_t, c_int64, c_int64, c_int64, c_int, _P, _P],
     ),
-    "pnft_stream_xent_saved_size": (c_size_t, [c_int64]),
-    "pnft_stream_xent_fwd_workspace_size": (c_size_t, [c_int64, c_int64]),
+    "pnft_stream_xent_saved_size": (c_size_t, [c_int64, c_int64]),
+    "pnft_stream_xent_fwd_workspace_size": (c_size_t, [c_int64, c_int64, c_int64, c_int]),
     "pnft_stream_xent_bwd": (
         c_int,
-        [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int, c_int, _P, c_int64, c_int, _P, c_int64, c_int, _P, c_size_t,
-         c_int64, c_int64, c_int64, c_int, _P, _P],
+        [_P, c_int64, _P, _P, c_int64, c_int, c_int, _P, c_int64, c_int, _P, c_int64, c_int, _P, c_size_t, c_int64, c_int64,
+         c_int64, c_int, _P, _P],
     ),
     "pnft_stream_xent_bwd_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
+    "pnft_act8_weight_grad": (
+        c_int,
+        [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, c_int, _P, c_size_t, c_int64, c_int64, c_int64, c_int, _P, _P],
+    ),
+    "pnft_act8_weight_grad_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
     "pnft_act8_pack": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64, c_int, _P]),
     "pnft_act8_unpack": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64, c_int, _P]),
 }

@@ -42,85 +42,113 @@ struct ActArgs {
   int8_t* e;
   int64_t lde;
   int64_t M;
-  int D, blocks, dtype, vec;
+  int D, dtype, vec;
 };
 
-// Eight columns per lane, 16 lanes per block of 128.
+// Eight columns from `col` of a row (zeros past its end).
+__device__ __forceinline__ void load8(const ActArgs& p, int64_t row, int col, float (&v)[8]) {
+  const int cnt = p.D - col;
+  if (p.dtype == PNFT_DTYPE_F32) {
+    const float* src = static_cast<const float*>(p.x) + row * p.ldx + col;
+    if (p.vec && cnt >= 8) {
+      const float4 a = __ldcs(reinterpret_cast<const float4*>(src)), c = __ldcs(reinterpret_cast<const float4*>(src) + 1);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = c.x, v[5] = c.y, v[6] = c.z, v[7] = c.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = k < cnt ? src[k] : 0.f;
+    }
+  } else {
+    tc::load_row16<8>(static_cast<const uint16_t*>(p.x) + row * p.ldx + col, v, cnt, p.vec, p.dtype == PNFT_DTYPE_BF16);
+  }
+}
+
+// A warp takes COLS columns of a row at a time: eight columns per lane, 16 lanes per block
+// of 128, AU loads in flight per lane (measured at 16384 x 1024 bf16: AU = 1 with a row
+// index by division 18.2 us, this 9.5).
+constexpr int AU = 4, COLS = 256 * AU;
+
 __global__ void __launch_bounds__(AT) act8_pack_kernel(ActArgs p) {
-  const int lane = threadIdx.x & 15;
-  const int64_t n = p.M * p.blocks;
+  const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
   int lo, hi;
   exponent_range(p.dtype, &lo, &hi);
-  for (int64_t i = ((int64_t)blockIdx.x * AT + threadIdx.x) / 16; i < (n + 1) / 2 * 2; i += (int64_t)gridDim.x * AT / 16) {
-    const int64_t row = i / p.blocks;
-    const int b = (int)(i - row * p.blocks), col = b * 128 + 8 * lane;
-    const int cnt = i < n ? p.D - col : 0;
-    float v[8];
-    if (p.dtype == PNFT_DTYPE_F32) {
-      const float* src = static_cast<const float*>(p.x) + row * p.ldx + col;
-      if (p.vec && cnt >= 8) {
-        const float4 a = reinterpret_cast<const float4*>(src)[0], c = reinterpret_cast<const float4*>(src)[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = c.x, v[5] = c.y, v[6] = c.z, v[7] = c.w;
-      } else {
+  for (int64_t row = (int64_t)blockIdx.x * (AT / 32) + (threadIdx.x >> 5); row < p.M; row += (int64_t)gridDim.x * (AT / 32)) {
+    const int c0 = blockIdx.y * COLS;
+    float v[AU][8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = k < cnt ? src[k] : 0.f;
+    for (int j = 0; j < AU; ++j) load8(p, row, c0 + 256 * j + 8 * lane, v[j]);
+#pragma unroll
+    for (int j = 0; j < AU; ++j) {
+      const int col = c0 + 256 * j + 8 * lane, cnt = p.D - col;
+      if (c0 + 256 * j >= p.D) break;  // the same for the whole warp
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (!(fabsf(v[j][k]) <= 3.402823466e38f)) v[j][k] = __int_as_float(0x7fc00000);
+        top = fmaxf(top, fabsf(v[j][k]));  // fmaxf leaves NaN out
       }
-    } else {
-      tc::load_row16<8>(static_cast<const uint16_t*>(p.x) + row * p.ldx + col, v, cnt, p.vec, p.dtype == PNFT_DTYPE_BF16);
-    }
-    float top = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (!(fabsf(v[k]) <= 3.402823466e38f)) v[k] = __int_as_float(0x7fc00000);
-      top = fmaxf(top, fabsf(v[k]));  // fmaxf leaves NaN out
-    }
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // top = f * 2^k, 1 <= f < 2 (subnormals fall below the range anyway): 448 = 1.75 * 2^8
+      const int bits = __float_as_int(top);
+      int e = (bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000);
+      e = max(lo, min(hi, top == 0.f ? lo : e));
+      const float scale = pow2(-e), end = e == hi ? 240.f : 448.f;
+      if (cnt <= 0) continue;
+      uint32_t w[2];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    // top = f * 2^k, 1 <= f < 2 (subnormals fall below the range anyway): 448 = 1.75 * 2^8
-    const int bits = __float_as_int(top);
-    int e = (bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000);
-    e = max(lo, min(hi, top == 0.f ? lo : e));
-    const float scale = pow2(-e), end = e == hi ? 240.f : 448.f;
-    if (cnt <= 0) continue;
-    uint32_t w[2];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float a = v[2 * k] * scale, c = v[2 * k + 1] * scale;
-      if (fabsf(a) > end) a = copysignf(end, a);  // leaves NaN alone
-      if (fabsf(c) > end) c = copysignf(end, c);
-      const uint32_t h = to_e4m3x2(a, c);
-      w[k / 2] = k & 1 ? w[k / 2] | (h << 16) : h;
+      for (int k = 0; k < 4; ++k) {
+        float a = v[j][2 * k] * scale, c = v[j][2 * k + 1] * scale;
+        if (fabsf(a) > end) a = copysignf(end, a);  // leaves NaN alone
+        if (fabsf(c) > end) c = copysignf(end, c);
+        const uint32_t h = to_e4m3x2(a, c);
+        w[k / 2] = k & 1 ? w[k / 2] | (h << 16) : h;
+      }
+      uint8_t* dst = p.q + row * p.ldq + col;
+      if (cnt >= 8) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+      } else {
+        for (int k = 0; k < cnt; ++k) dst[k] = (uint8_t)(w[k / 4] >> (8 * (k & 3)));
+      }
+      if (l == 0) p.e[row * p.lde + (c0 + 256 * j) / 128 + half] = (int8_t)e;
     }
-    uint8_t* dst = p.q + row * p.ldq + col;
-    if (cnt >= 8) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-    } else {
-      for (int k = 0; k < cnt; ++k) dst[k] = (uint8_t)(w[k / 4] >> (8 * (k & 3)));
-    }
-    if (lane == 0) p.e[row * p.lde + b] = (int8_t)e;
   }
 }
 
 __global__ void __launch_bounds__(AT) act8_unpack_kernel(ActArgs p, void* y, int64_t ldy) {
-  const int vecs = (p.D + 7) / 8;
-  const int64_t n = p.M * vecs;
-  for (int64_t i = (int64_t)blockIdx.x * AT + threadIdx.x; i < n; i += (int64_t)gridDim.x * AT) {
-    const int64_t row = i / vecs;
-    const int col = (int)(i - row * vecs) * 8, cnt = p.D - col;
-    const uint2 w = *reinterpret_cast<const uint2*>(p.q + row * p.ldq + col);
-    const float scale = pow2(p.e[row * p.lde + col / 128]);
-    const uint32_t u[4] = {w.x, w.x >> 16, w.y, w.y >> 16};
-    float v[8];
+  const int lane = threadIdx.x & 31;
+  for (int64_t row = (int64_t)blockIdx.x * (AT / 32) + (threadIdx.x >> 5); row < p.M; row += (int64_t)gridDim.x * (AT / 32)) {
+    const int c0 = blockIdx.y * COLS + 8 * lane;
+    uint2 w[AU];
+    int e[AU];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 f = from_e4m3x2(u[k] & 0xffffu);
-      v[2 * k] = f.x * scale, v[2 * k + 1] = f.y * scale;
+    for (int j = 0; j < AU; ++j) {
+      const int col = c0 + 256 * j;
+      if (col >= p.D) break;
+      w[j] = __ldcs(reinterpret_cast<const uint2*>(p.q + row * p.ldq + col));
+      e[j] = p.e[row * p.lde + col / 128];
     }
-    if (p.dtype == PNFT_DTYPE_F32)
-      tc::store_row32<8>(static_cast<float*>(y) + row * ldy + col, v, cnt, p.vec);
-    else
-      tc::store_row16<8>(static_cast<uint16_t*>(y) + row * ldy + col, v, cnt, p.vec, p.dtype == PNFT_DTYPE_BF16);
+#pragma unroll
+    for (int j = 0; j < AU; ++j) {
+      const int col = c0 + 256 * j, cnt = p.D - col;
+      if (cnt <= 0) break;
+      const float scale = pow2(e[j]);
+      const uint32_t u[4] = {w[j].x, w[j].x >> 16, w[j].y, w[j].y >> 16};
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = from_e4m3x2(u[k] & 0xffffu);
+        v[2 * k] = f.x * scale, v[2 * k + 1] = f.y * scale;
+      }
+      if (p.dtype == PNFT_DTYPE_F32)
+        tc::store_row32<8>(static_cast<float*>(y) + row * ldy + col, v, cnt, p.vec);
+      else
+        tc::store_row16<8>(static_cast<uint16_t*>(y) + row * ldy + col, v, cnt, p.vec, p.dtype == PNFT_DTYPE_BF16);
+    }
   }
+}
+
+dim3 act8_grid(int64_t M, int64_t D) {
+  return dim3((unsigned)std::min<int64_t>((M + AT / 32 - 1) / (AT / 32), (int64_t)tc::sm_count() * 16), (unsigned)((D + COLS - 1) / COLS));
 }
 
 int act8_check(const char* what, const void* x, int64_t ldx, const void* q, int64_t ldq, const void* e, int64_t lde,
@@ -144,10 +172,9 @@ extern "C" int pnft_act8_pack(const void* x, int64_t ldx, void* q, int64_t ldq, 
                               int64_t D, int dtype, void* stream) {
   if (int rc = act8_check("act8_pack", x, ldx, q, ldq, e, lde, M, D, dtype)) return rc;
   if (M == 0) return PNFT_OK;
-  ActArgs a{x, ldx, static_cast<uint8_t*>(q), ldq, e, lde, M, (int)D, (int)((D + 127) / 128), dtype,
+  ActArgs a{x, ldx, static_cast<uint8_t*>(q), ldq, e, lde, M, (int)D, dtype,
             tc::rows16(x, ldx, dtype == PNFT_DTYPE_F32 ? 4 : 2)};
-  const int64_t blocks = (M * a.blocks * 16 + AT - 1) / AT;
-  act8_pack_kernel<<<(unsigned)std::min<int64_t>(blocks, (int64_t)tc::sm_count() * 32), AT, 0, as_stream(stream)>>>(a);
+  act8_pack_kernel<<<act8_grid(M, D), AT, 0, as_stream(stream)>>>(a);
   return check_launch("act8_pack", 1);
 }
 
@@ -156,8 +183,61 @@ extern "C" int pnft_act8_unpack(const void* q, int64_t ldq, const int8_t* e, int
   if (int rc = act8_check("act8_unpack", y, ldy, q, ldq, e, lde, M, D, dtype)) return rc;
   if (M == 0) return PNFT_OK;
   ActArgs a{nullptr, 0, static_cast<uint8_t*>(const_cast<void*>(q)), ldq, const_cast<int8_t*>(e), lde, M, (int)D,
-            (int)((D + 127) / 128), dtype, tc::rows16(y, ldy, dtype == PNFT_DTYPE_F32 ? 4 : 2)};
-  const int64_t blocks = (M * ((D + 7) / 8) + AT - 1) / AT;
-  act8_unpack_kernel<<<(unsigned)std::min<int64_t>(blocks, (int64_t)tc::sm_count() * 32), AT, 0, as_stream(stream)>>>(a, y, ldy);
+            dtype, tc::rows16(y, ldy, dtype == PNFT_DTYPE_F32 ? 4 : 2)};
+  act8_unpack_kernel<<<act8_grid(M, D), AT, 0, as_stream(stream)>>>(a, y, ldy);
   return check_launch("act8_unpack", 1);
+}
+
+// Buffers of a weight gradient from 8 bits: the values as 16-bit rows, dy with aligned rows
+// where the caller's are not, and the product's partial sums.
+namespace {
+struct GradLayout {
+  int64_t ldx, ldy;
+  size_t x, y, part, total;
+};
+GradLayout grad_layout(int64_t M, int64_t N, int64_t D) {
+  GradLayout l;
+  l.ldx = (D + 7) / 8 * 8, l.ldy = (N + 7) / 8 * 8;
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t r = at;
+    at += (n + 255) / 256 * 256;
+    return r;
+  };
+  l.x = take(2 * (size_t)M * l.ldx);
+  l.y = take(N % 8 ? 2 * (size_t)M * l.ldy : 0);
+  l.part = take(pnft_weight_grad_workspace_size(M, N, D));
+  l.total = at;
+  return l;
+}
+}  // namespace
+
+extern "C" size_t pnft_act8_weight_grad_workspace_size(int64_t M, int64_t N, int64_t D) {
+  return M <= 0 || N <= 0 || D <= 0 ? 0 : grad_layout(M, N, D).total;
+}
+
+extern "C" int pnft_act8_weight_grad(const void* dy, int64_t lddy, const void* q, int64_t ldq, const int8_t* e, int64_t lde,
+                                     void* dw, int64_t lddw, int dw_dtype, void* workspace, size_t workspace_bytes, int64_t M,
+                                     int64_t N, int64_t D, int dtype, int32_t* status, void* stream) {
+  if (!tc::type16(dtype)) return fail(PNFT_EUNSUPPORTED, "act8_weight_grad: bfloat16 or float16 gradient expected");
+  if (M < 0 || N <= 0 || D <= 0 || lddy < N || lddw < D || !dw)
+    return fail(PNFT_EINVAL, "act8_weight_grad: bad shape M=%lld N=%lld D=%lld", (long long)M, (long long)N, (long long)D);
+  if (M == 0)
+    return pnft_weight_grad(nullptr, 0, nullptr, 0, dw, nullptr, lddw, N, N, dw_dtype, nullptr, 0, 0, N, D, dtype, status, stream);
+  if (!dy) return fail(PNFT_EINVAL, "act8_weight_grad: null pointer");
+  const GradLayout l = grad_layout(M, N, D);
+  if (!workspace || workspace_bytes < l.total || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(PNFT_EINVAL, "act8_weight_grad: workspace of %zu bytes < required %zu (16-byte aligned)", workspace_bytes, l.total);
+  if (N % 8 == 0 && !tc::rows16(dy, lddy, 2))
+    return fail(PNFT_EUNSUPPORTED, "act8_weight_grad: dy rows must be 16-byte aligned (or N not a multiple of 8)");
+  char* ws = static_cast<char*>(workspace);
+  int rc = pnft_act8_unpack(q, ldq, e, lde, ws + l.x, l.ldx, M, D, dtype, stream);
+  if (rc) return rc;
+  if (!tc::rows16(dy, lddy, 2)) {
+    rc = pnft_copy_rows16(dy, lddy, ws + l.y, l.ldy, M, N, stream);
+    if (rc) return rc;
+    dy = ws + l.y, lddy = l.ldy;
+  }
+  return pnft_weight_grad(dy, lddy, ws + l.x, l.ldx, dw, nullptr, lddw, N, N, dw_dtype, ws + l.part,
+                          pnft_weight_grad_workspace_size(M, N, D), M, N, D, dtype, status, stream);
 }

@@ -14,6 +14,7 @@
 // upper 16 bits of fp32 in two planes, the next 8 of both in a third: kept in 16 bits,
 // their rounding would add as much error to the gradients as the operands' own).
 #include "gemm_tc.cuh"
+#include "skinny.cuh"
 
 namespace pnft {
 namespace {
@@ -207,6 +208,48 @@ struct GatedEpi {
   }
 };
 
+// ------------------------------------------------------------------ a few rows
+// Forward for at most 64 rows: a block has 16 columns of h, four warps the products of
+// x with those rows of Wg and four with Wu's, each a quarter of K.
+struct SkinnyArgs {
+  const uint16_t *x, *wg, *wu;
+  int64_t ldx, ldwg, ldwu;
+  const void *bg, *bu;
+  int b_dtype, act;
+  uint16_t* h;
+  int64_t ldh;
+  int M, D, F;
+};
+template <int NT, bool VEC, bool BF16>
+__global__ void __launch_bounds__(32 * skinny::WARPS) gated_skinny_kernel(SkinnyArgs p) {
+  constexpr int N = 8 * NT;
+  __shared__ float red[skinny::WARPS][16][N + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int f0 = blockIdx.x * 16, side = warp >> 2;
+  const uint16_t* w = side ? p.wu : p.wg;
+  const int64_t ld = side ? p.ldwu : p.ldwg;
+  float acc[NT][4] = {};
+  // rows past F read the last one; their columns are not written
+  skinny::dot<NT, VEC, BF16>(w + min(f0 + g, p.F - 1) * ld, w + min(f0 + g + 8, p.F - 1) * ld, p.x, p.ldx, p.M, p.D, warp & 3,
+                             4, acc);
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    red[warp][g][8 * j + 2 * t] = acc[j][0], red[warp][g][8 * j + 2 * t + 1] = acc[j][1];
+    red[warp][g + 8][8 * j + 2 * t] = acc[j][2], red[warp][g + 8][8 * j + 2 * t + 1] = acc[j][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * p.M; i += 32 * skinny::WARPS) {
+    const int f = i & 15, n = i >> 4, col = f0 + f;
+    if (col >= p.F) continue;
+    float gv = (red[0][f][n] + red[1][f][n]) + (red[2][f][n] + red[3][f][n]);
+    float uv = (red[4][f][n] + red[5][f][n]) + (red[6][f][n] + red[7][f][n]);
+    if (p.bg) gv += load_any(p.bg, col, p.b_dtype);
+    if (p.bu) uv += load_any(p.bu, col, p.b_dtype);
+    const float a = p.act == PNFT_ACT_SILU ? act_value<false, PNFT_ACT_SILU>(gv, nullptr) : act_value<false, PNFT_ACT_GELU>(gv, nullptr);
+    store16(p.h + n * p.ldh + col, a * uv, BF16);
+  }
+}
+
 // ------------------------------------------------------------------ pointwise backward
 // dg, du from dh and the kept g, u (their three planes), with the column sums of dg and du
 // as stored for the biases' gradients; without dh only the sums of given dg, du. A block
@@ -382,6 +425,18 @@ extern "C" int pnft_gated_fwd(const void* x, int64_t ldx, const void* wg, int64_
   if (!h) return fail(PNFT_EINVAL, "gated_fwd: null output");
   if (ldh < F || (pre && ldp < F)) return fail(PNFT_EINVAL, "gated_fwd: row strides below the width");
   if (pre && !rows16(pre, ldp, 2)) return fail(PNFT_EINVAL, "gated_fwd: the kept rows must be 16-byte aligned");
+  if (b_dtype < PNFT_DTYPE_F32 || b_dtype > PNFT_DTYPE_F16) return fail(PNFT_EINVAL, "gated_fwd: unknown bias type %d", b_dtype);
+  if (ldx < D || ldwg < D || ldwu < D) return fail(PNFT_EUNSUPPORTED, "gated_fwd: x and weight rows must not overlap (aligned strides of at least D)");
+  if (M <= skinny::MAX_ROWS && !pre && x && wg && wu) {
+    const SkinnyArgs a{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(wg), static_cast<const uint16_t*>(wu),
+                       ldx, ldwg, ldwu, bg, bu, b_dtype, act, static_cast<uint16_t*>(h), ldh, (int)M, (int)D, (int)F};
+    const bool vec = D % 8 == 0 && rows16(x, ldx, 2) && rows16(wg, ldwg, 2) && rows16(wu, ldwu, 2);
+    return skinny::dispatch(M, vec, dtype == PNFT_DTYPE_BF16, [&](auto nt, auto v, auto b) {
+      gated_skinny_kernel<decltype(nt)::value, decltype(v)::value, decltype(b)::value>
+          <<<(unsigned)((F + 15) / 16), 32 * skinny::WARPS, 0, as_stream(stream)>>>(a);
+      return check_launch("gated_fwd", 1);
+    });
+  }
   if (int rc = gated_operands("gated_fwd", x, ldx, wg, ldwg, wu, ldwu, D)) return rc;
   Out o, k;
   int rc = make_out(&o, h, dtype, F, M, ldh, 1, 0, 64);

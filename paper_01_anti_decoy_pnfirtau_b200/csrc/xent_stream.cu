@@ -15,6 +15,7 @@
 // kernel sizes its work by that number. So nothing in a masked row, NaN and infinities
 // included, reaches a result.
 #include "gemm_tc.cuh"
+#include "skinny.cuh"
 
 namespace pnft {
 namespace {
@@ -280,6 +281,107 @@ __global__ void __launch_bounds__(256) xent_reduce_kernel(ReduceArgs p) {
   if (threadIdx.x == 0) *p.loss = (float)(p.mean ? red[0] / (double)n : red[0]);
 }
 
+// ------------------------------------------------------------------ a few rows
+// Loss of at most 64 rows without a gradient: every warp takes 16 words of the vocabulary
+// at a time and keeps each row's maximum and sum over them; a block joins its warps' and
+// leaves one pair per row. Rows to ignore are computed with the others (a column of the
+// product touches no other) and left out at the end.
+struct SkinnyArgs {
+  const uint16_t *h, *w;
+  int64_t ldh, ldw;
+  const int64_t* t;
+  int64_t ignore;
+  float *part_m, *part_s, *zt;  // [blocks][64], [64]
+  float *row_loss, *loss;
+  int M, D, V, blocks, mean;
+  int32_t* status;
+};
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  s = s * ex2(m - top) + s2 * ex2(m2 - top);
+  m = top;
+}
+template <int NT, bool VEC, bool BF16>
+__global__ void __launch_bounds__(32 * skinny::WARPS) xent_skinny_kernel(SkinnyArgs p) {
+  __shared__ float sm[skinny::WARPS][8 * NT], ss[skinny::WARPS][8 * NT];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float m[NT][2], s[NT][2];
+  int tgt[NT][2];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int n = 8 * j + 2 * t + k;
+      m[j][k] = kLow, s[j][k] = 0.f;
+      const int64_t v = n < p.M ? p.t[n] : -1;
+      tgt[j][k] = v >= 0 && v < p.V ? (int)v : -1;
+    }
+  for (int64_t v0 = (blockIdx.x * skinny::WARPS + warp) * 16; v0 < p.V; v0 += gridDim.x * skinny::WARPS * 16) {
+    float acc[NT][4] = {};
+    const int r0 = (int)v0 + g, r1 = r0 + 8;
+    skinny::dot<NT, VEC, BF16>(p.w + (int64_t)min(r0, p.V - 1) * p.ldw, p.w + (int64_t)min(r1, p.V - 1) * p.ldw, p.h, p.ldh, p.M,
+                               p.D, 0, 1, acc);
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (r0 == tgt[j][k]) p.zt[8 * j + 2 * t + k] = acc[j][k];
+        if (r1 == tgt[j][k]) p.zt[8 * j + 2 * t + k] = acc[j][k + 2];
+        const float a = r0 < p.V ? acc[j][k] : -INFINITY, b = r1 < p.V ? acc[j][k + 2] : -INFINITY;
+        const float top = max3(m[j][k], a * kLog2e, b * kLog2e);
+        s[j][k] = s[j][k] * ex2(m[j][k] - top) + ex2(fmaf(a, kLog2e, -top)) + ex2(fmaf(b, kLog2e, -top));
+        m[j][k] = top;
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1)
+        join(m[j][k], s[j][k], __shfl_xor_sync(0xffffffffu, m[j][k], o), __shfl_xor_sync(0xffffffffu, s[j][k], o));
+      if (g == 0) sm[warp][8 * j + 2 * t + k] = m[j][k], ss[warp][8 * j + 2 * t + k] = s[j][k];
+    }
+  __syncthreads();
+  const int n = threadIdx.x;
+  if (n >= p.M) return;
+  float a = sm[0][n], b = ss[0][n];
+  for (int k = 1; k < skinny::WARPS; ++k) join(a, b, sm[k][n], ss[k][n]);
+  p.part_m[blockIdx.x * skinny::MAX_ROWS + n] = a;
+  p.part_s[blockIdx.x * skinny::MAX_ROWS + n] = b;
+}
+
+// Joins the blocks' pairs, a warp per row, and sums the rows.
+__global__ void __launch_bounds__(1024) xent_skinny_reduce_kernel(SkinnyArgs p) {
+  __shared__ float losses[skinny::MAX_ROWS];
+  __shared__ int counted[skinny::MAX_ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int n = warp; n < p.M; n += 32) {
+    float m = kLow, s = 0.f;
+    for (int b = lane; b < p.blocks; b += 32) join(m, s, p.part_m[b * skinny::MAX_ROWS + n], p.part_s[b * skinny::MAX_ROWS + n]);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) join(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+    if (lane == 0) {
+      const int64_t t = p.t[n];
+      float loss = 0.f;
+      if (t != p.ignore) {
+        const bool good = t >= 0 && t < p.V;
+        loss = good ? kLn2 * (fmaf(-p.zt[n], kLog2e, m) + log2f(s)) : __int_as_float(0x7fc00000);
+        if (!good) report_status(p.status, PNFT_DEV_BAD_INDEX);
+      }
+      losses[n] = loss, counted[n] = t != p.ignore;
+      if (p.row_loss) p.row_loss[n] = loss;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && p.loss) {
+    double sum = 0.0;
+    int c = 0;
+    for (int n = 0; n < p.M; ++n) sum += losses[n], c += counted[n];
+    *p.loss = (float)(p.mean ? sum / (double)c : sum);
+  }
+}
+
 // ------------------------------------------------------------------ backward
 // The rows' factors: row i's gradient is multiplied by alpha * rs[i]. rs reaches from
 // -top to top with top 1 for bf16; 2^14 for fp16, so that the small probabilities of a
@@ -408,10 +510,13 @@ int strip_tiles(int64_t tiles_m, int tiles_n) {
   return best;
 }
 
+// What the backward needs: the rows that count (16-byte aligned, whole row tiles) and
+// their state.
 struct SavedLayout {
-  size_t counts, pos, idx, tgt, lse2, total;
+  int64_t ldc;
+  size_t hc, counts, pos, idx, tgt, lse2, total;
 };
-SavedLayout saved_layout(int64_t M) {
+SavedLayout saved_layout(int64_t M, int64_t D) {
   const int64_t Mp = up(std::max<int64_t>(M, 1), BM);
   SavedLayout l;
   size_t at = 0;
@@ -420,6 +525,8 @@ SavedLayout saved_layout(int64_t M) {
     at += (n + 255) / 256 * 256;
     return r;
   };
+  l.ldc = up(D, 8);
+  l.hc = take(2 * (size_t)Mp * l.ldc);
   l.counts = take(8);
   l.pos = take(4 * Mp);
   l.idx = take(4 * Mp);
@@ -428,8 +535,7 @@ SavedLayout saved_layout(int64_t M) {
   l.total = at;
   return l;
 }
-State state_of(void* saved, int64_t M) {
-  const SavedLayout l = saved_layout(M);
+State state_of(const SavedLayout& l, void* saved) {
   char* b = static_cast<char*>(saved);
   return State{reinterpret_cast<int32_t*>(b + l.counts), reinterpret_cast<int32_t*>(b + l.pos),
                reinterpret_cast<int32_t*>(b + l.idx), reinterpret_cast<int32_t*>(b + l.tgt),
@@ -507,10 +613,19 @@ int xent_check(const char* what, int64_t M, int64_t D, int64_t V, int dtype) {
 using namespace pnft;
 using namespace pnft::tc;
 
-extern "C" size_t pnft_stream_xent_saved_size(int64_t M) { return M < 0 ? 0 : saved_layout(M).total; }
+extern "C" size_t pnft_stream_xent_saved_size(int64_t M, int64_t D) {
+  return M <= 0 || D <= 0 ? 0 : saved_layout(M, D).total;
+}
 
-extern "C" size_t pnft_stream_xent_fwd_workspace_size(int64_t M, int64_t V) {
-  return M <= 0 || V <= 0 ? 0 : fwd_layout(M, V).total;
+// Blocks of the kernel for a few rows: 16 words per warp, at most four blocks per SM.
+static int skinny_blocks(int64_t V) {
+  return (int)std::min<int64_t>((V + 16 * skinny::WARPS - 1) / (16 * skinny::WARPS), 4 * (int64_t)sm_count());
+}
+
+extern "C" size_t pnft_stream_xent_fwd_workspace_size(int64_t M, int64_t V, int64_t D, int save) {
+  if (M <= 0 || V <= 0 || D <= 0) return 0;
+  if (!save && M <= skinny::MAX_ROWS) return sizeof(float) * skinny::MAX_ROWS * (2 * (size_t)skinny_blocks(V) + 1);
+  return fwd_layout(M, V).total + (save ? 0 : saved_layout(M, D).total);
 }
 
 extern "C" size_t pnft_stream_xent_bwd_workspace_size(int64_t M, int64_t V, int64_t D) {
@@ -518,31 +633,48 @@ extern "C" size_t pnft_stream_xent_bwd_workspace_size(int64_t M, int64_t V, int6
 }
 
 extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* targets,
-                                    int64_t ignore_index, void* hc, int64_t ldc, void* saved, float* row_loss,
-                                    float* loss, int mean, void* workspace, size_t workspace_bytes, int64_t M, int64_t V,
-                                    int64_t D, int dtype, int32_t* status, void* stream) {
+                                    int64_t ignore_index, void* saved, float* row_loss, float* loss, int mean,
+                                    void* workspace, size_t workspace_bytes, int64_t M, int64_t V, int64_t D, int dtype,
+                                    int32_t* status, void* stream) {
   if (int rc = xent_check("stream_xent_fwd", M, D, V, dtype)) return rc;
-  if (!saved || (!row_loss && !loss)) return fail(PNFT_EINVAL, "stream_xent_fwd: null output");
+  if (!row_loss && !loss) return fail(PNFT_EINVAL, "stream_xent_fwd: null output");
   if (M == 0) return fail(PNFT_EINVAL, "stream_xent_fwd: no rows");
-  if (!h || !w || !targets || !hc) return fail(PNFT_EINVAL, "stream_xent_fwd: null pointer");
-  if (ldh < D) return fail(PNFT_EINVAL, "stream_xent_fwd: row stride below the width");
-  if (!tma_rows_ok(hc, ldc, D) || !tma_rows_ok(w, ldw, D))
-    return fail(PNFT_EUNSUPPORTED, "stream_xent_fwd: weight and buffer rows must be 16-byte aligned (strides multiples of 8)");
+  if (!h || !w || !targets) return fail(PNFT_EINVAL, "stream_xent_fwd: null pointer");
+  if (ldh < D || ldw < D) return fail(PNFT_EINVAL, "stream_xent_fwd: row stride below the width");
   if (reinterpret_cast<uintptr_t>(saved) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(PNFT_EINVAL, "stream_xent_fwd: buffers must be 16-byte aligned");
-  const FwdLayout l = fwd_layout(M, V);
-  if (!workspace || workspace_bytes < l.total)
-    return fail(PNFT_EINVAL, "stream_xent_fwd: workspace of %zu bytes < required %zu", workspace_bytes, l.total);
-  if (!device_is_sm100()) return fail(PNFT_EUNSUPPORTED, "stream_xent_fwd: needs an sm_100 device");
-  const int64_t Mp = up(M, BM);
+  const size_t need = pnft_stream_xent_fwd_workspace_size(M, V, D, saved != nullptr);
+  if (!workspace || workspace_bytes < need)
+    return fail(PNFT_EINVAL, "stream_xent_fwd: workspace of %zu bytes < required %zu", workspace_bytes, need);
   char* ws = static_cast<char*>(workspace);
   cudaStream_t st = as_stream(stream);
+  if (!saved && M <= skinny::MAX_ROWS) {
+    const int blocks = skinny_blocks(V);
+    float* part = static_cast<float*>(workspace);
+    const SkinnyArgs a{static_cast<const uint16_t*>(h), static_cast<const uint16_t*>(w), ldh, ldw, targets, ignore_index, part,
+                       part + (size_t)blocks * skinny::MAX_ROWS, part + 2 * (size_t)blocks * skinny::MAX_ROWS, row_loss, loss,
+                       (int)M, (int)D, (int)V, blocks, mean, status};
+    const bool vec = D % 8 == 0 && rows16(h, ldh, 2) && rows16(w, ldw, 2);
+    return skinny::dispatch(M, vec, dtype == PNFT_DTYPE_BF16, [&](auto nt, auto v, auto b) {
+      xent_skinny_kernel<decltype(nt)::value, decltype(v)::value, decltype(b)::value><<<blocks, 32 * skinny::WARPS, 0, st>>>(a);
+      xent_skinny_reduce_kernel<<<1, 1024, 0, st>>>(a);
+      return check_launch("stream_xent_fwd", 2);
+    });
+  }
+  if (!tma_rows_ok(w, ldw, D))
+    return fail(PNFT_EUNSUPPORTED, "stream_xent_fwd: weight rows must be 16-byte aligned (strides multiples of 8)");
+  if (!device_is_sm100()) return fail(PNFT_EUNSUPPORTED, "stream_xent_fwd: needs an sm_100 device");
+  const FwdLayout l = fwd_layout(M, V);
+  const SavedLayout sl = saved_layout(M, D);
+  if (!saved) saved = ws + l.total;
+  const int64_t Mp = up(M, BM), ldc = sl.ldc;
+  char* hc = static_cast<char*>(saved) + sl.hc;
   CompactArgs c;
   memset(&c, 0, sizeof(c));
   c.t = targets, c.ignore = ignore_index;
   c.h = static_cast<const uint16_t*>(h), c.ldh = ldh;
-  c.hc = static_cast<uint16_t*>(hc), c.ldc = ldc;
-  c.s = state_of(saved, M);
+  c.hc = reinterpret_cast<uint16_t*>(hc), c.ldc = ldc;
+  c.s = state_of(sl, saved);
   c.zt = reinterpret_cast<float*>(ws + l.zt);
   c.row_loss = row_loss;
   c.M = M, c.V = (int)V, c.D = (int)D, c.Mp = Mp;
@@ -578,16 +710,15 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
   return check_launch("stream_xent reduction", 1);
 }
 
-extern "C" int pnft_stream_xent_bwd(const void* hc, int64_t ldc, const void* w, int64_t ldw, const void* saved,
-                                    const float* dloss, int64_t dloss_stride, int per_row, int mean, void* dh,
-                                    int64_t lddh, int dh_dtype, void* dw, int64_t lddw, int dw_dtype, void* workspace,
+extern "C" int pnft_stream_xent_bwd(const void* w, int64_t ldw, const void* saved, const float* dloss, int64_t dloss_stride,
+                                    int per_row, int mean, void* dh, int64_t lddh, int dh_dtype, void* dw, int64_t lddw, int dw_dtype, void* workspace,
                                     size_t workspace_bytes, int64_t M, int64_t V, int64_t D, int dtype, int32_t* status,
                                     void* stream) {
   if (int rc = xent_check("stream_xent_bwd", M, D, V, dtype)) return rc;
   if (M == 0) return fail(PNFT_EINVAL, "stream_xent_bwd: no rows");
-  if (!hc || !w || !saved || !dloss || (!dh && !dw)) return fail(PNFT_EINVAL, "stream_xent_bwd: null pointer");
-  if (!tma_rows_ok(hc, ldc, D) || !tma_rows_ok(w, ldw, D))
-    return fail(PNFT_EUNSUPPORTED, "stream_xent_bwd: weight and buffer rows must be 16-byte aligned (strides multiples of 8)");
+  if (!w || !saved || !dloss || (!dh && !dw)) return fail(PNFT_EINVAL, "stream_xent_bwd: null pointer");
+  if (!tma_rows_ok(w, ldw, D) || reinterpret_cast<uintptr_t>(saved) % 16)
+    return fail(PNFT_EUNSUPPORTED, "stream_xent_bwd: weight rows must be 16-byte aligned (strides multiples of 8)");
   if ((dh && lddh < D) || (dw && lddw < D)) return fail(PNFT_EINVAL, "stream_xent_bwd: row stride below the width");
   for (int t : {dh_dtype, dw_dtype})
     if (t < PNFT_DTYPE_F32 || t > PNFT_DTYPE_F16) return fail(PNFT_EINVAL, "stream_xent_bwd: unknown output type %d", t);
@@ -598,7 +729,10 @@ extern "C" int pnft_stream_xent_bwd(const void* hc, int64_t ldc, const void* w, 
   const int64_t Mp = up(M, BM), D4 = up(D, 4);
   char* ws = static_cast<char*>(workspace);
   cudaStream_t st = as_stream(stream);
-  const State s = state_of(const_cast<void*>(saved), M);
+  const SavedLayout sl = saved_layout(M, D);
+  const State s = state_of(sl, const_cast<void*>(saved));
+  const int64_t ldc = sl.ldc;
+  const char* hc = static_cast<const char*>(saved) + sl.hc;
   float* rs = reinterpret_cast<float*>(ws + l.rs);
   float* alpha = reinterpret_cast<float*>(ws + l.alpha);
   uint16_t* dz = reinterpret_cast<uint16_t*>(ws + l.dz);

@@ -272,13 +272,14 @@ def test_streamed_cross_entropy(cuda, shape, dt, reduction, ignored):
     with torch.no_grad():
         alone = streamed_cross_entropy(h, w, t, reduction=reduction)
     got = streamed_cross_entropy(h, w, t, reduction=reduction)
-    assert got.dtype == FP32 and torch.equal(alone, got.detach())
+    assert got.dtype == FP32
     gh, gw = torch.autograd.grad(got, (h, w), dloss)
     check_device_status(cuda)
     if reduction != "none":
         k = n if reduction == "mean" else 1
         loss, el = loss.sum() / k, el.sum() / k + 2.0 ** -23 * loss.sum() / k
     check("loss", got.detach(), (loss, el))
+    check("loss without gradient", alone, (loss, el))  # up to 64 rows: a kernel of its own
     check("dh", gh, dh)
     check("dw", gw, dw)
     assert torch.all(gh[t == -100] == 0)

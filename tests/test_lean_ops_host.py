@@ -30,9 +30,10 @@ def test_gated_fwd_refuses():
     refused(gated(pre=A, ldp=100), _lib.EINVAL, "stride")
     refused(gated(pre=A + 8), _lib.EINVAL, "aligned")
     refused(gated(ldh=127), _lib.EINVAL, "stride")
-    refused(gated(ldx=65), _lib.EUNSUPPORTED, "aligned")
-    refused(gated(x=A + 2), _lib.EUNSUPPORTED, "aligned")
+    refused(gated(M=65, ldx=65), _lib.EUNSUPPORTED, "aligned")
+    refused(gated(M=65, x=A + 2), _lib.EUNSUPPORTED, "aligned")
     refused(gated(ldx=56), _lib.EUNSUPPORTED, "aligned")
+    refused(gated(b_dtype=5), _lib.EINVAL, "bias type")
     assert gated(M=0, x=None) == _lib.OK
 
 
@@ -78,24 +79,31 @@ def test_weight_grad_refuses():
 
 def test_stream_xent_refuses():
     L = _lib.lib()
-    n = L.pnft_stream_xent_fwd_workspace_size(10, 1000)
-    fwd = lambda M=10, V=1000, dtype=BF16, ws=A, nb=n, ldc=64, saved=A, loss=A: L.pnft_stream_xent_fwd(  # noqa: E731
-        A, 64, A, 64, A, -100, A, ldc, saved, None, loss, 1, ws, nb, M, V, 64, dtype, None, None)
+    n = L.pnft_stream_xent_fwd_workspace_size(100, 1000, 64, 1)
+    assert L.pnft_stream_xent_fwd_workspace_size(100, 1000, 64, 0) > n  # the state goes there when it is not kept
+
+    def fwd(M=100, V=1000, dtype=BF16, ws=A, nb=n, ldh=64, ldw=64, saved=A, loss=A, h=A):
+        return L.pnft_stream_xent_fwd(h, ldh, A, ldw, A, -100, saved, None, loss, 1, ws, nb, M, V, 64, dtype, None, None)
+
     refused(fwd(M=0), _lib.EINVAL, "rows")
     refused(fwd(V=0), _lib.EINVAL, "shape")
     refused(fwd(dtype=FP32), _lib.EUNSUPPORTED, "float16")
     refused(fwd(loss=None), _lib.EINVAL, "null")
-    refused(fwd(saved=None), _lib.EINVAL, "null")
-    refused(fwd(ldc=60), _lib.EUNSUPPORTED, "aligned")
+    refused(fwd(h=None), _lib.EINVAL, "null")
+    refused(fwd(ldh=63), _lib.EINVAL, "stride")
+    refused(fwd(saved=A + 8), _lib.EINVAL, "aligned")
     refused(fwd(ws=None), _lib.EINVAL, "workspace")
     refused(fwd(nb=n - 1), _lib.EINVAL, "workspace")
+    refused(fwd(saved=None), _lib.EINVAL, "workspace")
+    refused(fwd(ldw=65), _lib.EUNSUPPORTED, "aligned")
     m = L.pnft_stream_xent_bwd_workspace_size(10, 1000, 64)
-    bwd = lambda dh=A, dw=A, nb=m, lddh=64, t=BF16: L.pnft_stream_xent_bwd(  # noqa: E731
-        A, 64, A, 64, A, A, 1, 0, 1, dh, lddh, t, dw, 64, t, A, nb, 10, 1000, 64, BF16, None, None)
+    bwd = lambda dh=A, dw=A, nb=m, lddh=64, t=BF16, ldw=64: L.pnft_stream_xent_bwd(  # noqa: E731
+        A, ldw, A, A, 1, 0, 1, dh, lddh, t, dw, 64, t, A, nb, 10, 1000, 64, BF16, None, None)
     refused(bwd(dh=None, dw=None), _lib.EINVAL, "null")
     refused(bwd(nb=m - 1), _lib.EINVAL, "workspace")
     refused(bwd(lddh=63), _lib.EINVAL, "stride")
     refused(bwd(t=5), _lib.EINVAL, "type")
+    refused(bwd(ldw=65), _lib.EUNSUPPORTED, "aligned")
 
 
 def test_stream_xent_memory_stays_small():
@@ -103,8 +111,8 @@ def test_stream_xent_memory_stays_small():
     33278, width 256) and a long batch: a fraction of the logits' 2 bytes per row and word."""
     L = _lib.lib()
     for M, V, D in ((16352, 33278, 256), (131072, 33278, 256), (4096, 128000, 2048)):
-        kept = L.pnft_stream_xent_saved_size(M) + 2 * M * D
-        work = max(L.pnft_stream_xent_fwd_workspace_size(M, V), L.pnft_stream_xent_bwd_workspace_size(M, V, D))
+        kept = L.pnft_stream_xent_saved_size(M, D)
+        work = max(L.pnft_stream_xent_fwd_workspace_size(M, V, D, 1), L.pnft_stream_xent_bwd_workspace_size(M, V, D))
         assert kept < 0.06 * 2 * M * V and work < 0.6 * 2 * M * V, (M, V, D, kept, work)
 
 
@@ -119,6 +127,15 @@ def test_act8_and_copies_refuse():
     refused(pack(lde=0), _lib.EINVAL, "stride")
     assert pack(M=0, x=None) == _lib.OK
     refused(L.pnft_copy_rows16(A, 8, A, 4, 2, 8, None), _lib.EINVAL, "layout")
+    n = L.pnft_act8_weight_grad_workspace_size(4, 16, 100)
+    grad = lambda dtype=BF16, lddy=16, dy=A, ws=A, nb=n, lddw=100, N=16: L.pnft_act8_weight_grad(  # noqa: E731
+        dy, lddy, A, 112, A, 112, A, lddw, FP32, ws, nb, 4, N, 100, dtype, None, None)
+    refused(grad(dtype=FP32), _lib.EUNSUPPORTED, "float16")
+    refused(grad(lddw=99), _lib.EINVAL, "shape")
+    refused(grad(lddy=15), _lib.EINVAL, "shape")
+    refused(grad(dy=None), _lib.EINVAL, "null")
+    refused(grad(nb=n - 1), _lib.EINVAL, "workspace")
+    refused(grad(lddy=17), _lib.EUNSUPPORTED, "aligned")
 
 
 def test_python_calls_refuse_cpu_tensors_and_bad_arguments():
