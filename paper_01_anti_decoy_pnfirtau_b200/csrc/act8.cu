@@ -45,61 +45,99 @@ struct ActArgs {
   int D, dtype, vec;
 };
 
-// Eight columns from `col` of a row (zeros past its end).
-__device__ __forceinline__ void load8(const ActArgs& p, int64_t row, int col, float (&v)[8]) {
-  const int cnt = p.D - col;
-  if (p.dtype == PNFT_DTYPE_F32) {
-    const float* src = static_cast<const float*>(p.x) + row * p.ldx + col;
-    if (p.vec && cnt >= 8) {
-      const float4 a = __ldcs(reinterpret_cast<const float4*>(src)), c = __ldcs(reinterpret_cast<const float4*>(src) + 1);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = c.x, v[5] = c.y, v[6] = c.z, v[7] = c.w;
+// Eight columns of a row as they are stored (16 or 32 bytes; zeros past the row's end).
+template <bool F32>
+struct Raw {
+  uint32_t w[F32 ? 8 : 4];
+  __device__ __forceinline__ void load(const void* x, int64_t at, int cnt, bool vec) {
+    constexpr int SIZE = F32 ? 4 : 2;
+    const char* src = static_cast<const char*>(x) + at * SIZE;
+    if (vec && cnt >= 8) {
+#pragma unroll
+      for (int i = 0; i < SIZE / 2; ++i) {
+        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(src) + i);
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+      }
+    } else if (F32) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[F32 ? k : 0] = k < cnt ? reinterpret_cast<const uint32_t*>(src)[k] : 0;
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = k < cnt ? src[k] : 0.f;
+      for (int k = 0; k < 4; ++k)
+        w[k] = (2 * k < cnt ? reinterpret_cast<const uint16_t*>(src)[2 * k] : 0u) |
+               (2 * k + 1 < cnt ? (uint32_t) reinterpret_cast<const uint16_t*>(src)[2 * k + 1] << 16 : 0u);
     }
-  } else {
-    tc::load_row16<8>(static_cast<const uint16_t*>(p.x) + row * p.ldx + col, v, cnt, p.vec, p.dtype == PNFT_DTYPE_BF16);
   }
-}
+  __device__ __forceinline__ float2 pair(int k, bool bf16) const {
+    if constexpr (F32) return make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+    return tc::unpack2(w[k], bf16);
+  }
+  // The largest magnitude's bits as fp32, NaN left out: magnitudes compare as integers, 16-bit
+  // ones two at a time.
+  __device__ __forceinline__ uint32_t top(bool bf16) const {
+    if constexpr (F32) {
+      float m = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(__uint_as_float(w[k])));
+      return __float_as_uint(m);
+    } else if (bf16) {
+      __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
+#pragma unroll
+      for (int k = 1; k < 4; ++k) m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[k])));
+      return __float_as_uint(fmaxf(fmaxf(__low2float(m), __high2float(m)), 0.f));
+    } else {
+      __half2 m = __habs2(*reinterpret_cast<const __half2*>(&w[0]));
+#pragma unroll
+      for (int k = 1; k < 4; ++k) m = __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&w[k])));
+      return __float_as_uint(fmaxf(fmaxf(__low2float(m), __high2float(m)), 0.f));
+    }
+  }
+};
 
 // A warp takes COLS columns of a row at a time: eight columns per lane, 16 lanes per block
-// of 128, AU loads in flight per lane (measured at 16384 x 1024 bf16: AU = 1 with a row
-// index by division 18.2 us, this 9.5).
+// of 128, AU loads in flight per lane.
 constexpr int AU = 4, COLS = 256 * AU;
 
+template <bool F32>
 __global__ void __launch_bounds__(AT) act8_pack_kernel(ActArgs p) {
   const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
+  const bool bf16 = p.dtype == PNFT_DTYPE_BF16;
   int lo, hi;
   exponent_range(p.dtype, &lo, &hi);
   for (int64_t row = (int64_t)blockIdx.x * (AT / 32) + (threadIdx.x >> 5); row < p.M; row += (int64_t)gridDim.x * (AT / 32)) {
     const int c0 = blockIdx.y * COLS;
-    float v[AU][8];
+    Raw<F32> v[AU];
 #pragma unroll
-    for (int j = 0; j < AU; ++j) load8(p, row, c0 + 256 * j + 8 * lane, v[j]);
+    for (int j = 0; j < AU; ++j) v[j].load(p.x, row * p.ldx + c0 + 256 * j + 8 * lane, p.D - (c0 + 256 * j + 8 * lane), p.vec);
 #pragma unroll
     for (int j = 0; j < AU; ++j) {
       const int col = c0 + 256 * j + 8 * lane, cnt = p.D - col;
       if (c0 + 256 * j >= p.D) break;  // the same for the whole warp
-      float top = 0.f;
+      uint32_t top = v[j].top(bf16);   // not negative: ordered as integers
+      if (__any_sync(0xffffffffu, top >= 0x7f800000u)) {  // an infinity: the largest of the finite ones, value by value
+        top = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (!(fabsf(v[j][k]) <= 3.402823466e38f)) v[j][k] = __int_as_float(0x7fc00000);
-        top = fmaxf(top, fabsf(v[j][k]));  // fmaxf leaves NaN out
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = v[j].pair(k, bf16);
+          const uint32_t a = __float_as_uint(fabsf(f.x)), c = __float_as_uint(fabsf(f.y));
+          top = max(top, max(a < 0x7f800000u ? a : 0u, c < 0x7f800000u ? c : 0u));
+        }
       }
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       // top = f * 2^k, 1 <= f < 2 (subnormals fall below the range anyway): 448 = 1.75 * 2^8
-      const int bits = __float_as_int(top);
-      int e = (bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000);
-      e = max(lo, min(hi, top == 0.f ? lo : e));
-      const float scale = pow2(-e), end = e == hi ? 240.f : 448.f;
+      int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffff) > 0x600000);
+      e = max(lo, min(hi, top == 0 ? lo : e));
       if (cnt <= 0) continue;
+      const float scale = pow2(-e), end = e == hi ? 240.f : 448.f;
       uint32_t w[2];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float a = v[j][2 * k] * scale, c = v[j][2 * k + 1] * scale;
-        if (fabsf(a) > end) a = copysignf(end, a);  // leaves NaN alone
-        if (fabsf(c) > end) c = copysignf(end, c);
+        const float2 f = v[j].pair(k, bf16);
+        // NaN stays NaN in the conversion; an infinity becomes one here; past `end` only in the largest exponent
+        float a = f.x * scale, c = f.y * scale;
+        a = fabsf(a) > end ? (fabsf(a) == INFINITY ? __int_as_float(0x7fc00000) : copysignf(end, a)) : a;
+        c = fabsf(c) > end ? (fabsf(c) == INFINITY ? __int_as_float(0x7fc00000) : copysignf(end, c)) : c;
         const uint32_t h = to_e4m3x2(a, c);
         w[k / 2] = k & 1 ? w[k / 2] | (h << 16) : h;
       }
@@ -174,7 +212,10 @@ extern "C" int pnft_act8_pack(const void* x, int64_t ldx, void* q, int64_t ldq, 
   if (M == 0) return PNFT_OK;
   ActArgs a{x, ldx, static_cast<uint8_t*>(q), ldq, e, lde, M, (int)D, dtype,
             tc::rows16(x, ldx, dtype == PNFT_DTYPE_F32 ? 4 : 2)};
-  act8_pack_kernel<<<act8_grid(M, D), AT, 0, as_stream(stream)>>>(a);
+  if (dtype == PNFT_DTYPE_F32)
+    act8_pack_kernel<true><<<act8_grid(M, D), AT, 0, as_stream(stream)>>>(a);
+  else
+    act8_pack_kernel<false><<<act8_grid(M, D), AT, 0, as_stream(stream)>>>(a);
   return check_launch("act8_pack", 1);
 }
 

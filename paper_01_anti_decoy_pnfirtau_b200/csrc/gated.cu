@@ -209,8 +209,11 @@ struct GatedEpi {
 };
 
 // ------------------------------------------------------------------ a few rows
-// Forward for at most 64 rows: a block has 16 columns of h, four warps the products of
-// x with those rows of Wg and four with Wu's, each a quarter of K.
+// From 33 rows on the tiles win (B200, bf16, cold L2: 1024 x 4096 weights 9.3 us here at 32
+// rows and 13.7 in tiles, 4096 x 16384 74 and 67; at one row 6.8 and 13.7, 51 and 67).
+constexpr int SKINNY_ROWS = 32;
+// Forward for few rows: a block has 16 columns of h; each of its warps takes an
+// eighth of K of the products of x with those rows of Wg and of Wu.
 struct SkinnyArgs {
   const uint16_t *x, *wg, *wu;
   int64_t ldx, ldwg, ldwu;
@@ -221,28 +224,36 @@ struct SkinnyArgs {
   int M, D, F;
 };
 template <int NT, bool VEC, bool BF16>
-__global__ void __launch_bounds__(32 * skinny::WARPS) gated_skinny_kernel(SkinnyArgs p) {
+__global__ void __launch_bounds__(32 * skinny::WARPS, 2) gated_skinny_kernel(SkinnyArgs p) {
   constexpr int N = 8 * NT;
-  __shared__ float red[skinny::WARPS][16][N + 1];
+  __shared__ float red[skinny::WARPS / 2][2][16][N + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int f0 = blockIdx.x * 16, side = warp >> 2;
-  const uint16_t* w = side ? p.wu : p.wg;
-  const int64_t ld = side ? p.ldwu : p.ldwg;
-  float acc[NT][4] = {};
+  const int f0 = blockIdx.x * 16;
   // rows past F read the last one; their columns are not written
-  skinny::dot<NT, VEC, BF16>(w + min(f0 + g, p.F - 1) * ld, w + min(f0 + g + 8, p.F - 1) * ld, p.x, p.ldx, p.M, p.D, warp & 3,
-                             4, acc);
+  const int64_t r0 = min(f0 + g, p.F - 1), r1 = min(f0 + g + 8, p.F - 1);
+  const uint16_t* const w[4] = {p.wg + r0 * p.ldwg, p.wg + r1 * p.ldwg, p.wu + r0 * p.ldwu, p.wu + r1 * p.ldwu};
+  float acc[2][NT][4] = {};
+  skinny::dot<2, NT, VEC, BF16>(w, p.x, p.ldx, p.M, p.D, warp, skinny::WARPS, acc);
+  // the upper warps' parts are added to the lower ones', which keep shared memory small
+  for (int half = 1; half >= 0; --half) {
+    if ((warp >> 2) == half) {
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    red[warp][g][8 * j + 2 * t] = acc[j][0], red[warp][g][8 * j + 2 * t + 1] = acc[j][1];
-    red[warp][g + 8][8 * j + 2 * t] = acc[j][2], red[warp][g + 8][8 * j + 2 * t + 1] = acc[j][3];
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float& v = red[warp & 3][r][g + 8 * (k >> 1)][8 * j + 2 * t + (k & 1)];
+            v = half ? acc[r][j][k] : v + acc[r][j][k];
+          }
+    }
+    __syncthreads();
   }
-  __syncthreads();
   for (int i = threadIdx.x; i < 16 * p.M; i += 32 * skinny::WARPS) {
     const int f = i & 15, n = i >> 4, col = f0 + f;
     if (col >= p.F) continue;
-    float gv = (red[0][f][n] + red[1][f][n]) + (red[2][f][n] + red[3][f][n]);
-    float uv = (red[4][f][n] + red[5][f][n]) + (red[6][f][n] + red[7][f][n]);
+    float gv = (red[0][0][f][n] + red[1][0][f][n]) + (red[2][0][f][n] + red[3][0][f][n]);
+    float uv = (red[0][1][f][n] + red[1][1][f][n]) + (red[2][1][f][n] + red[3][1][f][n]);
     if (p.bg) gv += load_any(p.bg, col, p.b_dtype);
     if (p.bu) uv += load_any(p.bu, col, p.b_dtype);
     const float a = p.act == PNFT_ACT_SILU ? act_value<false, PNFT_ACT_SILU>(gv, nullptr) : act_value<false, PNFT_ACT_GELU>(gv, nullptr);
@@ -253,8 +264,10 @@ __global__ void __launch_bounds__(32 * skinny::WARPS) gated_skinny_kernel(Skinny
 // ------------------------------------------------------------------ pointwise backward
 // dg, du from dh and the kept g, u (their three planes), with the column sums of dg and du
 // as stored for the biases' gradients; without dh only the sums of given dg, du. A block
-// takes 8 columns per lane (256 in all) of a run of rows, a warp two rows at a time.
-constexpr int PT = 256, PCOLS = 256, PBLOCKS = 2;  // blocks per SM
+// takes 8 columns per lane (256 in all) of a run of rows, a warp a row at a time. Bound by
+// HBM: 12 bytes per element; the loads of 32 warps per SM keep it busy (16 with two rows each
+// reached 3.8 TB/s).
+constexpr int PT = 256, PCOLS = 256, PBLOCKS = 4;  // blocks per SM
 struct PointArgs {
   const uint16_t* dh;
   int64_t lddh;
@@ -266,46 +279,48 @@ struct PointArgs {
   int M, F, bf16, rows, vec;
 };
 
-// 8 values of 24 bits from their upper 16 and a byte of the third plane.
-__device__ __forceinline__ void join24(const uint16_t* hi, const uint16_t* low, int n, bool up, float (&v)[8]) {
-  uint32_t h[4], l[4];
+// 8 values of g and of u with 24 bits from their upper 16 and the third plane's bytes.
+__device__ __forceinline__ void join24(const uint16_t* gp, const uint16_t* up, const uint16_t* lp, int n, float (&g)[8],
+                                       float (&u)[8]) {
+  uint32_t a[4], b[4], l[4];
   if (n >= 8) {
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(hi)), b = *reinterpret_cast<const uint4*>(low);
-    h[0] = a.x, h[1] = a.y, h[2] = a.z, h[3] = a.w, l[0] = b.x, l[1] = b.y, l[2] = b.z, l[3] = b.w;
+    const uint4 x = __ldcs(reinterpret_cast<const uint4*>(gp)), y = __ldcs(reinterpret_cast<const uint4*>(up)),
+                z = __ldcs(reinterpret_cast<const uint4*>(lp));
+    a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w, b[0] = y.x, b[1] = y.y, b[2] = y.z, b[3] = y.w;
+    l[0] = z.x, l[1] = z.y, l[2] = z.z, l[3] = z.w;
   } else {
+    auto pair = [&](const uint16_t* p, int k) {
+      return (2 * k < n ? p[2 * k] : 0u) | (2 * k + 1 < n ? (uint32_t)p[2 * k + 1] << 16 : 0u);
+    };
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      h[k] = (2 * k < n ? hi[2 * k] : 0u) | (2 * k + 1 < n ? (uint32_t)hi[2 * k + 1] << 16 : 0u);
-      l[k] = (2 * k < n ? low[2 * k] : 0u) | (2 * k + 1 < n ? (uint32_t)low[2 * k + 1] << 16 : 0u);
-    }
+    for (int k = 0; k < 4; ++k) a[k] = pair(gp, k), b[k] = pair(up, k), l[k] = pair(lp, k);
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    // bytes 3, 2: the upper half; byte 1: the low plane's byte (g's, or u's after it); byte 0: cleared
-    v[2 * k] = __uint_as_float(__byte_perm(h[k], l[k], up ? 0x1050 : 0x1040) & 0xffffff00u);
-    v[2 * k + 1] = __uint_as_float(__byte_perm(h[k], l[k], up ? 0x3270 : 0x3260) & 0xffffff00u);
+    // bytes 3, 2: the upper half; byte 1: the third plane's (g's, or u's above it); byte 0: cleared
+    g[2 * k] = __uint_as_float(__byte_perm(a[k], l[k], 0x1040) & 0xffffff00u);
+    g[2 * k + 1] = __uint_as_float(__byte_perm(a[k], l[k], 0x3260) & 0xffffff00u);
+    u[2 * k] = __uint_as_float(__byte_perm(b[k], l[k], 0x1050) & 0xffffff00u);
+    u[2 * k + 1] = __uint_as_float(__byte_perm(b[k], l[k], 0x3270) & 0xffffff00u);
   }
 }
 
-template <bool POINT, int ACT>
+template <bool POINT, bool SUMS, int ACT>
 __global__ void __launch_bounds__(PT, PBLOCKS) gated_point_kernel(PointArgs p) {
-  __shared__ float red[PT / 32][2][PCOLS];
+  __shared__ float red[SUMS ? PT / 32 : 1][2][PCOLS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col = blockIdx.x * PCOLS + 8 * lane, n = p.F - col;
   const bool bf16 = p.bf16;
-  float sg[8], su[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) sg[k] = su[k] = 0.f;
+  float sg[8] = {}, su[8] = {};
   const int64_t r0 = (int64_t)blockIdx.y * p.rows, r1 = std::min<int64_t>(p.M, r0 + p.rows);
   if (n > 0) {
-#pragma unroll 2
+#pragma unroll 1
     for (int64_t r = r0 + warp; r < r1; r += PT / 32) {
       float g[8], u[8];
       if (POINT) {
         float d[8];
+        join24(p.g + r * p.ldp + col, p.u + r * p.ldp + col, p.low + r * p.ldp + col, n, g, u);
         load_row16<8>(p.dh + r * p.lddh + col, d, n, p.vec, bf16);
-        join24(p.g + r * p.ldp + col, p.low + r * p.ldp + col, n, false, g);
-        join24(p.u + r * p.ldp + col, p.low + r * p.ldp + col, n, true, u);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           float da;
@@ -319,11 +334,13 @@ __global__ void __launch_bounds__(PT, PBLOCKS) gated_point_kernel(PointArgs p) {
         load_row16<8>(p.g + r * p.ldp + col, g, n, p.vec, bf16);
         load_row16<8>(p.u + r * p.ldp + col, u, n, p.vec, bf16);
       }
+      if (SUMS) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sg[k] += g[k], su[k] += u[k];
+        for (int k = 0; k < 8; ++k) sg[k] += g[k], su[k] += u[k];
+      }
     }
   }
-  if (!p.part) return;
+  if (!SUMS) return;
 #pragma unroll
   for (int k = 0; k < 8; ++k) red[warp][0][8 * lane + k] = sg[k], red[warp][1][8 * lane + k] = su[k];
   __syncthreads();
@@ -427,7 +444,7 @@ extern "C" int pnft_gated_fwd(const void* x, int64_t ldx, const void* wg, int64_
   if (pre && !rows16(pre, ldp, 2)) return fail(PNFT_EINVAL, "gated_fwd: the kept rows must be 16-byte aligned");
   if (b_dtype < PNFT_DTYPE_F32 || b_dtype > PNFT_DTYPE_F16) return fail(PNFT_EINVAL, "gated_fwd: unknown bias type %d", b_dtype);
   if (ldx < D || ldwg < D || ldwu < D) return fail(PNFT_EUNSUPPORTED, "gated_fwd: x and weight rows must not overlap (aligned strides of at least D)");
-  if (M <= skinny::MAX_ROWS && !pre && x && wg && wu) {
+  if (M <= SKINNY_ROWS && !pre && x && wg && wu) {
     const SkinnyArgs a{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(wg), static_cast<const uint16_t*>(wu),
                        ldx, ldwg, ldwu, bg, bu, b_dtype, act, static_cast<uint16_t*>(h), ldh, (int)M, (int)D, (int)F};
     const bool vec = D % 8 == 0 && rows16(x, ldx, 2) && rows16(wg, ldwg, 2) && rows16(wu, ldwu, 2);
@@ -492,11 +509,13 @@ int point(const uint16_t* dh, int64_t lddh, const void* pre, int64_t ldp, uint16
   p.rows = point_rows(M, F);
   const dim3 grid((unsigned)((F + PCOLS - 1) / PCOLS), (unsigned)((M + p.rows - 1) / p.rows));
   if (!dh)
-    gated_point_kernel<false, 0><<<grid, PT, 0, st>>>(p);
+    gated_point_kernel<false, true, 0><<<grid, PT, 0, st>>>(p);
   else if (act == PNFT_ACT_SILU)
-    gated_point_kernel<true, PNFT_ACT_SILU><<<grid, PT, 0, st>>>(p);
+    sums ? gated_point_kernel<true, true, PNFT_ACT_SILU><<<grid, PT, 0, st>>>(p)
+         : gated_point_kernel<true, false, PNFT_ACT_SILU><<<grid, PT, 0, st>>>(p);
   else
-    gated_point_kernel<true, PNFT_ACT_GELU><<<grid, PT, 0, st>>>(p);
+    sums ? gated_point_kernel<true, true, PNFT_ACT_GELU><<<grid, PT, 0, st>>>(p)
+         : gated_point_kernel<true, false, PNFT_ACT_GELU><<<grid, PT, 0, st>>>(p);
   if (sums)
     gated_bias_sum_kernel<<<(unsigned)((2 * F + 255) / 256), 256, 0, st>>>(p.part, (int)grid.y, (int)F, dbg, dbu, b_dtype);
   return check_launch("gated_bwd pointwise", sums ? 2 : 1);

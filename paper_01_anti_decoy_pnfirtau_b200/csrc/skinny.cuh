@@ -1,5 +1,5 @@
 // Products of a weight matrix with a few rows (single tokens, small batches of answers):
-//   acc[r, n] = sum_k W[r, k] x[n, k],   16 rows of W per warp, n < 8 NT <= 64
+//   acc[r, n] = sum_k W[r, k] x[n, k],   16 rows of W per warp, n < 8 NT <= 32
 // Bound by reading W once. A 256-row tcgen05 tile would be almost empty and leave half of
 // the SMs without a tile, so here every warp streams its own 16 rows straight from memory
 // into the fragments of mma.sync (m16n8k16, W as the 16-row operand, the tokens as the 8
@@ -12,7 +12,6 @@
 namespace pnft {
 namespace skinny {
 
-constexpr int MAX_ROWS = 64;  // of x
 constexpr int WARPS = 8;
 
 template <bool BF16>
@@ -49,22 +48,23 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int D) {
   }
 }
 
-// The lane's part of a warp's product: rows w0 (row lane / 4 of the 16) and w1 (8 below),
-// 32-wide steps first, first + stride, ... of K. acc[j]: rows (lane / 4, + 8) x tokens
-// 8 j + 2 (lane & 3) + {0, 1}, in mma.sync's order.
-template <int NT, bool VEC, bool BF16>
-__device__ __forceinline__ void dot(const uint16_t* w0, const uint16_t* w1, const uint16_t* x, int64_t ldx, int M, int D,
-                                    int first, int stride, float (&acc)[NT][4]) {
-  constexpr int U = NT <= 2 ? 4 : 2;  // steps in flight
+// The lane's part of a warp's product: RG groups of 16 rows (w[2 r]: the group's row
+// lane / 4, w[2 r + 1]: 8 below), 32-wide steps first, first + stride, ... of K.
+// acc[r][j]: rows (lane / 4, + 8) x tokens 8 j + 2 (lane & 3) + {0, 1}, in mma.sync's order.
+// The groups share the tokens' fragments, which come from L1.
+template <int RG, int NT, bool VEC, bool BF16>
+__device__ __forceinline__ void dot(const uint16_t* const (&w)[2 * RG], const uint16_t* x, int64_t ldx, int M, int D, int first,
+                                    int stride, float (&acc)[RG][NT][4]) {
+  constexpr int U = RG * NT <= 2 ? 4 : 2;  // steps in flight
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int steps = (D + 31) / 32;
   for (int s = first; s < steps; s += U * stride) {
-    uint4 a[U], b[U];
+    uint4 a[U][2 * RG];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int k = s + i * stride < steps ? 32 * (s + i * stride) + 8 * t : D;  // past the last step: zeros
-      a[i] = load8<VEC, true>(w0, k, D);
-      b[i] = load8<VEC, true>(w1, k, D);
+#pragma unroll
+      for (int r = 0; r < 2 * RG; ++r) a[i][r] = load8<VEC, true>(w[r], k, D);
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -74,15 +74,18 @@ __device__ __forceinline__ void dot(const uint16_t* w0, const uint16_t* w1, cons
       for (int j = 0; j < NT; ++j)
         v[j] = 8 * j + g < M ? load8<VEC, false>(x + (8 * j + g) * ldx, k, D) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        mma<BF16>(acc[j], a[i].x, b[i].x, a[i].y, b[i].y, v[j].x, v[j].y);
-        mma<BF16>(acc[j], a[i].z, b[i].z, a[i].w, b[i].w, v[j].z, v[j].w);
-      }
+      for (int r = 0; r < RG; ++r)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const uint4 &p = a[i][2 * r], &q = a[i][2 * r + 1];
+          mma<BF16>(acc[r][j], p.x, q.x, p.y, q.y, v[j].x, v[j].y);
+          mma<BF16>(acc[r][j], p.z, q.z, p.w, q.w, v[j].z, v[j].w);
+        }
     }
   }
 }
 
-// Calls f(NT, VEC, BF16 as integral constants) for M rows.
+// Calls f(NT, VEC, BF16 as integral constants) for M <= 32 rows.
 template <class F>
 int dispatch(int64_t M, bool vec, bool bf16, F f) {
   auto types = [&](auto nt) {
@@ -91,8 +94,8 @@ int dispatch(int64_t M, bool vec, bool bf16, F f) {
   };
   if (M <= 8) return types(std::integral_constant<int, 1>());
   if (M <= 16) return types(std::integral_constant<int, 2>());
-  if (M <= 32) return types(std::integral_constant<int, 4>());
-  return types(std::integral_constant<int, 8>());
+  if (M <= 24) return types(std::integral_constant<int, 3>());
+  return types(std::integral_constant<int, 4>());
 }
 
 }  // namespace skinny

@@ -282,7 +282,10 @@ __global__ void __launch_bounds__(256) xent_reduce_kernel(ReduceArgs p) {
 }
 
 // ------------------------------------------------------------------ a few rows
-// Loss of at most 64 rows without a gradient: every warp takes 16 words of the vocabulary
+// From 25 rows on the tiles win (B200, bf16, cold L2: 33278 x 256 weights 15 us here at one
+// row, 20 at 24 and 28 to 35 in tiles; 50021 x 1024 36, 45 and 47 to 54).
+constexpr int SKINNY_ROWS = 24;
+// Loss of few rows without a gradient: every warp takes 16 or 32 words of the vocabulary
 // at a time and keeps each row's maximum and sum over them; a block joins its warps' and
 // leaves one pair per row. Rows to ignore are computed with the others (a column of the
 // product touches no other) and left out at the end.
@@ -291,7 +294,7 @@ struct SkinnyArgs {
   int64_t ldh, ldw;
   const int64_t* t;
   int64_t ignore;
-  float *part_m, *part_s, *zt;  // [blocks][64], [64]
+  float *part_m, *part_s, *zt;  // [blocks][SKINNY_ROWS], [SKINNY_ROWS]
   float *row_loss, *loss;
   int M, D, V, blocks, mean;
   int32_t* status;
@@ -301,8 +304,10 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   s = s * ex2(m - top) + s2 * ex2(m2 - top);
   m = top;
 }
+// Groups of 16 words per warp: two share the rows' fragments when there are many rows.
+constexpr int skinny_groups(int nt) { return nt <= 2 ? 1 : 2; }
 template <int NT, bool VEC, bool BF16>
-__global__ void __launch_bounds__(32 * skinny::WARPS) xent_skinny_kernel(SkinnyArgs p) {
+__global__ void __launch_bounds__(32 * skinny::WARPS, NT <= 4 ? 2 : 1) xent_skinny_kernel(SkinnyArgs p) {
   __shared__ float sm[skinny::WARPS][8 * NT], ss[skinny::WARPS][8 * NT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float m[NT][2], s[NT][2];
@@ -316,22 +321,28 @@ __global__ void __launch_bounds__(32 * skinny::WARPS) xent_skinny_kernel(SkinnyA
       const int64_t v = n < p.M ? p.t[n] : -1;
       tgt[j][k] = v >= 0 && v < p.V ? (int)v : -1;
     }
-  for (int64_t v0 = (blockIdx.x * skinny::WARPS + warp) * 16; v0 < p.V; v0 += gridDim.x * skinny::WARPS * 16) {
-    float acc[NT][4] = {};
-    const int r0 = (int)v0 + g, r1 = r0 + 8;
-    skinny::dot<NT, VEC, BF16>(p.w + (int64_t)min(r0, p.V - 1) * p.ldw, p.w + (int64_t)min(r1, p.V - 1) * p.ldw, p.h, p.ldh, p.M,
-                               p.D, 0, 1, acc);
+  constexpr int RG = skinny_groups(NT);
+  for (int64_t v0 = (blockIdx.x * skinny::WARPS + warp) * (16 * RG); v0 < p.V; v0 += gridDim.x * skinny::WARPS * (16 * RG)) {
+    float acc[RG][NT][4] = {};
+    const uint16_t* w[2 * RG];
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+    for (int r = 0; r < 2 * RG; ++r) w[r] = p.w + min(v0 + g + 8 * r, (int64_t)p.V - 1) * p.ldw;
+    skinny::dot<RG, NT, VEC, BF16>(w, p.h, p.ldh, p.M, p.D, 0, 1, acc);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (r0 == tgt[j][k]) p.zt[8 * j + 2 * t + k] = acc[j][k];
-        if (r1 == tgt[j][k]) p.zt[8 * j + 2 * t + k] = acc[j][k + 2];
-        const float a = r0 < p.V ? acc[j][k] : -INFINITY, b = r1 < p.V ? acc[j][k + 2] : -INFINITY;
-        const float top = max3(m[j][k], a * kLog2e, b * kLog2e);
-        s[j][k] = s[j][k] * ex2(m[j][k] - top) + ex2(fmaf(a, kLog2e, -top)) + ex2(fmaf(b, kLog2e, -top));
-        m[j][k] = top;
-      }
+    for (int r = 0; r < RG; ++r) {
+      const int r0 = (int)v0 + 16 * r + g, r1 = r0 + 8;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (r0 == tgt[j][k]) p.zt[8 * j + 2 * t + k] = acc[r][j][k];
+          if (r1 == tgt[j][k]) p.zt[8 * j + 2 * t + k] = acc[r][j][k + 2];
+          const float a = r0 < p.V ? acc[r][j][k] : -INFINITY, b = r1 < p.V ? acc[r][j][k + 2] : -INFINITY;
+          const float top = max3(m[j][k], a * kLog2e, b * kLog2e);
+          s[j][k] = s[j][k] * ex2(m[j][k] - top) + ex2(fmaf(a, kLog2e, -top)) + ex2(fmaf(b, kLog2e, -top));
+          m[j][k] = top;
+        }
+    }
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j)
@@ -347,18 +358,19 @@ __global__ void __launch_bounds__(32 * skinny::WARPS) xent_skinny_kernel(SkinnyA
   if (n >= p.M) return;
   float a = sm[0][n], b = ss[0][n];
   for (int k = 1; k < skinny::WARPS; ++k) join(a, b, sm[k][n], ss[k][n]);
-  p.part_m[blockIdx.x * skinny::MAX_ROWS + n] = a;
-  p.part_s[blockIdx.x * skinny::MAX_ROWS + n] = b;
+  p.part_m[blockIdx.x * SKINNY_ROWS + n] = a;
+  p.part_s[blockIdx.x * SKINNY_ROWS + n] = b;
 }
 
 // Joins the blocks' pairs, a warp per row, and sums the rows.
 __global__ void __launch_bounds__(1024) xent_skinny_reduce_kernel(SkinnyArgs p) {
-  __shared__ float losses[skinny::MAX_ROWS];
-  __shared__ int counted[skinny::MAX_ROWS];
+  __shared__ float losses[SKINNY_ROWS];
+  __shared__ int counted[SKINNY_ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int n = warp; n < p.M; n += 32) {
     float m = kLow, s = 0.f;
-    for (int b = lane; b < p.blocks; b += 32) join(m, s, p.part_m[b * skinny::MAX_ROWS + n], p.part_s[b * skinny::MAX_ROWS + n]);
+#pragma unroll 8
+    for (int b = lane; b < p.blocks; b += 32) join(m, s, p.part_m[b * SKINNY_ROWS + n], p.part_s[b * SKINNY_ROWS + n]);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) join(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
     if (lane == 0) {
@@ -624,7 +636,7 @@ static int skinny_blocks(int64_t V) {
 
 extern "C" size_t pnft_stream_xent_fwd_workspace_size(int64_t M, int64_t V, int64_t D, int save) {
   if (M <= 0 || V <= 0 || D <= 0) return 0;
-  if (!save && M <= skinny::MAX_ROWS) return sizeof(float) * skinny::MAX_ROWS * (2 * (size_t)skinny_blocks(V) + 1);
+  if (!save && M <= SKINNY_ROWS) return sizeof(float) * SKINNY_ROWS * (2 * (size_t)skinny_blocks(V) + 1);
   return fwd_layout(M, V).total + (save ? 0 : saved_layout(M, D).total);
 }
 
@@ -648,11 +660,11 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
     return fail(PNFT_EINVAL, "stream_xent_fwd: workspace of %zu bytes < required %zu", workspace_bytes, need);
   char* ws = static_cast<char*>(workspace);
   cudaStream_t st = as_stream(stream);
-  if (!saved && M <= skinny::MAX_ROWS) {
+  if (!saved && M <= SKINNY_ROWS) {
     const int blocks = skinny_blocks(V);
     float* part = static_cast<float*>(workspace);
     const SkinnyArgs a{static_cast<const uint16_t*>(h), static_cast<const uint16_t*>(w), ldh, ldw, targets, ignore_index, part,
-                       part + (size_t)blocks * skinny::MAX_ROWS, part + 2 * (size_t)blocks * skinny::MAX_ROWS, row_loss, loss,
+                       part + (size_t)blocks * SKINNY_ROWS, part + 2 * (size_t)blocks * SKINNY_ROWS, row_loss, loss,
                        (int)M, (int)D, (int)V, blocks, mean, status};
     const bool vec = D % 8 == 0 && rows16(h, ldh, 2) && rows16(w, ldw, 2);
     return skinny::dispatch(M, vec, dtype == PNFT_DTYPE_BF16, [&](auto nt, auto v, auto b) {

@@ -202,7 +202,7 @@ def act8_weight_grad(dy: torch.Tensor, p: Act8, out_dtype: torch.dtype = torch.f
 # written once and read once by a pointwise backward kernel); below it the backward
 # computes them again, which costs 4 M D F operations but no memory traffic.
 _KEEP_FROM = 640
-_SKINNY = 64  # rows of the forward kernel that takes any row strides
+_FEW = 24  # rows up to which the forward kernels take any row strides
 
 
 def _gated_forward(x, wg, wu, bg, bu, act: int, dt: torch.dtype, keep: bool):
@@ -214,7 +214,7 @@ def _gated_forward(x, wg, wu, bg, bu, act: int, dt: torch.dtype, keep: bool):
     else:
         x2, shape = x.reshape(-1, D), (*x.shape[:-1], F_)
     M = x2.shape[0]
-    rows = _rows16 if keep or M > _SKINNY else _unit_rows
+    rows = _rows16 if keep or M > _FEW else _unit_rows
     x2, wg, wu = rows(x2, dt), rows(wg, dt), rows(wu, dt)
     h = torch.empty(shape, dtype=dt, device=dev)
     pre = torch.empty((3, M, _pad8(F_)), dtype=torch.int16, device=dev) if keep else None
@@ -338,7 +338,7 @@ def _xent_forward(h, weight, targets, ignore_index: int, reduction: str, dt: tor
     V, D = weight.shape
     h2 = _unit_rows(h if h.dim() == 2 else h.reshape(-1, D), dt)
     M = h2.shape[0]
-    w = _rows16(weight, dt) if save or M > _SKINNY else _unit_rows(weight, dt)
+    w = _rows16(weight, dt) if save or M > _FEW else _unit_rows(weight, dt)
     t = targets if targets.dim() == 1 else targets.reshape(-1)
     if t.dtype != torch.int64 or not t.is_contiguous():
         t = t.to(torch.int64).contiguous()

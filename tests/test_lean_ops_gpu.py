@@ -279,7 +279,7 @@ def test_streamed_cross_entropy(cuda, shape, dt, reduction, ignored):
         k = n if reduction == "mean" else 1
         loss, el = loss.sum() / k, el.sum() / k + 2.0 ** -23 * loss.sum() / k
     check("loss", got.detach(), (loss, el))
-    check("loss without gradient", alone, (loss, el))  # up to 64 rows: a kernel of its own
+    check("loss without gradient", alone, (loss, el))  # few rows: a kernel of its own
     check("dh", gh, dh)
     check("dw", gw, dw)
     assert torch.all(gh[t == -100] == 0)
