@@ -31,6 +31,71 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+// Pairs of fp32 in one 64-bit register: two products or sums per instruction.
+typedef uint64_t f32x2;
+__device__ __forceinline__ f32x2 pack(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x of two values. The special-function unit gives 16 exponentials per clock and SM, and a
+// tile of 256 columns from K = 256 leaves it exactly as many clocks as the tensor core needs:
+// so a part of the exponentials runs on the FMA pipe (POLY): x = n + f with |f| <= 1/2, and
+// 2^f by a polynomial of degree 5, fitted to a relative error of 7.5e-8, or of degree 4 to
+// 2.6e-6 where the result is rounded to 16 bits. x >= -126 there; NaN stays NaN.
+template <bool POLY, int DEGREE>
+__device__ __forceinline__ f32x2 exp2_pair(f32x2 x) {
+  const float2 v = unpack(x);
+  if (!POLY) return pack(ex2(v.x), ex2(v.y));
+  x = pack(max_nan(v.x, -126.f), max_nan(v.y, -126.f));
+  constexpr float kRound = 12582912.f + 127.f;  // 1.5 * 2^23: the sum's low bits are the rounded x, biased as an exponent
+  const f32x2 y = add2(x, pack(kRound, kRound));
+  const f32x2 f = fma2(add2(y, pack(-kRound, -kRound)), pack(-1.f, -1.f), x);
+  f32x2 q;
+  if (DEGREE == 5) {
+    q = fma2(f, pack(0.00132765f, 0.00132765f), pack(0.00967554f, 0.00967554f));
+    q = fma2(q, f, pack(0.05550713f, 0.05550713f));
+    q = fma2(q, f, pack(0.2402212f, 0.2402212f));
+    q = fma2(q, f, pack(0.69314697f, 0.69314697f));
+    q = fma2(q, f, pack(1.00000007f, 1.00000007f));
+  } else {
+    q = fma2(f, pack(0.0095701f, 0.0095701f), pack(0.05591786f, 0.05591786f));
+    q = fma2(q, f, pack(0.24024745f, 0.24024745f));
+    q = fma2(q, f, pack(0.69312181f, 0.69312181f));
+    q = fma2(q, f, pack(0.99999926f, 0.99999926f));
+  }
+  const float2 e = unpack(y);
+  return mul2(q, pack(__uint_as_float(__float_as_uint(e.x) << 23), __uint_as_float(__float_as_uint(e.y) << 23)));
+}
+// Pair i of 16 (32 columns): every POLY_EVERY-th goes to the FMA pipe.
+constexpr int POLY_EVERY = 3;
+
 // Device state of one call, in the caller's buffers (rows are compacted rows).
 struct State {
   int32_t* counts;   // [0] rows that count, [1] blocks of the reduction that are done
@@ -181,15 +246,19 @@ struct LseEpi {
       for (int i = 6; i < 30; i += 4) a = max3(a, z[i], z[i + 1]), b = max3(b, z[i + 2], z[i + 3]);
       a = max3(a, z[30], z[31]);
       const float nm = max3(m, a * kLog2e, b * kLog2e);
-      float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+      const f32x2 scale = pack(kLog2e, kLog2e), minus = pack(-nm, -nm);
+      f32x2 s0 = 0, s1 = 0;
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        s0 += ex2(fmaf(z[i], kLog2e, -nm));
-        s1 += ex2(fmaf(z[i + 1], kLog2e, -nm));
-        s2 += ex2(fmaf(z[i + 2], kLog2e, -nm));
-        s3 += ex2(fmaf(z[i + 3], kLog2e, -nm));
+      for (int i = 0; i < 16; ++i) {
+        const f32x2 x = fma2(pack(z[2 * i], z[2 * i + 1]), scale, minus);
+        const f32x2 e = i % POLY_EVERY == 0 ? exp2_pair<true, 5>(x) : exp2_pair<false, 5>(x);
+        if (i & 1)
+          s1 = add2(s1, e);
+        else
+          s0 = add2(s0, e);
       }
-      s = fmaf(s, ex2(m - nm), (s0 + s1) + (s2 + s3));
+      const float2 sum = unpack(add2(s0, s1));
+      s = fmaf(s, ex2(m - nm), sum.x + sum.y);
       m = nm;
     }
     if (q.item_last() && row < live) {
@@ -459,8 +528,13 @@ struct DzEpi {
       acc_load32(acc + c, false, z);
       if (c + 32 == (w.slice + 1) * (BN / 4)) release();
       const int col = q.nt * BN + c, n = row < live ? p.V - p.v0 - col : 0, tc = tgt - col;
+      const f32x2 scale = pack(kLog2e, kLog2e), minus = pack(-lse, -lse), factor = pack(rs, rs);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) z[i] = ex2(fmaf(z[i], kLog2e, -lse)) * rs;
+      for (int i = 0; i < 16; ++i) {
+        const f32x2 x = fma2(pack(z[2 * i], z[2 * i + 1]), scale, minus);
+        const float2 v = unpack(mul2(i % POLY_EVERY == 0 ? exp2_pair<true, 4>(x) : exp2_pair<false, 4>(x), factor));
+        z[2 * i] = v.x, z[2 * i + 1] = v.y;
+      }
       if ((unsigned)tc < 32u) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
@@ -578,11 +652,15 @@ FwdLayout fwd_layout(int64_t M, int64_t V) {
   return l;
 }
 
-// A piece's gradient buffer is about 64 MB, so that the two GEMMs find it in L2.
+// Columns per piece: its gradient buffer takes at most 288 MB (at least 1024 columns), and
+// the pieces are alike. Measured (B200, 16352 x 33278 x 256, bf16, kernels of forward and
+// backward): 64 MB, which the two products find in L2, 1433 us; 128 MB 1334; 192 MB 1223;
+// 272 MB 1166: fewer launches and longer sums are worth more than L2.
 int64_t piece_width(int64_t M, int64_t V) {
   const int64_t Mp = up(M, BM);
-  const int64_t w = std::max<int64_t>(1024, ((int64_t)64 << 20) / (2 * Mp) / BN * BN);
-  return std::min(w, up(V, BN));
+  const int64_t most = std::max<int64_t>(1024, ((int64_t)288 << 20) / (2 * Mp) / BN * BN);
+  const int64_t pieces = (V + most - 1) / most;
+  return up((V + pieces - 1) / pieces, BN);
 }
 struct BwdLayout {
   int64_t P;
