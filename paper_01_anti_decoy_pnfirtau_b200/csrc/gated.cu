@@ -407,6 +407,7 @@ int gated_gemm(const char* what, int mode, const void* x, int64_t ldx, const voi
   if (!rc) rc = map_kmajor(&a.tb[1], wu, D, F, ldwu);
   if (rc) return rc;
   a.s = plain_sched(M, 2 * ((F + BN / 2 - 1) / (BN / 2) * (BN / 2)), (D + BK - 1) / BK, 1);
+  runs_if_resident(&a.s, 2 * F, D);
   a.idesc = idesc(dtype, false, false);
   a.status = status;
   auto go = [&](auto m, auto c) {

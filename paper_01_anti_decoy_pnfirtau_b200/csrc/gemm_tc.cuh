@@ -35,7 +35,7 @@ constexpr int BN = 256, BK = 64;
 constexpr int HALF_BYTES = BM * BK * 2;    // a CTA's A rows, or its half of B, of one stage
 constexpr int STAGE_BYTES = 2 * HALF_BYTES;
 constexpr int GROUP_BYTES = 64 * BK * 2;   // MN-major: 64 columns x 64 K rows
-constexpr int STAGE_MAX = 226 * 1024;      // shared memory for the ring and the epilogue's buffers
+constexpr int STAGE_MAX = 225 * 1024;      // shared memory for the ring and the epilogue's buffers
 
 // ------------------------------------------------------------------ PTX of the pair
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -111,9 +111,12 @@ __device__ __forceinline__ void commit_pair(uint32_t bar) {
       : "memory");
 }
 
-// Which tiles there are and in which order: items of one split are taken group_m
-// row tiles at a time, the row tile running fastest, so the pairs in flight share
-// both operands in L2.
+// Which tiles there are and in which order. Strips: an item is tiles_per_strip column tiles
+// of one row tile and one split of K; items are taken group_m row tiles at a time, the row
+// tile running fastest, so the pairs in flight share both operands in L2. Runs (`runs`): the
+// tiles, row tile by row tile, are dealt to the pairs in equal contiguous runs, and an item
+// is a run's part of one row tile: the pairs end together, and a pair keeps its rows of A.
+// For a B that stays in L2 as a whole.
 struct Sched {
   int tiles_m;          // 256-row tiles (upper bound when live is given)
   int strips;           // items along N
@@ -123,50 +126,78 @@ struct Sched {
   int splits;           // splits of K
   int chunk;            // K blocks that one accumulator takes before the epilogue collects it
   int group_m;
+  int runs;
   int seg_kb;           // K blocks of the first pair of maps; the rest use the second
   const int32_t* live;  // device: rows that count (NULL: all)
   int live_m, live_k;   // the rows that count bound M / K
 };
 
+// First tile of pair p's run of `total` tiles over `pairs` pairs, and the pair of tile x.
+__host__ __device__ inline int64_t run_begin(int64_t total, int p, int pairs) { return total * p / pairs; }
+__host__ __device__ inline int run_owner(int64_t total, int64_t x, int pairs) {
+  return (int)(((x + 1) * pairs + total - 1) / total) - 1;
+}
+
 struct Args {
   CUtensorMap ta[2], tb[2];
   Sched s;
   uint32_t idesc;
+  int stages;  // of the ring
   int32_t* status;
 };
 
 struct Item {
   int mt, nt0, ntn, split, kb0, kbn;
   int row0;  // first row of this CTA
+  int slot;  // strip, or place of the run among those of its row tile
 };
 
 struct Walk {
-  int tiles_m, kb, items;
-  __device__ explicit Walk(const Sched& s) {
+  int tiles_m, kb, slots, pairs;
+  int64_t total;  // items, or tiles in runs
+  __device__ Walk(const Sched& s, int launched) {
     tiles_m = s.tiles_m, kb = s.kb;
     if (s.live) {
       const int n = *s.live;
       if (s.live_m) tiles_m = (n + PM - 1) / PM;
       if (s.live_k) kb = (n + BK - 1) / BK;
     }
-    items = tiles_m * s.strips * s.splits;
+    total = s.runs ? (int64_t)tiles_m * s.tiles_n : (int64_t)tiles_m * s.strips * s.splits;
+    pairs = s.runs ? run_pairs(total, launched) : launched;
+    slots = s.runs ? run_slots(tiles_m, pairs) : s.strips;
   }
-  __device__ Item at(const Sched& s, int i, int rank) const {
+  // Pairs that get a run: none is empty, also where fewer rows count than the launch was sized for.
+  __host__ __device__ static int run_pairs(int64_t total, int launched) { return (int)(total < launched ? total : launched); }
+  // Runs that a row tile may lie in.
+  __host__ __device__ static int run_slots(int tiles_m, int pairs) {
+    return tiles_m > 0 ? (pairs + tiles_m - 1) / tiles_m + 1 : 0;
+  }
+  // The item that starts at i of `end`.
+  __device__ Item at(const Sched& s, int64_t i, int64_t end, int rank, int pair) const {
     Item it;
-    const int per_split = tiles_m * s.strips;
-    it.split = i / per_split;
-    int r = i - it.split * per_split;
-    const int per = s.group_m * s.strips, g = r / per;
-    r -= g * per;
-    const int gm = min(s.group_m, tiles_m - g * s.group_m);
-    it.mt = g * s.group_m + r % gm;
+    if (s.runs) {
+      it.split = 0, it.kb0 = 0, it.kbn = kb;
+      it.mt = (int)(i / s.tiles_n);
+      const int64_t first = (int64_t)it.mt * s.tiles_n;
+      it.nt0 = (int)(i - first);
+      it.ntn = (int)min((int64_t)s.tiles_n, end - first) - it.nt0;
+      it.slot = pair - run_owner(total, first, pairs);
+    } else {
+      const int per_split = tiles_m * s.strips;
+      it.split = (int)(i / per_split);
+      int r = (int)(i - (int64_t)it.split * per_split);
+      const int per = s.group_m * s.strips, g = r / per;
+      r -= g * per;
+      const int gm = min(s.group_m, tiles_m - g * s.group_m);
+      it.mt = g * s.group_m + r % gm;
+      it.slot = r / gm;
+      it.nt0 = it.slot * s.tiles_per_strip;
+      it.ntn = min(s.tiles_per_strip, s.tiles_n - it.nt0);
+      // whole K blocks spread evenly over the splits
+      it.kb0 = (int)((int64_t)kb * it.split / s.splits);
+      it.kbn = (int)((int64_t)kb * (it.split + 1) / s.splits) - it.kb0;
+    }
     it.row0 = it.mt * PM + rank * BM;
-    const int strip = r / gm;
-    it.nt0 = strip * s.tiles_per_strip;
-    it.ntn = min(s.tiles_per_strip, s.tiles_n - it.nt0);
-    // whole K blocks spread evenly over the splits
-    it.kb0 = (int)((int64_t)kb * it.split / s.splits);
-    it.kbn = (int)((int64_t)kb * (it.split + 1) / s.splits) - it.kb0;
     return it;
   }
 };
@@ -176,16 +207,19 @@ struct Walk {
 struct Steps {
   const Walk& walk;
   const Sched& s;
-  int i, stride, rank, nt, kb;
+  int64_t i, end;
+  int pair, rank, nt, kb;
   Item it;
-  __device__ Steps(const Walk& w, const Sched& s_, int pair, int pairs, int rank_)
-      : walk(w), s(s_), i(pair), stride(pairs), rank(rank_) {
+  __device__ Steps(const Walk& w, const Sched& s_, int pair_, int rank_) : walk(w), s(s_), pair(pair_), rank(rank_) {
+    const bool run = s.runs && pair < w.pairs;
+    i = run ? run_begin(w.total, pair, w.pairs) : pair;
+    end = run ? run_begin(w.total, pair + 1, w.pairs) : s.runs ? 0 : w.total;
     load();
   }
   __device__ void load() {
-    if (i < walk.items) it = walk.at(s, i, rank), nt = it.nt0, kb = it.kb0;
+    if (i < end) it = walk.at(s, i, end, rank, pair), nt = it.nt0, kb = it.kb0;
   }
-  __device__ bool valid() const { return i < walk.items; }
+  __device__ bool valid() const { return i < end; }
   __device__ int kb_end() const { return min(kb + s.chunk, it.kb0 + it.kbn); }
   __device__ bool tile_first() const { return kb == it.kb0; }
   __device__ bool tile_last() const { return kb + s.chunk >= it.kb0 + it.kbn; }
@@ -198,7 +232,7 @@ struct Steps {
     }
     kb = it.kb0;
     if (++nt == it.nt0 + it.ntn) {
-      i += stride;
+      i += s.runs ? it.ntn : walk.pairs;
       load();
     }
   }
@@ -219,38 +253,48 @@ struct EpiWarp {
 // column is in registers), done() at the end.
 // DUAL_B: columns 0-127 of a tile come from tb[0] and 128-255 from tb[1], both at row
 // 128 * nt.
+// KEEP_A: an item's rows of A (all of K, at most a few hundred) stay in shared memory for
+// all of its tiles and the ring carries B alone: at K = 256 a tile's MMAs take 2048 clocks,
+// in which A and B together (128 KB per CTA) ask more of L2 than it gives.
+constexpr int MAX_STAGES = 14;
 template <class Epi>
-constexpr int stages() {
-  return (STAGE_MAX - Epi::WARPS * Epi::BOXES * Epi::BOX_BYTES) / STAGE_BYTES;
+constexpr int box_bytes() {
+  return Epi::WARPS * Epi::BOXES * Epi::BOX_BYTES;
 }
 template <class Epi>
-constexpr int smem_bytes() {
-  return stages<Epi>() * STAGE_BYTES + Epi::WARPS * Epi::BOXES * Epi::BOX_BYTES + 1024;
+constexpr int stages(bool keep_a, int kb) {
+  const int n = keep_a ? (STAGE_MAX - box_bytes<Epi>() - kb * HALF_BYTES) / HALF_BYTES : (STAGE_MAX - box_bytes<Epi>()) / STAGE_BYTES;
+  return n > MAX_STAGES ? MAX_STAGES : n;
 }
+constexpr int SMEM = STAGE_MAX + 1024;
 
-template <bool A_MN, bool B_MN, bool DUAL_B, class Epi>
+template <bool A_MN, bool B_MN, bool DUAL_B, bool KEEP_A, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS), 1)
     gemm_kernel(const __grid_constant__ Args p, const __grid_constant__ typename Epi::Params ep) {
-  constexpr int STAGES = stages<Epi>(), EPI_WARPS = Epi::WARPS;
+  static_assert(!KEEP_A || !A_MN, "kept rows of A are K-major");
+  constexpr int EPI_WARPS = Epi::WARPS, SLOT = KEEP_A ? HALF_BYTES : STAGE_BYTES;
+  const int stages = p.stages;
   extern __shared__ __align__(1024) uint8_t raw[];
   const uint32_t sb = (smem_u32(raw) + 1023u) & ~1023u;
-  __shared__ __align__(8) uint64_t bars[2 * STAGES + 5 + EPI_WARPS];  // full, empty, acc full x2, acc empty x2, done, warps
+  // full, empty, acc full x2, acc empty x2, done, A full, A empty, warps
+  __shared__ __align__(8) uint64_t bars[2 * MAX_STAGES + 7 + EPI_WARPS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const uint32_t b0 = smem_u32(bars);
   auto full = [&](int s) { return b0 + 8u * s; };
-  auto empty = [&](int s) { return b0 + 8u * (STAGES + s); };
-  auto acc_full = [&](int s) { return b0 + 8u * (2 * STAGES + s); };
-  auto acc_empty = [&](int s) { return b0 + 8u * (2 * STAGES + 2 + s); };
-  const uint32_t done = b0 + 8u * (2 * STAGES + 4);
-  auto warp_bar = [&](int w) { return b0 + 8u * (2 * STAGES + 5 + w); };
+  auto empty = [&](int s) { return b0 + 8u * (MAX_STAGES + s); };
+  auto acc_full = [&](int s) { return b0 + 8u * (2 * MAX_STAGES + s); };
+  auto acc_empty = [&](int s) { return b0 + 8u * (2 * MAX_STAGES + 2 + s); };
+  const uint32_t done = b0 + 8u * (2 * MAX_STAGES + 4), a_full = done + 8, a_empty = done + 16;
+  auto warp_bar = [&](int w) { return b0 + 8u * (2 * MAX_STAGES + 7 + w); };
+  const uint32_t ring = sb + (KEEP_A ? (uint32_t)p.s.kb * HALF_BYTES : 0u);
   const Abort ab{&abort_flag, p.status};
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(full(s), 1);   // the even CTA's: its producer's arrival, and the bytes of both CTAs
       mbar_init(empty(s), 1);  // the MMAs that read the stage, told to both CTAs
     }
@@ -259,6 +303,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
       mbar_init(acc_empty(s), 2 * EPI_WARPS);  // the even CTA's: the epilogue warps of both
     }
     mbar_init(done, 1);
+    mbar_init(a_full, 1);
+    mbar_init(a_empty, 1);
     for (int w = 0; w < EPI_WARPS; ++w) mbar_init(warp_bar(w), 1);
     fence_barrier_init();
   }
@@ -271,25 +317,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
   cluster_sync();  // the other CTA's barriers are ready for this one's arrivals
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
-  const Walk walk(p.s);
+  const Walk walk(p.s, pairs);
 
   if (warp == 0) {
     // -------------------------------------------------------------- TMA producer
     if (lane == 0) {
-      int st = 0, ph = 1, issued = 0;
+      int st = 0, ph = 1, issued = 0, items = 0;
       bool ok = true;
-      for (Steps q(walk, p.s, pair, pairs, rank); ok && q.valid(); q.next()) {
+      for (Steps q(walk, p.s, pair, rank); ok && q.valid(); q.next()) {
+        if (KEEP_A && q.item_first()) {
+          if (!mbar_wait(a_empty, (items & 1) ^ 1, ab)) break;
+          if (rank == 0) mbar_arrive_expect_tx(a_full, (uint32_t)(2 * HALF_BYTES * q.it.kbn));
+          for (int kb = 0; kb < q.it.kbn; ++kb)
+            tma_load_pair(sb + (uint32_t)kb * HALF_BYTES, &p.ta[0], map_rank(a_full, 0), kb * BK, q.it.row0);
+          ++items;
+        }
         for (int kb = q.kb; kb < q.kb_end(); ++kb) {
           if (!mbar_wait(empty(st), ph, ab)) {
             ok = false;
             break;
           }
-          if (rank == 0) mbar_arrive_expect_tx(full(st), 2 * STAGE_BYTES);
+          if (rank == 0) mbar_arrive_expect_tx(full(st), 2 * SLOT);
           const uint32_t bar = map_rank(full(st), 0);
           const int seg = kb >= p.s.seg_kb;
           const int k = (kb - (seg ? p.s.seg_kb : 0)) * BK;
-          const uint32_t sa = sb + (uint32_t)st * STAGE_BYTES, sB = sa + HALF_BYTES;
-          if (A_MN) {
+          const uint32_t sa = ring + (uint32_t)st * SLOT, sB = KEEP_A ? sa : sa + HALF_BYTES;
+          if (KEEP_A) {
+          } else if (A_MN) {
 #pragma unroll
             for (int g = 0; g < BM / 64; ++g) tma_load_pair(sa + g * GROUP_BYTES, &p.ta[seg], bar, q.it.row0 + 64 * g, k);
           } else {
@@ -305,24 +359,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
             tma_load_pair(sB, &p.tb[seg], bar, k, q.nt * BN + rank * (BN / 2));
           }
           ++issued;
-          if (++st == STAGES) st = 0, ph ^= 1;
+          if (++st == stages) st = 0, ph ^= 1;
         }
       }
       // Never leave a copy in flight into shared memory: the even CTA's barriers count the
       // copies of both, and the odd CTA stays until the even one comes to the final barrier.
       if (rank == 0) {
-        for (int n = 0; n < min(issued, STAGES); ++n) {
+        if (KEEP_A && items > 0) drain_wait(a_full, (items - 1) & 1);
+        for (int n = 0; n < min(issued, stages); ++n) {
           const int last = issued - 1 - n;
-          drain_wait(full(last % STAGES), (last / STAGES) & 1);
+          drain_wait(full(last % stages), (last / stages) & 1);
         }
       }
     }
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMA issuer (even CTA)
     if (rank == 0 && lane == 0) {
-      int st = 0, ph = 0, t = 0;
+      int st = 0, ph = 0, t = 0, items = 0;
       bool ok = true;
-      for (Steps q(walk, p.s, pair, pairs, rank); ok && q.valid(); q.next(), ++t) {
+      for (Steps q(walk, p.s, pair, rank); ok && q.valid(); q.next(), ++t) {
+        if (KEEP_A && q.item_first()) {
+          if (!mbar_wait(a_full, items & 1, ab)) break;
+          ++items;
+        }
         if (!mbar_wait(acc_empty(t & 1), ((t >> 1) & 1) ^ 1, ab)) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(t & 1) * BN;
@@ -332,15 +391,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
             break;
           }
           tc_fence_after();
-          const uint32_t sa = sb + (uint32_t)st * STAGE_BYTES;
-          const uint32_t da = sw128_desc(sa, A_MN ? GROUP_BYTES : 0), db = sw128_desc(sa + HALF_BYTES, B_MN ? GROUP_BYTES : 0);
+          const uint32_t slot = ring + (uint32_t)st * SLOT;
+          const uint32_t da = sw128_desc(KEEP_A ? sb + (uint32_t)kb * HALF_BYTES : slot, A_MN ? GROUP_BYTES : 0);
+          const uint32_t db = sw128_desc(KEEP_A ? slot : slot + HALF_BYTES, B_MN ? GROUP_BYTES : 0);
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk)  // 16 K: 32 bytes of a K-major row, 16 rows (2048 bytes) MN-major
             mma_pair(d, da + kk * (A_MN ? 128 : 2), db + kk * (B_MN ? 128 : 2), p.idesc, kb > q.kb || kk > 0);
           commit_pair(empty(st));
-          if (++st == STAGES) st = 0, ph ^= 1;
+          if (++st == stages) st = 0, ph ^= 1;
         }
         if (ok) commit_pair(acc_full(t & 1));
+        if (KEEP_A && ok && q.item_last()) commit_pair(a_empty);
       }
       commit_pair(done);
       drain_wait(done, 0);  // no MMA may still be writing TMEM, or reading either CTA's tiles, at teardown
@@ -348,10 +409,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
   } else {
     // -------------------------------------------------------------- epilogue
     const EpiWarp w{warp & 3, (warp - 2) >> 2, lane,
-                    sb + (uint32_t)(STAGES * STAGE_BYTES + (warp - 2) * Epi::BOXES * Epi::BOX_BYTES), warp_bar(warp - 2)};
+                    ring + (uint32_t)(stages * SLOT + (warp - 2) * Epi::BOXES * Epi::BOX_BYTES), warp_bar(warp - 2)};
     Epi epi(ep, w, ab);
     int t = 0;
-    for (Steps q(walk, p.s, pair, pairs, rank); q.valid(); q.next(), ++t) {
+    for (Steps q(walk, p.s, pair, rank); q.valid(); q.next(), ++t) {
       epi.prepare(q);
       if (!warp_wait(acc_full(t & 1), (t >> 1) & 1, ab)) break;
       tc_fence_after();
@@ -668,6 +729,8 @@ int sm_count();  // of the current device
 // least 8 K blocks (512 of K) each, since shorter ones cost more in partial sums than
 // they gain.
 int plan_splits(int64_t tiles, int64_t kb);
+// Pairs of SMs that a launch of `items` items takes.
+inline int pairs_of(int64_t items) { return (int)std::min<int64_t>(items, sm_count() / 2); }
 inline int64_t tiles_of(int64_t m, int64_t n) { return ((m + PM - 1) / PM) * ((n + BN - 1) / BN); }
 
 // Sums the splits' fp32 partials [splits][rows_total][ldp] in split order (bitwise
@@ -725,22 +788,33 @@ inline Sched plain_sched(int64_t m, int64_t n, int64_t kb, int splits) {
   return s;
 }
 
-template <bool A_MN, bool B_MN, bool DUAL_B, class Epi>
-int launch(const char* what, const Args& a, const typename Epi::Params& ep, cudaStream_t st) {
-  const int64_t items = (int64_t)a.s.tiles_m * a.s.strips * a.s.splits;
+// Runs where all of B (n rows of k elements) stays in L2 beside what streams through it.
+inline void runs_if_resident(Sched* s, int64_t n, int64_t k) { s->runs = n * k * 2 <= ((int64_t)48 << 20); }
+
+template <bool A_MN, bool B_MN, bool DUAL_B, bool KEEP_A, class Epi>
+int launch_kernel(const char* what, Args a, const typename Epi::Params& ep, cudaStream_t st) {
+  const int64_t items = (int64_t)a.s.tiles_m * (a.s.runs ? a.s.tiles_n : a.s.strips) * a.s.splits;
   if (items <= 0) return PNFT_OK;
   if (items > (1 << 30)) return fail(PNFT_EUNSUPPORTED, "%s: too many tiles", what);
-  auto* k = gemm_kernel<A_MN, B_MN, DUAL_B, Epi>;
-  constexpr int smem = smem_bytes<Epi>();
+  auto* k = gemm_kernel<A_MN, B_MN, DUAL_B, KEEP_A, Epi>;
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel has its shared memory
   const uint64_t bit = 1ull << (current_device() & 63);
   if (!(ready.load(std::memory_order_acquire) & bit)) {
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-      return check_launch(what, 0);
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return check_launch(what, 0);
     ready.fetch_or(bit, std::memory_order_release);
   }
-  k<<<(unsigned)(2 * std::min<int64_t>(items, sm_count() / 2)), 32 * (2 + Epi::WARPS), smem, st>>>(a, ep);
+  a.stages = stages<Epi>(KEEP_A, a.s.kb);
+  k<<<(unsigned)(2 * pairs_of(items)), 32 * (2 + Epi::WARPS), SMEM, st>>>(a, ep);
   return check_launch(what, 1);
+}
+template <bool A_MN, bool B_MN, bool DUAL_B, class Epi>
+int launch(const char* what, const Args& a, const typename Epi::Params& ep, cudaStream_t st) {
+  if constexpr (!A_MN) {
+    // rows of A are kept where that leaves the ring at least four stages and an item has several tiles
+    if ((a.s.runs || a.s.tiles_per_strip > 1) && a.s.splits == 1 && a.s.chunk >= a.s.kb && stages<Epi>(true, a.s.kb) >= 4)
+      return launch_kernel<A_MN, B_MN, DUAL_B, true, Epi>(what, a, ep, st);
+  }
+  return launch_kernel<A_MN, B_MN, DUAL_B, false, Epi>(what, a, ep, st);
 }
 
 // C = A B^T with the plain epilogue; K in chunks of 2048 for an fp32 C (see StoreEpi).
@@ -752,9 +826,9 @@ int launch_store(const char* what, Args a, const StoreEpi<false>::Params& ep, cu
     typename StoreEpi<true>::Params e;
     static_assert(sizeof(e) == sizeof(ep), "same parameters");
     memcpy(&e, &ep, sizeof(e));
-    return launch<A_MN, B_MN, false, StoreEpi<true>>(what, a, e, st);
+    return launch_kernel<A_MN, B_MN, false, false, StoreEpi<true>>(what, a, e, st);
   }
-  return launch<A_MN, B_MN, false, StoreEpi<false>>(what, a, ep, st);
+  return launch_kernel<A_MN, B_MN, false, false, StoreEpi<false>>(what, a, ep, st);
 }
 
 // An operand that TMA can read: 16-byte base, row stride a multiple of 8 elements

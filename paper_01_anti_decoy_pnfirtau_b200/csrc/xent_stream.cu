@@ -201,12 +201,11 @@ __global__ void __launch_bounds__(CT) xent_compact_kernel(CompactArgs p) {
 struct LseEpi {
   static constexpr int WARPS = 16, BOXES = 0, BOX_BYTES = 0;
   struct Params {
-    float *part_m, *part_s;  // [strips * 4][Mp]
+    float *part_m, *part_s;  // [row tile][slot][quarter][256]
     float* zt;
     const int32_t* tgt;
     const int32_t* live;
-    int64_t Mp;
-    int V, strip_tiles;
+    int V;
   };
   const Params& p;
   EpiWarp w;
@@ -262,7 +261,7 @@ struct LseEpi {
       m = nm;
     }
     if (q.item_last() && row < live) {
-      const int64_t at = (int64_t)(q.it.nt0 / p.strip_tiles * 4 + w.slice) * p.Mp + row;
+      const int64_t at = (((int64_t)q.it.mt * q.walk.slots + q.it.slot) * 4 + w.slice) * PM + row % PM;
       p.part_m[at] = m;
       p.part_s[at] = s;
     }
@@ -277,8 +276,7 @@ struct ReduceArgs {
   float* row_loss;  // [M], or NULL
   float* loss;      // scalar, or NULL
   double* block_sum;
-  int64_t Mp;
-  int parts, mean;
+  int runs, tiles_n, slots, pairs, mean;
 };
 // A block takes ROWS rows, 256 / ROWS threads each: many threads per row when there are
 // few rows, which then have many strips.
@@ -291,10 +289,20 @@ __global__ void __launch_bounds__(256) xent_reduce_kernel(ReduceArgs p) {
   const int n = p.s.counts[0];
   const int r = threadIdx.x % ROWS, lane = threadIdx.x / ROWS;
   const int64_t i = (int64_t)blockIdx.x * ROWS + r;
+  // the pairs of the row's tile: one per strip, or one per run that the tile lies in
+  const int tiles_m = (n + PM - 1) / PM;
+  const int64_t mt = i / PM, total = (int64_t)tiles_m * p.tiles_n;
+  int slots = p.slots, parts = 4 * slots;
+  if (p.runs && i < n) {
+    const int pairs = Walk::run_pairs(total, p.pairs);
+    slots = Walk::run_slots(tiles_m, pairs);
+    parts = 4 * (run_owner(total, (mt + 1) * p.tiles_n - 1, pairs) - run_owner(total, mt * p.tiles_n, pairs) + 1);
+  }
+  const float *pm = p.part_m + mt * slots * 4 * PM + i % PM, *ps = p.part_s + mt * slots * 4 * PM + i % PM;
   float m = kLow;
   if (i < n) {
 #pragma unroll 4
-    for (int k = lane; k < p.parts; k += LANES) m = fmaxf(m, p.part_m[k * p.Mp + i]);
+    for (int k = lane; k < parts; k += LANES) m = fmaxf(m, pm[k * PM]);
   }
   top[threadIdx.x] = m;
   __syncthreads();
@@ -306,7 +314,7 @@ __global__ void __launch_bounds__(256) xent_reduce_kernel(ReduceArgs p) {
   float s = 0.f;
   if (i < n) {
 #pragma unroll 4
-    for (int k = lane; k < p.parts; k += LANES) s += p.part_s[k * p.Mp + i] * ex2(p.part_m[k * p.Mp + i] - m);
+    for (int k = lane; k < parts; k += LANES) s += ps[k * PM] * ex2(pm[k * PM] - m);
   }
   sum[threadIdx.x] = s;
   __syncthreads();
@@ -629,15 +637,21 @@ State state_of(const SavedLayout& l, void* saved) {
 }
 
 struct FwdLayout {
-  int per, strips;
+  int runs, pairs, tiles_n, per, strips;
   size_t zt, part_m, part_s, sums, total;
 };
-FwdLayout fwd_layout(int64_t M, int64_t V) {
-  const int64_t Mp = up(M, BM);
+FwdLayout fwd_layout(int64_t M, int64_t V, int64_t D) {
+  const int64_t Mp = up(M, BM), tiles_m = (M + PM - 1) / PM;
   FwdLayout l;
-  const int tiles_n = (int)((V + BN - 1) / BN);
-  l.per = strip_tiles((M + PM - 1) / PM, tiles_n);
-  l.strips = (tiles_n + l.per - 1) / l.per;
+  Sched s;
+  runs_if_resident(&s, V, D);
+  l.runs = s.runs;
+  l.tiles_n = (int)((V + BN - 1) / BN);
+  l.pairs = pairs_of(tiles_m * l.tiles_n);
+  l.per = l.runs ? 1 : strip_tiles(tiles_m, l.tiles_n);
+  l.strips = (l.tiles_n + l.per - 1) / l.per;
+  // in runs a row tile lies in at most pairs / row tiles + 2, for any number of rows that count
+  const size_t parts = 4 * PM * (size_t)(l.runs ? l.pairs + 2 * tiles_m : tiles_m * l.strips);
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t r = at;
@@ -645,8 +659,8 @@ FwdLayout fwd_layout(int64_t M, int64_t V) {
     return r;
   };
   l.zt = take(4 * Mp);
-  l.part_m = take(4 * Mp * 4 * l.strips);
-  l.part_s = take(4 * Mp * 4 * l.strips);
+  l.part_m = take(4 * parts);
+  l.part_s = take(4 * parts);
   l.sums = take(8 * std::max<int64_t>(64, (M + 31) / 32));
   l.total = at;
   return l;
@@ -715,7 +729,7 @@ static int skinny_blocks(int64_t V) {
 extern "C" size_t pnft_stream_xent_fwd_workspace_size(int64_t M, int64_t V, int64_t D, int save) {
   if (M <= 0 || V <= 0 || D <= 0) return 0;
   if (!save && M <= SKINNY_ROWS) return sizeof(float) * SKINNY_ROWS * (2 * (size_t)skinny_blocks(V) + 1);
-  return fwd_layout(M, V).total + (save ? 0 : saved_layout(M, D).total);
+  return fwd_layout(M, V, D).total + (save ? 0 : saved_layout(M, D).total);
 }
 
 extern "C" size_t pnft_stream_xent_bwd_workspace_size(int64_t M, int64_t V, int64_t D) {
@@ -754,7 +768,7 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
   if (!tma_rows_ok(w, ldw, D))
     return fail(PNFT_EUNSUPPORTED, "stream_xent_fwd: weight rows must be 16-byte aligned (strides multiples of 8)");
   if (!device_is_sm100()) return fail(PNFT_EUNSUPPORTED, "stream_xent_fwd: needs an sm_100 device");
-  const FwdLayout l = fwd_layout(M, V);
+  const FwdLayout l = fwd_layout(M, V, D);
   const SavedLayout sl = saved_layout(M, D);
   if (!saved) saved = ws + l.total;
   const int64_t Mp = up(M, BM), ldc = sl.ldc;
@@ -781,6 +795,7 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
   if (!rc) rc = map_kmajor(&a.tb[0], w, D, V, ldw);
   if (rc) return rc;
   a.s = plain_sched(M, V, (D + BK - 1) / BK, 1);
+  a.s.runs = l.runs;
   a.s.strips = l.strips;
   a.s.tiles_per_strip = l.per;
   a.s.group_m = a.s.tiles_m;
@@ -789,10 +804,11 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
   a.idesc = idesc(dtype, false, false);
   a.status = status;
   LseEpi::Params ep{reinterpret_cast<float*>(ws + l.part_m), reinterpret_cast<float*>(ws + l.part_s), c.zt, c.s.tgt,
-                    c.s.counts, Mp, (int)V, l.per};
+                    c.s.counts, (int)V};
   rc = launch<false, false, false, LseEpi>("stream_xent forward", a, ep, st);
   if (rc) return rc;
-  ReduceArgs r{ep.part_m, ep.part_s, c.zt, c.s, row_loss, loss, reinterpret_cast<double*>(ws + l.sums), Mp, 4 * l.strips, mean};
+  ReduceArgs r{ep.part_m, ep.part_s, c.zt, c.s, row_loss, loss, reinterpret_cast<double*>(ws + l.sums),
+               l.runs, l.tiles_n, l.strips, l.pairs, mean};
   if (M > 64)
     xent_reduce_kernel<32><<<(unsigned)((M + 31) / 32), 256, 0, st>>>(r);
   else
@@ -842,6 +858,7 @@ extern "C" int pnft_stream_xent_bwd(const void* w, int64_t ldw, const void* save
     if (!rc) rc = map_kmajor(&a.tb[0], wp, D, n, ldw);
     if (rc) break;
     a.s = plain_sched(M, n, (D + BK - 1) / BK, 1);
+    runs_if_resident(&a.s, n, D);
     a.s.live = s.counts;
     a.s.live_m = 1;
     a.idesc = idesc(dtype, false, false);
