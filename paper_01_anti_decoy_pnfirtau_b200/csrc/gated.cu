@@ -82,6 +82,7 @@ __device__ __forceinline__ void add_bias(float (&v)[W], const void* bias, int dt
 enum { FWD, KEEP, BWD };
 template <int MODE, int ACT>
 struct GatedEpi {
+  static constexpr bool PING_PONG = false;
   static constexpr int WARPS = 16, W = 32, ROW_BYTES = 2 * W;
   static constexpr int OUTS = MODE == KEEP ? 3 : 2;                                       // boxes for results
   static constexpr int BOXES = OUTS + (MODE == BWD), BOX_BYTES = 32 * ROW_BYTES;          // and one for dh
@@ -98,9 +99,10 @@ struct GatedEpi {
   Boxes<OUTS, ROW_BYTES> boxes;
   int phase, issued;
   __device__ GatedEpi(const Params& p_, const EpiWarp& w_, const Abort& ab_)
-      : p(p_), w(w_), ab(ab_), boxes(EpiWarp{w_.quad, w_.slice, w_.lane, w_.smem + (MODE == BWD ? BOX_BYTES : 0), w_.bar}),
+      : p(p_), w(w_), ab(ab_), boxes(EpiWarp{w_.quad, w_.group, w_.slice, w_.lane, w_.smem + (MODE == BWD ? BOX_BYTES : 0), w_.bar}),
         phase(0), issued(0) {}
   __device__ int col0(const Steps& q) const { return q.nt * (BN / 2) + w.slice * W; }
+  __device__ void end(const Steps&) {}
   __device__ void load_dh(const Steps& q) {
     if (w.lane == 0) {
       mbar_arrive_expect_tx(w.bar, BOX_BYTES);

@@ -238,17 +238,21 @@ struct Steps {
   }
 };
 
-// What an epilogue warp has: its TMEM lane quadrant, its slice of the columns (of 2 or 4),
-// its boxes in shared memory and a barrier for loads into them.
+// What an epilogue warp has: its group (ping-pong epilogues have two, which take the
+// accumulators in turn), its TMEM lane quadrant, its slice of the columns (of 2 or 4), its
+// boxes in shared memory and a barrier for loads into them.
 struct EpiWarp {
-  int quad, slice, lane;
+  int quad, group, slice, lane;
   uint32_t smem, bar;
   __device__ int row() const { return 32 * quad + lane; }
 };
 
 // Epi: WARPS (8, or 16 where the arithmetic per element is what takes the time: a warp's
 // chain of TMEM load, exponentials and stores has long latencies, and 16 warps of at most 96
-// registers hide them twice as well), BOXES of BOX_BYTES per warp; tile(steps, acc, release) for every accumulator
+// registers hide them twice as well), PING_PONG (the warps form two groups, one per
+// accumulator: while one group is at its loads, the other keeps the arithmetic pipes busy,
+// where all warps in step would use one after the other), BOXES of BOX_BYTES per warp;
+// prepare(steps) and end(steps) for every accumulator, tile(steps, acc, release) between them for those of the warp's group
 // (acc: its TMEM address with the warp's lanes; release() hands it back once its last
 // column is in registers), done() at the end.
 // DUAL_B: columns 0-127 of a tile come from tb[0] and 128-255 from tb[1], both at row
@@ -300,7 +304,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(acc_full(s), 1);
-      mbar_init(acc_empty(s), 2 * EPI_WARPS);  // the even CTA's: the epilogue warps of both
+      mbar_init(acc_empty(s), Epi::PING_PONG ? EPI_WARPS : 2 * EPI_WARPS);  // the even CTA's: the epilogue warps of both
     }
     mbar_init(done, 1);
     mbar_init(a_full, 1);
@@ -408,12 +412,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
     }
   } else {
     // -------------------------------------------------------------- epilogue
-    const EpiWarp w{warp & 3, (warp - 2) >> 2, lane,
+    const int part = (warp - 2) >> 2;
+    const EpiWarp w{warp & 3, Epi::PING_PONG ? part & 1 : 0, Epi::PING_PONG ? part >> 1 : part, lane,
                     ring + (uint32_t)(stages * SLOT + (warp - 2) * Epi::BOXES * Epi::BOX_BYTES), warp_bar(warp - 2)};
     Epi epi(ep, w, ab);
     int t = 0;
     for (Steps q(walk, p.s, pair, rank); q.valid(); q.next(), ++t) {
       epi.prepare(q);
+      if (Epi::PING_PONG && (t & 1) != w.group) {
+        epi.end(q);
+        continue;
+      }
       if (!warp_wait(acc_full(t & 1), (t >> 1) & 1, ab)) break;
       tc_fence_after();
       const uint32_t release = map_rank(acc_empty(t & 1), 0);
@@ -422,6 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(release);
       });
+      epi.end(q);
     }
     epi.done();
   }
@@ -639,6 +649,7 @@ struct Out {
 template <bool PROMOTE>
 struct StoreEpi {
   static constexpr int WARPS = 8, BOXES = 2, BOX_BYTES = 4096;
+  static constexpr bool PING_PONG = false;
   struct Params {
     Out c[2];
     int row_split;
@@ -657,6 +668,7 @@ struct StoreEpi {
     for (float& v : sum) v = 0.f;
   }
   __device__ void prepare(const Steps&) {}
+  __device__ void end(const Steps&) {}
   __device__ void done() { boxes.finish(); }
   __device__ __forceinline__ void out32(const Steps& q, int c, float (&v)[32], uint32_t& box) {
     int row = q.it.row0 + 32 * w.quad;

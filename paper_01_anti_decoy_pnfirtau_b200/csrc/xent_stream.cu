@@ -58,43 +58,14 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
-// 2^x of two values. The special-function unit gives 16 exponentials per clock and SM, and a
-// tile of 256 columns from K = 256 leaves it exactly as many clocks as the tensor core needs:
-// so a part of the exponentials runs on the FMA pipe (POLY): x = n + f with |f| <= 1/2, and
-// 2^f by a polynomial of degree 5, fitted to a relative error of 7.5e-8, or of degree 4 to
-// 2.6e-6 where the result is rounded to 16 bits. x >= -126 there; NaN stays NaN.
-template <bool POLY, int DEGREE>
+// 2^x of two values, both on the special-function unit. At K = 256 that unit (16 per clock
+// and SM) is as busy as the tensor core, yet moving every third or second exponential to a
+// polynomial on the FMA pipe made the forward slower (16352 x 33278 x 256: 217 us without,
+// 227 and 237 with): the instructions cost more clock than the unit does.
 __device__ __forceinline__ f32x2 exp2_pair(f32x2 x) {
   const float2 v = unpack(x);
-  if (!POLY) return pack(ex2(v.x), ex2(v.y));
-  x = pack(max_nan(v.x, -126.f), max_nan(v.y, -126.f));
-  constexpr float kRound = 12582912.f + 127.f;  // 1.5 * 2^23: the sum's low bits are the rounded x, biased as an exponent
-  const f32x2 y = add2(x, pack(kRound, kRound));
-  const f32x2 f = fma2(add2(y, pack(-kRound, -kRound)), pack(-1.f, -1.f), x);
-  f32x2 q;
-  if (DEGREE == 5) {
-    q = fma2(f, pack(0.00132765f, 0.00132765f), pack(0.00967554f, 0.00967554f));
-    q = fma2(q, f, pack(0.05550713f, 0.05550713f));
-    q = fma2(q, f, pack(0.2402212f, 0.2402212f));
-    q = fma2(q, f, pack(0.69314697f, 0.69314697f));
-    q = fma2(q, f, pack(1.00000007f, 1.00000007f));
-  } else {
-    q = fma2(f, pack(0.0095701f, 0.0095701f), pack(0.05591786f, 0.05591786f));
-    q = fma2(q, f, pack(0.24024745f, 0.24024745f));
-    q = fma2(q, f, pack(0.69312181f, 0.69312181f));
-    q = fma2(q, f, pack(0.99999926f, 0.99999926f));
-  }
-  const float2 e = unpack(y);
-  return mul2(q, pack(__uint_as_float(__float_as_uint(e.x) << 23), __uint_as_float(__float_as_uint(e.y) << 23)));
+  return pack(ex2(v.x), ex2(v.y));
 }
-// Pair i of 16 (32 columns): every POLY_EVERY-th goes to the FMA pipe.
-constexpr int POLY_EVERY = 3;
 
 // Device state of one call, in the caller's buffers (rows are compacted rows).
 struct State {
@@ -196,12 +167,13 @@ __global__ void __launch_bounds__(CT) xent_compact_kernel(CompactArgs p) {
 }
 
 // ------------------------------------------------------------------ forward epilogue
-// Per row and quarter of the columns: running maximum (times log2 e) and sum of
-// 2^(z log2 e - max), both fp32, over the tiles of a strip.
+// Per row, half of the columns and group of warps: running maximum (times log2 e) and sum of
+// 2^(z log2 e - max), both fp32, over the group's tiles of an item.
 struct LseEpi {
   static constexpr int WARPS = 16, BOXES = 0, BOX_BYTES = 0;
+  static constexpr bool PING_PONG = true;
   struct Params {
-    float *part_m, *part_s;  // [row tile][slot][quarter][256]
+    float *part_m, *part_s;  // [row tile][slot][group and half][256]
     float* zt;
     const int32_t* tgt;
     const int32_t* live;
@@ -219,51 +191,55 @@ struct LseEpi {
     tgt = row < live ? p.tgt[row] : -1;
   }
   __device__ void done() {}
+  __device__ void end(const Steps& q) {  // also of a group that had no tile of the item: maximum and sum of nothing
+    const int row = q.it.row0 + w.row();
+    if (!q.item_last() || row >= live) return;
+    const int64_t at = (((int64_t)q.it.mt * q.walk.slots + q.it.slot) * 4 + 2 * w.group + w.slice) * PM + row % PM;
+    p.part_m[at] = m;
+    p.part_s[at] = s;
+  }
   template <class Release>
   __device__ __forceinline__ void tile(const Steps& q, uint32_t acc, Release release) {
-    const int row = q.it.row0 + w.row();
+    constexpr int W = 64;
 #pragma unroll 1
-    for (int c = w.slice * (BN / 4); c < (w.slice + 1) * (BN / 4); c += 32) {
-      float z[32];
-      acc_load32(acc + c, false, z);
-      if (c + 32 == (w.slice + 1) * (BN / 4)) release();
-      const int col = q.nt * BN + c, n = p.V - col;
-      if (n < 32) {
+    for (int c = w.slice * (BN / 2); c < (w.slice + 1) * (BN / 2); c += W) {
+      uint32_t z[2][W / 2];
+      tmem_load32x2(acc + c, z[0], acc + c + W / 2, z[1]);
+      if (c + W == (w.slice + 1) * (BN / 2)) release();
+      const int row = q.it.row0 + w.row(), col = q.nt * BN + c, n = p.V - col;
+      auto at = [&](int i) { return __uint_as_float(z[i / (W / 2)][i % (W / 2)]); };
+      if (n < W) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i >= n) z[i] = -INFINITY;
+        for (int i = 0; i < W; ++i)
+          if (i >= n) z[i / (W / 2)][i % (W / 2)] = 0xff800000u;  // -infinity
       }
       const int tc = tgt - col;
-      if ((unsigned)tc < 32u) {
+      if ((unsigned)tc < (unsigned)W) {
         float v = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v = i == tc ? z[i] : v;
+        for (int i = 0; i < W; ++i) v = i == tc ? at(i) : v;
         p.zt[row] = v;
       }
-      float a = max3(z[0], z[1], z[2]), b = max3(z[3], z[4], z[5]);
+      float top[4];
 #pragma unroll
-      for (int i = 6; i < 30; i += 4) a = max3(a, z[i], z[i + 1]), b = max3(b, z[i + 2], z[i + 3]);
-      a = max3(a, z[30], z[31]);
-      const float nm = max3(m, a * kLog2e, b * kLog2e);
-      const f32x2 scale = pack(kLog2e, kLog2e), minus = pack(-nm, -nm);
-      f32x2 s0 = 0, s1 = 0;
+      for (int k = 0; k < 4; ++k) top[k] = max3(at(k), at(k + 4), at(k + 8));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const f32x2 x = fma2(pack(z[2 * i], z[2 * i + 1]), scale, minus);
-        const f32x2 e = i % POLY_EVERY == 0 ? exp2_pair<true, 5>(x) : exp2_pair<false, 5>(x);
-        if (i & 1)
-          s1 = add2(s1, e);
-        else
-          s0 = add2(s0, e);
+      for (int i = 12; i < W - 4; i += 8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top[k] = max3(top[k], at(i + k), at(i + k + 4));
       }
-      const float2 sum = unpack(add2(s0, s1));
-      s = fmaf(s, ex2(m - nm), sum.x + sum.y);
+      top[0] = max3(top[0], at(W - 4), at(W - 3)), top[1] = max3(top[1], at(W - 2), at(W - 1));
+      const float nm = fmaxf(m, kLog2e * max3(top[0], top[1], fmaxf(top[2], top[3])));
+      const f32x2 scale = pack(kLog2e, kLog2e), minus = pack(-nm, -nm);
+      f32x2 sum[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < W / 2; ++i) {
+        const f32x2 x = fma2(pack(at(2 * i), at(2 * i + 1)), scale, minus);
+        sum[i & 3] = add2(sum[i & 3], exp2_pair(x));
+      }
+      const float2 t = unpack(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+      s = fmaf(s, ex2(m - nm), t.x + t.y);
       m = nm;
-    }
-    if (q.item_last() && row < live) {
-      const int64_t at = (((int64_t)q.it.mt * q.walk.slots + q.it.slot) * 4 + w.slice) * PM + row % PM;
-      p.part_m[at] = m;
-      p.part_s[at] = s;
     }
   }
 };
@@ -506,6 +482,7 @@ __global__ void __launch_bounds__(1024) xent_scale_kernel(ScaleArgs p) {
 // past the vocabulary (the two GEMMs run over whole 64-deep blocks of both).
 struct DzEpi {
   static constexpr int WARPS = 16, BOXES = 1, BOX_BYTES = 4096;
+  static constexpr bool PING_PONG = false;
   struct Params {
     Out dz;
     const float *lse2, *rs;
@@ -525,6 +502,7 @@ struct DzEpi {
     rs = row < live ? p.rs[row] : 0.f;
     tgt = row < live ? p.tgt[row] - p.v0 : -1;
   }
+  __device__ void end(const Steps&) {}
   __device__ void done() { boxes.finish(); }
   template <class Release>
   __device__ __forceinline__ void tile(const Steps& q, uint32_t acc, Release release) {
@@ -540,7 +518,7 @@ struct DzEpi {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const f32x2 x = fma2(pack(z[2 * i], z[2 * i + 1]), scale, minus);
-        const float2 v = unpack(mul2(i % POLY_EVERY == 0 ? exp2_pair<true, 4>(x) : exp2_pair<false, 4>(x), factor));
+        const float2 v = unpack(mul2(exp2_pair(x), factor));
         z[2 * i] = v.x, z[2 * i + 1] = v.y;
       }
       if ((unsigned)tc < 32u) {
