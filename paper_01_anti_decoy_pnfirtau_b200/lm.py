@@ -14,6 +14,12 @@ split-K tcgen05 GEMM, and the head's loss and logit gradient in one pass over
 the logits. With ``fused_step_ops=False`` the blocks are nn.LayerNorm, nn.Linear,
 nn.GELU and F.cross_entropy. Parameters and state_dict keys are the same either
 way.
+
+Options beyond the reference's model: a gated feed-forward (``LMConfig.ffn``
+``"swiglu"`` or ``"geglu"``), and two that make a training step keep less
+(lm_lean_ops): ``streamed_loss`` (the loss without the head's logits) and
+``checkpoint_8bit`` (the inputs of the attention's projections and of the gated
+feed-forward's layers kept in 8 bits for the backward).
 """
 from __future__ import annotations
 
@@ -23,6 +29,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .lm_lean_ops import gated_mlp, streamed_cross_entropy
 from .lm_ops import Bf16Casts, LayerNorm, Linear, add_layer_norm, head_cross_entropy, mlp_gelu
 from .pnfirtau_attention import PnFirConfig, PnFirTauFlashMHA, PnFirTauMHA, PnFirTauTritonMHA
 
@@ -42,17 +49,43 @@ class LMConfig:
     silence_gamma: float | None = 0.5
     tau_init: float = 0.0
     fir_k: int = 7
+    ffn: str = "gelu"  # "gelu" (the reference's), "swiglu" or "geglu"
+
+
+_GATES = {"swiglu": "silu", "geglu": "gelu"}
+
+
+class GatedFFN(nn.Module):
+    """``down(act(gate(x)) * up(x))`` with biases, as the reference's feed-forward has;
+    ``fused``: the product on this library's kernel (``gated_mlp``), else plain modules."""
+
+    def __init__(self, d_model: int, d_ff: int, kind: str, dropout: float = 0.0, fused: bool = True):
+        super().__init__()
+        if kind not in _GATES:
+            raise ValueError(f"GatedFFN: kind {kind!r} (one of {sorted(_GATES)})")
+        self.act, self.fused, self.checkpoint_8bit = _GATES[kind], fused, False
+        self.gate, self.up = nn.Linear(d_model, d_ff), nn.Linear(d_model, d_ff)
+        self.down = (Linear if fused else nn.Linear)(d_ff, d_model)
+        self.drop = nn.Dropout(dropout)
+
+    def forward(self, x: torch.Tensor, casts: Bf16Casts | None = None) -> torch.Tensor:
+        if self.fused:
+            y = gated_mlp(x, self.gate, self.up, self.down, self.act, checkpoint_8bit=self.checkpoint_8bit, casts=casts)
+        else:
+            y = self.down((F.silu if self.act == "silu" else F.gelu)(self.gate(x)) * self.up(x))
+        return self.drop(y)
 
 
 class Block(nn.Module):
     """exp4_wikitext2_lm.py:183-200."""
 
-    def __init__(self, d_model: int, attn: nn.Module, dropout: float, d_ff: int, norm=nn.LayerNorm):
+    def __init__(self, d_model: int, attn: nn.Module, dropout: float, d_ff: int, norm=nn.LayerNorm,
+                 ffn: nn.Module | None = None):
         super().__init__()
         self.ln1 = norm(d_model)
         self.attn = attn
         self.ln2 = norm(d_model)
-        self.ffn = nn.Sequential(nn.Linear(d_model, d_ff), nn.GELU(), nn.Linear(d_ff, d_model), nn.Dropout(dropout))
+        self.ffn = ffn if ffn is not None else nn.Sequential(nn.Linear(d_model, d_ff), nn.GELU(), nn.Linear(d_ff, d_model), nn.Dropout(dropout))
         self.drop = nn.Dropout(dropout)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
@@ -61,13 +94,24 @@ class Block(nn.Module):
 
 
 class PnFirLM(nn.Module):
-    """exp4_wikitext2_lm.py:203-247 (``WikiLM``) with a pn_fir_tau variant."""
+    """exp4_wikitext2_lm.py:203-247 (``WikiLM``) with a pn_fir_tau variant.
+    ``streamed_loss`` and ``checkpoint_8bit`` (module docstring) need ``fused_step_ops``
+    and a bf16 computation; ``checkpoint_8bit`` covers the attention's projections and,
+    where ``cfg.ffn`` is gated, the feed-forward (``mlp_gelu`` keeps its 16-bit
+    activations)."""
 
-    def __init__(self, cfg: LMConfig = LMConfig(), variant: str = "pn_fir_tau_flash", fused_step_ops: bool = True):
+    def __init__(self, cfg: LMConfig = LMConfig(), variant: str = "pn_fir_tau_flash", fused_step_ops: bool = True,
+                 streamed_loss: bool = False, checkpoint_8bit: bool = False):
         super().__init__()
+        if (streamed_loss or checkpoint_8bit) and not fused_step_ops:
+            raise ValueError("PnFirLM: streamed_loss and checkpoint_8bit need fused_step_ops")
+        if cfg.ffn != "gelu" and cfg.ffn not in _GATES:
+            raise ValueError(f"PnFirLM: ffn {cfg.ffn!r} (one of {['gelu', *sorted(_GATES)]})")
         self.cfg = cfg
         self.variant = variant
         self.fused_step_ops = fused_step_ops
+        self.streamed_loss = streamed_loss
+        gated = cfg.ffn in _GATES
         norm = LayerNorm if fused_step_ops else nn.LayerNorm
         self.embed = nn.Embedding(cfg.vocab, cfg.d_model)
         self.pos = nn.Embedding(cfg.max_seq, cfg.d_model)
@@ -76,13 +120,18 @@ class PnFirLM(nn.Module):
                            tau_init=cfg.tau_init, fir_k=cfg.fir_k, dropout=cfg.dropout, causal_mask=True, bias=False)
         cls = _VARIANTS[variant]
         self.blocks = nn.ModuleList(
-            Block(cfg.d_model, cls(acfg), cfg.dropout, cfg.d_ff, norm) for _ in range(cfg.n_layers))
+            Block(cfg.d_model, cls(acfg), cfg.dropout, cfg.d_ff, norm,
+                  GatedFFN(cfg.d_model, cfg.d_ff, cfg.ffn, cfg.dropout, fused_step_ops) if gated else None)
+            for _ in range(cfg.n_layers))
         self.ln_f = norm(cfg.d_model)
         if fused_step_ops:
             # the attention's projections with the library's weight-gradient GEMM (same parameters)
             for blk in self.blocks:
                 for name in ("qkv", "out"):
                     setattr(blk.attn, name, Linear.sharing(getattr(blk.attn, name)))
+                    getattr(blk.attn, name).checkpoint_8bit = checkpoint_8bit
+                if gated:
+                    blk.ffn.checkpoint_8bit = blk.ffn.down.checkpoint_8bit = checkpoint_8bit
         self.head = nn.Linear(cfg.d_model, cfg.vocab, bias=False)
         self.head.weight = self.embed.weight
         self._casts: Bf16Casts | None = None  # bf16 copies of the GEMM parameters (_step_casts)
@@ -95,13 +144,16 @@ class PnFirLM(nn.Module):
         copy of the logits is needed. ``targets`` (``[B, N-1]``, the ids of
         positions 1..N-1): the mean next-token cross-entropy of positions 0..N-2
         instead of logits (one kernel pass over the logits with
-        ``fused_step_ops``, else F.cross_entropy)."""
+        ``fused_step_ops``, no logits at all with ``streamed_loss``, else
+        F.cross_entropy)."""
         B, N = idx.shape
         pos = torch.arange(N, device=idx.device).unsqueeze(0)
         h = self.drop(self.embed(idx) + self.pos(pos))
         casts = self._step_casts(idx.device)
         h = self._trunk_fused(h, casts) if self.fused_step_ops else self._trunk(h)
         if targets is not None:
+            if self.streamed_loss:
+                return streamed_cross_entropy(h[:, :-1], self.head.weight, targets, casts=casts)
             if self.fused_step_ops:
                 return head_cross_entropy(h[:, :-1], self.head.weight, targets, casts=casts)
             logits = self._padded_logits(h)
@@ -125,9 +177,12 @@ class PnFirLM(nn.Module):
             return None
         if self._casts is None:
             lins = [lin for blk in self.blocks for lin in (blk.attn.qkv, blk.attn.out)]
+            gated = [blk.ffn for blk in self.blocks if isinstance(blk.ffn, GatedFFN)]
+            lins += [f.down for f in gated]
             params = [t for lin in lins for t in (lin.weight, lin.bias)]
-            params += [t for blk in self.blocks for t in (blk.ffn[0].weight, blk.ffn[0].bias, blk.ffn[2].weight,
-                                                          blk.ffn[2].bias)]
+            params += [t for f in gated for t in (f.gate.weight, f.up.weight)]
+            params += [t for blk in self.blocks if not isinstance(blk.ffn, GatedFFN)
+                       for t in (blk.ffn[0].weight, blk.ffn[0].bias, blk.ffn[2].weight, blk.ffn[2].bias)]
             params.append(self.head.weight)
             if torch.cuda.is_current_stream_capturing() or any(
                     t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.device != dev)
@@ -150,7 +205,10 @@ class PnFirLM(nn.Module):
             att = blk.drop(blk.attn(a))
             ln2 = blk.ln2
             h, b = add_layer_norm(h, att, ln2.normalized_shape, ln2.weight, ln2.bias, ln2.eps)
-            f = blk.ffn[3](mlp_gelu(b, blk.ffn[0], blk.ffn[2], casts))
+            if isinstance(blk.ffn, GatedFFN):
+                f = blk.ffn(b, casts)
+            else:
+                f = blk.ffn[3](mlp_gelu(b, blk.ffn[0], blk.ffn[2], casts))
             nxt = blocks[i + 1].ln1 if i + 1 < len(blocks) else self.ln_f
             h, a = add_layer_norm(h, f, nxt.normalized_shape, nxt.weight, nxt.bias, nxt.eps)
         return a

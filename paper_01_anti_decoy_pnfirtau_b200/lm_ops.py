@@ -43,6 +43,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
+from .lm_lean_ops import Act8, act8_pack, act8_weight_grad
 from .pnfirtau_ops import _check_pending, _require_cuda, _status_ptr, _stream
 
 _LN_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
@@ -430,13 +431,17 @@ def mlp_gelu(x: torch.Tensor, fc1: nn.Linear, fc2: nn.Linear, casts: "Bf16Casts 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, dt: torch.dtype, pre=None):
+    def forward(ctx, x, weight, bias, dt: torch.dtype, pre=None, in8: bool = False):
         _require_cuda("Linear", x, weight)
         D = x.shape[-1]
         x2 = x.reshape(-1, D).to(dt)
         x2 = x2 if x2.stride(-1) == 1 else x2.contiguous()
         w, b = pre if pre is not None else (weight.to(dt), _cast(bias, dt))  # pre: cast by Bf16Casts
         y = torch.addmm(b, x2, w.t()) if bias is not None else torch.mm(x2, w.t())
+        ctx.act8 = None
+        if in8 and ctx.needs_input_grad[1]:  # only the weight's gradient reads x
+            p = act8_pack(x2)
+            x2, ctx.act8 = p.data, (p.shape, p.dtype)
         ctx.save_for_backward(x2, w)
         ctx.x_shape, ctx.x_dtype = x.shape, x.dtype
         ctx.p_dtypes = (weight.dtype, None if bias is None else bias.dtype)
@@ -445,21 +450,22 @@ class _LinearFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         x2, w = ctx.saved_tensors
-        dt, dev = x2.dtype, x2.device
+        dt, dev = w.dtype, x2.device
         Dout = w.shape[0]
         g2 = _rows(g, Dout, dt, like=dt)
         dx = dw = db = None
         if ctx.needs_input_grad[0]:
             dx = torch.mm(g2, w).to(ctx.x_dtype).view(ctx.x_shape)
         if ctx.needs_input_grad[1]:
-            dw = _weight_grad(g2, x2).to(ctx.p_dtypes[0])
+            dw = act8_weight_grad(g2, Act8(x2, *ctx.act8)) if ctx.act8 is not None else _weight_grad(g2, x2)
+            dw = dw.to(ctx.p_dtypes[0])
         if ctx.needs_input_grad[2]:
             db = torch.empty(Dout, dtype=torch.float32, device=dev)
             ws, nb = _colsum_ws(g2.shape[0], Dout, dev)
             _lib.check(_lib.lib().pnft_colsum(g2.data_ptr(), g2.stride(0), db.data_ptr(), ws.data_ptr(), nb,
                                               g2.shape[0], Dout, _ln_code(dt, "Linear"), _stream(dev)), "pnft_colsum")
             db = db.to(ctx.p_dtypes[1])
-        return dx, dw, db, None, None
+        return dx, dw, db, None, None, None
 
 
 class Linear(nn.Linear):
@@ -469,9 +475,14 @@ class Linear(nn.Linear):
     with the fixed-order column sum. ``Linear.sharing(lin)`` wraps an existing
     layer's parameters without re-initialising anything. ``casts`` (plain
     attribute, default None): a ``Bf16Casts`` whose current bf16 copies of the
-    parameters the bf16 GEMM uses instead of casting them per call."""
+    parameters the bf16 GEMM uses instead of casting them per call.
+    ``checkpoint_8bit`` (plain attribute, default False): the backward keeps the
+    input in 8 bits (``act8_pack``) and takes the weight gradient from that
+    (``act8_weight_grad``); output and input gradient do not change. Needs a bf16
+    computation."""
 
     casts: "Bf16Casts | None" = None
+    checkpoint_8bit: bool = False
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         dt = _autocast_dtype(x)
@@ -479,7 +490,9 @@ class Linear(nn.Linear):
             dt = torch.float32
         c = self.casts
         pre = c.lookup(self.weight, self.bias) if c is not None and dt == torch.bfloat16 else None
-        return _LinearFn.apply(x, self.weight, self.bias, dt, pre)
+        if self.checkpoint_8bit and dt != torch.bfloat16:
+            raise RuntimeError(f"Linear: checkpoint_8bit needs a bfloat16 computation (input or CUDA autocast), got {dt}")
+        return _LinearFn.apply(x, self.weight, self.bias, dt, pre, self.checkpoint_8bit)
 
     @classmethod
     def sharing(cls, lin: nn.Linear) -> "Linear":
