@@ -769,8 +769,8 @@ inline int dtype_size(int dtype) { return dtype == PNFT_DTYPE_F32 ? 4 : 2; }
 inline int make_out(Out* o, void* base, int dtype, int64_t cols, int64_t rows, int64_t ld, int64_t slices = 1,
                     int64_t slice_stride = 0, int row_bytes = 128) {
   memset(o, 0, sizeof(*o));
+  if (!base) return PNFT_OK;  // no rows: nothing is written
   o->base = base, o->ld = ld, o->rows = (int)rows, o->cols = (int)cols;
-  if (!base) return PNFT_OK;
   o->tma = rows16(base, ld, dtype_size(dtype)) && ld < ((int64_t)1 << 37);
   return o->tma ? tma_map_out(&o->map, base, dtype_size(dtype), cols, rows, ld, slices, slice_stride, 32, row_bytes) : PNFT_OK;
 }

@@ -421,18 +421,15 @@ def streamed_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch
     if h.dtype not in _DTYPES or weight.dtype not in _DTYPES:
         raise RuntimeError(f"streamed_cross_entropy: float32, bfloat16 or float16 tensors expected, got {h.dtype} and {weight.dtype}")
     dt = _compute_dtype(h, "streamed_cross_entropy")
-    need = torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad)
     if targets.numel() == 0:  # as F.cross_entropy: nothing, 0, or 0 / 0; gradients of zeros
-        if reduction == "none":
-            return h.float().sum(-1)
-        zero = h.float().sum() + (weight[:0].float().sum() if need else 0.0)
-        return zero if reduction == "sum" else zero * math.nan
+        zero = (h.float().sum(-1) if reduction == "none" else h.float().sum()) + weight[:0].float().sum()
+        return zero * math.nan if reduction == "mean" else zero
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return streamed_cross_entropy(h, weight, targets, ignore_index, reduction=reduction, casts=casts)
     copy = casts.lookup(weight) if casts is not None and dt == torch.bfloat16 else None
     copy = None if copy is None else copy[0]
-    if need:
+    if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad):
         return _StreamXentFn.apply(h, weight, targets, int(ignore_index), reduction, dt, copy)
     return _xent_forward(h, weight if copy is None else copy, targets, int(ignore_index), reduction, dt, False)[0]
 
