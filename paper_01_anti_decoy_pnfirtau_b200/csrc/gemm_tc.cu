@@ -22,8 +22,8 @@ int sm_count() {
   return n;
 }
 
-int plan_splits(int64_t tiles, int64_t kb) {
-  const int64_t want = std::max<int64_t>(1, sm_count() / 2 / std::max<int64_t>(1, tiles));
+int plan_splits(int64_t tiles, int64_t kb, int rounds) {
+  const int64_t want = std::max<int64_t>(1, rounds * (sm_count() / 2) / std::max<int64_t>(1, tiles));
   return (int)std::max<int64_t>(1, std::min(want, kb / 8));
 }
 

@@ -116,7 +116,8 @@ __device__ __forceinline__ void commit_pair(uint32_t bar) {
 // tile running fastest, so the pairs in flight share both operands in L2. Runs (`runs`): the
 // tiles, row tile by row tile, are dealt to the pairs in equal contiguous runs, and an item
 // is a run's part of one row tile: the pairs end together, and a pair keeps its rows of A.
-// For a B that stays in L2 as a whole.
+// For a B that stays in L2 as a whole. strips = 0: strips as fit the number of row tiles (the
+// rows that count, known on the device alone), see auto_strips.
 struct Sched {
   int tiles_m;          // 256-row tiles (upper bound when live is given)
   int strips;           // items along N
@@ -138,6 +139,22 @@ __host__ __device__ inline int run_owner(int64_t total, int64_t x, int pairs) {
   return (int)(((x + 1) * pairs + total - 1) / total) - 1;
 }
 
+// Strips per row tile: those of one to four equal rounds of items over the pairs, the one
+// with the fewest tiles in a row, counting a third of a tile for an item's start and end.
+__host__ __device__ inline int auto_strips(int tiles_m, int tiles_n, int pairs) {
+  int best = 1;
+  float least = 3e38f;
+  for (int r = 0; r <= 4 && tiles_m > 0; ++r) {
+    int strips = r * pairs / tiles_m;
+    strips = strips < 1 ? 1 : strips > tiles_n ? tiles_n : strips;
+    const int per = (tiles_n + strips - 1) / strips;
+    strips = (tiles_n + per - 1) / per;
+    const float cost = (float)((tiles_m * strips + pairs - 1) / pairs) * ((float)per + 0.333f);
+    if (cost < least) least = cost, best = strips;
+  }
+  return best;
+}
+
 struct Args {
   CUtensorMap ta[2], tb[2];
   Sched s;
@@ -154,6 +171,7 @@ struct Item {
 
 struct Walk {
   int tiles_m, kb, slots, pairs;
+  int strips, per_strip, group_m;
   int64_t total;  // items, or tiles in runs
   __device__ Walk(const Sched& s, int launched) {
     tiles_m = s.tiles_m, kb = s.kb;
@@ -162,9 +180,15 @@ struct Walk {
       if (s.live_m) tiles_m = (n + PM - 1) / PM;
       if (s.live_k) kb = (n + BK - 1) / BK;
     }
-    total = s.runs ? (int64_t)tiles_m * s.tiles_n : (int64_t)tiles_m * s.strips * s.splits;
+    strips = s.strips, per_strip = s.tiles_per_strip, group_m = s.group_m;
+    if (strips == 0) {
+      strips = auto_strips(tiles_m, s.tiles_n, launched);
+      per_strip = (s.tiles_n + strips - 1) / strips;
+      group_m = max(tiles_m, 1);
+    }
+    total = s.runs ? (int64_t)tiles_m * s.tiles_n : (int64_t)tiles_m * strips * s.splits;
     pairs = s.runs ? run_pairs(total, launched) : launched;
-    slots = s.runs ? run_slots(tiles_m, pairs) : s.strips;
+    slots = s.runs ? run_slots(tiles_m, pairs) : strips;
   }
   // Pairs that get a run: none is empty, also where fewer rows count than the launch was sized for.
   __host__ __device__ static int run_pairs(int64_t total, int launched) { return (int)(total < launched ? total : launched); }
@@ -183,16 +207,16 @@ struct Walk {
       it.ntn = (int)min((int64_t)s.tiles_n, end - first) - it.nt0;
       it.slot = pair - run_owner(total, first, pairs);
     } else {
-      const int per_split = tiles_m * s.strips;
+      const int per_split = tiles_m * strips;
       it.split = (int)(i / per_split);
       int r = (int)(i - (int64_t)it.split * per_split);
-      const int per = s.group_m * s.strips, g = r / per;
+      const int per = group_m * strips, g = r / per;
       r -= g * per;
-      const int gm = min(s.group_m, tiles_m - g * s.group_m);
-      it.mt = g * s.group_m + r % gm;
+      const int gm = min(group_m, tiles_m - g * group_m);
+      it.mt = g * group_m + r % gm;
       it.slot = r / gm;
-      it.nt0 = it.slot * s.tiles_per_strip;
-      it.ntn = min(s.tiles_per_strip, s.tiles_n - it.nt0);
+      it.nt0 = it.slot * per_strip;
+      it.ntn = min(per_strip, s.tiles_n - it.nt0);
       // whole K blocks spread evenly over the splits
       it.kb0 = (int)((int64_t)kb * it.split / s.splits);
       it.kbn = (int)((int64_t)kb * (it.split + 1) / s.splits) - it.kb0;
@@ -737,10 +761,10 @@ struct StoreEpi {
 // ------------------------------------------------------------------ host side
 int current_device();
 int sm_count();  // of the current device
-// Splits of K for an output of `tiles` tiles: about one work item per pair of SMs, at
+// Splits of K for an output of `tiles` tiles: about `rounds` work items per pair of SMs, at
 // least 8 K blocks (512 of K) each, since shorter ones cost more in partial sums than
 // they gain.
-int plan_splits(int64_t tiles, int64_t kb);
+int plan_splits(int64_t tiles, int64_t kb, int rounds = 1);
 // Pairs of SMs that a launch of `items` items takes.
 inline int pairs_of(int64_t items) { return (int)std::min<int64_t>(items, sm_count() / 2); }
 inline int64_t tiles_of(int64_t m, int64_t n) { return ((m + PM - 1) / PM) * ((n + BN - 1) / BN); }
@@ -805,7 +829,7 @@ inline void runs_if_resident(Sched* s, int64_t n, int64_t k) { s->runs = n * k *
 
 template <bool A_MN, bool B_MN, bool DUAL_B, bool KEEP_A, class Epi>
 int launch_kernel(const char* what, Args a, const typename Epi::Params& ep, cudaStream_t st) {
-  const int64_t items = (int64_t)a.s.tiles_m * (a.s.runs ? a.s.tiles_n : a.s.strips) * a.s.splits;
+  const int64_t items = (int64_t)a.s.tiles_m * (a.s.runs || !a.s.strips ? a.s.tiles_n : a.s.strips) * a.s.splits;
   if (items <= 0) return PNFT_OK;
   if (items > (1 << 30)) return fail(PNFT_EUNSUPPORTED, "%s: too many tiles", what);
   auto* k = gemm_kernel<A_MN, B_MN, DUAL_B, KEEP_A, Epi>;
@@ -823,7 +847,7 @@ template <bool A_MN, bool B_MN, bool DUAL_B, class Epi>
 int launch(const char* what, const Args& a, const typename Epi::Params& ep, cudaStream_t st) {
   if constexpr (!A_MN) {
     // rows of A are kept where that leaves the ring at least four stages and an item has several tiles
-    if ((a.s.runs || a.s.tiles_per_strip > 1) && a.s.splits == 1 && a.s.chunk >= a.s.kb && stages<Epi>(true, a.s.kb) >= 4)
+    if ((a.s.runs || !a.s.strips) && a.s.splits == 1 && a.s.chunk >= a.s.kb && stages<Epi>(true, a.s.kb) >= 4)
       return launch_kernel<A_MN, B_MN, DUAL_B, true, Epi>(what, a, ep, st);
   }
   return launch_kernel<A_MN, B_MN, DUAL_B, false, Epi>(what, a, ep, st);

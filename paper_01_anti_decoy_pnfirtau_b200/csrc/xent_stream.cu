@@ -252,7 +252,7 @@ struct ReduceArgs {
   float* row_loss;  // [M], or NULL
   float* loss;      // scalar, or NULL
   double* block_sum;
-  int runs, tiles_n, slots, pairs, mean;
+  int runs, tiles_n, pairs, mean;
 };
 // A block takes ROWS rows, 256 / ROWS threads each: many threads per row when there are
 // few rows, which then have many strips.
@@ -268,8 +268,12 @@ __global__ void __launch_bounds__(256) xent_reduce_kernel(ReduceArgs p) {
   // the pairs of the row's tile: one per strip, or one per run that the tile lies in
   const int tiles_m = (n + PM - 1) / PM;
   const int64_t mt = i / PM, total = (int64_t)tiles_m * p.tiles_n;
-  int slots = p.slots, parts = 4 * slots;
-  if (p.runs && i < n) {
+  int slots = 1, parts = 4;
+  if (i < n && !p.runs) {
+    slots = auto_strips(tiles_m, p.tiles_n, p.pairs);
+    parts = 4 * slots;
+  }
+  if (i < n && p.runs) {
     const int pairs = Walk::run_pairs(total, p.pairs);
     slots = Walk::run_slots(tiles_m, pairs);
     parts = 4 * (run_owner(total, (mt + 1) * p.tiles_n - 1, pairs) - run_owner(total, mt * p.tiles_n, pairs) + 1);
@@ -567,21 +571,6 @@ __global__ void __launch_bounds__(256) xent_dh_kernel(const float* __restrict__ 
 // ------------------------------------------------------------------ plans
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Column tiles per strip: the fewest rounds of tiles over the pairs of SMs, counting a third of a
-// tile for each strip's start and end.
-int strip_tiles(int64_t tiles_m, int tiles_n) {
-  const int sms = sm_count() / 2;  // pairs
-  int best = 1;
-  double cost = 1e300;
-  for (int strips = 1; strips <= std::min(tiles_n, 2 * sms); ++strips) {
-    const int per = (tiles_n + strips - 1) / strips;
-    const int64_t items = tiles_m * ((tiles_n + per - 1) / per);
-    const double c = (double)((items + sms - 1) / sms) * (per + 1.0 / 3);
-    if (c < cost) cost = c, best = per;
-  }
-  return best;
-}
-
 // What the backward needs: the rows that count (16-byte aligned, whole row tiles) and
 // their state.
 struct SavedLayout {
@@ -615,7 +604,7 @@ State state_of(const SavedLayout& l, void* saved) {
 }
 
 struct FwdLayout {
-  int runs, pairs, tiles_n, per, strips;
+  int runs, pairs, tiles_n;
   size_t zt, part_m, part_s, sums, total;
 };
 FwdLayout fwd_layout(int64_t M, int64_t V, int64_t D) {
@@ -626,10 +615,9 @@ FwdLayout fwd_layout(int64_t M, int64_t V, int64_t D) {
   l.runs = s.runs;
   l.tiles_n = (int)((V + BN - 1) / BN);
   l.pairs = pairs_of(tiles_m * l.tiles_n);
-  l.per = l.runs ? 1 : strip_tiles(tiles_m, l.tiles_n);
-  l.strips = (l.tiles_n + l.per - 1) / l.per;
-  // in runs a row tile lies in at most pairs / row tiles + 2, for any number of rows that count
-  const size_t parts = 4 * PM * (size_t)(l.runs ? l.pairs + 2 * tiles_m : tiles_m * l.strips);
+  // a row tile lies in at most pairs / row tiles + 2 runs, or has 4 pairs / row tiles strips (at least
+  // one), for any number of rows that count
+  const size_t parts = 4 * PM * (size_t)(l.runs ? l.pairs + 2 * tiles_m : 4 * l.pairs + tiles_m);
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t r = at;
@@ -663,7 +651,8 @@ BwdLayout bwd_layout(int64_t M, int64_t V, int64_t D) {
   const int64_t Mp = up(M, BM), D4 = up(D, 4);
   BwdLayout l;
   l.P = piece_width(M, V);
-  l.dh_splits = plan_splits(tiles_of(M, D), l.P / BK);
+  // few tiles: two rounds, which become one where half of the rows count
+  l.dh_splits = plan_splits(tiles_of(M, D), l.P / BK, 4 * tiles_of(M, D) <= sm_count() / 2 ? 2 : 1);
   l.dw_splits = plan_splits(tiles_of(l.P, D), Mp / BK);
   size_t at = 0;
   auto take = [&](size_t n) {
@@ -774,9 +763,7 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
   if (rc) return rc;
   a.s = plain_sched(M, V, (D + BK - 1) / BK, 1);
   a.s.runs = l.runs;
-  a.s.strips = l.strips;
-  a.s.tiles_per_strip = l.per;
-  a.s.group_m = a.s.tiles_m;
+  a.s.strips = 0;
   a.s.live = c.s.counts;
   a.s.live_m = 1;
   a.idesc = idesc(dtype, false, false);
@@ -786,7 +773,7 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
   rc = launch<false, false, false, LseEpi>("stream_xent forward", a, ep, st);
   if (rc) return rc;
   ReduceArgs r{ep.part_m, ep.part_s, c.zt, c.s, row_loss, loss, reinterpret_cast<double*>(ws + l.sums),
-               l.runs, l.tiles_n, l.strips, l.pairs, mean};
+               l.runs, l.tiles_n, l.pairs, mean};
   if (M > 64)
     xent_reduce_kernel<32><<<(unsigned)((M + 31) / 32), 256, 0, st>>>(r);
   else

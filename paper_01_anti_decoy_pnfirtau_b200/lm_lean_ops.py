@@ -55,11 +55,15 @@ def _context(dev: torch.device) -> tuple[int, int]:
 
 def _elsewhere(dev: torch.device) -> bool:
     """``dev`` is not the current device (a call then runs under ``torch.cuda.device(dev)``)."""
-    return torch.cuda.current_device() != dev.index
+    return torch._C._cuda_getDevice() != dev.index
+
+
+def _new(rows: int, cols: int, dt: torch.dtype, dev: torch.device) -> torch.Tensor:
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dt, device=dev)  # cheaper to call than empty
 
 
 def _bytes(n: int, dev: torch.device) -> torch.Tensor:
-    return torch.empty(n or 16, dtype=torch.uint8, device=dev)
+    return torch.empty_strided((n or 16,), (1,), dtype=torch.uint8, device=dev)
 
 
 def _pad8(n: int) -> int:
@@ -74,6 +78,10 @@ def _ld(t: torch.Tensor) -> int:
 
 def _unit_rows(t: torch.Tensor, dt: torch.dtype) -> torch.Tensor:
     """``t`` (2-D) in ``dt`` with unit column stride and rows that do not overlap."""
+    if t.dtype is dt:
+        ld, unit = t.stride()
+        if unit == 1 and ld >= t.shape[1]:
+            return t
     if t.dtype != dt:
         t = t.to(dt)
     rows, cols = t.shape
@@ -83,11 +91,15 @@ def _unit_rows(t: torch.Tensor, dt: torch.dtype) -> torch.Tensor:
 def _rows16(t: torch.Tensor, dt: torch.dtype) -> torch.Tensor:
     """``t`` (2-D) in ``dt`` as rows that a TMA map takes: unit column stride, row stride
     a multiple of 8 elements, 16-byte base. A view of ``t`` when it is that already."""
+    if t.dtype is dt and t.data_ptr() % 16 == 0:
+        ld, unit = t.stride()
+        if unit == 1 and ld % 8 == 0 and ld >= t.shape[1]:
+            return t
     t = _unit_rows(t, dt)
     if t.data_ptr() % 16 == 0 and _ld(t) % 8 == 0:
         return t
     rows, cols = t.shape
-    out = torch.empty((rows, _pad8(cols)), dtype=dt, device=t.device)[:, :cols]
+    out = _new(rows, _pad8(cols), dt, t.device)[:, :cols]
     rc = _lib.lib().pnft_copy_rows16(t.data_ptr(), _ld(t), out.data_ptr(), _pad8(cols), rows, cols, _context(t.device)[1])
     _lib.check(rc, "pnft_copy_rows16")
     return out
@@ -137,8 +149,7 @@ def act8_pack(x: torch.Tensor) -> Act8:
     D = shape[-1]
     x2 = _unit_rows(x if x.dim() == 2 else x.reshape(-1, D), x.dtype)
     M = x2.shape[0]
-    p = Act8(torch.empty((M, (D + 15) // 16 * 16 + ((D + 127) // 128 + 15) // 16 * 16), dtype=torch.uint8, device=dev), shape,
-             x.dtype)
+    p = Act8(_new(M, (D + 15) // 16 * 16 + ((D + 127) // 128 + 15) // 16 * 16, torch.uint8, dev), shape, x.dtype)
     q, ldq, e, lde, _, _ = p._layout()
     rc = _lib.lib().pnft_act8_pack(x2.data_ptr(), x2.stride(0) if M > 1 else D, q, ldq, e, lde, M, D, code, _context(dev)[1])
     _lib.check(rc, "pnft_act8_pack")
@@ -149,7 +160,7 @@ def _act8_rows(p: Act8, dt: torch.dtype, width: int) -> torch.Tensor:
     """The values as rows of ``width`` columns of ``dt`` (those past ``p.width`` undefined)."""
     q, ldq, e, lde, M, D = p._layout()
     dev = p.data.device
-    y = torch.empty((M, width), dtype=dt, device=dev)
+    y = _new(M, width, dt, dev)
     rc = _lib.lib().pnft_act8_unpack(q, ldq, e, lde, y.data_ptr(), width, M, D, _DTYPES[dt], _context(dev)[1])
     _lib.check(rc, "pnft_act8_unpack")
     return y
@@ -186,7 +197,7 @@ def act8_weight_grad(dy: torch.Tensor, p: Act8, out_dtype: torch.dtype = torch.f
     if dy2.shape[0] != M:
         raise RuntimeError(f"act8_weight_grad: {dy2.shape[0]} rows of gradient but {M} of activation")
     dy2 = _rows16(dy2, dy.dtype) if N % 8 == 0 else _unit_rows(dy2, dy.dtype)
-    dw = torch.empty((N, D), dtype=out_dtype, device=dev)
+    dw = _new(N, D, out_dtype, dev)
     L = _lib.lib()
     nbytes = L.pnft_act8_weight_grad_workspace_size(M, N, D)
     ws = _bytes(nbytes, dev)
@@ -209,15 +220,13 @@ def _gated_forward(x, wg, wu, bg, bu, act: int, dt: torch.dtype, keep: bool):
     """(h, x's rows, the weights' rows, the kept pre-activations or None)."""
     dev = x.device
     F_, D = wg.shape
-    if x.dim() == 2:
-        x2, shape = x, (x.shape[0], F_)
-    else:
-        x2, shape = x.reshape(-1, D), (*x.shape[:-1], F_)
+    flat = x.dim() == 2
+    x2 = x if flat else x.reshape(-1, D)
     M = x2.shape[0]
     rows = _rows16 if keep or M > _FEW else _unit_rows
     x2, wg, wu = rows(x2, dt), rows(wg, dt), rows(wu, dt)
-    h = torch.empty(shape, dtype=dt, device=dev)
-    pre = torch.empty((3, M, _pad8(F_)), dtype=torch.int16, device=dev) if keep else None
+    h = _new(M, F_, dt, dev)
+    pre = _new(3 * M, _pad8(F_), torch.int16, dev) if keep else None
     b = bg if bg is not None else bu
     status, stream = _context(dev)
     rc = _lib.lib().pnft_gated_fwd(
@@ -225,7 +234,7 @@ def _gated_forward(x, wg, wu, bg, bu, act: int, dt: torch.dtype, keep: bool):
         _lib.DTYPE_F32 if b is None else _DTYPES[b.dtype], h.data_ptr(), F_, _ptr(pre), _pad8(F_), M, D, F_, act, _DTYPES[dt],
         status, stream)
     _lib.check(rc, "pnft_gated_fwd")
-    return h, x2, wg, wu, pre
+    return h if flat else h.view(*x.shape[:-1], F_), x2, wg, wu, pre
 
 
 class _GatedLinearFn(torch.autograd.Function):
@@ -267,9 +276,9 @@ def _gated_backward(ctx, dh):
     M = x2.shape[0]
     dh = dh.reshape(-1, F_)
     dh = _rows16(dh, dt) if F_ % 8 == 0 else _unit_rows(dh, dt)
-    dx = torch.empty(x_shape, dtype=x_dtype, device=dev) if nx else None
-    dwg = torch.empty((F_, D), dtype=w_dtype, device=dev) if nwg else None
-    dwu = torch.empty((F_, D), dtype=w_dtype, device=dev) if nwu else None
+    dx = _new(M, D, x_dtype, dev) if nx else None
+    dwg = _new(F_, D, w_dtype, dev) if nwg else None
+    dwu = _new(F_, D, w_dtype, dev) if nwu else None
     b = bg if bg is not None else bu
     b_dtype = torch.float32 if b is None else b.dtype
     dbg = torch.empty(F_, dtype=b_dtype, device=dev) if nbg and bg is not None else None
@@ -283,6 +292,8 @@ def _gated_backward(ctx, dh):
         _pad8(F_), dh.data_ptr(), _ld(dh), _ptr(dx), D, _DTYPES[x_dtype], _ptr(dwg), _ptr(dwu), D, _DTYPES[w_dtype], _ptr(dbg),
         _ptr(dbu), ws.data_ptr(), nbytes, M, D, F_, act, _DTYPES[dt], status, stream)
     _lib.check(rc, "pnft_gated_bwd")
+    if nx and len(x_shape) != 2:
+        dx = dx.view(x_shape)
     return dx, dwg, dwu, dbg, dbu, None, None, None, None
 
 
@@ -299,7 +310,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     and is the gradient at that 8-bit ``x``: it computes the pre-activations again from it.
     The forward's result does not change. ``casts``: an ``lm_ops.Bf16Casts`` with current
     bf16 copies of the weights, used when the dtype is bf16."""
-    biases = tuple(b for b in (b_gate, b_up) if b is not None)
+    biases = () if b_gate is None and b_up is None else tuple(b for b in (b_gate, b_up) if b is not None)
     dev = _require_cuda("gated_linear", x, w_gate, w_up, *biases)
     act = _ACTS.get(activation)
     if act is None:
@@ -307,7 +318,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     if x.dim() == 0 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or x.shape[-1] != w_gate.shape[1]:
         raise RuntimeError(f"gated_linear: x {tuple(x.shape)}, weights {tuple(w_gate.shape)} and {tuple(w_up.shape)}: [..., D] "
                            "and twice [F, D] expected")
-    if w_gate.numel() == 0:
+    if 0 in w_gate.shape:
         raise RuntimeError(f"gated_linear: empty weights {tuple(w_gate.shape)}")
     for b in biases:
         if b.shape != w_gate.shape[:1]:
@@ -383,8 +394,8 @@ def _xent_backward(ctx, dloss):
     per_row = reduction == "none"
     if per_row:
         dloss = dloss.reshape(-1)
-    dh = torch.empty(h_shape, dtype=h_dtype, device=dev) if ctx.needs_input_grad[0] else None
-    dw = torch.empty((V, D), dtype=w_dtype, device=dev) if ctx.needs_input_grad[1] else None
+    dh = _new(M, D, h_dtype, dev) if ctx.needs_input_grad[0] else None
+    dw = _new(V, D, w_dtype, dev) if ctx.needs_input_grad[1] else None
     nbytes = L.pnft_stream_xent_bwd_workspace_size(M, V, D)
     ws = _bytes(nbytes, dev)
     status, stream = _context(dev)
@@ -392,6 +403,8 @@ def _xent_backward(ctx, dloss):
                                 per_row, reduction == "mean", _ptr(dh), D, _DTYPES[h_dtype], _ptr(dw), D, _DTYPES[w_dtype],
                                 ws.data_ptr(), nbytes, M, V, D, _DTYPES[dt], status, stream)
     _lib.check(rc, "pnft_stream_xent_bwd")
+    if dh is not None and len(h_shape) != 2:
+        dh = dh.view(h_shape)
     return dh, dw, None, None, None, None, None
 
 
