@@ -100,6 +100,8 @@ constexpr int AU = 4, COLS = 256 * AU;
 
 template <bool F32>
 __global__ void __launch_bounds__(AT) act8_pack_kernel(ActArgs p) {
+  tc::launch_next();
+  tc::wait_previous();
   const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
   const bool bf16 = p.dtype == PNFT_DTYPE_BF16;
   int lo, hi;
@@ -153,6 +155,8 @@ __global__ void __launch_bounds__(AT) act8_pack_kernel(ActArgs p) {
 }
 
 __global__ void __launch_bounds__(AT) act8_unpack_kernel(ActArgs p, void* y, int64_t ldy) {
+  tc::launch_next();
+  tc::wait_previous();
   const int lane = threadIdx.x & 31;
   for (int64_t row = (int64_t)blockIdx.x * (AT / 32) + (threadIdx.x >> 5); row < p.M; row += (int64_t)gridDim.x * (AT / 32)) {
     const int c0 = blockIdx.y * COLS + 8 * lane;
@@ -212,10 +216,8 @@ extern "C" int pnft_act8_pack(const void* x, int64_t ldx, void* q, int64_t ldq, 
   if (M == 0) return PNFT_OK;
   ActArgs a{x, ldx, static_cast<uint8_t*>(q), ldq, e, lde, M, (int)D, dtype,
             tc::rows16(x, ldx, dtype == PNFT_DTYPE_F32 ? 4 : 2)};
-  if (dtype == PNFT_DTYPE_F32)
-    act8_pack_kernel<true><<<act8_grid(M, D), AT, 0, as_stream(stream)>>>(a);
-  else
-    act8_pack_kernel<false><<<act8_grid(M, D), AT, 0, as_stream(stream)>>>(a);
+  tc::launch_dependent(dtype == PNFT_DTYPE_F32 ? act8_pack_kernel<true> : act8_pack_kernel<false>, act8_grid(M, D), AT, 0,
+                       as_stream(stream), a);
   return check_launch("act8_pack", 1);
 }
 
@@ -225,7 +227,7 @@ extern "C" int pnft_act8_unpack(const void* q, int64_t ldq, const int8_t* e, int
   if (M == 0) return PNFT_OK;
   ActArgs a{nullptr, 0, static_cast<uint8_t*>(const_cast<void*>(q)), ldq, const_cast<int8_t*>(e), lde, M, (int)D,
             dtype, tc::rows16(y, ldy, dtype == PNFT_DTYPE_F32 ? 4 : 2)};
-  act8_unpack_kernel<<<act8_grid(M, D), AT, 0, as_stream(stream)>>>(a, y, ldy);
+  tc::launch_dependent(act8_unpack_kernel, act8_grid(M, D), AT, 0, as_stream(stream), a, y, ldy);
   return check_launch("act8_unpack", 1);
 }
 

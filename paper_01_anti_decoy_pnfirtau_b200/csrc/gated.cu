@@ -227,6 +227,8 @@ struct SkinnyArgs {
 };
 template <int NT, bool VEC, bool BF16>
 __global__ void __launch_bounds__(32 * skinny::WARPS, 2) gated_skinny_kernel(SkinnyArgs p) {
+  launch_next();
+  wait_previous();
   constexpr int N = 8 * NT;
   __shared__ float red[skinny::WARPS / 2][2][16][N + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -309,6 +311,8 @@ __device__ __forceinline__ void join24(const uint16_t* gp, const uint16_t* up, c
 
 template <bool POINT, bool SUMS, int ACT>
 __global__ void __launch_bounds__(PT, PBLOCKS) gated_point_kernel(PointArgs p) {
+  launch_next();
+  wait_previous();
   __shared__ float red[SUMS ? PT / 32 : 1][2][PCOLS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col = blockIdx.x * PCOLS + 8 * lane, n = p.F - col;
@@ -358,6 +362,8 @@ __global__ void __launch_bounds__(PT, PBLOCKS) gated_point_kernel(PointArgs p) {
 
 __global__ void __launch_bounds__(256) gated_bias_sum_kernel(const float* __restrict__ part, int blocks, int F, void* dbg,
                                                              void* dbu, int dtype) {
+  launch_next();
+  wait_previous();
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= 2 * F) return;
   float t = 0.f;
@@ -452,8 +458,8 @@ extern "C" int pnft_gated_fwd(const void* x, int64_t ldx, const void* wg, int64_
                        ldx, ldwg, ldwu, bg, bu, b_dtype, act, static_cast<uint16_t*>(h), ldh, (int)M, (int)D, (int)F};
     const bool vec = D % 8 == 0 && rows16(x, ldx, 2) && rows16(wg, ldwg, 2) && rows16(wu, ldwu, 2);
     return skinny::dispatch(M, vec, dtype == PNFT_DTYPE_BF16, [&](auto nt, auto v, auto b) {
-      gated_skinny_kernel<decltype(nt)::value, decltype(v)::value, decltype(b)::value>
-          <<<(unsigned)((F + 15) / 16), 32 * skinny::WARPS, 0, as_stream(stream)>>>(a);
+      launch_dependent(gated_skinny_kernel<decltype(nt)::value, decltype(v)::value, decltype(b)::value>,
+                       dim3((unsigned)((F + 15) / 16)), 32 * skinny::WARPS, 0, as_stream(stream), a);
       return check_launch("gated_fwd", 1);
     });
   }
@@ -512,15 +518,16 @@ int point(const uint16_t* dh, int64_t lddh, const void* pre, int64_t ldp, uint16
   p.rows = point_rows(M, F);
   const dim3 grid((unsigned)((F + PCOLS - 1) / PCOLS), (unsigned)((M + p.rows - 1) / p.rows));
   if (!dh)
-    gated_point_kernel<false, true, 0><<<grid, PT, 0, st>>>(p);
+    launch_dependent(gated_point_kernel<false, true, 0>, grid, PT, 0, st, p);
   else if (act == PNFT_ACT_SILU)
-    sums ? gated_point_kernel<true, true, PNFT_ACT_SILU><<<grid, PT, 0, st>>>(p)
-         : gated_point_kernel<true, false, PNFT_ACT_SILU><<<grid, PT, 0, st>>>(p);
+    launch_dependent(sums ? gated_point_kernel<true, true, PNFT_ACT_SILU> : gated_point_kernel<true, false, PNFT_ACT_SILU>, grid, PT, 0,
+                     st, p);
   else
-    sums ? gated_point_kernel<true, true, PNFT_ACT_GELU><<<grid, PT, 0, st>>>(p)
-         : gated_point_kernel<true, false, PNFT_ACT_GELU><<<grid, PT, 0, st>>>(p);
+    launch_dependent(sums ? gated_point_kernel<true, true, PNFT_ACT_GELU> : gated_point_kernel<true, false, PNFT_ACT_GELU>, grid, PT, 0,
+                     st, p);
   if (sums)
-    gated_bias_sum_kernel<<<(unsigned)((2 * F + 255) / 256), 256, 0, st>>>(p.part, (int)grid.y, (int)F, dbg, dbu, b_dtype);
+    launch_dependent(gated_bias_sum_kernel, dim3((unsigned)((2 * F + 255) / 256)), 256, 0, st, p.part, (int)grid.y, (int)F, dbg, dbu,
+                     b_dtype);
   return check_launch("gated_bwd pointwise", sums ? 2 : 1);
 }
 

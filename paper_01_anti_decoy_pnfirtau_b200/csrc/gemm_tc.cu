@@ -33,6 +33,8 @@ namespace {
 __global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict__ part, int64_t ldp,
                                                          int64_t split_stride, int splits, SumArgs o,
                                                          int rows_total) {
+  launch_next();
+  wait_previous();
   const int n4 = (o.cols + 3) / 4;
   const float alpha = o.alpha ? *o.alpha : 1.f;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)rows_total * n4; i += (int64_t)gridDim.x * 256) {
@@ -70,6 +72,8 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict
 template <typename W>
 __global__ void __launch_bounds__(256) copy_rows_kernel(const char* __restrict__ src, int64_t ss, char* __restrict__ dst,
                                                         int64_t ds, int64_t rows, int64_t words) {
+  launch_next();
+  wait_previous();
   const int lane = threadIdx.x & 31;
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
     const W* from = reinterpret_cast<const W*>(src + r * ss);
@@ -92,7 +96,7 @@ int sum_splits(const float* part, int64_t ldp, int64_t split_stride, int splits,
                int rows_total, cudaStream_t st) {
   const int64_t items = (int64_t)rows_total * ((out.cols + 3) / 4);
   const int64_t blocks = std::min<int64_t>((items + 255) / 256, (int64_t)sm_count() * 8);
-  sum_splits_kernel<<<(unsigned)blocks, 256, 0, st>>>(part, ldp, split_stride, splits, out, rows_total);
+  launch_dependent(sum_splits_kernel, dim3((unsigned)blocks), 256, 0, st, part, ldp, split_stride, splits, out, rows_total);
   return check_launch("split sum", 1);
 }
 
@@ -194,10 +198,10 @@ extern "C" int pnft_copy_rows16(const void* src, int64_t lds, void* dst, int64_t
   char* d = static_cast<char*>(dst);
   cudaStream_t st = as_stream(stream);
   if (w == 16)
-    copy_rows_kernel<uint4><<<grid, 256, 0, st>>>(s, lds * 2, d, ldd * 2, rows, words);
+    launch_dependent(copy_rows_kernel<uint4>, dim3(grid), 256, 0, st, s, lds * 2, d, ldd * 2, rows, words);
   else if (w == 4)
-    copy_rows_kernel<uint32_t><<<grid, 256, 0, st>>>(s, lds * 2, d, ldd * 2, rows, words);
+    launch_dependent(copy_rows_kernel<uint32_t>, dim3(grid), 256, 0, st, s, lds * 2, d, ldd * 2, rows, words);
   else
-    copy_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(s, lds * 2, d, ldd * 2, rows, words);
+    launch_dependent(copy_rows_kernel<uint16_t>, dim3(grid), 256, 0, st, s, lds * 2, d, ldd * 2, rows, words);
   return check_launch("copy_rows16", 1);
 }

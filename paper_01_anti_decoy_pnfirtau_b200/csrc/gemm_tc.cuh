@@ -37,6 +37,25 @@ constexpr int STAGE_BYTES = 2 * HALF_BYTES;
 constexpr int GROUP_BYTES = 64 * BK * 2;   // MN-major: 64 columns x 64 K rows
 constexpr int STAGE_MAX = 225 * 1024;      // shared memory for the ring and the epilogue's buffers
 
+// ------------------------------------------------------------------ dependent launches
+// The kernels of one call follow each other on a stream. Each lets the next be launched at
+// once and waits itself, before it touches memory, until the one before has completed: the
+// launch, the barriers and the TMEM allocation of a kernel then pass while the one before
+// still runs. Every thread of a kernel calls it.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class K, class... A>
+inline void launch_dependent(K* kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t c;
+  memset(&c, 0, sizeof(c));
+  c.gridDim = grid, c.blockDim = dim3((unsigned)threads), c.dynamicSmemBytes = smem, c.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &attr, c.numAttrs = 1;
+  (void)cudaLaunchKernelEx(&c, kernel, args...);  // its error is the pending one that check_launch reads
+}
+
 // ------------------------------------------------------------------ PTX of the pair
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -308,6 +327,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
   __shared__ __align__(8) uint64_t bars[2 * MAX_STAGES + 7 + EPI_WARPS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
+  launch_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const uint32_t b0 = smem_u32(bars);
@@ -345,6 +365,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
   cluster_sync();  // the other CTA's barriers are ready for this one's arrivals
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
+  wait_previous();
   const Walk walk(p.s, pairs);
 
   if (warp == 0) {
@@ -840,7 +861,7 @@ int launch_kernel(const char* what, Args a, const typename Epi::Params& ep, cuda
     ready.fetch_or(bit, std::memory_order_release);
   }
   a.stages = stages<Epi>(KEEP_A, a.s.kb);
-  k<<<(unsigned)(2 * pairs_of(items)), 32 * (2 + Epi::WARPS), SMEM, st>>>(a, ep);
+  launch_dependent(k, dim3((unsigned)(2 * pairs_of(items))), 32 * (2 + Epi::WARPS), SMEM, st, a, ep);
   return check_launch(what, 1);
 }
 template <bool A_MN, bool B_MN, bool DUAL_B, class Epi>

@@ -104,25 +104,17 @@ __device__ __forceinline__ int block_total(int v, int* red) {
   return t;
 }
 
-__device__ __forceinline__ void copy_row(uint16_t* dst, const uint16_t* src, int D, bool vec, int lane) {
-  if (vec) {
-#pragma unroll 8
-    for (int i = lane; i < D / 8; i += 32) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
-    for (int i = D / 8 * 8 + lane; i < D; i += 32) dst[i] = src[i];
-  } else {
-    for (int i = lane; i < D; i += 32) dst[i] = src[i];
-  }
-}
-
 // Block b owns rows [b * rows, ...): it counts the rows that count before them (every
-// block reads all earlier targets: at most 1024 blocks, a few bytes per row), places its
+// block reads all earlier targets: at most 512 blocks, a few bytes per row), places its
 // own in order and copies them.
 __global__ void __launch_bounds__(CT) xent_compact_kernel(CompactArgs p) {
-  __shared__ int red[CT / 32];
+  __shared__ int red[CT / 32], place[CT];
+  launch_next();
+  wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t r0 = (int64_t)blockIdx.x * p.rows, r1 = std::min<int64_t>(p.M, r0 + p.rows);
   int n = 0;
-#pragma unroll 4
+#pragma unroll 8
   for (int64_t r = threadIdx.x; r < r0; r += CT) n += p.t[r] != p.ignore;
   int base = block_total(n, red);
   for (int64_t c0 = r0; c0 < r1; c0 += CT) {
@@ -139,6 +131,7 @@ __global__ void __launch_bounds__(CT) xent_compact_kernel(CompactArgs p) {
       total += red[k];
     }
     at += __popc(vote & ((1u << lane) - 1));
+    place[threadIdx.x] = counts ? at : -1;
     if (r < r1) p.s.pos[r] = counts ? at : -1;
     if (counts) {
       p.s.idx[at] = (int)r;
@@ -152,11 +145,21 @@ __global__ void __launch_bounds__(CT) xent_compact_kernel(CompactArgs p) {
       p.row_loss[r] = 0.f;
     }
     base += total;
-  }
-  __syncthreads();
-  for (int64_t r = r0 + warp; r < r1; r += CT / 32) {
-    const int at = p.s.pos[r];
-    if (at >= 0) copy_row(p.hc + at * p.ldc, p.h + r * p.ldh, p.D, p.vec, lane);
+    __syncthreads();
+    // the rows themselves: 16 bytes at a time where both sides allow it, four in flight per thread
+    const int rows = (int)std::min<int64_t>(CT, r1 - c0), vecs = p.vec ? p.D / 8 : 0, rest = p.D - 8 * vecs;
+    const uint16_t* h = p.h + c0 * p.ldh;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < rows * vecs; i += CT) {
+      const int k = i / vecs, v = i - k * vecs;
+      if (place[k] >= 0)
+        reinterpret_cast<uint4*>(p.hc + place[k] * p.ldc)[v] = __ldcs(reinterpret_cast<const uint4*>(h + k * p.ldh) + v);
+    }
+#pragma unroll 4
+    for (int i = threadIdx.x; i < rows * rest; i += CT) {
+      const int k = i / rest, v = 8 * vecs + i - k * rest;
+      if (place[k] >= 0) p.hc[place[k] * p.ldc + v] = h[k * p.ldh + v];
+    }
   }
   if (r1 == p.M) {  // the last block knows the number of rows; zeros up to the tile's end
     if (threadIdx.x == 0) p.s.counts[0] = base, p.s.counts[1] = 0;
@@ -262,6 +265,8 @@ __global__ void __launch_bounds__(256) xent_reduce_kernel(ReduceArgs p) {
   __shared__ float top[256], sum[256];
   __shared__ int last;
   constexpr int LANES = 256 / ROWS;
+  launch_next();
+  wait_previous();
   const int n = p.s.counts[0];
   const int r = threadIdx.x % ROWS, lane = threadIdx.x / ROWS;
   const int64_t i = (int64_t)blockIdx.x * ROWS + r;
@@ -366,6 +371,8 @@ constexpr int skinny_groups(int nt) { return nt <= 2 ? 1 : 2; }
 template <int NT, bool VEC, bool BF16>
 __global__ void __launch_bounds__(32 * skinny::WARPS, NT <= 4 ? 2 : 1) xent_skinny_kernel(SkinnyArgs p) {
   __shared__ float sm[skinny::WARPS][8 * NT], ss[skinny::WARPS][8 * NT];
+  launch_next();
+  wait_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float m[NT][2], s[NT][2];
   int tgt[NT][2];
@@ -423,6 +430,8 @@ __global__ void __launch_bounds__(32 * skinny::WARPS, NT <= 4 ? 2 : 1) xent_skin
 __global__ void __launch_bounds__(1024) xent_skinny_reduce_kernel(SkinnyArgs p) {
   __shared__ float losses[SKINNY_ROWS];
   __shared__ int counted[SKINNY_ROWS];
+  launch_next();
+  wait_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int n = warp; n < p.M; n += 32) {
     float m = kLow, s = 0.f;
@@ -465,6 +474,8 @@ struct ScaleArgs {
 };
 __global__ void __launch_bounds__(1024) xent_scale_kernel(ScaleArgs p) {
   __shared__ float red[32];
+  launch_next();
+  wait_previous();
   const int n = p.s.counts[0];
   if (!p.per_row) {
     for (int i = threadIdx.x; i < n; i += 1024) p.rs[i] = p.top;
@@ -547,6 +558,8 @@ struct DzEpi {
 __global__ void __launch_bounds__(256) xent_dh_kernel(const float* __restrict__ acc, int64_t lda, const int32_t* __restrict__ pos,
                                                       const float* __restrict__ alpha, void* dh, int64_t lddh, int dtype,
                                                       int64_t M, int D) {
+  launch_next();
+  wait_previous();
   const float a = *alpha;
   const int lane = threadIdx.x & 31;
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < M; r += (int64_t)gridDim.x * 8) {
@@ -627,7 +640,7 @@ FwdLayout fwd_layout(int64_t M, int64_t V, int64_t D) {
   l.zt = take(4 * Mp);
   l.part_m = take(4 * parts);
   l.part_s = take(4 * parts);
-  l.sums = take(8 * std::max<int64_t>(64, (M + 31) / 32));
+  l.sums = take(8 * std::max<int64_t>(64, (M + 7) / 8));
   l.total = at;
   return l;
 }
@@ -727,8 +740,9 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
                        (int)M, (int)D, (int)V, blocks, mean, status};
     const bool vec = D % 8 == 0 && rows16(h, ldh, 2) && rows16(w, ldw, 2);
     return skinny::dispatch(M, vec, dtype == PNFT_DTYPE_BF16, [&](auto nt, auto v, auto b) {
-      xent_skinny_kernel<decltype(nt)::value, decltype(v)::value, decltype(b)::value><<<blocks, 32 * skinny::WARPS, 0, st>>>(a);
-      xent_skinny_reduce_kernel<<<1, 1024, 0, st>>>(a);
+      launch_dependent(xent_skinny_kernel<decltype(nt)::value, decltype(v)::value, decltype(b)::value>, dim3((unsigned)blocks),
+                       32 * skinny::WARPS, 0, st, a);
+      launch_dependent(xent_skinny_reduce_kernel, dim3(1), 1024, 0, st, a);
       return check_launch("stream_xent_fwd", 2);
     });
   }
@@ -749,10 +763,10 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
   c.zt = reinterpret_cast<float*>(ws + l.zt);
   c.row_loss = row_loss;
   c.M = M, c.V = (int)V, c.D = (int)D, c.Mp = Mp;
-  c.rows = (int)std::max<int64_t>(8, (M + 1023) / 1024);
+  c.rows = (int)std::max<int64_t>(8, (M + 511) / 512);
   c.vec = rows16(h, ldh, 2);
   c.status = status;
-  xent_compact_kernel<<<(unsigned)((M + c.rows - 1) / c.rows), CT, 0, st>>>(c);
+  launch_dependent(xent_compact_kernel, dim3((unsigned)((M + c.rows - 1) / c.rows)), CT, 0, st, c);
   int rc = check_launch("stream_xent compaction", 1);
   if (rc) return rc;
 
@@ -775,9 +789,9 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
   ReduceArgs r{ep.part_m, ep.part_s, c.zt, c.s, row_loss, loss, reinterpret_cast<double*>(ws + l.sums),
                l.runs, l.tiles_n, l.pairs, mean};
   if (M > 64)
-    xent_reduce_kernel<32><<<(unsigned)((M + 31) / 32), 256, 0, st>>>(r);
+    launch_dependent(xent_reduce_kernel<8>, dim3((unsigned)((M + 7) / 8)), 256, 0, st, r);
   else
-    xent_reduce_kernel<1><<<(unsigned)M, 256, 0, st>>>(r);
+    launch_dependent(xent_reduce_kernel<1>, dim3((unsigned)M), 256, 0, st, r);
   return check_launch("stream_xent reduction", 1);
 }
 
@@ -810,7 +824,8 @@ extern "C" int pnft_stream_xent_bwd(const void* w, int64_t ldw, const void* save
   float* acc = reinterpret_cast<float*>(ws + l.acc);
   float* part = reinterpret_cast<float*>(ws + l.part);
   const bool bf16 = dtype == PNFT_DTYPE_BF16;
-  xent_scale_kernel<<<1, 1024, 0, st>>>(ScaleArgs{s, dloss, dloss_stride, rs, alpha, per_row, mean, bf16 ? 1.f : 16384.f});
+  launch_dependent(xent_scale_kernel, dim3(1), 1024, 0, st,
+                   ScaleArgs{s, dloss, dloss_stride, rs, alpha, per_row, mean, bf16 ? 1.f : 16384.f});
   int rc = check_launch("stream_xent scale", 1);
   for (int64_t v0 = 0; !rc && v0 < V; v0 += l.P) {
     const int64_t n = std::min(l.P, V - v0);
@@ -888,7 +903,7 @@ extern "C" int pnft_stream_xent_bwd(const void* w, int64_t ldw, const void* save
     }
   }
   if (rc || !dh) return rc;
-  xent_dh_kernel<<<(unsigned)std::min<int64_t>((M + 7) / 8, (int64_t)sm_count() * 16), 256, 0, st>>>(
-      acc, D4, s.pos, alpha, dh, lddh, dh_dtype, M, (int)D);
+  launch_dependent(xent_dh_kernel, dim3((unsigned)std::min<int64_t>((M + 7) / 8, (int64_t)sm_count() * 16)), 256, 0, st,
+                   (const float*)acc, D4, (const int32_t*)s.pos, (const float*)alpha, dh, lddh, dh_dtype, M, (int)D);
   return check_launch("stream_xent dh rows", 1);
 }
