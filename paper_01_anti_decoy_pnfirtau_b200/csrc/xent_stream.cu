@@ -16,56 +16,13 @@
 // included, reaches a result.
 #include "gemm_tc.cuh"
 #include "skinny.cuh"
+#include "xent_dzdh.cuh"
 
 namespace pnft {
 namespace {
 
 using namespace tc;
-
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kLow = -1e30f;  // running maximum before any logit: finite, so that low - low is 0
-
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// Pairs of fp32 in one 64-bit register: two products or sums per instruction.
-typedef uint64_t f32x2;
-__device__ __forceinline__ f32x2 pack(float a, float b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpack(f32x2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-// 2^x of two values, both on the special-function unit. At K = 256 that unit (16 per clock
-// and SM) is as busy as the tensor core, yet moving every third or second exponential to a
-// polynomial on the FMA pipe made the forward slower (16352 x 33278 x 256: 217 us without,
-// 227 and 237 with): the instructions cost more clock than the unit does.
-__device__ __forceinline__ f32x2 exp2_pair(f32x2 x) {
-  const float2 v = unpack(x);
-  return pack(ex2(v.x), ex2(v.y));
-}
+using namespace xent;
 
 // Device state of one call, in the caller's buffers (rows are compacted rows).
 struct State {
@@ -557,26 +514,19 @@ struct DzEpi {
 // dh[r] = alpha * acc[compacted row of r], 0 for rows that do not count.
 __global__ void __launch_bounds__(256) xent_dh_kernel(const float* __restrict__ acc, int64_t lda, const int32_t* __restrict__ pos,
                                                       const float* __restrict__ alpha, void* dh, int64_t lddh, int dtype,
-                                                      int64_t M, int D) {
+                                                      int64_t M, int D, int vec) {
   launch_next();
   wait_previous();
   const float a = *alpha;
   const int lane = threadIdx.x & 31;
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < M; r += (int64_t)gridDim.x * 8) {
     const int at = pos[r];
+#pragma unroll 4
     for (int c = 4 * lane; c < D; c += 128) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (at >= 0) {
-        v = *reinterpret_cast<const float4*>(acc + at * lda + c);
-        v.x *= a, v.y *= a, v.z *= a, v.w *= a;
-      }
-      const float f[4] = {v.x, v.y, v.z, v.w};
-      for (int k = 0; k < 4 && c + k < D; ++k) {
-        if (dtype == PNFT_DTYPE_F32)
-          static_cast<float*>(dh)[r * lddh + c + k] = f[k];
-        else
-          store16(static_cast<uint16_t*>(dh) + r * lddh + c + k, f[k], dtype == PNFT_DTYPE_BF16);
-      }
+      if (at >= 0) v = *reinterpret_cast<const float4*>(acc + at * lda + c);
+      const float f[4] = {v.x * a, v.y * a, v.z * a, v.w * a};
+      store_row4(dh, r * lddh + c, f, D - c, dtype, vec);
     }
   }
 }
@@ -655,11 +605,17 @@ int64_t piece_width(int64_t M, int64_t V) {
   const int64_t pieces = (V + most - 1) / most;
   return up((V + pieces - 1) / pieces, BN);
 }
+constexpr int FUSED_WIDTH = 256;  // up to this width dz and dh come from one kernel
 struct BwdLayout {
   int64_t P;
   int dh_splits, dw_splits;
   size_t rs, alpha, dz, acc, part, total;
 };
+// Shares of dh that the fused kernel leaves: one per row tile and run that meet.
+int64_t dh_shares(int64_t M, int64_t P) {
+  const int64_t tiles_m = (M + PM - 1) / PM;
+  return tiles_m + pairs_of(tiles_m * (P / BN));
+}
 BwdLayout bwd_layout(int64_t M, int64_t V, int64_t D) {
   const int64_t Mp = up(M, BM), D4 = up(D, 4);
   BwdLayout l;
@@ -677,11 +633,24 @@ BwdLayout bwd_layout(int64_t M, int64_t V, int64_t D) {
   l.alpha = take(4);
   l.dz = take(2 * (size_t)Mp * l.P);
   l.acc = take(4 * (size_t)Mp * D4);
-  const size_t a = l.dh_splits > 1 ? 4 * (size_t)l.dh_splits * Mp * D4 : 0;
+  const size_t a = D <= FUSED_WIDTH ? 4 * (size_t)dh_shares(M, l.P) * PM * D4 : l.dh_splits > 1 ? 4 * (size_t)l.dh_splits * Mp * D4 : 0;
   const size_t b = l.dw_splits > 1 ? 4 * (size_t)l.dw_splits * l.P * D4 : 0;
-  l.part = take(std::max(a, b));
+  l.part = take(std::max(a, b));  // the shares are joined before the splits of dW are written
   l.total = at;
   return l;
+}
+
+template <int NB>
+int launch_dzdh(const DzDhArgs& f, int pairs, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};  // devices on which the kernel has its shared memory
+  const uint64_t bit = 1ull << (current_device() & 63);
+  if (!(ready.load(std::memory_order_acquire) & bit)) {
+    if (cudaFuncSetAttribute(xent_dzdh_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess)
+      return check_launch("stream_xent dz and dh", 0);
+    ready.fetch_or(bit, std::memory_order_release);
+  }
+  launch_dependent(xent_dzdh_kernel<NB>, dim3((unsigned)(2 * pairs)), 32 * (2 + DZDH_WARPS), SMEM, st, f);
+  return check_launch("stream_xent dz and dh", 1);
 }
 
 int xent_check(const char* what, int64_t M, int64_t D, int64_t V, int dtype) {
@@ -833,6 +802,35 @@ extern "C" int pnft_stream_xent_bwd(const void* w, int64_t ldw, const void* save
     Args a;
     memset(&a, 0, sizeof(a));
     a.status = status;
+    if (dh && D <= FUSED_WIDTH) {  // dz and dh of the piece
+      const int tiles_n = (int)((n + BN - 1) / BN), kd = (int)((D + BK - 1) / BK), nb = D <= 128 ? 64 : 128;
+      DzDhArgs f;
+      memset(&f, 0, sizeof(f));
+      f.s = plain_sched(M, n, kd, 1);
+      f.s.runs = 1;
+      f.s.live = s.counts;
+      f.s.live_m = 1;
+      const int pairs = pairs_of((int64_t)f.s.tiles_m * tiles_n);
+      rc = tma_map_rows(&f.th, hc, D, Mp, ldc, BM);
+      if (!rc) rc = tma_map_rows(&f.tw1, wp, D, n, ldw, BM);
+      if (!rc) rc = tma_map_rows(&f.tw2, wp, D, n, ldw, BK);
+      if (!rc) rc = tma_map_out(&f.tdz, dz, 2, l.P, Mp, l.P, 1, 0, 32);
+      if (!rc) rc = tma_map_out(&f.tpart, part, 4, D, PM, D4, f.s.tiles_m + pairs, PM * D4, 32);
+      if (rc) break;
+      f.lse2 = s.lse2, f.rs = rs, f.tgt = s.tgt, f.live = s.counts;
+      f.v0 = (int)v0, f.V = (int)V, f.D = (int)D, f.Mp = (int)Mp, f.bf16 = bf16, f.store_dz = dw != nullptr;
+      f.stages = dzdh_stages(kd);
+      f.idesc1 = idesc(dtype, false, false);
+      f.idesc2 = idesc_f16(PM, 2 * nb, bf16 ? 1 : 0, 0, 1);
+      f.status = status;
+      rc = nb == 64 ? launch_dzdh<64>(f, pairs, st) : launch_dzdh<128>(f, pairs, st);
+      if (rc) break;
+      const JoinArgs j{part, acc, D4, s.counts, s.pos, alpha, dh, lddh, M, (int)D, dh_dtype, tiles_n, pairs, v0 == 0, v0 + l.P >= V,
+                       rows16(dh, lddh, dtype_size(dh_dtype))};
+      launch_dependent(xent_join_kernel, dim3((unsigned)std::min<int64_t>((M + 7) / 8, (int64_t)sm_count() * 16)), 256, 0, st, j);
+      rc = check_launch("stream_xent dh rows", 1);
+      if (rc) break;
+    } else {
     // dz of the piece
     rc = map_kmajor(&a.ta[0], hc, D, Mp, ldc);
     if (!rc) rc = map_kmajor(&a.tb[0], wp, D, n, ldw);
@@ -875,6 +873,7 @@ extern "C" int pnft_stream_xent_bwd(const void* w, int64_t ldw, const void* save
       }
       if (rc) break;
     }
+    }
     if (dw) {  // the piece's rows of dW = dz^T h
       rc = map_mnmajor(&a.ta[0], dz, n, Mp, l.P);
       if (!rc) rc = map_mnmajor(&a.tb[0], hc, D, Mp, ldc);
@@ -902,8 +901,9 @@ extern "C" int pnft_stream_xent_bwd(const void* w, int64_t ldw, const void* save
       }
     }
   }
-  if (rc || !dh) return rc;
+  if (rc || !dh || D <= FUSED_WIDTH) return rc;
   launch_dependent(xent_dh_kernel, dim3((unsigned)std::min<int64_t>((M + 7) / 8, (int64_t)sm_count() * 16)), 256, 0, st,
-                   (const float*)acc, D4, (const int32_t*)s.pos, (const float*)alpha, dh, lddh, dh_dtype, M, (int)D);
+                   (const float*)acc, D4, (const int32_t*)s.pos, (const float*)alpha, dh, lddh, dh_dtype, M, (int)D,
+                   (int)rows16(dh, lddh, dtype_size(dh_dtype)));
   return check_launch("stream_xent dh rows", 1);
 }
