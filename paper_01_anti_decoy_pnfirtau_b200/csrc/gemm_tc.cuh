@@ -46,10 +46,9 @@ __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.lau
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <class K, class... A>
 inline void launch_dependent(K* kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, const A&... args) {
-  cudaLaunchConfig_t c;
-  memset(&c, 0, sizeof(c));
+  cudaLaunchConfig_t c = {};
   c.gridDim = grid, c.blockDim = dim3((unsigned)threads), c.dynamicSmemBytes = smem, c.stream = st;
-  cudaLaunchAttribute attr;
+  cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   c.attrs = &attr, c.numAttrs = 1;

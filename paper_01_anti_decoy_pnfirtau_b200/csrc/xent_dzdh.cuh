@@ -7,9 +7,9 @@
 // epilogue turns them into dz, 16 bits, written into shared memory as the K-major operand
 // of MMA 2, dh += dz W (the other 256 columns), and from there by TMA to memory. A tile of
 // W serves both products: rows x 64 columns, 128-byte swizzled, is K-major for the first
-// and MN-major for the second. MMA 1 of tile j + 1 is issued before MMA 2 of tile j, so
-// the tensor core has work while the epilogue of tile j runs: single buffers of S and dz
-// suffice. The tiles of all rows are dealt to the pairs in equal runs; a run's part of a
+// and MN-major for the second. MMA 1 of tile j + 1 is issued before MMA 2 of tile j, also
+// where tile j + 1 begins another row tile, so the tensor core has work while the epilogue
+// of tile j runs: single buffers of S and dz suffice. The tiles of all rows are dealt to the pairs in equal runs; a run's part of a
 // row tile leaves its share of dh in fp32, and a last kernel adds the shares in order.
 #pragma once
 
@@ -119,18 +119,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + DZDH_WARPS
         }
         return true;
       };
+      int before = -1;  // the tile whose words are still to be loaded for MMA 2
+      bool ok = true;
       for (Steps q(walk, p.s, pair, rank); q.valid(); q.next()) {
         if (q.item_first()) {
-          if (!mbar_wait(h_empty, (items & 1) ^ 1, ab)) break;
+          if (!(ok = mbar_wait(h_empty, (items & 1) ^ 1, ab))) break;
           if (rank == 0) mbar_arrive_expect_tx(h_full, (uint32_t)(2 * HALF_BYTES * kd));
           for (int kb = 0; kb < kd; ++kb)
             tma_load_pair(sh + (uint32_t)kb * HALF_BYTES, &p.th, map_rank(h_full, 0), kb * BK, q.it.row0);
           ++items;
         }
-        if (!load1(q.nt)) break;
-        if (!q.item_first() && !load2(q.nt - 1)) break;
-        if (q.item_last() && !load2(q.nt)) break;
+        if (!(ok = load1(q.nt) && (before < 0 || load2(before)))) break;
+        before = q.nt;
       }
+      if (ok && before >= 0) load2(before);
       if (rank == 0) {  // never leave a copy in flight (see gemm_kernel)
         if (items > 0) drain_wait(h_full, (items - 1) & 1);
         for (int n = 0; n < min(issued, stages); ++n) {
@@ -142,7 +144,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + DZDH_WARPS
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMA issuer (even CTA)
     if (rank == 0 && lane == 0) {
-      int st = 0, ph = 0, items = 0, t1 = 0, t2 = 0;
+      int st = 0, ph = 0, items = 0, shares = 0, t1 = 0, t2 = 0;
       auto next = [&]() {
         commit_pair(empty(st));
         if (++st == stages) st = 0, ph ^= 1;
@@ -162,8 +164,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + DZDH_WARPS
         ++t1;
         return true;
       };
-      auto mma2 = [&](bool first) {  // dh (+)= dz W
-        if (first && !mbar_wait(dh_empty, ((items - 1) & 1) ^ 1, ab)) return false;
+      bool first = false, last = false;  // of its item: the tile whose MMA 2 is still to come
+      auto mma2 = [&]() {  // dh (+)= dz W
+        if (first && !mbar_wait(dh_empty, (shares++ & 1) ^ 1, ab)) return false;
         if (!mbar_wait(dz_full, t2 & 1, ab)) return false;
         tc_fence_after();
         for (int k = 0; k < BN / BK; ++k) {
@@ -176,23 +179,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + DZDH_WARPS
           next();
         }
         commit_pair(dz_empty);
+        if (last) commit_pair(dh_full);
         ++t2;
         return true;
       };
+      bool ok = true;
       for (Steps q(walk, p.s, pair, rank); q.valid(); q.next()) {
-        const bool first = q.item_first(), last = q.item_last();
-        if (first) {
-          if (!mbar_wait(h_full, items & 1, ab)) break;
-          ++items;
-        }
-        if (!mma1()) break;
-        if (last) commit_pair(h_empty);
-        if (!first && !mma2(q.nt - 1 == q.it.nt0)) break;
-        if (last) {
-          if (!mma2(first)) break;
-          commit_pair(dh_full);
-        }
+        if (q.item_first() && !(ok = mbar_wait(h_full, items++ & 1, ab))) break;
+        if (!(ok = mma1())) break;
+        if (q.item_last()) commit_pair(h_empty);
+        if (t1 > 1 && !(ok = mma2())) break;
+        first = q.item_first(), last = q.item_last();
       }
+      if (ok && t1 > 0) mma2();
       commit_pair(done);
       drain_wait(done, 0);
     }
@@ -205,7 +204,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + DZDH_WARPS
     const uint32_t to_s = map_rank(s_empty, 0), to_dz = map_rank(dz_full, 0), to_dh = map_rank(dh_empty, 0);
     const int live = *p.live;
     float lse = 0.f, rs = 0.f;
-    int tgt = -1, t = 0, items = 0;
+    int tgt = -1, t = 0, shares = 0, share_of = -1;  // the row tile whose share of dh is still to be written
+    bool ok = true;
+    auto write_share = [&]() {
+      if (!warp_wait(dh_full, shares & 1, ab)) return false;
+      ++shares;
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = w.slice * (N2 / 4); c < min((w.slice + 1) * (N2 / 4), p.D); c += 32) {
+        float v[32];
+        acc_load32(dh_acc + lanes + c, false, v);
+        const uint32_t s = box.take();
+        box.put32(s, v);
+        box.store(s, &p.tpart, c, rank * BM + 32 * w.quad, share_of + pair);
+      }
+      share_of = -1;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(to_dh);
+      return true;
+    };
     for (Steps q(walk, p.s, pair, rank); q.valid(); q.next(), ++t) {
       const int row = q.it.row0 + w.row();
       if (q.item_first()) {
@@ -213,7 +231,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + DZDH_WARPS
         rs = row < live ? p.rs[row] : 0.f;
         tgt = row < live ? p.tgt[row] - p.v0 : -1;
       }
-      if (!warp_wait(s_full, t & 1, ab)) break;
+      if (!(ok = warp_wait(s_full, t & 1, ab))) break;
       tc_fence_after();
       uint32_t z[2][32];
       tmem_load32x2(tmem + lanes + w.slice * 64, z[0], tmem + lanes + w.slice * 64 + 32, z[1]);
@@ -246,7 +264,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + DZDH_WARPS
         for (int i = 0; i < 16; ++i) d[h][i] = pack2(v[2 * i], v[2 * i + 1], p.bf16);
       }
       // free once MMA 2 of the tile before and the warp's own store out of it have read it
-      if (!warp_wait(dz_empty, (t & 1) ^ 1, ab)) break;
+      if (!(ok = warp_wait(dz_empty, (t & 1) ^ 1, ab))) break;
+      if (share_of >= 0 && !(ok = write_share())) break;  // through the same box, the item before being complete
       const uint32_t b = box.take();
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -255,28 +274,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + DZDH_WARPS
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        // the writes of both CTAs have to be visible to the even one's MMA: a release over the cluster
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(to_dz) : "memory");
+        // Each CTA's tensor core reads its own shared memory: the proxy fence above has made the warp's
+        // writes visible there, and the arrival on the even CTA's barrier comes after it. (A release over
+        // the whole cluster adds a memory barrier per warp and tile.)
+        asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(to_dz) : "memory");
         if (p.store_dz && q.it.row0 < p.Mp) tma_store_3d(&p.tdz, b, col, q.it.row0 + 32 * w.quad, 0);
         bulk_commit();
       }
-      if (!q.item_last()) continue;
-      // the run's share of dh for these rows
-      if (!warp_wait(dh_full, items & 1, ab)) break;
-      ++items;
-      tc_fence_after();
-#pragma unroll 1
-      for (int c = w.slice * (N2 / 4); c < min((w.slice + 1) * (N2 / 4), p.D); c += 32) {
-        float v[32];
-        acc_load32(dh_acc + lanes + c, false, v);
-        const uint32_t s = box.take();
-        box.put32(s, v);
-        box.store(s, &p.tpart, c, rank * BM + 32 * w.quad, q.it.mt + pair);
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(to_dh);
+      if (q.item_last()) share_of = q.it.mt;
     }
+    if (ok && share_of >= 0) write_share();
     box.finish();
   }
   // ---------------------------------------------------------------- teardown
