@@ -116,7 +116,8 @@ __global__ void __launch_bounds__(AT) act8_pack_kernel(ActArgs p) {
       const int col = c0 + 256 * j + 8 * lane, cnt = p.D - col;
       if (c0 + 256 * j >= p.D) break;  // the same for the whole warp
       uint32_t top = v[j].top(bf16);   // not negative: ordered as integers
-      if (__any_sync(0xffffffffu, top >= 0x7f800000u)) {  // an infinity: the largest of the finite ones, value by value
+      const bool odd = top >= 0x7f800000u;
+      if (__any_sync(0xffffffffu, odd)) {  // an infinity: the largest of the finite ones, value by value
         top = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -130,19 +131,30 @@ __global__ void __launch_bounds__(AT) act8_pack_kernel(ActArgs p) {
       // top = f * 2^k, 1 <= f < 2 (subnormals fall below the range anyway): 448 = 1.75 * 2^8
       int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffff) > 0x600000);
       e = max(lo, min(hi, top == 0 ? lo : e));
-      if (cnt <= 0) continue;
-      const float scale = pow2(-e), end = e == hi ? 240.f : 448.f;
+      const float scale = pow2(-e);
       uint32_t w[2];
+      // Magnitudes are at most 448 after scaling, and NaN stays NaN in the conversion: only infinities
+      // and the largest exponent (where values end at 240) need a look at each value.
+      if (!__any_sync(0xffffffffu, odd || e == hi)) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = v[j].pair(k, bf16);
-        // NaN stays NaN in the conversion; an infinity becomes one here; past `end` only in the largest exponent
-        float a = f.x * scale, c = f.y * scale;
-        a = fabsf(a) > end ? (fabsf(a) == INFINITY ? __int_as_float(0x7fc00000) : copysignf(end, a)) : a;
-        c = fabsf(c) > end ? (fabsf(c) == INFINITY ? __int_as_float(0x7fc00000) : copysignf(end, c)) : c;
-        const uint32_t h = to_e4m3x2(a, c);
-        w[k / 2] = k & 1 ? w[k / 2] | (h << 16) : h;
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = v[j].pair(k, bf16);
+          const uint32_t h = to_e4m3x2(f.x * scale, f.y * scale);
+          w[k / 2] = k & 1 ? w[k / 2] | (h << 16) : h;
+        }
+      } else {
+        const float end = e == hi ? 240.f : 448.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = v[j].pair(k, bf16);
+          float a = f.x * scale, c = f.y * scale;
+          a = fabsf(a) > end ? (fabsf(a) == INFINITY ? __int_as_float(0x7fc00000) : copysignf(end, a)) : a;
+          c = fabsf(c) > end ? (fabsf(c) == INFINITY ? __int_as_float(0x7fc00000) : copysignf(end, c)) : c;
+          const uint32_t h = to_e4m3x2(a, c);
+          w[k / 2] = k & 1 ? w[k / 2] | (h << 16) : h;
+        }
       }
+      if (cnt <= 0) continue;
       uint8_t* dst = p.q + row * p.ldq + col;
       if (cnt >= 8) {
         *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
