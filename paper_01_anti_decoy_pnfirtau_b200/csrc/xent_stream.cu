@@ -440,12 +440,15 @@ __global__ void __launch_bounds__(1024) xent_scale_kernel(ScaleArgs p) {
     return;
   }
   float m = 0.f;
-  for (int i = threadIdx.x; i < n; i += 1024) m = fmaxf(m, fabsf(p.dloss[p.s.idx[i] * p.stride]));
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    const float v = fabsf(p.dloss[p.s.idx[i] * p.stride]);
+    m = v < INFINITY ? fmaxf(m, v) : m;  // an infinite or NaN factor stays its own row's
+  }
   m = group_max<32>(m);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
   __syncthreads();
   m = group_max<32>(red[threadIdx.x & 31]);
-  if (!(m > 0.f)) m = 1.f;  // all zero (or NaN alone, which the factors carry)
+  if (!(m > 0.f)) m = 1.f;  // all zero, or none finite
   for (int i = threadIdx.x; i < n; i += 1024) p.rs[i] = p.dloss[p.s.idx[i] * p.stride] / m * p.top;
   if (threadIdx.x == 0) *p.alpha = m / p.top;
 }

@@ -264,6 +264,20 @@ def test_xent_zero_and_huge_upstream_gradients(cuda):
 
 
 # ------------------------------------------------------------------ streams, graphs, reruns, differences
+@pytest.mark.parametrize("D", [64, 320])
+def test_xent_infinite_upstream_gradient_of_one_row(cuda, D):
+    h, w = rand(70, D, seed=8), rand(300, D, std=D ** -0.5, seed=9)
+    t = torch.arange(70, device=cuda)
+    dloss = torch.ones(70, device=cuda)
+    want = xent_all(h, w, t, dloss=dloss, reduction="none")[1]
+    for bad in (float("inf"), float("nan")):
+        dloss[33] = bad
+        dh = xent_all(h, w, t, dloss=dloss, reduction="none")[1]
+        rest = torch.arange(70, device=cuda) != 33
+        assert not torch.isfinite(dh[33]).any()
+        assert torch.equal(dh[rest], want[rest])
+
+
 def test_calls_on_another_stream(cuda):
     x, wg, wu, t, w = rand(500, 256), rand(384, 256, std=0.05, seed=1), rand(384, 256, std=0.05, seed=2), torch.randint(0, 999, (500,), device=cuda), rand(999, 256, std=0.1, seed=3)
     want = gated_all(x, wg, wu), xent_all(x, w, t), act8_weight_grad(x, act8_pack(x))
