@@ -309,6 +309,37 @@ def test_two_streams_at_once(cuda):
         same(a, b)
 
 
+def test_offsets_past_32_bits(cuda):
+    """The far end of tensors of more than 2^31 elements. bf16 results of two summation orders
+    of fp32 sums differ by one rounding each at most: 2^-8 relative in all."""
+    far = slice(-300, None)
+    M, D, F_ = 66_000, 64, 33_000  # h, dh, and dg beside du
+    x, wg, wu = rand(M, D), rand(F_, D, std=D ** -0.5, seed=1), rand(F_, D, std=D ** -0.5, seed=2)
+    dh = rand(1, F_, seed=3).expand(M, F_).contiguous()
+    xa = x.detach().requires_grad_(True)
+    h = gated_linear(xa, wg, wu)
+    dx, = torch.autograd.grad(h, xa, dh)
+    xb = x[far].detach().requires_grad_(True)
+    hb = gated_linear(xb, wg, wu)
+    assert torch.equal(h[far], hb)
+    assert rel_l2(dx[far], torch.autograd.grad(hb, xb, dh[far])[0]) < 2 ** -8
+    del h, dh, dx
+    M, D = 2_100_000, 1032
+    x = rand(4096, D).repeat(M // 4096 + 1, 1)[:M]
+    assert torch.equal(act8_unpack(act8_pack(x))[far], act8_unpack(act8_pack(x[far])))
+    del x
+    V, D, M = 2_200_000, 1000, 64
+    w, h = rand(V, D, std=D ** -0.5), rand(M, D, seed=5)
+    t = V - 1 - torch.arange(M, device=cuda)
+    loss, gh, gw = xent_all(h, w, t, reduction="sum")
+    z = torch.cat([h.float() @ c.float().t() for c in w.split(550_000)], 1)
+    p = torch.softmax(z, 1)
+    assert abs(loss.item() - F.cross_entropy(z, t, reduction="sum").item()) < 1e-4 * loss.item()
+    p[torch.arange(M), t] -= 1
+    # two roundings to bf16, of dz and of the result, and TF32 or fp32 sums in the plain form
+    assert rel_l2(gw[-300:], p[:, -300:].t() @ h.float()) < 2 ** -8 + 2 ** -9
+
+
 @pytest.mark.parametrize("M", [8, 600])
 def test_forward_captured_and_replayed_on_new_inputs(cuda, M):
     x, w, t = rand(M, 128), rand(2000, 128, std=0.1, seed=1), torch.randint(0, 2000, (M,), device=cuda)
