@@ -133,7 +133,7 @@ __device__ __forceinline__ void commit_pair(uint32_t bar) {
 // of one row tile and one split of K; items are taken group_m row tiles at a time, the row
 // tile running fastest, so the pairs in flight share both operands in L2. Runs (`runs`): the
 // tiles, row tile by row tile, are dealt to the pairs in equal contiguous runs, and an item
-// is a run's part of one row tile: the pairs end together, and a pair keeps its rows of A.
+// is a run's part of one row tile: the pairs end together, and a pair finds its rows of A in L2 for many tiles.
 // For a B that stays in L2 as a whole. strips = 0: strips as fit the number of row tiles (the
 // rows that count, known on the device alone), see auto_strips.
 struct Sched {
@@ -177,7 +177,6 @@ struct Args {
   CUtensorMap ta[2], tb[2];
   Sched s;
   uint32_t idesc;
-  int stages;  // of the ring
   int32_t* status;
 };
 
@@ -299,31 +298,24 @@ struct EpiWarp {
 // column is in registers), done() at the end.
 // DUAL_B: columns 0-127 of a tile come from tb[0] and 128-255 from tb[1], both at row
 // 128 * nt.
-// KEEP_A: an item's rows of A (all of K, at most a few hundred) stay in shared memory for
-// all of its tiles and the ring carries B alone: at K = 256 a tile's MMAs take 2048 clocks,
-// in which A and B together (128 KB per CTA) ask more of L2 than it gives.
-constexpr int MAX_STAGES = 14;
 template <class Epi>
 constexpr int box_bytes() {
   return Epi::WARPS * Epi::BOXES * Epi::BOX_BYTES;
 }
 template <class Epi>
-constexpr int stages(bool keep_a, int kb) {
-  const int n = keep_a ? (STAGE_MAX - box_bytes<Epi>() - kb * HALF_BYTES) / HALF_BYTES : (STAGE_MAX - box_bytes<Epi>()) / STAGE_BYTES;
-  return n > MAX_STAGES ? MAX_STAGES : n;
+constexpr int stages() {
+  return (STAGE_MAX - box_bytes<Epi>()) / STAGE_BYTES;
 }
 constexpr int SMEM = STAGE_MAX + 1024;
 
-template <bool A_MN, bool B_MN, bool DUAL_B, bool KEEP_A, class Epi>
+template <bool A_MN, bool B_MN, bool DUAL_B, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS), 1)
     gemm_kernel(const __grid_constant__ Args p, const __grid_constant__ typename Epi::Params ep) {
-  static_assert(!KEEP_A || !A_MN, "kept rows of A are K-major");
-  constexpr int EPI_WARPS = Epi::WARPS, SLOT = KEEP_A ? HALF_BYTES : STAGE_BYTES;
-  const int stages = p.stages;
+  constexpr int EPI_WARPS = Epi::WARPS, STAGES = stages<Epi>();
   extern __shared__ __align__(1024) uint8_t raw[];
-  const uint32_t sb = (smem_u32(raw) + 1023u) & ~1023u;
-  // full, empty, acc full x2, acc empty x2, done, A full, A empty, warps
-  __shared__ __align__(8) uint64_t bars[2 * MAX_STAGES + 7 + EPI_WARPS];
+  const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
+  // full, empty, acc full x2, acc empty x2, done, warps
+  __shared__ __align__(8) uint64_t bars[2 * STAGES + 5 + EPI_WARPS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   launch_next();
@@ -331,17 +323,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
   const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const uint32_t b0 = smem_u32(bars);
   auto full = [&](int s) { return b0 + 8u * s; };
-  auto empty = [&](int s) { return b0 + 8u * (MAX_STAGES + s); };
-  auto acc_full = [&](int s) { return b0 + 8u * (2 * MAX_STAGES + s); };
-  auto acc_empty = [&](int s) { return b0 + 8u * (2 * MAX_STAGES + 2 + s); };
-  const uint32_t done = b0 + 8u * (2 * MAX_STAGES + 4), a_full = done + 8, a_empty = done + 16;
-  auto warp_bar = [&](int w) { return b0 + 8u * (2 * MAX_STAGES + 7 + w); };
-  const uint32_t ring = sb + (KEEP_A ? (uint32_t)p.s.kb * HALF_BYTES : 0u);
+  auto empty = [&](int s) { return b0 + 8u * (STAGES + s); };
+  auto acc_full = [&](int s) { return b0 + 8u * (2 * STAGES + s); };
+  auto acc_empty = [&](int s) { return b0 + 8u * (2 * STAGES + 2 + s); };
+  const uint32_t done = b0 + 8u * (2 * STAGES + 4);
+  auto warp_bar = [&](int w) { return b0 + 8u * (2 * STAGES + 5 + w); };
   const Abort ab{&abort_flag, p.status};
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int s = 0; s < stages; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(full(s), 1);   // the even CTA's: its producer's arrival, and the bytes of both CTAs
       mbar_init(empty(s), 1);  // the MMAs that read the stage, told to both CTAs
     }
@@ -350,8 +341,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
       mbar_init(acc_empty(s), Epi::PING_PONG ? EPI_WARPS : 2 * EPI_WARPS);  // the even CTA's: the epilogue warps of both
     }
     mbar_init(done, 1);
-    mbar_init(a_full, 1);
-    mbar_init(a_empty, 1);
     for (int w = 0; w < EPI_WARPS; ++w) mbar_init(warp_bar(w), 1);
     fence_barrier_init();
   }
@@ -370,28 +359,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
   if (warp == 0) {
     // -------------------------------------------------------------- TMA producer
     if (lane == 0) {
-      int st = 0, ph = 1, issued = 0, items = 0;
+      int st = 0, ph = 1, issued = 0;
       bool ok = true;
       for (Steps q(walk, p.s, pair, rank); ok && q.valid(); q.next()) {
-        if (KEEP_A && q.item_first()) {
-          if (!mbar_wait(a_empty, (items & 1) ^ 1, ab)) break;
-          if (rank == 0) mbar_arrive_expect_tx(a_full, (uint32_t)(2 * HALF_BYTES * q.it.kbn));
-          for (int kb = 0; kb < q.it.kbn; ++kb)
-            tma_load_pair(sb + (uint32_t)kb * HALF_BYTES, &p.ta[0], map_rank(a_full, 0), kb * BK, q.it.row0);
-          ++items;
-        }
         for (int kb = q.kb; kb < q.kb_end(); ++kb) {
           if (!mbar_wait(empty(st), ph, ab)) {
             ok = false;
             break;
           }
-          if (rank == 0) mbar_arrive_expect_tx(full(st), 2 * SLOT);
+          if (rank == 0) mbar_arrive_expect_tx(full(st), 2 * STAGE_BYTES);
           const uint32_t bar = map_rank(full(st), 0);
           const int seg = kb >= p.s.seg_kb;
           const int k = (kb - (seg ? p.s.seg_kb : 0)) * BK;
-          const uint32_t sa = ring + (uint32_t)st * SLOT, sB = KEEP_A ? sa : sa + HALF_BYTES;
-          if (KEEP_A) {
-          } else if (A_MN) {
+          const uint32_t sa = ring + (uint32_t)st * STAGE_BYTES, sB = sa + HALF_BYTES;
+          if (A_MN) {
 #pragma unroll
             for (int g = 0; g < BM / 64; ++g) tma_load_pair(sa + g * GROUP_BYTES, &p.ta[seg], bar, q.it.row0 + 64 * g, k);
           } else {
@@ -407,29 +388,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
             tma_load_pair(sB, &p.tb[seg], bar, k, q.nt * BN + rank * (BN / 2));
           }
           ++issued;
-          if (++st == stages) st = 0, ph ^= 1;
+          if (++st == STAGES) st = 0, ph ^= 1;
         }
       }
       // Never leave a copy in flight into shared memory: the even CTA's barriers count the
       // copies of both, and the odd CTA stays until the even one comes to the final barrier.
       if (rank == 0) {
-        if (KEEP_A && items > 0) drain_wait(a_full, (items - 1) & 1);
-        for (int n = 0; n < min(issued, stages); ++n) {
+        for (int n = 0; n < min(issued, STAGES); ++n) {
           const int last = issued - 1 - n;
-          drain_wait(full(last % stages), (last / stages) & 1);
+          drain_wait(full(last % STAGES), (last / STAGES) & 1);
         }
       }
     }
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMA issuer (even CTA)
     if (rank == 0 && lane == 0) {
-      int st = 0, ph = 0, t = 0, items = 0;
+      int st = 0, ph = 0, t = 0;
       bool ok = true;
       for (Steps q(walk, p.s, pair, rank); ok && q.valid(); q.next(), ++t) {
-        if (KEEP_A && q.item_first()) {
-          if (!mbar_wait(a_full, items & 1, ab)) break;
-          ++items;
-        }
         if (!mbar_wait(acc_empty(t & 1), ((t >> 1) & 1) ^ 1, ab)) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(t & 1) * BN;
@@ -439,17 +415,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
             break;
           }
           tc_fence_after();
-          const uint32_t slot = ring + (uint32_t)st * SLOT;
-          const uint32_t da = sw128_desc(KEEP_A ? sb + (uint32_t)kb * HALF_BYTES : slot, A_MN ? GROUP_BYTES : 0);
-          const uint32_t db = sw128_desc(KEEP_A ? slot : slot + HALF_BYTES, B_MN ? GROUP_BYTES : 0);
+          const uint32_t slot = ring + (uint32_t)st * STAGE_BYTES;
+          const uint32_t da = sw128_desc(slot, A_MN ? GROUP_BYTES : 0);
+          const uint32_t db = sw128_desc(slot + HALF_BYTES, B_MN ? GROUP_BYTES : 0);
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk)  // 16 K: 32 bytes of a K-major row, 16 rows (2048 bytes) MN-major
             mma_pair(d, da + kk * (A_MN ? 128 : 2), db + kk * (B_MN ? 128 : 2), p.idesc, kb > q.kb || kk > 0);
           commit_pair(empty(st));
-          if (++st == stages) st = 0, ph ^= 1;
+          if (++st == STAGES) st = 0, ph ^= 1;
         }
         if (ok) commit_pair(acc_full(t & 1));
-        if (KEEP_A && ok && q.item_last()) commit_pair(a_empty);
       }
       commit_pair(done);
       drain_wait(done, 0);  // no MMA may still be writing TMEM, or reading either CTA's tiles, at teardown
@@ -458,7 +433,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + Epi::WARPS
     // -------------------------------------------------------------- epilogue
     const int part = (warp - 2) >> 2;
     const EpiWarp w{warp & 3, Epi::PING_PONG ? part & 1 : 0, Epi::PING_PONG ? part >> 1 : part, lane,
-                    ring + (uint32_t)(stages * SLOT + (warp - 2) * Epi::BOXES * Epi::BOX_BYTES), warp_bar(warp - 2)};
+                    ring + (uint32_t)(STAGES * STAGE_BYTES + (warp - 2) * Epi::BOXES * Epi::BOX_BYTES), warp_bar(warp - 2)};
     Epi epi(ep, w, ab);
     int t = 0;
     for (Steps q(walk, p.s, pair, rank); q.valid(); q.next(), ++t) {
@@ -844,35 +819,28 @@ inline Sched plain_sched(int64_t m, int64_t n, int64_t kb, int splits) {
   return s;
 }
 
-// Runs where all of B (n rows of k elements) stays in L2 beside what streams through it.
-inline void runs_if_resident(Sched* s, int64_t n, int64_t k) { s->runs = n * k * 2 <= ((int64_t)48 << 20); }
+// Runs where all of B (n rows of k elements) stays in L2 beside what streams through it. Measured
+// (B200, bf16), runs against strips, by the size of B: gated product 16384 x 1024 x 4096, 17 MB, 182
+// and 196 us; cross entropy's forward 16352 x 33278 x 256, 17 MB, 247 and 278; 8192 x 50021 x 512,
+// 51 MB, 294 and 308; gated product 8192 x 2048 x 8192, 67 MB, 404 and 368; cross entropy
+// 8192 x 50021 x 1024, 102 MB, 633 and 562.
+inline void runs_if_resident(Sched* s, int64_t n, int64_t k) { s->runs = n * k * 2 <= ((int64_t)56 << 20); }
 
-template <bool A_MN, bool B_MN, bool DUAL_B, bool KEEP_A, class Epi>
-int launch_kernel(const char* what, Args a, const typename Epi::Params& ep, cudaStream_t st) {
+template <bool A_MN, bool B_MN, bool DUAL_B, class Epi>
+int launch(const char* what, const Args& a, const typename Epi::Params& ep, cudaStream_t st) {
   const int64_t items = (int64_t)a.s.tiles_m * (a.s.runs || !a.s.strips ? a.s.tiles_n : a.s.strips) * a.s.splits;
   if (items <= 0) return PNFT_OK;
   if (items > (1 << 30)) return fail(PNFT_EUNSUPPORTED, "%s: too many tiles", what);
-  auto* k = gemm_kernel<A_MN, B_MN, DUAL_B, KEEP_A, Epi>;
+  auto* k = gemm_kernel<A_MN, B_MN, DUAL_B, Epi>;
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel has its shared memory
   const uint64_t bit = 1ull << (current_device() & 63);
   if (!(ready.load(std::memory_order_acquire) & bit)) {
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return check_launch(what, 0);
     ready.fetch_or(bit, std::memory_order_release);
   }
-  a.stages = stages<Epi>(KEEP_A, a.s.kb);
   launch_dependent(k, dim3((unsigned)(2 * pairs_of(items))), 32 * (2 + Epi::WARPS), SMEM, st, a, ep);
   return check_launch(what, 1);
 }
-template <bool A_MN, bool B_MN, bool DUAL_B, class Epi>
-int launch(const char* what, const Args& a, const typename Epi::Params& ep, cudaStream_t st) {
-  if constexpr (!A_MN) {
-    // rows of A are kept where that leaves the ring at least four stages and an item has several tiles
-    if ((a.s.runs || !a.s.strips) && a.s.splits == 1 && a.s.chunk >= a.s.kb && stages<Epi>(true, a.s.kb) >= 4)
-      return launch_kernel<A_MN, B_MN, DUAL_B, true, Epi>(what, a, ep, st);
-  }
-  return launch_kernel<A_MN, B_MN, DUAL_B, false, Epi>(what, a, ep, st);
-}
-
 // C = A B^T with the plain epilogue; K in chunks of 2048 for an fp32 C (see StoreEpi).
 constexpr int PROMOTE_KB = 32;
 template <bool A_MN, bool B_MN>
@@ -882,9 +850,9 @@ int launch_store(const char* what, Args a, const StoreEpi<false>::Params& ep, cu
     typename StoreEpi<true>::Params e;
     static_assert(sizeof(e) == sizeof(ep), "same parameters");
     memcpy(&e, &ep, sizeof(e));
-    return launch_kernel<A_MN, B_MN, false, false, StoreEpi<true>>(what, a, e, st);
+    return launch<A_MN, B_MN, false, StoreEpi<true>>(what, a, e, st);
   }
-  return launch_kernel<A_MN, B_MN, false, false, StoreEpi<false>>(what, a, ep, st);
+  return launch<A_MN, B_MN, false, StoreEpi<false>>(what, a, ep, st);
 }
 
 // An operand that TMA can read: 16-byte base, row stride a multiple of 8 elements

@@ -209,10 +209,12 @@ def act8_weight_grad(dy: torch.Tensor, p: Act8, out_dtype: torch.dtype = torch.f
 
 
 # ---------------------------------------------------------------- gated product
-# From this input width on the forward keeps the pre-activations (3 bytes of each element,
+# From this input width on the forward keeps the pre-activations (6 bytes of each pair,
 # written once and read once by a pointwise backward kernel); below it the backward
-# computes them again, which costs 4 M D F operations but no memory traffic.
-_KEEP_FROM = 640
+# computes them again, which costs 4 M D F operations but no memory traffic. Forward and
+# backward on a B200 (bf16, 16384 rows, F = 4 D), kept against computed again: D = 512
+# 286 and 249 us, 768 503 and 480, 1024 820 and 840, 2048 2700 and 3102.
+_KEEP_FROM = 896
 _FEW = 24  # rows up to which the forward kernels take any row strides
 
 
