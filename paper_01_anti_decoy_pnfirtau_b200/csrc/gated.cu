@@ -21,7 +21,7 @@ namespace {
 
 using namespace tc;
 
-constexpr float kSqrtHalf = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143268f, kLog2e = 1.4426950408889634f;
+constexpr float kInvSqrt2Pi = 0.39894228040143268f, kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float fast_ex2(float x) {
   float r;
@@ -34,9 +34,16 @@ __device__ __forceinline__ float fast_rcp(float x) {
   return r;
 }
 
-// act(g); deriv: also act'(g). The exponentials and the quotient are the fast ones
-// (a few units of 2^-23): the results are rounded to 16 bits. GELU's normal
-// distribution goes through erfc, which keeps its relative accuracy for g << 0.
+// act(g); deriv: also act'(g). The exponentials and the quotients are the fast ones
+// (a few units of 2^-23; results below 2^-126 are 0): the results are rounded to 16 bits.
+// GELU's normal distribution: for a = |g| and t = 1 / (1 + 0.3 a)
+//   Phi(-a) = exp(-a^2 / 2) t Q(t),
+// where t Q(t) stands for exp(a^2 / 2) erfc(a / sqrt 2) / 2, Q the polynomial of degree 7
+// with the least relative error on 0 <= a <= 14 (1.5e-7; fitted by reweighted least
+// squares). With fp32's rounding the relative error is 2^-20 up to a = 3 and 2^-17 where
+// Phi(-a) ends, so the far negative side keeps its digits; Phi(a) = 1 - Phi(-a). It shares
+// its exponential with the derivative (B200, 4095 x 1000 x 2731 with biases: the forward kernel
+// 55 us and the backward one 57, 61 and 64 with erfcf).
 template <bool DERIV, int ACT>
 __device__ __forceinline__ float act_value(float g, float* deriv) {
   if (ACT == PNFT_ACT_SILU) {
@@ -44,8 +51,17 @@ __device__ __forceinline__ float act_value(float g, float* deriv) {
     if (DERIV) *deriv = s * (1.f + g * (1.f - s));
     return g * s;
   }
-  const float cdf = 0.5f * erfcf(-kSqrtHalf * g);
-  if (DERIV) *deriv = cdf + g * (kInvSqrt2Pi * fast_ex2(-0.5f * kLog2e * g * g));
+  const float a = fabsf(g), t = fast_rcp(fmaf(0.3f, a, 1.f)), e = fast_ex2(-0.5f * kLog2e * a * a);
+  float q = 0.0356748118f;
+  q = fmaf(q, t, -0.157203222f);
+  q = fmaf(q, t, 0.206353707f);
+  q = fmaf(q, t, -0.0536837867f);
+  q = fmaf(q, t, 0.128561677f);
+  q = fmaf(q, t, 0.0999134846f);
+  q = fmaf(q, t, 0.120753956f);
+  q = fmaf(q, t, 0.119629299f);
+  const float tail = q * t * e, cdf = g < 0.f ? tail : 1.f - tail;
+  if (DERIV) *deriv = cdf + g * (kInvSqrt2Pi * e);
   return g * cdf;
 }
 
