@@ -509,9 +509,7 @@ BwdLayout bwd_layout(int64_t M, int64_t D, int64_t F) {
   l.d = take(2 * (size_t)M * 2 * l.Fp);
   l.dh = take(F % 8 ? 2 * (size_t)M * l.Fp : 0);
   l.bias = take(sizeof(float) * 2 * (size_t)F * (size_t)((M + point_rows(M, F) - 1) / point_rows(M, F)));
-  const int s = plan_splits(tiles_of(M, D), 2 * ((F + BK - 1) / BK));
-  const size_t dx = s > 1 ? sizeof(float) * (size_t)s * (size_t)M * (size_t)((D + 3) / 4 * 4) : 0;
-  l.part = take(std::max(dx, pnft_weight_grad_workspace_size(M, 2 * l.Fp, D)));
+  l.part = take(std::max(product_workspace(M, D, 2 * ((F + BK - 1) / BK)), pnft_weight_grad_workspace_size(M, 2 * l.Fp, D)));
   l.total = at;
   return l;
 }
@@ -557,26 +555,11 @@ int gated_dx(const uint16_t* dg, const uint16_t* du, int64_t ldd, const void* wg
   if (!rc) rc = map_mnmajor(&a.tb[0], wg, D, F, ldwg);
   if (!rc) rc = map_mnmajor(&a.tb[1], wu, D, F, ldwu);
   if (rc) return rc;
-  const int kb = (int)((F + BK - 1) / BK), splits = plan_splits(tiles_of(M, D), 2 * kb);
-  a.s = plain_sched(M, D, 2 * kb, splits);
-  a.s.seg_kb = kb;
+  const int kb = (int)((F + BK - 1) / BK);
   a.idesc = idesc(dtype, false, true);
   a.status = status;
-  StoreEpi<false>::Params out;
-  memset(&out, 0, sizeof(out));
-  out.row_split = 0x7fffffff;
-  out.dtype = dx_dtype;
-  if (splits == 1) {
-    rc = make_out(&out.c[0], dx, dx_dtype, D, M, lddx);
-    return rc ? rc : launch_store<false, true>("gated_bwd dx", a, out, st);
-  }
-  const int64_t ldp = (D + 3) / 4 * 4;
-  out.dtype = PNFT_DTYPE_F32;
-  rc = make_out(&out.c[0], part, PNFT_DTYPE_F32, D, M, ldp, splits, M * ldp);
-  if (!rc) rc = launch_store<false, true>("gated_bwd dx", a, out, st);
-  if (rc) return rc;
-  const SumArgs sum{{dx, nullptr}, lddx, 0x7fffffff, (int)M, (int)D, nullptr, dx_dtype, 0, rows16(dx, lddx, dtype_size(dx_dtype))};
-  return sum_splits(static_cast<const float*>(part), ldp, M * ldp, splits, sum, (int)M, st);
+  const SumArgs c{{dx, nullptr}, lddx, 0x7fffffff, (int)M, (int)D, nullptr, dx_dtype, 0, rows16(dx, lddx, dtype_size(dx_dtype))};
+  return product<false, true>("gated_bwd dx", a, c, static_cast<float*>(part), M, D, 2 * kb, kb, nullptr, st);
 }
 
 }  // namespace

@@ -27,20 +27,59 @@ int plan_splits(int64_t tiles, int64_t kb, int rounds) {
   return (int)std::max<int64_t>(1, std::min(want, kb / 8));
 }
 
+// A round of whole tiles takes 0.42 us per K block; split tiles take a launch more and write and
+// read their partials (0.09 us each, from L2). Measured (B200, weight gradient from 8 bits, fp32
+// out), the last round split and whole: 8192 rows into 4096 x 4096 (34 of 256 tiles in the last
+// round, split in 2) 218 and 228 us; 4096 into 5632 x 1000 (14 of 88, in 5) 53 and 65; 2048 into
+// 2560 x 2560 (26 of 100, K too short: whole) 38.
+Plan plan_product(int64_t tiles, int64_t kb) {
+  const int pairs = sm_count() / 2;
+  if (tiles <= pairs) return Plan{plan_splits(tiles, kb), 0};
+  const int rest = (int)(tiles % pairs);
+  Plan best{1, 0};
+  float least = rest ? 0.42f * (float)kb : 0.f;
+  for (int n = 2; n <= 8 && kb / n >= 8; ++n) {
+    const float cost = 0.42f * (float)kb * (float)((rest * n + pairs - 1) / pairs) / (float)n + 4.f + 0.09f * (float)(rest * n);
+    if (cost < least) least = cost, best = Plan{n, (int)(tiles - rest)};
+  }
+  return best;
+}
+
+size_t product_workspace(int64_t M, int64_t N, int64_t kb) {
+  if (M <= 0 || N <= 0 || kb <= 0) return 0;
+  const int64_t tiles = tiles_of(M, N);
+  const Plan p = plan_product(tiles, kb);
+  if (p.splits == 1) return 0;
+  if (p.whole) return sizeof(float) * (size_t)(PM * BN) * (size_t)(tiles - p.whole) * (size_t)p.splits;
+  return sizeof(float) * (size_t)p.splits * (size_t)M * (size_t)((N + 3) / 4 * 4);
+}
+
 namespace {
 
+// Where the split tiles behind whole ones lie (sum_splits_kernel<true>).
+struct TailArgs {
+  int tiles_m, tiles_n, group_m, whole;
+};
+
 // Four columns per thread; partial rows are 16-byte aligned (ldp a multiple of 4).
+template <bool TAIL>
 __global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict__ part, int64_t ldp,
                                                          int64_t split_stride, int splits, SumArgs o,
-                                                         int rows_total) {
+                                                         int rows_total, TailArgs tail) {
   launch_next();
   wait_previous();
-  const int n4 = (o.cols + 3) / 4;
+  const int n4 = TAIL ? BN / 4 : (o.cols + 3) / 4;
   const float alpha = o.alpha ? *o.alpha : 1.f;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)rows_total * n4; i += (int64_t)gridDim.x * 256) {
     int row = (int)(i / n4);
-    const int c = (int)(i - (int64_t)row * n4) * 4;
+    int c = (int)(i - (int64_t)row * n4) * 4;
     const float* src = part + (int64_t)row * ldp + c;
+    if (TAIL) {  // a row of a tile: its place in the matrix
+      int mt, nt;
+      item_order(tail.whole + row / PM, tail.tiles_m, tail.tiles_n, tail.group_m, &mt, &nt);
+      row = mt * PM + row % PM, c += nt * BN;
+      if (c >= o.cols) continue;
+    }
     const int side = row >= o.row_split;
     if (side) row -= o.row_split;
     if (row >= o.rows || !(side ? o.c[1] : o.c[0])) continue;
@@ -96,7 +135,16 @@ int sum_splits(const float* part, int64_t ldp, int64_t split_stride, int splits,
                int rows_total, cudaStream_t st) {
   const int64_t items = (int64_t)rows_total * ((out.cols + 3) / 4);
   const int64_t blocks = std::min<int64_t>((items + 255) / 256, (int64_t)sm_count() * 8);
-  launch_dependent(sum_splits_kernel, dim3((unsigned)blocks), 256, 0, st, part, ldp, split_stride, splits, out, rows_total);
+  launch_dependent(sum_splits_kernel<false>, dim3((unsigned)blocks), 256, 0, st, part, ldp, split_stride, splits, out, rows_total,
+                   TailArgs{});
+  return check_launch("split sum", 1);
+}
+
+int sum_tail(const float* part, const Sched& s, const SumArgs& out, cudaStream_t st) {
+  const int rows = (s.tiles_m * s.tiles_n - s.whole) * PM;
+  const int64_t blocks = std::min<int64_t>((int64_t)rows * (BN / 4) / 256, (int64_t)sm_count() * 8);
+  launch_dependent(sum_splits_kernel<true>, dim3((unsigned)blocks), 256, 0, st, part, (int64_t)BN, (int64_t)rows * BN, s.splits, out,
+                   rows, TailArgs{s.tiles_m, s.tiles_n, s.group_m, s.whole});
   return check_launch("split sum", 1);
 }
 
@@ -105,8 +153,6 @@ int sum_splits(const float* part, int64_t ldp, int64_t split_stride, int splits,
 
 using namespace pnft;
 using namespace pnft::tc;
-
-static int wgrad_splits(int64_t K, int64_t M, int64_t N) { return plan_splits(tiles_of(M, N), (K + BK - 1) / BK); }
 
 namespace pnft {
 namespace tc {
@@ -119,38 +165,18 @@ int weight_grad(const char* what, const void* dy, int64_t lddy, const void* x, i
   int rc = map_mnmajor(&a.ta[0], dy, M, K, lddy);
   if (!rc) rc = map_mnmajor(&a.tb[0], x, N, K, ldx);
   if (rc) return rc;
-  const int splits = wgrad_splits(K, M, N);
-  a.s = plain_sched(M, N, (K + BK - 1) / BK, splits);
   a.idesc = idesc(dtype, true, true);
   a.status = status;
-  StoreEpi<false>::Params out;
-  memset(&out, 0, sizeof(out));
-  out.row_split = (int)row_split;
-  out.dtype = c_dtype;
-  if (splits == 1) {
-    rc = make_out(&out.c[0], c0, c_dtype, N, rows, ldc);
-    if (!rc && row_split < M) rc = make_out(&out.c[1], c1, c_dtype, N, rows, ldc);
-    return rc ? rc : launch_store<true, true>(what, a, out, st);
-  }
-  const int64_t ldp = (N + 3) / 4 * 4;
-  out.row_split = 0x7fffffff;
-  out.dtype = PNFT_DTYPE_F32;
-  rc = make_out(&out.c[0], workspace, PNFT_DTYPE_F32, N, M, ldp, splits, M * ldp);
-  if (!rc) rc = launch_store<true, true>(what, a, out, st);
-  if (rc) return rc;
-  const SumArgs sum{{c0, c1}, ldc, (int)row_split, (int)rows, (int)N, nullptr, c_dtype, 0,
-                    rows16(c0, ldc, dtype_size(c_dtype)) && rows16(c1, ldc, dtype_size(c_dtype))};
-  return sum_splits(static_cast<const float*>(workspace), ldp, M * ldp, splits, sum, (int)M, st);
+  const SumArgs c{{c0, c1}, ldc, (int)row_split, (int)rows, (int)N, nullptr, c_dtype, 0,
+                  rows16(c0, ldc, dtype_size(c_dtype)) && rows16(c1, ldc, dtype_size(c_dtype))};
+  return product<true, true>(what, a, c, static_cast<float*>(workspace), M, N, (K + BK - 1) / BK, 0, nullptr, st);
 }
 
 }  // namespace tc
 }  // namespace pnft
 
-
 extern "C" size_t pnft_weight_grad_workspace_size(int64_t K, int64_t M, int64_t N) {
-  if (K <= 0 || M <= 0 || N <= 0) return 0;
-  const int s = wgrad_splits(K, M, N);
-  return s > 1 ? sizeof(float) * (size_t)s * (size_t)M * (size_t)((N + 3) / 4 * 4) : 0;
+  return K <= 0 ? 0 : product_workspace(M, N, (K + BK - 1) / BK);
 }
 
 extern "C" int pnft_weight_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* c0, void* c1, int64_t ldc,

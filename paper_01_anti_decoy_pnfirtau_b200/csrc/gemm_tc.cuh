@@ -143,6 +143,7 @@ struct Sched {
   int tiles_per_strip;  // column tiles per item
   int kb;               // 64-deep K blocks (upper bound when live_k)
   int splits;           // splits of K
+  int whole;            // the first tiles, which are not split (strips of one tile)
   int chunk;            // K blocks that one accumulator takes before the epilogue collects it
   int group_m;
   int runs;
@@ -184,7 +185,17 @@ struct Item {
   int mt, nt0, ntn, split, kb0, kbn;
   int row0;  // first row of this CTA
   int slot;  // strip, or place of the run among those of its row tile
+  int part;  // place among the split items behind whole tiles, or -1
 };
+
+// Row tile and strip of item r: group_m row tiles at a time, the row tile running fastest.
+__host__ __device__ inline void item_order(int r, int tiles_m, int strips, int group_m, int* mt, int* strip) {
+  const int per = group_m * strips, g = r / per;
+  r -= g * per;
+  const int gm = tiles_m - g * group_m < group_m ? tiles_m - g * group_m : group_m;
+  *mt = g * group_m + r % gm;
+  *strip = r / gm;
+}
 
 struct Walk {
   int tiles_m, kb, slots, pairs;
@@ -203,7 +214,7 @@ struct Walk {
       per_strip = (s.tiles_n + strips - 1) / strips;
       group_m = max(tiles_m, 1);
     }
-    total = s.runs ? (int64_t)tiles_m * s.tiles_n : (int64_t)tiles_m * strips * s.splits;
+    total = s.runs ? (int64_t)tiles_m * s.tiles_n : s.whole + (int64_t)(tiles_m * strips - s.whole) * s.splits;
     pairs = s.runs ? run_pairs(total, launched) : launched;
     slots = s.runs ? run_slots(tiles_m, pairs) : strips;
   }
@@ -217,26 +228,24 @@ struct Walk {
   __device__ Item at(const Sched& s, int64_t i, int64_t end, int rank, int pair) const {
     Item it;
     if (s.runs) {
-      it.split = 0, it.kb0 = 0, it.kbn = kb;
+      it.split = 0, it.kb0 = 0, it.kbn = kb, it.part = -1;
       it.mt = (int)(i / s.tiles_n);
       const int64_t first = (int64_t)it.mt * s.tiles_n;
       it.nt0 = (int)(i - first);
       it.ntn = (int)min((int64_t)s.tiles_n, end - first) - it.nt0;
       it.slot = pair - run_owner(total, first, pairs);
     } else {
-      const int per_split = tiles_m * strips;
-      it.split = (int)(i / per_split);
-      int r = (int)(i - (int64_t)it.split * per_split);
-      const int per = group_m * strips, g = r / per;
-      r -= g * per;
-      const int gm = min(group_m, tiles_m - g * group_m);
-      it.mt = g * group_m + r % gm;
-      it.slot = r / gm;
+      const int per_split = tiles_m * strips - s.whole, j = (int)i - s.whole;
+      const bool split = j >= 0;
+      it.split = split ? j / per_split : 0;
+      it.part = split && s.whole > 0 ? j : -1;
+      item_order(split ? s.whole + j - it.split * per_split : (int)i, tiles_m, strips, group_m, &it.mt, &it.slot);
       it.nt0 = it.slot * per_strip;
       it.ntn = min(per_strip, s.tiles_n - it.nt0);
       // whole K blocks spread evenly over the splits
-      it.kb0 = (int)((int64_t)kb * it.split / s.splits);
-      it.kbn = (int)((int64_t)kb * (it.split + 1) / s.splits) - it.kb0;
+      const int splits = split ? s.splits : 1;
+      it.kb0 = (int)((int64_t)kb * it.split / splits);
+      it.kbn = (int)((int64_t)kb * (it.split + 1) / splits) - it.kb0;
     }
     it.row0 = it.mt * PM + rank * BM;
     return it;
@@ -662,7 +671,7 @@ struct Out {
 // ------------------------------------------------------------------ plain epilogue
 // C = alpha * acc as fp32, bf16 or fp16: the rows of two matrices one after the other
 // (row_split, a multiple of 128, rows apart), or the fp32 partials of the splits (slices),
-// or added to an fp32 C. PROMOTE: an item's accumulators (chunks of K) are collected in
+// or added to an fp32 C; of split tiles behind whole ones the fp32 partials, tile by tile. PROMOTE: an item's accumulators (chunks of K) are collected in
 // fp32 registers: the tensor core's own sum over K loses about 2^-24 per 16 products,
 // which an fp32 C would show.
 template <bool PROMOTE>
@@ -671,6 +680,7 @@ struct StoreEpi {
   static constexpr bool PING_PONG = false;
   struct Params {
     Out c[2];
+    Out part;  // partials of the split tiles behind whole ones: a slice of 256 x 256 each
     int row_split;
     const float* alpha;  // device scalar (NULL: 1)
     int dtype;           // of C
@@ -690,6 +700,12 @@ struct StoreEpi {
   __device__ void end(const Steps&) {}
   __device__ void done() { boxes.finish(); }
   __device__ __forceinline__ void out32(const Steps& q, int c, float (&v)[32], uint32_t& box) {
+    if (q.it.part >= 0) {
+      const uint32_t b = boxes.take();
+      boxes.put32(b, v);
+      boxes.store(b, &p.part.map, c, q.it.row0 % PM + 32 * w.quad, q.it.part);
+      return;
+    }
     int row = q.it.row0 + 32 * w.quad;
     const int part = row >= p.row_split;
     if (part) row -= p.row_split;
@@ -780,6 +796,18 @@ int weight_grad(const char* what, const void* dy, int64_t lddy, const void* x, i
 int sum_splits(const float* part, int64_t ldp, int64_t split_stride, int splits, const SumArgs& out, int rows_total,
                cudaStream_t st);
 
+// How a product's tiles are dealt: in whole rounds over the pairs, and the rest of them (all,
+// if there are fewer than pairs) in `splits` splits of K each, so that no round is half empty.
+struct Plan {
+  int splits;
+  int whole;  // tiles that are not split
+};
+Plan plan_product(int64_t tiles, int64_t kb);
+// Bytes of partial sums of an M x N product.
+size_t product_workspace(int64_t M, int64_t N, int64_t kb);
+// The same for the tiles from `s.whole` on, whose partials lie tile by tile.
+int sum_tail(const float* part, const Sched& s, const SumArgs& out, cudaStream_t st);
+
 inline bool rows16(const void* p, int64_t ld, int size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0;
 }
@@ -828,7 +856,8 @@ inline void runs_if_resident(Sched* s, int64_t n, int64_t k) { s->runs = n * k *
 
 template <bool A_MN, bool B_MN, bool DUAL_B, class Epi>
 int launch(const char* what, const Args& a, const typename Epi::Params& ep, cudaStream_t st) {
-  const int64_t items = (int64_t)a.s.tiles_m * (a.s.runs || !a.s.strips ? a.s.tiles_n : a.s.strips) * a.s.splits;
+  const int64_t tiles = (int64_t)a.s.tiles_m * (a.s.runs || !a.s.strips ? a.s.tiles_n : a.s.strips);
+  const int64_t items = a.s.whole + (tiles - a.s.whole) * a.s.splits;
   if (items <= 0) return PNFT_OK;
   if (items > (1 << 30)) return fail(PNFT_EUNSUPPORTED, "%s: too many tiles", what);
   auto* k = gemm_kernel<A_MN, B_MN, DUAL_B, Epi>;
@@ -845,7 +874,7 @@ int launch(const char* what, const Args& a, const typename Epi::Params& ep, cuda
 constexpr int PROMOTE_KB = 32;
 template <bool A_MN, bool B_MN>
 int launch_store(const char* what, Args a, const StoreEpi<false>::Params& ep, cudaStream_t st) {
-  if (ep.dtype == PNFT_DTYPE_F32 && a.s.kb > PROMOTE_KB * a.s.splits) {
+  if (ep.dtype == PNFT_DTYPE_F32 && a.s.kb > PROMOTE_KB * (a.s.whole ? 1 : a.s.splits)) {
     a.s.chunk = PROMOTE_KB;
     typename StoreEpi<true>::Params e;
     static_assert(sizeof(e) == sizeof(ep), "same parameters");
@@ -853,6 +882,42 @@ int launch_store(const char* what, Args a, const StoreEpi<false>::Params& ep, cu
     return launch<A_MN, B_MN, false, StoreEpi<true>>(what, a, e, st);
   }
   return launch<A_MN, B_MN, false, StoreEpi<false>>(what, a, ep, st);
+}
+
+// alpha A B^T (M x N, kb K blocks, the operands' maps in `a`) into C as planned: one matrix of M
+// rows, or two (row_split). `work` has product_workspace's bytes; seg_kb: K blocks of the first
+// pair of maps (0: all); live: device number of K that count.
+template <bool A_MN, bool B_MN>
+int product(const char* what, Args a, const SumArgs& c, float* work, int64_t M, int64_t N, int64_t kb, int64_t seg_kb,
+            const int32_t* live, cudaStream_t st) {
+  const Plan plan = plan_product(tiles_of(M, N), kb);
+  a.s = plain_sched(M, N, kb, plan.splits);
+  if (seg_kb) a.s.seg_kb = (int)seg_kb;
+  a.s.whole = plan.whole;
+  a.s.live = live;
+  a.s.live_k = live != nullptr;
+  typename StoreEpi<false>::Params out;
+  memset(&out, 0, sizeof(out));
+  const bool apart = plan.splits > 1 && !plan.whole;
+  const int64_t ldp = (N + 3) / 4 * 4;
+  int rc = PNFT_OK;
+  if (apart) {
+    out.row_split = 0x7fffffff;
+    out.dtype = PNFT_DTYPE_F32;
+    rc = make_out(&out.c[0], work, PNFT_DTYPE_F32, N, M, ldp, plan.splits, M * ldp);
+  } else {
+    out.row_split = c.row_split;
+    out.dtype = c.dtype;
+    out.alpha = c.alpha;
+    rc = make_out(&out.c[0], c.c[0], c.dtype, N, c.rows, c.ldc);
+    if (!rc && c.row_split < M) rc = make_out(&out.c[1], c.c[1], c.dtype, N, c.rows, c.ldc);
+    const int64_t parts = (tiles_of(M, N) - plan.whole) * plan.splits;
+    if (!rc && plan.whole) rc = make_out(&out.part, work, PNFT_DTYPE_F32, BN, PM, BN, parts, PM * BN);
+  }
+  if (!rc) rc = launch_store<A_MN, B_MN>(what, a, out, st);
+  if (rc || plan.splits == 1) return rc;
+  if (apart) return sum_splits(work, ldp, M * ldp, plan.splits, c, (int)M, st);
+  return sum_tail(work, a.s, c, st);
 }
 
 // An operand that TMA can read: 16-byte base, row stride a multiple of 8 elements

@@ -611,7 +611,7 @@ int64_t piece_width(int64_t M, int64_t V) {
 constexpr int FUSED_WIDTH = 256;  // up to this width dz and dh come from one kernel
 struct BwdLayout {
   int64_t P;
-  int dh_splits, dw_splits;
+  int dh_splits;
   size_t rs, alpha, dz, acc, part, total;
 };
 // Shares of dh that the fused kernel leaves: one per row tile and run that meet.
@@ -625,7 +625,6 @@ BwdLayout bwd_layout(int64_t M, int64_t V, int64_t D) {
   l.P = piece_width(M, V);
   // few tiles: two rounds, which become one where half of the rows count
   l.dh_splits = plan_splits(tiles_of(M, D), l.P / BK, 4 * tiles_of(M, D) <= sm_count() / 2 ? 2 : 1);
-  l.dw_splits = plan_splits(tiles_of(l.P, D), Mp / BK);
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t r = at;
@@ -637,7 +636,7 @@ BwdLayout bwd_layout(int64_t M, int64_t V, int64_t D) {
   l.dz = take(2 * (size_t)Mp * l.P);
   l.acc = take(4 * (size_t)Mp * D4);
   const size_t a = D <= FUSED_WIDTH ? 4 * (size_t)dh_shares(M, l.P) * PM * D4 : l.dh_splits > 1 ? 4 * (size_t)l.dh_splits * Mp * D4 : 0;
-  const size_t b = l.dw_splits > 1 ? 4 * (size_t)l.dw_splits * l.P * D4 : 0;
+  const size_t b = std::max(product_workspace(l.P, D, Mp / BK), product_workspace((V - 1) % l.P + 1, D, Mp / BK));
   l.part = take(std::max(a, b));  // the shares are joined before the splits of dW are written
   l.total = at;
   return l;
@@ -881,27 +880,11 @@ extern "C" int pnft_stream_xent_bwd(const void* w, int64_t ldw, const void* save
       rc = map_mnmajor(&a.ta[0], dz, n, Mp, l.P);
       if (!rc) rc = map_mnmajor(&a.tb[0], hc, D, Mp, ldc);
       if (rc) break;
-      a.s = plain_sched(n, D, (Mp + BK - 1) / BK, l.dw_splits);
-      a.s.live = s.counts;
-      a.s.live_k = 1;
       a.idesc = idesc(dtype, true, true);
       const int size = dtype_size(dw_dtype);
       void* dst = static_cast<char*>(dw) + v0 * lddw * size;
-      StoreEpi<false>::Params out;
-      memset(&out, 0, sizeof(out));
-      out.row_split = 0x7fffffff;
-      if (l.dw_splits > 1) {
-        out.dtype = PNFT_DTYPE_F32;
-        rc = make_out(&out.c[0], part, PNFT_DTYPE_F32, D, n, D4, l.dw_splits, l.P * D4);
-        if (!rc) rc = launch_store<true, true>("stream_xent dW", a, out, st);
-        const SumArgs sum{{dst, nullptr}, lddw, 0x7fffffff, (int)n, (int)D, alpha, dw_dtype, 0, rows16(dst, lddw, size)};
-        if (!rc) rc = sum_splits(part, D4, l.P * D4, l.dw_splits, sum, (int)n, st);
-      } else {
-        out.dtype = dw_dtype;
-        out.alpha = alpha;
-        rc = make_out(&out.c[0], dst, dw_dtype, D, n, lddw);
-        if (!rc) rc = launch_store<true, true>("stream_xent dW", a, out, st);
-      }
+      const SumArgs c{{dst, nullptr}, lddw, 0x7fffffff, (int)n, (int)D, alpha, dw_dtype, 0, rows16(dst, lddw, size)};
+      rc = product<true, true>("stream_xent dW", a, c, part, n, D, Mp / BK, 0, s.counts, st);
     }
   }
   if (rc || !dh || D <= FUSED_WIDTH) return rc;

@@ -93,9 +93,10 @@ def gated_inputs(M, D, F, dt, bias, seed, device):
     return x, wg, wu, bg, bu, r(M, F)
 
 
-# (M, D, F): one token; a few; a tile's edges on each side; K tails; odd widths; one column; wide
+# (M, D, F): one token; a few; a tile's edges on each side; K tails; odd widths; one column; wide;
+# products whose last round of tiles is split along K
 GATED = [(1, 64, 128), (3, 256, 1024), (17, 100, 77), (127, 64, 129), (128, 128, 128), (129, 72, 127), (300, 1, 5),
-         (5, 1001, 1), (33, 520, 2731), (1000, 256, 1024), (257, 2048, 640)]
+         (5, 1001, 1), (33, 520, 2731), (1000, 256, 1024), (257, 2048, 640), (4200, 1300, 1800)]
 
 
 @pytest.mark.parametrize("shape", GATED)
@@ -202,7 +203,7 @@ def test_act8_strides_and_shape(cuda):
 
 
 @pytest.mark.parametrize("dt", [BF16, FP16])
-@pytest.mark.parametrize("M,N,D", [(1, 8, 128), (5, 3, 1), (64, 256, 1024), (1000, 129, 257), (4099, 256, 1000), (0, 16, 24)])
+@pytest.mark.parametrize("M,N,D", [(1, 8, 128), (5, 3, 1), (64, 256, 1024), (1000, 129, 257), (4099, 256, 1000), (0, 16, 24), (4001, 2500, 2309)])
 def test_act8_weight_grad(cuda, dt, M, N, D):
     g = torch.Generator(device=cuda).manual_seed(M + N + D)
     x = torch.randn(M, D, device=cuda, generator=g).to(dt)
@@ -244,9 +245,10 @@ def xent_oracle(h, w, t, up, dt, ignore=-100):
     return (loss, torch.where(live, el, 0.0)), (dh, edh + e * (dh.abs() + edh) + tiny), (dw, edw + e * (dw.abs() + edw) + tiny)
 
 
-# (M, V, D): one token; a tile's edges; a vocabulary of one; odd widths; several pieces
+# (M, V, D): one token; a tile's edges; a vocabulary of one; odd widths; several pieces;
+# a dW whose last round of tiles is split along K
 XENT = [(1, 1000, 64), (1, 33278, 256), (5, 1, 8), (7, 257, 72), (128, 256, 128), (129, 255, 1), (300, 1025, 1001),
-        (1000, 5000, 256), (64, 50021, 776), (2100, 40000, 64)]
+        (1000, 5000, 256), (64, 50021, 776), (2100, 40000, 64), (4000, 20001, 300)]
 
 
 @pytest.mark.parametrize("shape", XENT)
