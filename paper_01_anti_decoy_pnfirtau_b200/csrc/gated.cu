@@ -93,6 +93,24 @@ __device__ __forceinline__ void add_bias(float (&v)[W], const void* bias, int dt
   }
 }
 
+// Sums of 16 values of every lane over the warp: lanes 2 k and 2 k + 1 return value k's, in
+// an order that depends on the lanes alone.
+__device__ __forceinline__ float column_sums(const float (&x)[16], int lane) {
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = x[i];
+#pragma unroll
+  for (int n = 8; n > 0; n /= 2) {  // a lane hands half of its values to the lane 2 n away
+    const bool upper = lane & (2 * n);
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float other = __shfl_xor_sync(0xffffffffu, upper ? v[i] : v[i + n], 2 * n);
+      v[i] = (upper ? v[i + n] : v[i]) + other;
+    }
+  }
+  return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
+}
+
 // FWD: h. KEEP: h and the three planes of g, u. BWD: dg, du from dh and the recomputed g, u.
 // A warp has 32 columns of g and of u of a tile, and takes them 16 at a time (96 registers).
 enum { FWD, KEEP, BWD };
@@ -108,6 +126,7 @@ struct GatedEpi {
     Out h;            // FWD, KEEP: h; BWD: dg
     Out k;            // KEEP: the planes; BWD: du
     CUtensorMap dh;   // BWD
+    float* sums;      // BWD: [32-row blocks][2][columns] sums of dg and du for the biases, or NULL
   };
   const Params& p;
   EpiWarp w;
@@ -186,6 +205,20 @@ struct GatedEpi {
           if (next.valid()) load_dh(next);
         }
         if (!live) continue;
+        if (p.sums) {  // before the rounding to 16 bits
+          const bool in = row + w.lane < p.h.rows;
+          float s[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = in ? g[i] : 0.f;
+          const float sg = column_sums(s, w.lane);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = in ? u[i] : 0.f;
+          const float su = column_sums(s, w.lane);
+          if (w.lane / 2 < n) {
+            float* at = p.sums + (int64_t)(row / 32) * 2 * p.h.cols + col + c + w.lane / 2;
+            at[w.lane & 1 ? p.h.cols : 0] = w.lane & 1 ? su : sg;
+          }
+        }
         boxes.put16(b[0], c, g, bf16);
         boxes.put16(b[OUTS - 1], c, u, bf16);
       } else {
@@ -283,8 +316,7 @@ __global__ void __launch_bounds__(32 * skinny::WARPS, 2) gated_skinny_kernel(Ski
 
 // ------------------------------------------------------------------ pointwise backward
 // dg, du from dh and the kept g, u (their three planes), with the column sums of dg and du
-// as stored for the biases' gradients; without dh only the sums of given dg, du. A block
-// takes 8 columns per lane (256 in all) of a run of rows, a warp a row at a time. Bound by
+// before their rounding for the biases' gradients. A block takes 8 columns per lane (256 in all) of a run of rows, a warp a row at a time. Bound by
 // HBM: 12 bytes per element; the loads of 32 warps per SM keep it busy (16 with two rows each
 // reached 3.8 TB/s).
 constexpr int PT = 256, PCOLS = 256, PBLOCKS = 4;  // blocks per SM
@@ -325,7 +357,7 @@ __device__ __forceinline__ void join24(const uint16_t* gp, const uint16_t* up, c
   }
 }
 
-template <bool POINT, bool SUMS, int ACT>
+template <bool SUMS, int ACT>
 __global__ void __launch_bounds__(PT, PBLOCKS) gated_point_kernel(PointArgs p) {
   launch_next();
   wait_previous();
@@ -339,23 +371,18 @@ __global__ void __launch_bounds__(PT, PBLOCKS) gated_point_kernel(PointArgs p) {
 #pragma unroll 1
     for (int64_t r = r0 + warp; r < r1; r += PT / 32) {
       float g[8], u[8];
-      if (POINT) {
-        float d[8];
-        join24(p.g + r * p.ldp + col, p.u + r * p.ldp + col, p.low + r * p.ldp + col, n, g, u);
-        load_row16<8>(p.dh + r * p.lddh + col, d, n, p.vec, bf16);
+      float d[8];
+      join24(p.g + r * p.ldp + col, p.u + r * p.ldp + col, p.low + r * p.ldp + col, n, g, u);
+      load_row16<8>(p.dh + r * p.lddh + col, d, n, p.vec, bf16);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          float da;
-          const float a = act_value<true, ACT>(g[k], &da);
-          g[k] = d[k] * u[k] * da;
-          u[k] = d[k] * a;
-        }
-        store_row16<8>(p.dg + r * p.ldd + col, g, n, true, bf16);
-        store_row16<8>(p.du + r * p.ldd + col, u, n, true, bf16);
-      } else {
-        load_row16<8>(p.g + r * p.ldp + col, g, n, p.vec, bf16);
-        load_row16<8>(p.u + r * p.ldp + col, u, n, p.vec, bf16);
+      for (int k = 0; k < 8; ++k) {
+        float da;
+        const float a = act_value<true, ACT>(g[k], &da);
+        g[k] = d[k] * u[k] * da;
+        u[k] = d[k] * a;
       }
+      store_row16<8>(p.dg + r * p.ldd + col, g, n, true, bf16);
+      store_row16<8>(p.du + r * p.ldd + col, u, n, true, bf16);
       if (SUMS) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) sg[k] += g[k], su[k] += u[k];
@@ -376,14 +403,22 @@ __global__ void __launch_bounds__(PT, PBLOCKS) gated_point_kernel(PointArgs p) {
   }
 }
 
-__global__ void __launch_bounds__(256) gated_bias_sum_kernel(const float* __restrict__ part, int blocks, int F, void* dbg,
+// Adds the blocks' column sums: 32 columns per block, eight threads each, in a fixed order.
+__global__ void __launch_bounds__(256) gated_bias_sum_kernel(const float* __restrict__ part, int64_t blocks, int F, void* dbg,
                                                              void* dbu, int dtype) {
+  __shared__ float red[8][32];
   launch_next();
   wait_previous();
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= 2 * F) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
   float t = 0.f;
-  for (int b = 0; b < blocks; ++b) t += part[(int64_t)b * 2 * F + i];
+  if (i < 2 * F) {
+#pragma unroll 8
+    for (int64_t b = warp; b < blocks; b += 8) t += part[b * 2 * F + i];
+  }
+  red[warp][lane] = t;
+  __syncthreads();
+  if (warp > 0 || i >= 2 * F) return;
+  for (int k = 1; k < 8; ++k) t += red[k][lane];
   void* dst = i < F ? dbg : dbu;
   const int c = i < F ? i : i - F;
   if (!dst) return;
@@ -391,6 +426,10 @@ __global__ void __launch_bounds__(256) gated_bias_sum_kernel(const float* __rest
     static_cast<float*>(dst)[c] = t;
   else
     store16(static_cast<uint16_t*>(dst) + c, t, dtype == PNFT_DTYPE_BF16);
+}
+int bias_sum(const float* part, int64_t blocks, int64_t F, void* dbg, void* dbu, int dtype, cudaStream_t st) {
+  launch_dependent(gated_bias_sum_kernel, dim3((unsigned)((2 * F + 31) / 32)), 256, 0, st, part, blocks, (int)F, dbg, dbu, dtype);
+  return check_launch("gated_bwd biases", 1);
 }
 
 // Rows per block of the pointwise kernel: one wave of PBLOCKS per SM.
@@ -411,18 +450,19 @@ int gated_check(const char* what, int64_t M, int64_t D, int64_t F, int act, int 
 
 template <int MODE, int ACT>
 int gated_launch(const char* what, const Args& a, const void* bg, const void* bu, int b_dtype, int dtype, const Out& h,
-                 const Out& k, const CUtensorMap* dh, cudaStream_t st) {
+                 const Out& k, const CUtensorMap* dh, float* sums, cudaStream_t st) {
   typename GatedEpi<MODE, ACT>::Params ep;
   memset(&ep, 0, sizeof(ep));
   ep.bg = bg, ep.bu = bu, ep.b_dtype = b_dtype, ep.bf16 = dtype == PNFT_DTYPE_BF16;
   ep.h = h, ep.k = k;
   if (dh) ep.dh = *dh;
+  ep.sums = sums;
   return launch<false, false, true, GatedEpi<MODE, ACT>>(what, a, ep, st);
 }
 
 int gated_gemm(const char* what, int mode, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
                int64_t ldwu, const void* bg, const void* bu, int b_dtype, const Out& h, const Out& k, const CUtensorMap* dh,
-               int64_t M, int64_t D, int64_t F, int act, int dtype, int32_t* status, cudaStream_t st) {
+               float* sums, int64_t M, int64_t D, int64_t F, int act, int dtype, int32_t* status, cudaStream_t st) {
   if (b_dtype < PNFT_DTYPE_F32 || b_dtype > PNFT_DTYPE_F16) return fail(PNFT_EINVAL, "%s: unknown bias type %d", what, b_dtype);
   Args a;
   memset(&a, 0, sizeof(a));
@@ -435,7 +475,7 @@ int gated_gemm(const char* what, int mode, const void* x, int64_t ldx, const voi
   a.idesc = idesc(dtype, false, false);
   a.status = status;
   auto go = [&](auto m, auto c) {
-    return gated_launch<decltype(m)::value, decltype(c)::value>(what, a, bg, bu, b_dtype, dtype, h, k, dh, st);
+    return gated_launch<decltype(m)::value, decltype(c)::value>(what, a, bg, bu, b_dtype, dtype, h, k, dh, sums, st);
   };
   auto with_act = [&](auto m) {
     return act == PNFT_ACT_SILU ? go(m, std::integral_constant<int, PNFT_ACT_SILU>()) : go(m, std::integral_constant<int, PNFT_ACT_GELU>());
@@ -484,7 +524,7 @@ extern "C" int pnft_gated_fwd(const void* x, int64_t ldx, const void* wg, int64_
   int rc = make_out(&o, h, dtype, F, M, ldh, 1, 0, 64);
   if (!rc) rc = make_out(&k, pre, dtype, F, M, ldp, 3, M * ldp, 64);
   if (rc) return rc;
-  return gated_gemm("gated_fwd", pre ? KEEP : FWD, x, ldx, wg, ldwg, wu, ldwu, bg, bu, b_dtype, o, k, nullptr, M, D, F, act,
+  return gated_gemm("gated_fwd", pre ? KEEP : FWD, x, ldx, wg, ldwg, wu, ldwu, bg, bu, b_dtype, o, k, nullptr, nullptr, M, D, F, act,
                     dtype, status, as_stream(stream));
 }
 
@@ -508,7 +548,7 @@ BwdLayout bwd_layout(int64_t M, int64_t D, int64_t F) {
   };
   l.d = take(2 * (size_t)M * 2 * l.Fp);
   l.dh = take(F % 8 ? 2 * (size_t)M * l.Fp : 0);
-  l.bias = take(sizeof(float) * 2 * (size_t)F * (size_t)((M + point_rows(M, F) - 1) / point_rows(M, F)));
+  l.bias = take(sizeof(float) * 2 * (size_t)F * (size_t)std::max((M + point_rows(M, F) - 1) / point_rows(M, F), (M + 31) / 32));
   l.part = take(std::max(product_workspace(M, D, 2 * ((F + BK - 1) / BK)), pnft_weight_grad_workspace_size(M, 2 * l.Fp, D)));
   l.total = at;
   return l;
@@ -519,30 +559,19 @@ int point(const uint16_t* dh, int64_t lddh, const void* pre, int64_t ldp, uint16
   const bool sums = dbg || dbu;
   PointArgs p;
   memset(&p, 0, sizeof(p));
-  if (dh) {
-    p.dh = dh, p.lddh = lddh;
-    p.g = static_cast<const uint16_t*>(pre), p.u = p.g + M * ldp, p.low = p.u + M * ldp, p.ldp = ldp;
-    p.vec = rows16(dh, lddh, 2);
-  } else {
-    p.g = dg, p.u = du, p.ldp = ldd, p.vec = 1;
-  }
+  p.dh = dh, p.lddh = lddh, p.vec = rows16(dh, lddh, 2);
+  p.g = static_cast<const uint16_t*>(pre), p.u = p.g + M * ldp, p.low = p.u + M * ldp, p.ldp = ldp;
   p.dg = dg, p.du = du, p.ldd = ldd;
   p.part = sums ? part : nullptr;
   p.M = (int)M, p.F = (int)F, p.bf16 = dtype == PNFT_DTYPE_BF16;
   p.rows = point_rows(M, F);
   const dim3 grid((unsigned)((F + PCOLS - 1) / PCOLS), (unsigned)((M + p.rows - 1) / p.rows));
-  if (!dh)
-    launch_dependent(gated_point_kernel<false, true, 0>, grid, PT, 0, st, p);
-  else if (act == PNFT_ACT_SILU)
-    launch_dependent(sums ? gated_point_kernel<true, true, PNFT_ACT_SILU> : gated_point_kernel<true, false, PNFT_ACT_SILU>, grid, PT, 0,
-                     st, p);
+  if (act == PNFT_ACT_SILU)
+    launch_dependent(sums ? gated_point_kernel<true, PNFT_ACT_SILU> : gated_point_kernel<false, PNFT_ACT_SILU>, grid, PT, 0, st, p);
   else
-    launch_dependent(sums ? gated_point_kernel<true, true, PNFT_ACT_GELU> : gated_point_kernel<true, false, PNFT_ACT_GELU>, grid, PT, 0,
-                     st, p);
-  if (sums)
-    launch_dependent(gated_bias_sum_kernel, dim3((unsigned)((2 * F + 255) / 256)), 256, 0, st, p.part, (int)grid.y, (int)F, dbg, dbu,
-                     b_dtype);
-  return check_launch("gated_bwd pointwise", sums ? 2 : 1);
+    launch_dependent(sums ? gated_point_kernel<true, PNFT_ACT_GELU> : gated_point_kernel<false, PNFT_ACT_GELU>, grid, PT, 0, st, p);
+  if (int rc = check_launch("gated_bwd pointwise", 1)) return rc;
+  return sums ? bias_sum(p.part, grid.y, F, dbg, dbu, b_dtype, st) : PNFT_OK;
 }
 
 int gated_dx(const uint16_t* dg, const uint16_t* du, int64_t ldd, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
@@ -617,9 +646,10 @@ extern "C" int pnft_gated_bwd(const void* x, int64_t ldx, const void* wg, int64_
     if (!rc) rc = make_out(&u, du, dtype, F, M, ldd, 1, 0, 64);
     if (!rc) rc = tma_map_out(&map, d, 2, F, M, ldh, 1, 0, 32, 64);
     if (!rc)
-      rc = gated_gemm("gated_bwd", BWD, x, ldx, wg, ldwg, wu, ldwu, bg, bu, b_dtype, g, u, &map, M, D, F, act, dtype, status, st);
+      rc = gated_gemm("gated_bwd", BWD, x, ldx, wg, ldwg, wu, ldwu, bg, bu, b_dtype, g, u, &map, dbg || dbu ? bias : nullptr, M, D, F, act,
+                      dtype, status, st);
     if (!rc && (dbg || dbu))
-      rc = point(nullptr, 0, nullptr, 0, dg, du, ldd, dbg, dbu, b_dtype, bias, M, F, act, dtype, st);
+      rc = bias_sum(bias, (M + 31) / 32, F, dbg, dbu, b_dtype, st);
   }
   if (!rc && dx) rc = gated_dx(dg, du, ldd, wg, ldwg, wu, ldwu, dx, lddx, dx_dtype, ws + l.part, M, D, F, dtype, status, st);
   if (!rc && (dwg || dwu))
