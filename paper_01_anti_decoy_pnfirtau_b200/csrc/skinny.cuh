@@ -51,14 +51,28 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int D) {
 // The lane's part of a warp's product: RG groups of 16 rows (w[2 r]: the group's row
 // lane / 4, w[2 r + 1]: 8 below), 32-wide steps first, first + stride, ... of K.
 // acc[r][j]: rows (lane / 4, + 8) x tokens 8 j + 2 (lane & 3) + {0, 1}, in mma.sync's order.
-// The groups share the tokens' fragments, which come from L1.
-template <int RG, int NT, bool VEC, bool BF16>
+// The groups share the tokens' fragments, which come from L1. FOLD: after 16 steps (512 of
+// K) the sums go into a second set of accumulators: the tensor core's own sum over K
+// truncates, which an fp32 result would show.
+template <bool FOLD, int RG, int NT, bool VEC, bool BF16>
 __device__ __forceinline__ void dot(const uint16_t* const (&w)[2 * RG], const uint16_t* x, int64_t ldx, int M, int D, int first,
                                     int stride, float (&acc)[RG][NT][4]) {
   constexpr int U = RG * NT <= 2 ? 4 : 2;  // steps in flight
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int steps = (D + 31) / 32;
+  float part[FOLD ? RG : 1][NT][4] = {};
+  auto fold = [&]() {
+#pragma unroll
+    for (int r = 0; r < RG; ++r)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[r][j][k] += part[FOLD ? r : 0][j][k], part[FOLD ? r : 0][j][k] = 0.f;
+  };
+  int since = 0;
   for (int s = first; s < steps; s += U * stride) {
+    if (FOLD && since >= 16) fold(), since = 0;
+    since += U;
     uint4 a[U][2 * RG];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -78,15 +92,17 @@ __device__ __forceinline__ void dot(const uint16_t* const (&w)[2 * RG], const ui
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           const uint4 &p = a[i][2 * r], &q = a[i][2 * r + 1];
-          mma<BF16>(acc[r][j], p.x, q.x, p.y, q.y, v[j].x, v[j].y);
-          mma<BF16>(acc[r][j], p.z, q.z, p.w, q.w, v[j].z, v[j].w);
+          float(&sum)[4] = FOLD ? part[FOLD ? r : 0][j] : acc[r][j];
+          mma<BF16>(sum, p.x, q.x, p.y, q.y, v[j].x, v[j].y);
+          mma<BF16>(sum, p.z, q.z, p.w, q.w, v[j].z, v[j].w);
         }
     }
   }
+  if (FOLD) fold();
 }
 
-// Calls f(NT, VEC, BF16 as integral constants) for M <= 32 rows.
-template <class F>
+// Calls f(NT, VEC, BF16 as integral constants) for M <= 8 MAX_NT rows.
+template <int MAX_NT, class F>
 int dispatch(int64_t M, bool vec, bool bf16, F f) {
   auto types = [&](auto nt) {
     if (vec) return bf16 ? f(nt, std::true_type(), std::true_type()) : f(nt, std::true_type(), std::false_type());
@@ -94,8 +110,10 @@ int dispatch(int64_t M, bool vec, bool bf16, F f) {
   };
   if (M <= 8) return types(std::integral_constant<int, 1>());
   if (M <= 16) return types(std::integral_constant<int, 2>());
-  if (M <= 24) return types(std::integral_constant<int, 3>());
-  return types(std::integral_constant<int, 4>());
+  if constexpr (MAX_NT > 3) {
+    if (M > 24) return types(std::integral_constant<int, 4>());
+  }
+  return types(std::integral_constant<int, 3>());
 }
 
 }  // namespace skinny

@@ -128,10 +128,15 @@ __global__ void __launch_bounds__(CT) xent_compact_kernel(CompactArgs p) {
 
 // ------------------------------------------------------------------ forward epilogue
 // Per row, half of the columns and group of warps: running maximum (times log2 e) and sum of
-// 2^(z log2 e - max), both fp32, over the group's tiles of an item.
+// 2^(z log2 e - max), both fp32, over the group's tiles of an item. PROMOTE: a tile's
+// accumulators (chunks of K) are collected in fp32 registers first: the tensor core's own sum
+// over K truncates, which an fp32 loss shows (1.1e-6 of it at width 2048, 2.7e-6 at 4096). The
+// registers for that leave room for 8 warps, enough where a tile has MMAs of more than 16 K blocks.
+template <bool PROMOTE>
 struct LseEpi {
-  static constexpr int WARPS = 16, BOXES = 0, BOX_BYTES = 0;
-  static constexpr bool PING_PONG = true;
+  static constexpr int WARPS = PROMOTE ? 8 : 16, BOXES = 0, BOX_BYTES = 0;
+  static constexpr bool PING_PONG = !PROMOTE;
+  static constexpr int W = 64;
   struct Params {
     float *part_m, *part_s;  // [row tile][slot][group and half][256]
     float* zt;
@@ -143,7 +148,12 @@ struct LseEpi {
   EpiWarp w;
   float m, s;
   int tgt, live;
-  __device__ LseEpi(const Params& p_, const EpiWarp& w_, const Abort&) : p(p_), w(w_) { live = *p.live; }
+  float sum[PROMOTE ? BN / 2 : 1];
+  __device__ LseEpi(const Params& p_, const EpiWarp& w_, const Abort&) : p(p_), w(w_) {
+    live = *p.live;
+#pragma unroll
+    for (float& v : sum) v = 0.f;
+  }
   __device__ void prepare(const Steps& q) {
     if (!q.item_first()) return;
     m = kLow, s = 0.f;
@@ -157,49 +167,75 @@ struct LseEpi {
     const int64_t at = (((int64_t)q.it.mt * q.walk.slots + q.it.slot) * 4 + 2 * w.group + w.slice) * PM + row % PM;
     p.part_m[at] = m;
     p.part_s[at] = s;
+    if (PROMOTE) p.part_m[at + 2 * PM] = kLow, p.part_s[at + 2 * PM] = 0.f;  // there is no second group
+  }
+  // The logits z of columns col on.
+  __device__ __forceinline__ void take(float (&z)[W], int row, int col) {
+    const int n = p.V - col;
+    if (n < W) {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (i >= n) z[i] = __int_as_float(0xff800000);  // -infinity
+    }
+    const int tc = tgt - col;
+    if ((unsigned)tc < (unsigned)W) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) v = i == tc ? z[i] : v;
+      p.zt[row] = v;
+    }
+    float top[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top[k] = max3(z[k], z[k + 4], z[k + 8]);
+#pragma unroll
+    for (int i = 12; i < W - 4; i += 8) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top[k] = max3(top[k], z[i + k], z[i + k + 4]);
+    }
+    top[0] = max3(top[0], z[W - 4], z[W - 3]), top[1] = max3(top[1], z[W - 2], z[W - 1]);
+    const float nm = fmaxf(m, kLog2e * max3(top[0], top[1], fmaxf(top[2], top[3])));
+    const f32x2 scale = pack(kLog2e, kLog2e), minus = pack(-nm, -nm);
+    f32x2 sums[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      const f32x2 x = fma2(pack(z[2 * i], z[2 * i + 1]), scale, minus);
+      sums[i & 3] = add2(sums[i & 3], exp2_pair(x));
+    }
+    const float2 t = unpack(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+    s = fmaf(s, ex2(m - nm), t.x + t.y);
+    m = nm;
   }
   template <class Release>
   __device__ __forceinline__ void tile(const Steps& q, uint32_t acc, Release release) {
-    constexpr int W = 64;
+    const int row = q.it.row0 + w.row(), c0 = w.slice * (BN / 2);
+    if constexpr (PROMOTE) {
+#pragma unroll
+      for (int c = 0; c < BN / 2; c += 16) {
+        uint32_t r[16];
+        tmem_load16(acc + c0 + c, r);
+        if (c + 16 == BN / 2) release();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[c + i] += __uint_as_float(r[i]);
+      }
+      if (!q.tile_last()) return;
+#pragma unroll
+      for (int c = 0; c < BN / 2; c += W) {
+        float z[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) z[i] = sum[c + i], sum[c + i] = 0.f;
+        take(z, row, q.nt * BN + c0 + c);
+      }
+    } else {
 #pragma unroll 1
-    for (int c = w.slice * (BN / 2); c < (w.slice + 1) * (BN / 2); c += W) {
-      uint32_t z[2][W / 2];
-      tmem_load32x2(acc + c, z[0], acc + c + W / 2, z[1]);
-      if (c + W == (w.slice + 1) * (BN / 2)) release();
-      const int row = q.it.row0 + w.row(), col = q.nt * BN + c, n = p.V - col;
-      auto at = [&](int i) { return __uint_as_float(z[i / (W / 2)][i % (W / 2)]); };
-      if (n < W) {
+      for (int c = c0; c < c0 + BN / 2; c += W) {
+        uint32_t r[2][W / 2];
+        tmem_load32x2(acc + c, r[0], acc + c + W / 2, r[1]);
+        if (c + W == c0 + BN / 2) release();
+        float z[W];
 #pragma unroll
-        for (int i = 0; i < W; ++i)
-          if (i >= n) z[i / (W / 2)][i % (W / 2)] = 0xff800000u;  // -infinity
+        for (int i = 0; i < W; ++i) z[i] = __uint_as_float(r[i / (W / 2)][i % (W / 2)]);
+        take(z, row, q.nt * BN + c);
       }
-      const int tc = tgt - col;
-      if ((unsigned)tc < (unsigned)W) {
-        float v = 0.f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) v = i == tc ? at(i) : v;
-        p.zt[row] = v;
-      }
-      float top[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) top[k] = max3(at(k), at(k + 4), at(k + 8));
-#pragma unroll
-      for (int i = 12; i < W - 4; i += 8) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top[k] = max3(top[k], at(i + k), at(i + k + 4));
-      }
-      top[0] = max3(top[0], at(W - 4), at(W - 3)), top[1] = max3(top[1], at(W - 2), at(W - 1));
-      const float nm = fmaxf(m, kLog2e * max3(top[0], top[1], fmaxf(top[2], top[3])));
-      const f32x2 scale = pack(kLog2e, kLog2e), minus = pack(-nm, -nm);
-      f32x2 sum[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < W / 2; ++i) {
-        const f32x2 x = fma2(pack(at(2 * i), at(2 * i + 1)), scale, minus);
-        sum[i & 3] = add2(sum[i & 3], exp2_pair(x));
-      }
-      const float2 t = unpack(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
-      s = fmaf(s, ex2(m - nm), t.x + t.y);
-      m = nm;
     }
   }
 };
@@ -326,7 +362,7 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 // Groups of 16 words per warp: two share the rows' fragments when there are many rows.
 constexpr int skinny_groups(int nt) { return nt <= 2 ? 1 : 2; }
 template <int NT, bool VEC, bool BF16>
-__global__ void __launch_bounds__(32 * skinny::WARPS, NT <= 4 ? 2 : 1) xent_skinny_kernel(SkinnyArgs p) {
+__global__ void __launch_bounds__(32 * skinny::WARPS, 2) xent_skinny_kernel(SkinnyArgs p) {
   __shared__ float sm[skinny::WARPS][8 * NT], ss[skinny::WARPS][8 * NT];
   launch_next();
   wait_previous();
@@ -348,7 +384,7 @@ __global__ void __launch_bounds__(32 * skinny::WARPS, NT <= 4 ? 2 : 1) xent_skin
     const uint16_t* w[2 * RG];
 #pragma unroll
     for (int r = 0; r < 2 * RG; ++r) w[r] = p.w + min(v0 + g + 8 * r, (int64_t)p.V - 1) * p.ldw;
-    skinny::dot<RG, NT, VEC, BF16>(w, p.h, p.ldh, p.M, p.D, 0, 1, acc);
+    skinny::dot<true, RG, NT, VEC, BF16>(w, p.h, p.ldh, p.M, p.D, 0, 1, acc);
 #pragma unroll
     for (int r = 0; r < RG; ++r) {
       const int r0 = (int)v0 + 16 * r + g, r1 = r0 + 8;
@@ -608,6 +644,7 @@ int64_t piece_width(int64_t M, int64_t V) {
   const int64_t pieces = (V + most - 1) / most;
   return up((V + pieces - 1) / pieces, BN);
 }
+constexpr int LSE_KB = 16;        // K blocks that the forward leaves to one accumulator
 constexpr int FUSED_WIDTH = 256;  // up to this width dz and dh come from one kernel
 struct BwdLayout {
   int64_t P;
@@ -710,7 +747,7 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
                        part + (size_t)blocks * SKINNY_ROWS, part + 2 * (size_t)blocks * SKINNY_ROWS, row_loss, loss,
                        (int)M, (int)D, (int)V, blocks, mean, status};
     const bool vec = D % 8 == 0 && rows16(h, ldh, 2) && rows16(w, ldw, 2);
-    return skinny::dispatch(M, vec, dtype == PNFT_DTYPE_BF16, [&](auto nt, auto v, auto b) {
+    return skinny::dispatch<SKINNY_ROWS / 8>(M, vec, dtype == PNFT_DTYPE_BF16, [&](auto nt, auto v, auto b) {
       launch_dependent(xent_skinny_kernel<decltype(nt)::value, decltype(v)::value, decltype(b)::value>, dim3((unsigned)blocks),
                        32 * skinny::WARPS, 0, st, a);
       launch_dependent(xent_skinny_reduce_kernel, dim3(1), 1024, 0, st, a);
@@ -753,11 +790,16 @@ extern "C" int pnft_stream_xent_fwd(const void* h, int64_t ldh, const void* w, i
   a.s.live_m = 1;
   a.idesc = idesc(dtype, false, false);
   a.status = status;
-  LseEpi::Params ep{reinterpret_cast<float*>(ws + l.part_m), reinterpret_cast<float*>(ws + l.part_s), c.zt, c.s.tgt,
-                    c.s.counts, (int)V};
-  rc = launch<false, false, false, LseEpi>("stream_xent forward", a, ep, st);
+  float *part_m = reinterpret_cast<float*>(ws + l.part_m), *part_s = reinterpret_cast<float*>(ws + l.part_s);
+  auto run = [&](auto promote) {
+    typename LseEpi<decltype(promote)::value>::Params ep{part_m, part_s, c.zt, c.s.tgt, c.s.counts, (int)V};
+    return launch<false, false, false, LseEpi<decltype(promote)::value>>("stream_xent forward", a, ep, st);
+  };
+  const int chunks = (a.s.kb + LSE_KB - 1) / LSE_KB;
+  a.s.chunk = (a.s.kb + chunks - 1) / chunks;
+  rc = chunks > 1 ? run(std::true_type()) : run(std::false_type());
   if (rc) return rc;
-  ReduceArgs r{ep.part_m, ep.part_s, c.zt, c.s, row_loss, loss, reinterpret_cast<double*>(ws + l.sums),
+  ReduceArgs r{part_m, part_s, c.zt, c.s, row_loss, loss, reinterpret_cast<double*>(ws + l.sums),
                l.runs, l.tiles_n, l.pairs, mean};
   if (M > 64)
     launch_dependent(xent_reduce_kernel<8>, dim3((unsigned)((M + 7) / 8)), 256, 0, st, r);
