@@ -847,12 +847,16 @@ inline Sched plain_sched(int64_t m, int64_t n, int64_t kb, int splits) {
   return s;
 }
 
-// Runs where all of B (n rows of k elements) stays in L2 beside what streams through it. Measured
-// (B200, bf16), runs against strips, by the size of B: gated product 16384 x 1024 x 4096, 17 MB, 182
-// and 196 us; cross entropy's forward 16352 x 33278 x 256, 17 MB, 247 and 278; 8192 x 50021 x 512,
-// 51 MB, 294 and 308; gated product 8192 x 2048 x 8192, 67 MB, 404 and 368; cross entropy
-// 8192 x 50021 x 1024, 102 MB, 633 and 562.
-inline void runs_if_resident(Sched* s, int64_t n, int64_t k) { s->runs = n * k * 2 <= ((int64_t)56 << 20); }
+// Runs where all of B (n rows of k elements) and the rows of A that the pairs are at (256 each) stay in
+// L2 beside what streams through it. Measured (B200, bf16), runs against strips in us, by the sum of
+// both. Gated product: 16384 x 512 x 2048 (21 MB) 55, 65; x 1024 x 4096 (50 MB) 181, 194; x 1536 x 4096
+// (75 MB) 275, 271; x 2048 x 1024 (75 MB) 90, 93; x 2048 x 2048 (84 MB) 190, 177; x 2048 x 6000 (116 MB)
+// 713, 535. Cross entropy's forward: 8192 x 50021 x 512 (60 MB) 291, 303; 8192 x 10000 x 2048 (75 MB)
+// 252, 270; 8192 x 50021 x 1024 (119 MB) 633, 562.
+inline void runs_if_resident(Sched* s, int64_t n, int64_t k) {
+  const int64_t rows = (int64_t)PM * std::min(s->tiles_m, sm_count() / 2);
+  s->runs = (n + rows) * k * 2 <= ((int64_t)76 << 20);
+}
 
 template <bool A_MN, bool B_MN, bool DUAL_B, class Epi>
 int launch(const char* what, const Args& a, const typename Epi::Params& ep, cudaStream_t st) {

@@ -612,7 +612,7 @@ struct FwdLayout {
 FwdLayout fwd_layout(int64_t M, int64_t V, int64_t D) {
   const int64_t Mp = up(M, BM), tiles_m = (M + PM - 1) / PM;
   FwdLayout l;
-  Sched s;
+  Sched s = plain_sched(M, V, 1, 1);
   runs_if_resident(&s, V, D);
   l.runs = s.runs;
   l.tiles_n = (int)((V + BN - 1) / BN);
