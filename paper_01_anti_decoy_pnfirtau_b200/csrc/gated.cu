@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(32 * skinny::WARPS, 2) gated_skinny_kernel(Ski
 // ------------------------------------------------------------------ pointwise backward
 // dg, du from dh and the kept g, u (their three planes), with the column sums of dg and du
 // before their rounding for the biases' gradients. A block takes 8 columns per lane (256 in all) of a run of rows, a warp a row at a time. Bound by
-// HBM: 12 bytes per element; the loads of 32 warps per SM keep it busy (16 with two rows each
+// HBM: 12 bytes per element (B200, 8192 x 8192: 128 us, 6.3 TB/s); the loads of 32 warps per SM keep it busy (16 with two rows each
 // reached 3.8 TB/s).
 constexpr int PT = 256, PCOLS = 256, PBLOCKS = 4;  // blocks per SM
 struct PointArgs {

@@ -14,6 +14,10 @@
 // other accumulator, so a tile's epilogue overlaps the next tile's MMAs. Either operand
 // may be K-major (rows of K) or MN-major (K rows of M or N), so no caller transposes
 // anything. Rows, columns and K past the end are zero-filled by TMA.
+//
+// Bound by the tensor core from K of about 1024 on, and by the power limit in long runs. Measured (B200,
+// bf16, single calls): the gated product 16384 x 2048 x 2048 178 us (1.55 PFLOP/s), 16384 x 512 x 2048
+// 55 us (1.25), cross entropy's forward 8192 x 50021 x 512 291 us (1.44), 16352 x 33278 x 256 240 us (1.16).
 #pragma once
 
 #include <string.h>

@@ -132,6 +132,8 @@ __global__ void __launch_bounds__(CT) xent_compact_kernel(CompactArgs p) {
 // accumulators (chunks of K) are collected in fp32 registers first: the tensor core's own sum
 // over K truncates, which an fp32 loss shows (1.1e-6 of it at width 2048, 2.7e-6 at 4096). The
 // registers for that leave room for 8 warps, enough where a tile has MMAs of more than 16 K blocks.
+// At K = 256 a tile's exponentials take as long as its MMAs: 16352 x 33278 x 256 takes 217 us from warm
+// L2 (1.28 PFLOP/s), 190 with an epilogue of loads alone.
 template <bool PROMOTE>
 struct LseEpi {
   static constexpr int WARPS = PROMOTE ? 8 : 16, BOXES = 0, BOX_BYTES = 0;
