@@ -246,6 +246,15 @@ def test_gradients_of_a_part_of_the_inputs(cuda):
     assert torch.equal(torch.autograd.grad(streamed_cross_entropy(h, ww, t), ww)[0], dw)
 
 
+def test_one_gradient_of_a_product_with_a_split_last_round(cuda):
+    x, wg, wu, dh = rand(4200, 1300), rand(1800, 1300, std=0.03, seed=1), rand(1800, 1300, std=0.03, seed=2), rand(4200, 1800, seed=3)
+    full = gated_all(x, wg, wu, dh=dh)
+    for i in range(3):
+        leaves = [t.detach().clone() for t in (x, wg, wu)]
+        leaves[i].requires_grad_(True)
+        assert torch.equal(torch.autograd.grad(gated_linear(*leaves), leaves[i], dh)[0], full[1 + i]), i
+
+
 def test_xent_zero_and_huge_upstream_gradients(cuda):
     h, w, t = rand(70, 64), rand(300, 64, std=0.2, seed=1), torch.randint(0, 300, (70,), device=cuda)
     for dt in (BF16, FP16):
@@ -397,6 +406,26 @@ def test_backward_captured_and_replayed_on_new_inputs(cuda):
         t[:ignored] = -100
         g.replay()
         same([o.detach() for o in out], xent_all(h, w, t))
+
+
+@pytest.mark.parametrize("D", [72, 1000])
+def test_a_graph_is_differentiated_twice_and_checks_its_tensors(cuda, D):
+    """retain_graph, another upstream gradient for each pass; an input changed in place since raises."""
+    x, wg, wu = (rand(*s, std=D ** -0.5, seed=i).requires_grad_(True) for i, s in enumerate([(200, D), (130, D), (130, D)]))
+    w, t = rand(1000, 130, seed=9).requires_grad_(True), torch.arange(200, device=cuda)
+    for in8 in (False, True):
+        h = gated_linear(x, wg, wu, checkpoint_8bit=in8)
+        loss = streamed_cross_entropy(h, w, t, reduction="none")
+        up = rand(200, dt=FP32, seed=3)
+        a = torch.autograd.grad(loss, (x, wg, wu, w), up, retain_graph=True)
+        b = torch.autograd.grad(loss, (x, wg, wu, w), torch.zeros_like(up), retain_graph=True)
+        assert all(not torch.any(g) for g in b)
+        same(torch.autograd.grad(loss, (x, wg, wu, w), up), a)
+    h = gated_linear(x, wg, wu)
+    with torch.no_grad():
+        wg.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(h.sum(), x)
 
 
 def test_reruns_are_bitwise_equal(cuda):
