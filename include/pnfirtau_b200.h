@@ -466,7 +466,7 @@ PNFT_API int pnft_weight_grad(const void* dy, int64_t lddy, const void* x, int64
 
 PNFT_API size_t pnft_weight_grad_workspace_size(int64_t K, int64_t M, int64_t N);
 
-/* dst[r, c] = src[r, c] for 16-bit elements, any row strides (elements). */
+/* dst[r, c] = src[r, c] for 16-bit elements: any rows into 16-byte aligned ones (strides in elements). */
 PNFT_API int pnft_copy_rows16(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols,
                      void* stream);
 

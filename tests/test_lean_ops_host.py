@@ -127,6 +127,8 @@ def test_act8_and_copies_refuse():
     refused(pack(lde=0), _lib.EINVAL, "stride")
     assert pack(M=0, x=None) == _lib.OK
     refused(L.pnft_copy_rows16(A, 8, A, 4, 2, 8, None), _lib.EINVAL, "layout")
+    refused(L.pnft_copy_rows16(A, 8, A, 9, 2, 8, None), _lib.EUNSUPPORTED, "aligned")
+    refused(L.pnft_copy_rows16(A, 8, A + 2, 8, 2, 8, None), _lib.EUNSUPPORTED, "aligned")
     n = L.pnft_act8_weight_grad_workspace_size(4, 16, 100)
     grad = lambda dtype=BF16, lddy=16, dy=A, ws=A, nb=n, lddw=100, N=16: L.pnft_act8_weight_grad(  # noqa: E731
         dy, lddy, A, 112, A, 112, A, lddw, FP32, ws, nb, 4, N, 100, dtype, None, None)
