@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(PT, PBLOCKS) gated_point_kernel(PointArgs p) {
 }
 
 // Adds the blocks' column sums: 32 columns per block, eight threads each, in a fixed order.
-__global__ void __launch_bounds__(256) gated_bias_sum_kernel(const float* __restrict__ part, int64_t blocks, int F, void* dbg,
+__global__ void __launch_bounds__(256) gated_bias_sum_kernel(const float* part, int64_t blocks, int F, void* dbg,
                                                              void* dbu, int dtype) {
   __shared__ float red[8][32];
   launch_next();

@@ -63,7 +63,7 @@ struct TailArgs {
 
 // Four columns per thread; partial rows are 16-byte aligned (ldp a multiple of 4).
 template <bool TAIL>
-__global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict__ part, int64_t ldp,
+__global__ void __launch_bounds__(256) sum_splits_kernel(const float* part, int64_t ldp,
                                                          int64_t split_stride, int splits, SumArgs o,
                                                          int rows_total, TailArgs tail) {
   launch_next();
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict
 
 // dst[r] = src[r]: a warp per row, eight words in flight per lane.
 template <typename W>
-__global__ void __launch_bounds__(256) copy_rows_kernel(const char* __restrict__ src, int64_t ss, char* __restrict__ dst,
+__global__ void __launch_bounds__(256) copy_rows_kernel(const char* src, int64_t ss, char* dst,
                                                         int64_t ds, int64_t rows, int64_t words) {
   launch_next();
   wait_previous();
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const char* __restrict__
 // of a word is loaded by the aligned words behind its first element, and each word that is
 // stored takes its lower half from the lane before (13.7 us for 4095 x 2731 from cold
 // L2, 15.3 element by element).
-__global__ void __launch_bounds__(256) copy_rows2_kernel(const uint16_t* __restrict__ src, int64_t ss, uint16_t* __restrict__ dst,
+__global__ void __launch_bounds__(256) copy_rows2_kernel(const uint16_t* src, int64_t ss, uint16_t* dst,
                                                          int64_t ds, int64_t rows, int64_t cols) {
   launch_next();
   wait_previous();

@@ -45,7 +45,10 @@ constexpr int STAGE_MAX = 225 * 1024;      // shared memory for the ring and the
 // The kernels of one call follow each other on a stream. Each lets the next be launched at
 // once and waits itself, before it touches memory, until the one before has completed: the
 // launch, the barriers and the TMEM allocation of a kernel then pass while the one before
-// still runs. Every thread of a kernel calls it.
+// still runs. Every thread of a kernel calls it. So what such a kernel reads may have been
+// written while it was resident: its loads are ordinary ones (never the read-only path, which
+// is for data that is constant as long as the kernel lives, and no restrict pointers to const,
+// which let the compiler take that path or move a load above the wait).
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <class K, class... A>

@@ -36,12 +36,12 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int D) {
   if constexpr (VEC) {
     if (k >= D) return make_uint4(0, 0, 0, 0);
     const uint4* p = reinterpret_cast<const uint4*>(row + k);
-    return STREAM ? __ldcs(p) : __ldg(p);
+    return STREAM ? __ldcs(p) : *p;
   } else {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = k + 2 * i < D ? __ldg(row + k + 2 * i) : 0, hi = k + 2 * i + 1 < D ? __ldg(row + k + 2 * i + 1) : 0;
+      const uint32_t lo = k + 2 * i < D ? row[k + 2 * i] : 0, hi = k + 2 * i + 1 < D ? row[k + 2 * i + 1] : 0;
       w[i] = lo | (hi << 16);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);

@@ -553,21 +553,27 @@ struct DzEpi {
 };
 
 // dh[r] = alpha * acc[compacted row of r], 0 for rows that do not count.
-__global__ void __launch_bounds__(256) xent_dh_kernel(const float* __restrict__ acc, int64_t lda, const int32_t* __restrict__ pos,
-                                                      const float* __restrict__ alpha, void* dh, int64_t lddh, int dtype,
-                                                      int64_t M, int D, int vec) {
+__global__ void __launch_bounds__(256) xent_dh_kernel(const float* acc, int64_t lda, const int32_t* pos, const float* alpha,
+                                                      void* dh, int64_t lddh, int dtype, int64_t M, int D, int vec) {
   launch_next();
   wait_previous();
   const float a = *alpha;
   const int lane = threadIdx.x & 31;
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < M; r += (int64_t)gridDim.x * 8) {
     const int at = pos[r];
-#pragma unroll 4
-    for (int c = 4 * lane; c < D; c += 128) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (at >= 0) v = *reinterpret_cast<const float4*>(acc + at * lda + c);
-      const float f[4] = {v.x * a, v.y * a, v.z * a, v.w * a};
-      store_row4(dh, r * lddh + c, f, D - c, dtype, vec);
+    for (int c0 = 4 * lane; c0 < D; c0 += 512) {  // four loads in flight before the first store
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int c = c0 + 128 * k;
+        v[k] = at >= 0 && c < D ? *reinterpret_cast<const float4*>(acc + at * lda + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int c = c0 + 128 * k;
+        const float f[4] = {v[k].x * a, v[k].y * a, v[k].z * a, v[k].w * a};
+        if (c < D) store_row4(dh, r * lddh + c, f, D - c, dtype, vec);
+      }
     }
   }
 }
