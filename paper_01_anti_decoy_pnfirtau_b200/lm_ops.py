@@ -295,7 +295,10 @@ class Bf16Casts:
 
     A copy is handed out only while its parameter still has the storage and the
     version counter seen at the last ``refresh()`` (an in-place update such as
-    an optimizer step makes it stale until the next refresh). ``padded``: rows
+    an optimizer step makes it stale until the next refresh). A refresh from a
+    parameter that changed counts as an in-place change of its copy: the backward
+    of a graph that saved the copy before raises, as one that saved the parameter
+    would. ``padded``: rows
     to pad a 2-D parameter to (its copy's extra rows stay zero), as the LM head's
     GEMM wants. The device table of addresses is written outside CUDA graph
     capture (the first refresh); a refresh inside a capture records only the
@@ -335,7 +338,11 @@ class Bf16Casts:
         n = max(t.numel() for t in self.params)
         _lib.check(_lib.lib().pnft_cast_bf16(self._table.data_ptr(), len(self.params), n, _stream(self.device)),
                    "pnft_cast_bf16")
-        self._seen = [(t.data_ptr(), t._version) for t in self.params]
+        seen = [(t.data_ptr(), t._version) for t in self.params]
+        changed = [c for c, now, was in zip(self.copies, seen, self._seen) if now != was and not c.is_inference()]
+        if changed:
+            torch.autograd.graph.increment_version(changed)
+        self._seen = seen
 
     def _current(self, t: torch.Tensor) -> int:
         i = self.index.get(id(t), -1)

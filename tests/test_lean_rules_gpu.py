@@ -1,0 +1,59 @@
+"""Calls of the lean training-step operators at the edges of what they allow."""
+import pytest
+import torch
+
+from paper_01_anti_decoy_pnfirtau_b200 import gated_linear, streamed_cross_entropy
+from paper_01_anti_decoy_pnfirtau_b200.lm_ops import Bf16Casts, Linear, mlp_gelu
+
+pytestmark = pytest.mark.gpu
+BF16, FP32 = torch.bfloat16, torch.float32
+
+
+def rand(*shape, dt=BF16, std=1.0, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed + sum(shape))
+    return (torch.randn(*shape, device="cuda", generator=g) * std).to(dt)
+
+
+# ------------------------------------------------------------------ parameter copies
+def copied_calls():
+    """An input, and (call, parameters) of every operator that takes parameter copies."""
+    x = rand(40, 32).requires_grad_(True)
+    a, b, w = (torch.nn.Parameter(rand(64, 32, dt=FP32, std=0.3, seed=i)) for i in range(3))
+    t = torch.arange(40, device="cuda")
+    lin = Linear(32, 64).to("cuda")
+    fc1, fc2 = torch.nn.Linear(32, 64).to("cuda"), torch.nn.Linear(64, 32).to("cuda")
+
+    def linear(casts):
+        lin.casts = casts
+        return lin(x)
+
+    return x, {
+        "gated": (lambda casts: gated_linear(x, a, b, casts=casts), [a, b]),
+        "gated8": (lambda casts: gated_linear(x, a, b, checkpoint_8bit=True, casts=casts), [a, b]),
+        "xent": (lambda casts: streamed_cross_entropy(x, w, t, casts=casts), [w]),
+        "linear": (linear, list(lin.parameters())),
+        "mlp": (lambda casts: mlp_gelu(x, fc1, fc2, casts), [*fc1.parameters(), *fc2.parameters()]),
+    }
+
+
+@pytest.mark.parametrize("name", ["gated", "gated8", "xent", "linear", "mlp"])
+def test_a_graph_on_parameter_copies_refreshed_since(cuda, name):
+    """Copies refreshed from parameters that changed raise in the backward of a graph made before, as an in-place
+    change of the parameters themselves does; refreshed from the same parameters they do not."""
+    x, calls = copied_calls()
+    call, params = calls[name]
+    casts = Bf16Casts(params)
+    casts.refresh()
+    with torch.autocast("cuda", dtype=BF16):
+        first, want = call(casts), call(None)
+        casts.refresh()  # another forward in between, say of the next micro-batch
+        second = call(casts)
+    for out in (first, second):
+        got = torch.autograd.grad(out.float().sum(), [x, *params], retain_graph=True)
+        for g, r in zip(got, torch.autograd.grad(want.float().sum(), [x, *params], retain_graph=True)):
+            assert torch.equal(g, r)
+    with torch.no_grad():
+        params[0].mul_(2)
+    casts.refresh()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(first.float().sum(), x)

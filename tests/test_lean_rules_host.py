@@ -1,7 +1,9 @@
 """Rules of the lean training-step operators that can be checked without a GPU."""
 import re
 
-from paper_01_anti_decoy_pnfirtau_b200 import _build
+import torch
+
+from paper_01_anti_decoy_pnfirtau_b200 import _build, lm_ops
 
 
 def code(path):
@@ -27,3 +29,33 @@ def test_kernels_launched_early_wait():
         if "wait_previous()" in text:
             assert text.count("__global__") == len(re.findall(r"(?<!void )wait_previous\(\);", text)), f.name
             assert text.count("__global__") == len(re.findall(r"(?<!void )launch_next\(\);", text)), f.name
+
+
+def test_refreshed_copies_of_changed_parameters_count_as_changed(monkeypatch):
+    """A copy's version moves when it is refreshed from a parameter that changed, and only then: autograd sees by it
+    that a tensor saved for a backward holds other values now."""
+    calls = []
+
+    class Library:
+        def pnft_cast_bf16(self, *args):
+            calls.append(args)
+            return 0
+
+    monkeypatch.setattr(lm_ops._lib, "lib", Library)
+    monkeypatch.setattr(lm_ops, "_stream", lambda dev: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    a, b, head = (torch.nn.Parameter(torch.randn(6, 4)) for _ in range(3))
+    casts = lm_ops.Bf16Casts([a, b, head], padded={id(head): 8})
+    versions = lambda: [c._version for c in casts.copies]  # noqa: E731
+    casts.refresh()
+    first = versions()
+    casts.refresh()
+    assert versions() == first and len(calls) == 2
+    with torch.no_grad():
+        b.add_(1)
+        head.add_(1)
+    casts.refresh()
+    assert [x > y for x, y in zip(versions(), first)] == [False, True, True]
+    a.data = a.data.clone()  # another storage
+    casts.refresh()
+    assert versions()[0] > first[0]
