@@ -19,13 +19,16 @@ reference's language-model experiments (experiments/exp4_wikitext2_lm.py:183-259
 
 Operands are bfloat16 or float16: under CUDA autocast the inputs are cast to the
 autocast dtype, else the input's dtype counts; float32 without autocast raises. CUDA
-only; a CPU tensor raises. Results are bitwise reproducible on a given GPU.
+only; a CPU tensor raises. Results are bitwise reproducible on a given GPU. Forward-mode
+tangents and tracing (``torch.jit.trace``, ``make_fx``) are refused; the ``act8_*`` calls
+are not differentiable: their results require no gradient, whatever their inputs do.
 """
 from __future__ import annotations
 
 import math
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn as nn
 
 from . import _lib
@@ -40,6 +43,19 @@ def _compute_dtype(x: torch.Tensor, what: str) -> torch.dtype:
     if dt not in _TYPES16:
         raise RuntimeError(f"{what}: bfloat16 or float16 expected (or CUDA autocast to one of them), got {dt}")
     return dt
+
+
+def _plain_values(what: str, *tensors: torch.Tensor | None) -> None:
+    """Raises where a call would lose what follows the values: the kernels write through addresses, so a tangent
+    would vanish and a trace would hold an uninitialised buffer in the call's place."""
+    if torch._C._get_tracing_state() is not None or (
+            torch._C._len_torch_dispatch_stack() > 0
+            and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
+        raise RuntimeError(f"{what}: cannot be traced")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what}: forward-mode differentiation is not available")
 
 
 def _context(dev: torch.device) -> tuple[int, int]:
@@ -137,6 +153,7 @@ def act8_pack(x: torch.Tensor) -> Act8:
     128 columns e4m3 values times the least power of two that brings the block's largest
     magnitude to 448 or less, rounded to nearest even. NaN and infinities become NaN."""
     dev = _require_cuda("act8_pack", x)
+    _plain_values("act8_pack", x)
     code = _DTYPES.get(x.dtype)
     if code is None:
         raise RuntimeError(f"act8_pack: float32, bfloat16 or float16 expected, got {x.dtype}")
@@ -169,6 +186,7 @@ def _act8_rows(p: Act8, dt: torch.dtype, width: int) -> torch.Tensor:
 def act8_unpack(p: Act8) -> torch.Tensor:
     """The tensor that ``p`` stands for, in the shape and dtype that were packed (exact:
     the dtype holds every packed value)."""
+    _plain_values("act8_unpack", p.data)
     if _elsewhere(p.data.device):
         with torch.cuda.device(p.data.device):
             return act8_unpack(p)
@@ -181,6 +199,7 @@ def act8_weight_grad(dy: torch.Tensor, p: Act8, out_dtype: torch.dtype = torch.f
     from its output's gradient ``dy`` (``[..., N]``, bfloat16 or float16, as many rows as
     ``x``) and its input kept in 8 bits; fp32 sums."""
     dev = _require_cuda("act8_weight_grad", dy, p.data)
+    _plain_values("act8_weight_grad", dy)
     if dy.dtype not in _TYPES16 or out_dtype not in _DTYPES:
         raise RuntimeError(f"act8_weight_grad: bfloat16 or float16 gradient and a float32, bfloat16 or float16 result expected, "
                            f"got {dy.dtype} and {out_dtype}")
@@ -314,6 +333,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     bf16 copies of the weights, used when the dtype is bf16."""
     biases = () if b_gate is None and b_up is None else tuple(b for b in (b_gate, b_up) if b is not None)
     dev = _require_cuda("gated_linear", x, w_gate, w_up, *biases)
+    _plain_values("gated_linear", x, w_gate, w_up, *biases)
     act = _ACTS.get(activation)
     if act is None:
         raise ValueError(f"gated_linear: activation {activation!r} (one of {sorted(_ACTS)})")
@@ -423,6 +443,7 @@ def streamed_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch
     and is reported by ``check_device_status()`` or the next call. ``casts``: an
     ``lm_ops.Bf16Casts`` with a current bf16 copy of ``weight``. Twice differentiating raises."""
     dev = _require_cuda("streamed_cross_entropy", h, weight, targets)
+    _plain_values("streamed_cross_entropy", h, weight)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"streamed_cross_entropy: reduction {reduction!r}")
     if h.dim() == 0 or weight.dim() != 2 or h.shape[-1] != weight.shape[1]:

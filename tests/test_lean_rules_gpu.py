@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from paper_01_anti_decoy_pnfirtau_b200 import gated_linear, streamed_cross_entropy
+from paper_01_anti_decoy_pnfirtau_b200 import act8_pack, act8_unpack, act8_weight_grad, gated_linear, streamed_cross_entropy
 from paper_01_anti_decoy_pnfirtau_b200.lm_ops import Bf16Casts, Linear, mlp_gelu
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +57,44 @@ def test_a_graph_on_parameter_copies_refreshed_since(cuda, name):
     casts.refresh()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(first.float().sum(), x)
+
+
+# ------------------------------------------------------------------ forward mode, tracing
+def raw_calls():
+    x, w, t = rand(40, 64), rand(96, 64, std=0.1, seed=1), torch.arange(40, device="cuda")
+    bias, p = rand(96, seed=2), act8_pack(x)
+    return {
+        "gated x": (lambda v: gated_linear(v, w, w), x),
+        "gated weight": (lambda v: gated_linear(x, w, v), w),
+        "gated bias": (lambda v: gated_linear(x, w, w, v), bias),
+        "xent h": (lambda v: streamed_cross_entropy(v, w, t), x),
+        "xent weight": (lambda v: streamed_cross_entropy(x, v, t), w),
+        "pack": (lambda v: act8_unpack(act8_pack(v)), x),
+        "weight grad": (lambda v: act8_weight_grad(v, p), x),
+    }
+
+
+@pytest.mark.parametrize("name", ["gated x", "gated weight", "gated bias", "xent h", "xent weight", "pack", "weight grad"])
+def test_forward_mode_and_tracing_are_refused(cuda, name):
+    """A tangent would be lost and a trace would hold no operator; without tangents a dual level changes nothing."""
+    import torch.autograd.forward_ad as fwAD
+
+    call, v = raw_calls()[name]
+    want = call(v)
+    with fwAD.dual_level():
+        assert torch.equal(call(v), want)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(fwAD.make_dual(v, torch.ones_like(v)))
+    with pytest.raises(RuntimeError, match="trac"):
+        torch.jit.trace(call, (v,))
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    with pytest.raises(RuntimeError, match="trac"):
+        make_fx(call)(v)
+    assert torch.equal(call(v), want)
+
+
+def test_act8_results_require_no_gradient(cuda):
+    x, dy = rand(20, 64).requires_grad_(True), rand(20, 32, seed=1).requires_grad_(True)
+    p = act8_pack(x)
+    assert not act8_unpack(p).requires_grad and not act8_weight_grad(dy, p).requires_grad
