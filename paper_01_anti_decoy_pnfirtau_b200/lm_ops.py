@@ -486,7 +486,7 @@ class Linear(nn.Linear):
     ``checkpoint_8bit`` (plain attribute, default False): the backward keeps the
     input in 8 bits (``act8_pack``) and takes the weight gradient from that
     (``act8_weight_grad``); output and input gradient do not change. Needs a bf16
-    computation."""
+    computation, except where gradients are disabled (no backward, nothing kept)."""
 
     casts: "Bf16Casts | None" = None
     checkpoint_8bit: bool = False
@@ -497,9 +497,10 @@ class Linear(nn.Linear):
             dt = torch.float32
         c = self.casts
         pre = c.lookup(self.weight, self.bias) if c is not None and dt == torch.bfloat16 else None
-        if self.checkpoint_8bit and dt != torch.bfloat16:
+        in8 = self.checkpoint_8bit and torch.is_grad_enabled()  # without a backward nothing is kept
+        if in8 and dt != torch.bfloat16:
             raise RuntimeError(f"Linear: checkpoint_8bit needs a bfloat16 computation (input or CUDA autocast), got {dt}")
-        return _LinearFn.apply(x, self.weight, self.bias, dt, pre, self.checkpoint_8bit)
+        return _LinearFn.apply(x, self.weight, self.bias, dt, pre, in8)
 
     @classmethod
     def sharing(cls, lin: nn.Linear) -> "Linear":

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from paper_01_anti_decoy_pnfirtau_b200 import act8_pack, act8_unpack, act8_weight_grad, gated_linear, streamed_cross_entropy
+from paper_01_anti_decoy_pnfirtau_b200 import lm_ops
 from paper_01_anti_decoy_pnfirtau_b200.lm_ops import Bf16Casts, Linear, mlp_gelu
 
 pytestmark = pytest.mark.gpu
@@ -98,3 +99,20 @@ def test_act8_results_require_no_gradient(cuda):
     x, dy = rand(20, 64).requires_grad_(True), rand(20, 32, seed=1).requires_grad_(True)
     p = act8_pack(x)
     assert not act8_unpack(p).requires_grad and not act8_weight_grad(dy, p).requires_grad
+
+
+# ------------------------------------------------------------------ evaluation
+def test_linear_packs_its_input_for_a_backward_alone(cuda, monkeypatch):
+    """With checkpoint_8bit set a call that no backward follows packs nothing, and takes any type as before."""
+    torch.manual_seed(0)
+    lin, x = Linear(100, 77).to(cuda), rand(33, 100)
+    with torch.no_grad():
+        want, want32 = lin(x), lin(x.float())
+    lin.checkpoint_8bit = True
+    packed = []
+    monkeypatch.setattr(lm_ops, "act8_pack", lambda t: packed.append(t.shape) or act8_pack(t))
+    for context in (torch.no_grad, torch.inference_mode):
+        with context():
+            assert torch.equal(lin(x), want) and torch.equal(lin(x.float()), want32)
+    assert not packed
+    assert torch.equal(lin(x).detach(), want) and packed == [(33, 100)]
