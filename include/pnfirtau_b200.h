@@ -423,12 +423,17 @@ PNFT_API int pnft_cast_bf16(const int64_t* table, int count, int64_t max_n, void
  * status: as the flash entry points (bounded pipeline waits).
  * ------------------------------------------------------------------------- */
 
+/* Calls without a backward of up to so many rows have kernels of their own, which take any row
+ * strides (at least the width) and any 2-byte alignment. */
+#define PNFT_GATED_FEW_ROWS 32 /* pnft_gated_fwd without pre */
+#define PNFT_XENT_FEW_ROWS 24  /* pnft_stream_xent_fwd without saved */
+
 #define PNFT_ACT_SILU 0
 #define PNFT_ACT_GELU 1 /* the exact (erf) form */
 
 /* Gated feed-forward product h[M x F] = act(x Wg^T + bg) * (x Wu^T + bu), x [M x D],
- * Wg and Wu [F x D], one kernel (calls of up to 32 rows without pre have one of their
- * own, which takes any row strides >= D). bg / bu [F] of type b_dtype (each may be NULL). h is
+ * Wg and Wu [F x D], one kernel (calls of up to PNFT_GATED_FEW_ROWS rows without pre have
+ * one of their own). bg / bu [F] of type b_dtype (each may be NULL). h is
  * written in `dtype`. pre (may be NULL): the pre-activations x Wg^T + bg and x Wu^T + bu
  * kept for pnft_gated_bwd with 24 bits each, as three matrices [M x ldp] of 16-bit
  * words one after the other (ldp a multiple of 8, 16-byte aligned).
@@ -478,8 +483,8 @@ PNFT_API int pnft_copy_rows16(const void* src, int64_t lds, void* dst, int64_t l
  * ignore_index gives NaN and sets the status word to PNFT_DEV_BAD_INDEX. Rows to
  * ignore are left out of all work; what they hold reaches no result.
  * saved (pnft_stream_xent_saved_size(M, D) bytes, 16-byte aligned): the rows that
- * count and their state, kept for the backward; NULL when there will be none (calls of
- * up to 24 rows then take a kernel of their own). h: any row stride >= D; W: 16-byte
+ * count and their state, kept for the backward; NULL when there will be none (calls of up
+ * to PNFT_XENT_FEW_ROWS rows then take a kernel of their own). h: any row stride >= D; W: 16-byte
  * aligned rows, except in those small calls. workspace:
  * pnft_stream_xent_fwd_workspace_size(M, V, D, saved != NULL) bytes, 16-byte aligned.
  * M >= 1.

@@ -20,6 +20,7 @@ FLASH_FORCE_GENERIC, FLASH_DETERMINISTIC, FLASH_PREFER_SM100 = 0x1, 0x2, 0x4
 FLASH_TEST_STALL = 0x100  # test-only: the tcgen05 kernels take their timeout path
 FIR_FUSED_TAPS = 7  # PNFT_FIR_FUSED_TAPS
 ACT_SILU, ACT_GELU = 0, 1
+GATED_FEW_ROWS, XENT_FEW_ROWS = 32, 24  # PNFT_GATED_FEW_ROWS, PNFT_XENT_FEW_ROWS
 GELU_TABLE_FLOATS = 10240  # PNFT_GELU_TABLE_FLOATS
 
 _I64x4 = c_int64 * 4

@@ -264,7 +264,7 @@ struct GatedEpi {
 // ------------------------------------------------------------------ a few rows
 // From 33 rows on the tiles win (B200, bf16, cold L2: 1024 x 4096 weights 9.3 us here at 32
 // rows and 13.7 in tiles, 4096 x 16384 74 and 67; at one row 6.8 and 13.7, 51 and 67).
-constexpr int SKINNY_ROWS = 32;
+constexpr int SKINNY_ROWS = PNFT_GATED_FEW_ROWS;
 // Forward for few rows: a block has 16 columns of h; each of its warps takes an
 // eighth of K of the products of x with those rows of Wg and of Wu.
 struct SkinnyArgs {

@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(256) xent_reduce_kernel(ReduceArgs p) {
 // ------------------------------------------------------------------ a few rows
 // From 25 rows on the tiles win (B200, bf16, cold L2: 33278 x 256 weights 15 us here at one
 // row, 20 at 24 and 28 to 35 in tiles; 50021 x 1024 36, 45 and 47 to 54).
-constexpr int SKINNY_ROWS = 24;
+constexpr int SKINNY_ROWS = PNFT_XENT_FEW_ROWS;
 // Loss of few rows without a gradient: every warp takes 16 or 32 words of the vocabulary
 // at a time and keeps each row's maximum and sum over them; a block joins its warps' and
 // leaves one pair per row. Rows to ignore are computed with the others (a column of the

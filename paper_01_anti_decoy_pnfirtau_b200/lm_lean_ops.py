@@ -234,7 +234,11 @@ def act8_weight_grad(dy: torch.Tensor, p: Act8, out_dtype: torch.dtype = torch.f
 # backward on a B200 (bf16, 16384 rows, F = 4 D), kept against computed again: D = 512
 # 286 and 249 us, 768 503 and 480, 1024 820 and 840, 2048 2700 and 3102.
 _KEEP_FROM = 896
-_FEW = 24  # rows up to which the forward kernels take any row strides
+# Rows up to which a call that keeps nothing leaves unaligned rows as they are: all that the few-row
+# kernel takes where the width is no multiple of 8, since aligned copies gain no vector loads there
+# (B200, 32 rows from cold L2, copied against in place: 1001 x 4096 35 and 22 us, 2047 x 5461 115
+# and 57); fewer where they do (2-byte aligned views, 1024 x 4096 27 and 25, 4096 x 16384 210 and 270).
+_FEW_VECTOR = 24
 
 
 def _gated_forward(x, wg, wu, bg, bu, act: int, dt: torch.dtype, keep: bool):
@@ -244,7 +248,8 @@ def _gated_forward(x, wg, wu, bg, bu, act: int, dt: torch.dtype, keep: bool):
     flat = x.dim() == 2
     x2 = x if flat else x.reshape(-1, D)
     M = x2.shape[0]
-    rows = _rows16 if keep or M > _FEW else _unit_rows
+    few = _lib.GATED_FEW_ROWS if D % 8 else _FEW_VECTOR
+    rows = _rows16 if keep or M > few else _unit_rows
     x2, wg, wu = rows(x2, dt), rows(wg, dt), rows(wu, dt)
     h = _new(M, F_, dt, dev)
     pre = _new(3 * M, _pad8(F_), torch.int16, dev) if keep else None
@@ -371,7 +376,7 @@ def _xent_forward(h, weight, targets, ignore_index: int, reduction: str, dt: tor
     V, D = weight.shape
     h2 = _unit_rows(h if h.dim() == 2 else h.reshape(-1, D), dt)
     M = h2.shape[0]
-    w = _rows16(weight, dt) if save or M > _FEW else _unit_rows(weight, dt)
+    w = _rows16(weight, dt) if save or M > _lib.XENT_FEW_ROWS else _unit_rows(weight, dt)
     t = targets if targets.dim() == 1 else targets.reshape(-1)
     if t.dtype != torch.int64 or not t.is_contiguous():
         t = t.to(torch.int64).contiguous()

@@ -3,11 +3,12 @@ import pytest
 import torch
 
 from paper_01_anti_decoy_pnfirtau_b200 import act8_pack, act8_unpack, act8_weight_grad, gated_linear, streamed_cross_entropy
+from paper_01_anti_decoy_pnfirtau_b200 import lm_lean_ops as lean
 from paper_01_anti_decoy_pnfirtau_b200 import lm_ops
 from paper_01_anti_decoy_pnfirtau_b200.lm_ops import Bf16Casts, Linear, mlp_gelu
 
 pytestmark = pytest.mark.gpu
-BF16, FP32 = torch.bfloat16, torch.float32
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 
 
 def rand(*shape, dt=BF16, std=1.0, seed=0):
@@ -116,3 +117,23 @@ def test_linear_packs_its_input_for_a_backward_alone(cuda, monkeypatch):
             assert torch.equal(lin(x), want) and torch.equal(lin(x.float()), want32)
     assert not packed
     assert torch.equal(lin(x).detach(), want) and packed == [(33, 100)]
+
+
+# ------------------------------------------------------------------ few rows
+@pytest.mark.parametrize("M", [24, 25, 31, 32, 33])
+@pytest.mark.parametrize("dt", [BF16, FP16])
+def test_gated_few_rows_take_rows_as_they_are(cuda, M, dt, monkeypatch):
+    """Without a gradient, up to 32 rows of an odd width are read in place; 2-byte aligned views equal their copies."""
+    from test_lean_ops_gpu import check, gated_inputs, gated_oracle
+
+    copied = []
+    monkeypatch.setattr(lean, "_rows16", lambda t, d, f=lean._rows16: copied.append(t.shape) or f(t, d))
+    for D in (77, 1001):
+        x, wg, wu, bg, bu, dh = gated_inputs(M, D, 61, dt, True, M + D, cuda)
+        want = gated_oracle(x, wg, wu, bg, bu, dh, "gelu", dt, kept=False)[0]
+        check("h", gated_linear(x, wg, wu, bg, bu, "gelu"), want)
+    assert (not copied) == (M <= 32)
+    base = rand(200, 66, dt=dt)
+    for cols in (slice(1, 65), slice(1, 64)):
+        x, w = base[:M, cols], base[100:, cols]
+        assert torch.equal(gated_linear(x, w, w), gated_linear(x.contiguous(), w.contiguous(), w.contiguous()))

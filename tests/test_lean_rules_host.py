@@ -3,7 +3,7 @@ import re
 
 import torch
 
-from paper_01_anti_decoy_pnfirtau_b200 import _build, lm_ops
+from paper_01_anti_decoy_pnfirtau_b200 import _build, _lib, lm_ops
 
 
 def code(path):
@@ -59,3 +59,11 @@ def test_refreshed_copies_of_changed_parameters_count_as_changed(monkeypatch):
     a.data = a.data.clone()  # another storage
     casts.refresh()
     assert versions()[0] > first[0]
+
+
+def test_limits_of_the_few_row_calls_agree():
+    """The Python calls leave rows unaligned up to the number of rows that the C entry points take so."""
+    header = (_build.INCLUDE / "pnfirtau_b200.h").read_text()
+    limit = lambda name: int(re.search(rf"#define {name} (\d+)", header).group(1))  # noqa: E731
+    assert _lib.GATED_FEW_ROWS == limit("PNFT_GATED_FEW_ROWS")
+    assert _lib.XENT_FEW_ROWS == limit("PNFT_XENT_FEW_ROWS")
