@@ -415,6 +415,7 @@ class _StreamXentFn(torch.autograd.Function):
 def _xent_backward(ctx, dloss):
     saved, w = ctx.saved_tensors
     M, dt, reduction, h_shape, h_dtype, w_dtype = ctx.meta
+    w = _rows16(w, dt)  # a copy only where a hook brought the saved rows back without their padding
     V, D = w.shape
     dev = w.device
     L = _lib.lib()

@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from paper_01_anti_decoy_pnfirtau_b200 import act8_pack, act8_unpack, act8_weight_grad, gated_linear, streamed_cross_entropy
+from paper_01_anti_decoy_pnfirtau_b200 import (act8_pack, act8_unpack, act8_weight_grad, check_device_status, gated_linear,
+                                               streamed_cross_entropy)
 from paper_01_anti_decoy_pnfirtau_b200 import lm_lean_ops as lean
 from paper_01_anti_decoy_pnfirtau_b200 import lm_ops
 from paper_01_anti_decoy_pnfirtau_b200.lm_ops import Bf16Casts, Linear, mlp_gelu
@@ -137,3 +138,31 @@ def test_gated_few_rows_take_rows_as_they_are(cuda, M, dt, monkeypatch):
     for cols in (slice(1, 65), slice(1, 64)):
         x, w = base[:M, cols], base[100:, cols]
         assert torch.equal(gated_linear(x, w, w), gated_linear(x.contiguous(), w.contiguous(), w.contiguous()))
+
+
+# ------------------------------------------------------------------ saved tensors
+@pytest.mark.parametrize("D", [64, 77, 1001])
+def test_saved_tensors_that_were_moved_come_back(cuda, D):
+    """A backward whose saved tensors were kept on the host, and one that computes its forward again."""
+    from torch.utils.checkpoint import checkpoint
+
+    x, wg, wu, w = (rand(n, D, std=D ** -0.5, seed=i).requires_grad_(True) for i, n in enumerate((50, 130, 130, 300)))
+    t = torch.arange(50, device=cuda)
+    lin = Linear(D, 40).to(cuda).bfloat16()
+    lin.checkpoint_8bit = True
+    calls = {
+        "gated": (lambda: gated_linear(x, wg, wu), (x, wg, wu)),
+        "gated8": (lambda: gated_linear(x, wg, wu, checkpoint_8bit=True), (x, wg, wu)),
+        "xent": (lambda: streamed_cross_entropy(x, w, t), (x, w)),
+        "linear8": (lambda: lin(x), (x, lin.weight)),
+    }
+    for name, (call, leaves) in calls.items():
+        want = torch.autograd.grad(call().float().sum(), leaves)
+        for pinned in (False, True):
+            with torch.autograd.graph.save_on_cpu(pin_memory=pinned):
+                out = call()
+            for g, r in zip(torch.autograd.grad(out.float().sum(), leaves), want):
+                assert torch.equal(g, r), name
+        for g, r in zip(torch.autograd.grad(checkpoint(call, use_reentrant=False).float().sum(), leaves), want):
+            assert torch.equal(g, r), name
+    check_device_status(cuda)
