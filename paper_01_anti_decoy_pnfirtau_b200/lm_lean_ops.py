@@ -122,6 +122,10 @@ def _rows16(t: torch.Tensor, dt: torch.dtype) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- 8-bit activations
+def _act8_row_bytes(D: int) -> int:
+    return (D + 15) // 16 * 16 + ((D + 127) // 128 + 15) // 16 * 16
+
+
 class Act8:
     """An activation in 8 bits: ``data`` holds a row's e4m3 bytes (padded to a multiple of
     16) and behind them one int8 exponent per block of 128 columns; an element's value is
@@ -141,11 +145,18 @@ class Act8:
         return self.data.numel()
 
     def _layout(self):
-        """(bytes' address, row stride, exponents' address, row stride, rows, columns)."""
-        rows, ld = self.data.shape
-        D = self.shape[-1]
-        at = self.data.data_ptr()
-        return at, ld, at + (D + 15) // 16 * 16, ld, rows, D
+        """(bytes' address, row stride, exponents' address, row stride, rows, columns), once the
+        buffer is known to hold what ``shape`` says."""
+        data, shape = self.data, self.shape
+        D = shape[-1] if len(shape) else 0
+        q, ld = (D + 15) // 16 * 16, _act8_row_bytes(D)
+        at = data.data_ptr()
+        if (D == 0 or data.dtype is not torch.uint8 or data.dim() != 2 or data.shape[1] != ld or data.stride(1) != 1
+                or data.shape[0] != math.prod(shape[:-1]) or (data.shape[0] > 1 and data.stride(0) != ld) or at % 16
+                or self.dtype not in _DTYPES):
+            raise RuntimeError(f"Act8: {data.dtype} buffer {tuple(data.shape)} with strides {data.stride()} does not hold "
+                               f"{tuple(shape)} of {self.dtype} in 8 bits")
+        return at, ld, at + q, ld, data.shape[0], D
 
 
 def act8_pack(x: torch.Tensor) -> Act8:
@@ -166,7 +177,7 @@ def act8_pack(x: torch.Tensor) -> Act8:
     D = shape[-1]
     x2 = _unit_rows(x if x.dim() == 2 else x.reshape(-1, D), x.dtype)
     M = x2.shape[0]
-    p = Act8(_new(M, (D + 15) // 16 * 16 + ((D + 127) // 128 + 15) // 16 * 16, torch.uint8, dev), shape, x.dtype)
+    p = Act8(_new(M, _act8_row_bytes(D), torch.uint8, dev), shape, x.dtype)
     q, ldq, e, lde, _, _ = p._layout()
     rc = _lib.lib().pnft_act8_pack(x2.data_ptr(), x2.stride(0) if M > 1 else D, q, ldq, e, lde, M, D, code, _context(dev)[1])
     _lib.check(rc, "pnft_act8_pack")
@@ -186,9 +197,10 @@ def _act8_rows(p: Act8, dt: torch.dtype, width: int) -> torch.Tensor:
 def act8_unpack(p: Act8) -> torch.Tensor:
     """The tensor that ``p`` stands for, in the shape and dtype that were packed (exact:
     the dtype holds every packed value)."""
+    dev = _require_cuda("act8_unpack", p.data)
     _plain_values("act8_unpack", p.data)
-    if _elsewhere(p.data.device):
-        with torch.cuda.device(p.data.device):
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
             return act8_unpack(p)
     y = _act8_rows(p, p.dtype, p.width)
     return y if y.shape == p.shape else y.view(p.shape)

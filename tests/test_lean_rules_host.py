@@ -1,8 +1,10 @@
 """Rules of the lean training-step operators that can be checked without a GPU."""
 import re
 
+import pytest
 import torch
 
+import paper_01_anti_decoy_pnfirtau_b200 as P
 from paper_01_anti_decoy_pnfirtau_b200 import _build, _lib, lm_ops
 
 
@@ -67,3 +69,18 @@ def test_limits_of_the_few_row_calls_agree():
     limit = lambda name: int(re.search(rf"#define {name} (\d+)", header).group(1))  # noqa: E731
     assert _lib.GATED_FEW_ROWS == limit("PNFT_GATED_FEW_ROWS")
     assert _lib.XENT_FEW_ROWS == limit("PNFT_XENT_FEW_ROWS")
+
+
+def test_act8_refuses_buffers_that_do_not_hold_its_shape():
+    """The kernels read what shape says: the buffer has to hold it."""
+    P.Act8(torch.zeros(4, 1024, dtype=torch.uint8), torch.Size((2, 2, 1000)), torch.bfloat16)._layout()
+    good = dict(data=torch.zeros(4, 1024, dtype=torch.uint8), shape=torch.Size((4, 1000)), dtype=torch.bfloat16)
+    for bad in (dict(data=torch.zeros(4, 1008, dtype=torch.uint8)), dict(data=torch.zeros(3, 1024, dtype=torch.uint8)),
+                dict(data=torch.zeros(4, 1024, dtype=torch.int8)), dict(data=torch.zeros(4 * 1024, dtype=torch.uint8)),
+                dict(data=torch.zeros(4, 2048, dtype=torch.uint8)[:, ::2]), dict(shape=torch.Size((4, 1025))),
+                dict(shape=torch.Size((5, 1000))), dict(shape=torch.Size(())), dict(shape=torch.Size((4, 0))),
+                dict(dtype=torch.float64), dict(data=torch.zeros(4 * 1024 + 8, dtype=torch.uint8)[8:].view(4, 1024))):
+        with pytest.raises(RuntimeError, match="Act8"):
+            P.Act8(**{**good, **bad})._layout()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        P.act8_unpack(P.Act8(**good))
