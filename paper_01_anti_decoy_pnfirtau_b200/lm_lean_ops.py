@@ -148,15 +148,15 @@ class Act8:
         """(bytes' address, row stride, exponents' address, row stride, rows, columns), once the
         buffer is known to hold what ``shape`` says."""
         data, shape = self.data, self.shape
-        D = shape[-1] if len(shape) else 0
-        q, ld = (D + 15) // 16 * 16, _act8_row_bytes(D)
-        at = data.data_ptr()
-        if (D == 0 or data.dtype is not torch.uint8 or data.dim() != 2 or data.shape[1] != ld or data.stride(1) != 1
-                or data.shape[0] != math.prod(shape[:-1]) or (data.shape[0] > 1 and data.stride(0) != ld) or at % 16
+        n = len(shape)
+        D = shape[-1] if n else 0
+        rows = shape[0] if n == 2 else math.prod(shape[:-1])
+        ld, at = _act8_row_bytes(D), data.data_ptr()
+        if (D == 0 or data.shape != (rows, ld) or data.dtype is not torch.uint8 or not data.is_contiguous() or at % 16
                 or self.dtype not in _DTYPES):
             raise RuntimeError(f"Act8: {data.dtype} buffer {tuple(data.shape)} with strides {data.stride()} does not hold "
                                f"{tuple(shape)} of {self.dtype} in 8 bits")
-        return at, ld, at + q, ld, data.shape[0], D
+        return at, ld, at + (D + 15) // 16 * 16, ld, rows, D
 
 
 def act8_pack(x: torch.Tensor) -> Act8:
@@ -177,11 +177,13 @@ def act8_pack(x: torch.Tensor) -> Act8:
     D = shape[-1]
     x2 = _unit_rows(x if x.dim() == 2 else x.reshape(-1, D), x.dtype)
     M = x2.shape[0]
-    p = Act8(_new(M, _act8_row_bytes(D), torch.uint8, dev), shape, x.dtype)
-    q, ldq, e, lde, _, _ = p._layout()
-    rc = _lib.lib().pnft_act8_pack(x2.data_ptr(), x2.stride(0) if M > 1 else D, q, ldq, e, lde, M, D, code, _context(dev)[1])
+    ld = _act8_row_bytes(D)
+    data = _new(M, ld, torch.uint8, dev)
+    q = data.data_ptr()
+    rc = _lib.lib().pnft_act8_pack(x2.data_ptr(), x2.stride(0) if M > 1 else D, q, ld, q + (D + 15) // 16 * 16, ld, M, D, code,
+                                   _context(dev)[1])
     _lib.check(rc, "pnft_act8_pack")
-    return p
+    return Act8(data, shape, x.dtype)
 
 
 def _act8_rows(p: Act8, dt: torch.dtype, width: int) -> torch.Tensor:
