@@ -166,3 +166,139 @@ def test_saved_tensors_that_were_moved_come_back(cuda, D):
         for g, r in zip(torch.autograd.grad(checkpoint(call, use_reentrant=False).float().sum(), leaves), want):
             assert torch.equal(g, r), name
     check_device_status(cuda)
+
+
+# ------------------------------------------------------------------ precision of what is kept and summed in fp32
+@pytest.mark.parametrize("D", [520, 1000])
+@pytest.mark.parametrize("name", ["silu", "gelu"])
+def test_backward_sees_preactivations_of_at_least_24_bits(cuda, D, name):
+    """Bias gradients of one row are dg and du themselves, in fp32. g and u are multiples of 2^-8 below 2^7, exact
+    in the sums; kept with 24 bits (width 1000) they lose less than 2^-15 of their size, computed again nothing.
+    |act'| <= 1.13, |act''| <= 0.8; the fast exponential and quotient cost 2^-18."""
+    from test_lean_ops_gpu import act
+
+    g0 = torch.Generator(device=cuda).manual_seed(D)
+    Fh = 2000
+    x = torch.randint(-3, 4, (1, D), device=cuda, generator=g0).float()
+    wg, wu = (torch.randint(-8, 9, (Fh, D), device=cuda, generator=g0) / 256.0 for _ in range(2))
+    bg, bu = (torch.zeros(Fh, device=cuda).requires_grad_(True) for _ in range(2))
+    dh = rand(1, Fh, seed=1)
+    with torch.autocast("cuda", dtype=BF16):
+        h = gated_linear(x, wg, wu, bg, bu, name)
+    dg, du = (t.double() for t in torch.autograd.grad(h, (bg, bu), dh))
+    g, u = (x.double() @ w.double().T for w in (wg, wu))
+    assert float(g.abs().max()) < 128 and float(u.abs().max()) < 128
+    a, da = act(g, name)
+    d, lost, fast = dh.double(), 2.0 ** -15 if D == 1000 else 0.0, 2.0 ** -18
+    eg, eu = lost * g.abs(), lost * u.abs()
+    want_g, want_u = (d * u * da)[0], (d * a)[0]
+    bound_g = (d.abs() * (eu * 1.13 + (u.abs() + eu) * (0.8 * eg + fast * (1 + g.abs()))))[0] + 1e-30
+    bound_u = (d.abs() * (1.13 * eg + fast * g.abs()))[0] + 1e-30
+    assert torch.all((dg - want_g).abs() <= bound_g) and torch.all((du - want_u).abs() <= bound_u)
+    # and pre-activations rounded to 16 bits would be seen here
+    r = u.to(BF16).double()
+    assert float(((d * r * da)[0] - want_g).abs().sub(bound_g).max()) > 0
+
+
+def test_fp32_weight_gradient_of_many_rows(cuda):
+    """Products of positive numbers over 65536 rows, one tile after the other without splits. The tensor core adds 16
+    products at a time and loses at most two steps (2^-22) of the running sum each time; it sums 2048 rows (128 times,
+    so 64.5 2^-22 of the piece's sum, 10% more as the pieces' rows are not all alike), and 32 pieces are added in fp32."""
+    M, N, D = 65536, 2048, 2048
+    g = torch.Generator(device=cuda).manual_seed(1)
+    x, dy = ((torch.rand(M, n, device=cuda, generator=g) + 0.5).to(BF16) for n in (D, N))
+    p = act8_pack(x)
+    got = act8_weight_grad(dy, p)
+    x8, want = act8_unpack(p), torch.zeros(N, D, dtype=torch.float64, device=cuda)
+    for i in range(0, M, 8192):
+        want += dy[i:i + 8192].double().T @ x8[i:i + 8192].double()
+    worst = float(((got.double() - want) / want).abs().max())
+    assert worst <= 1.1 * 64.5 * 2.0 ** -22 + 32 * 2.0 ** -24, worst
+
+
+@pytest.mark.parametrize("M,grad", [(200, True), (200, False), (20, False)])
+def test_fp32_loss_of_a_wide_model(cuda, M, grad):
+    """Logits that are sums of 32768 positive products, against a target whose logit is 0: the loss has the logits' own
+    relative error. Sums of the tensor core as above, in pieces of 1024 (64 additions; few rows 512 and 32), which are
+    added in fp32; the logarithm and its base cost 2^-20."""
+    D, V = 32768, 300
+    g = torch.Generator(device=cuda).manual_seed(2)
+    h = (torch.rand(M, D, device=cuda, generator=g) + 0.5).to(BF16).requires_grad_(grad)
+    w = ((torch.rand(V, D, device=cuda, generator=g) + 0.5) * (30.0 / D)).to(BF16)
+    w[0] = 0
+    rows = streamed_cross_entropy(h, w, torch.zeros(M, dtype=torch.int64, device=cuda), reduction="none").detach()
+    z = h.detach().double() @ w.double().T
+    want = torch.logsumexp(z, 1) - z[:, 0]
+    piece, adds = (16.5, 64) if M <= 24 and not grad else (32.5, 32)
+    bound = 1.1 * piece * 2.0 ** -22 + adds * 2.0 ** -24 + 2.0 ** -20
+    worst = float(((rows.double() - want) / want).abs().max())
+    assert worst <= bound, (worst, bound)
+
+
+# ------------------------------------------------------------------ threads, whole steps
+def test_two_threads_at_once(cuda):
+    """Calls from two threads, each on its own stream, with backward passes."""
+    import threading
+
+    w, wg, wu = rand(3000, 256, std=0.1, seed=9), rand(512, 256, std=0.06, seed=1), rand(512, 256, std=0.06, seed=2)
+    t = torch.arange(300, device=cuda)
+    xs = [rand(300, 256, seed=20 + i) for i in range(2)]
+
+    def step(x):
+        leaves = [v.clone().requires_grad_(True) for v in (x, wg, wu, w)]
+        h = gated_linear(*leaves[:3], checkpoint_8bit=True)
+        loss = streamed_cross_entropy(h[:, :256], leaves[3], t)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    out, failed = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    out[i] = step(xs[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed, failed
+    for a, b in zip(out, want):
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+    check_device_status(cuda)
+
+
+def test_lean_lm_step_replayed_bit_for_bit(cuda):
+    """With the attention's ordered backward the captured step and eager ones agree in every bit, and so do the
+    parameters after three steps (deterministic mode also fills uninitialised memory with NaN)."""
+    from paper_01_anti_decoy_pnfirtau_b200.lm import GraphedTrainStep, LMConfig, PnFirLM, make_optimizer, train_step
+
+    was, warn = torch.are_deterministic_algorithms_enabled(), torch.is_deterministic_algorithms_warn_only_enabled()
+    torch.use_deterministic_algorithms(True, warn_only=True)
+    try:
+        models = []
+        for _ in range(2):
+            torch.manual_seed(0)
+            cfg = LMConfig(vocab=1003, d_model=128, n_heads=2, n_layers=2, d_ff=344, max_seq=128, ffn="swiglu")
+            models.append(PnFirLM(cfg, streamed_loss=True, checkpoint_8bit=True).to(cuda))
+        a, b = models
+        gen = torch.Generator(device=cuda).manual_seed(2)
+        batches = [torch.randint(0, 1003, (4, 64), device=cuda, generator=gen) for _ in range(3)]
+        oa, ob = make_optimizer(a, capturable=True), make_optimizer(b, capturable=True)
+        step = GraphedTrainStep(b, ob, batches[0])
+        start = [p.detach().clone() for p in b.parameters()]
+        for idx in batches:
+            assert torch.equal(train_step(a, oa, idx), step.step(idx))
+        step.close()
+        for (n, p), (_, q), s in zip(a.named_parameters(), b.named_parameters(), start):
+            assert torch.equal(p, q) and not torch.equal(q, s), n
+    finally:
+        torch.use_deterministic_algorithms(was, warn_only=warn)
+    check_device_status(cuda)
