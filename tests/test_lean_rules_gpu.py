@@ -203,17 +203,18 @@ def test_backward_sees_preactivations_of_at_least_24_bits(cuda, D, name):
 def test_fp32_weight_gradient_of_many_rows(cuda):
     """Products of positive numbers over 65536 rows, one tile after the other without splits. The tensor core adds 16
     products at a time and loses at most two steps (2^-22) of the running sum each time; it sums 2048 rows (128 times,
-    so 64.5 2^-22 of the piece's sum, 10% more as the pieces' rows are not all alike), and 32 pieces are added in fp32."""
+    so 64.5 2^-22 of the piece's sum; half more, as numbers from 1/16 to 16 make its rows unlike), and 32 pieces are
+    added in fp32. Over so many octaves the products have more bits than the sum, so that every addition loses some."""
     M, N, D = 65536, 2048, 2048
     g = torch.Generator(device=cuda).manual_seed(1)
-    x, dy = ((torch.rand(M, n, device=cuda, generator=g) + 0.5).to(BF16) for n in (D, N))
+    x, dy = (torch.exp2(8 * torch.rand(M, n, device=cuda, generator=g) - 4).to(BF16) for n in (D, N))
     p = act8_pack(x)
     got = act8_weight_grad(dy, p)
     x8, want = act8_unpack(p), torch.zeros(N, D, dtype=torch.float64, device=cuda)
     for i in range(0, M, 8192):
         want += dy[i:i + 8192].double().T @ x8[i:i + 8192].double()
     worst = float(((got.double() - want) / want).abs().max())
-    assert worst <= 1.1 * 64.5 * 2.0 ** -22 + 32 * 2.0 ** -24, worst
+    assert worst <= 1.5 * 64.5 * 2.0 ** -22 + 32 * 2.0 ** -24, worst
 
 
 @pytest.mark.parametrize("M,grad", [(200, True), (200, False), (20, False)])
