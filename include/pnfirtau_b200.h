@@ -447,6 +447,7 @@ PNFT_API int pnft_gated_fwd(const void* x, int64_t ldx, const void* wg, int64_t 
  * (from `pre`, or computed again from x when pre is NULL):
  *   dg = dh * u * act'(g), du = dh * act(g)              (rounded to `dtype`)
  *   dx = dg Wg + du Wu, dwg = dg^T x, dwu = du^T x, dbg / dbu = column sums
+ * (float16: dg and du past 65504 are infinite)
  * dh [M x F]: 16-byte aligned rows, or any rows when F is no multiple of 8 or `pre` is
  * given. Sums run in a fixed order. workspace: pnft_gated_bwd_workspace_size bytes,
  * 16-byte aligned. */

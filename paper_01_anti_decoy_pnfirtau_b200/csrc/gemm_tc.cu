@@ -31,7 +31,7 @@ int plan_splits(int64_t tiles, int64_t kb, int rounds) {
 // read their partials (0.09 us each, from L2). Measured (B200, weight gradient from 8 bits, fp32
 // out), the last round split and whole: 8192 rows into 4096 x 4096 (34 of 256 tiles in the last
 // round, split in 2) 218 and 228 us; 4096 into 5632 x 1000 (14 of 88, in 5) 53 and 65; 2048 into
-// 2560 x 2560 (26 of 100, K too short: whole) 38.
+// 2560 x 2560 (26 of 100, K too short: whole) 38. The three times are a fit to these shapes.
 Plan plan_product(int64_t tiles, int64_t kb) {
   const int pairs = sm_count() / 2;
   if (tiles <= pairs) return Plan{plan_splits(tiles, kb), 0};

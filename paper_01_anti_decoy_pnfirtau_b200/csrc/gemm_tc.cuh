@@ -17,7 +17,8 @@
 //
 // Bound by the tensor core from K of about 1024 on, and by the power limit in long runs. Measured (B200,
 // bf16, single calls): the gated product 16384 x 2048 x 2048 178 us (1.55 PFLOP/s), 16384 x 512 x 2048
-// 55 us (1.25), cross entropy's forward 8192 x 50021 x 512 291 us (1.44), 16352 x 33278 x 256 240 us (1.16).
+// 55 us (1.25), cross entropy's forward 8192 x 50021 x 512 291 us (1.44), 16352 x 33278 x 256 240 us (1.16;
+// whole calls: the rows' compaction and the join of the strips take 25 us of that).
 #pragma once
 
 #include <string.h>
@@ -78,8 +79,8 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   return r;
 }
 // Arrival on a barrier of either CTA that publishes no memory (TMEM reads are ordered by
-// tcgen05.wait and tcgen05.fence): a release at cluster scope would cost a memory barrier
-// per warp and tile, which took a fifth of the epilogue's time.
+// tcgen05.wait and tcgen05.fence), so it is relaxed: a release at cluster scope took a
+// fifth of the epilogue's time.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -166,7 +167,9 @@ __host__ __device__ inline int run_owner(int64_t total, int64_t x, int pairs) {
 }
 
 // Strips per row tile: those of one to four equal rounds of items over the pairs, the one
-// with the fewest tiles in a row, counting a third of a tile for an item's start and end.
+// with the fewest tiles in a row, counting a third of a tile for an item's start and end (which
+// decides between equal counts only: cross entropy's forward with no such share, a third and a
+// whole tile, B200: 300 x 50021 x 512 47, 45, 47 us; 4096 x 131072 x 512 383 each).
 __host__ __device__ inline int auto_strips(int tiles_m, int tiles_n, int pairs) {
   int best = 1;
   float least = 3e38f;
@@ -842,6 +845,8 @@ inline uint32_t idesc(int dtype, bool a_mn, bool b_mn) {
   return idesc_f16(PM, BN, dtype == PNFT_DTYPE_BF16 ? 1 : 0, a_mn, b_mn);
 }
 
+// Strips go eight row tiles at a time. Measured (B200, bf16) with 4, 8 and 16: gated forward 8192 x 2048 x 8192
+// 358, 350, 346 us and its backward 842, 850, 858; cross entropy's backward 4096 x 128000 x 2048 4.81, 4.75, 4.61 ms.
 inline Sched plain_sched(int64_t m, int64_t n, int64_t kb, int splits) {
   Sched s;
   memset(&s, 0, sizeof(s));
@@ -881,7 +886,9 @@ int launch(const char* what, const Args& a, const typename Epi::Params& ep, cuda
   launch_dependent(k, dim3((unsigned)(2 * pairs_of(items))), 32 * (2 + Epi::WARPS), SMEM, st, a, ep);
   return check_launch(what, 1);
 }
-// C = A B^T with the plain epilogue; K in chunks of 2048 for an fp32 C (see StoreEpi).
+// C = A B^T with the plain epilogue; K in chunks of 2048 for an fp32 C (see StoreEpi). Chunks of 1024, 2048, 4096
+// and none (B200, weight gradient from 8 bits, 8192 rows into 4096 x 4096): 211, 203, 199, 193 us; the largest
+// relative error over 65536 rows of positive numbers 2.2e-6, 4.3e-6, 1.0e-5, 3.0e-4.
 constexpr int PROMOTE_KB = 32;
 template <bool A_MN, bool B_MN>
 int launch_store(const char* what, Args a, const StoreEpi<false>::Params& ep, cudaStream_t st) {

@@ -57,7 +57,9 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int D) {
 template <bool FOLD, int RG, int NT, bool VEC, bool BF16>
 __device__ __forceinline__ void dot(const uint16_t* const (&w)[2 * RG], const uint16_t* x, int64_t ldx, int M, int D, int first,
                                     int stride, float (&acc)[RG][NT][4]) {
-  constexpr int U = RG * NT <= 2 ? 4 : 2;  // steps in flight
+  // Steps in flight: four while their registers allow it. B200, four against two: one row of 50021 x 1024 37 and
+  // 41 us; 32 rows of the gated 4096 x 16384 88 and 78.
+  constexpr int U = RG * NT <= 2 ? 4 : 2;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int steps = (D + 31) / 32;
   float part[FOLD ? RG : 1][NT][4] = {};

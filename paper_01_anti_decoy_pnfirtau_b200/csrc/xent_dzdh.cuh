@@ -280,8 +280,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * (2 + DZDH_WARPS
       __syncwarp();
       if (lane == 0) {
         // Each CTA's tensor core reads its own shared memory: the proxy fence above has made the warp's
-        // writes visible there, and the arrival on the even CTA's barrier comes after it. (A release over
-        // the whole cluster adds a memory barrier per warp and tile.)
+        // writes visible there, and the arrival on the even CTA's barrier comes after it. No other memory
+        // is published by it.
         asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(to_dz) : "memory");
         if (p.store_dz && q.it.row0 < p.Mp) tma_store_3d(&p.tdz, b, col, q.it.row0 + 32 * w.quad, 0);
         bulk_commit();

@@ -45,8 +45,8 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
 }
 // 2^x of two values, both on the special-function unit. At K = 256 that unit (16 per clock
 // and SM) is as busy as the tensor core, yet moving every third or second exponential to a
-// polynomial on the FMA pipe made the forward slower (16352 x 33278 x 256: 217 us without,
-// 227 and 237 with): the instructions cost more clock than the unit does.
+// polynomial on the FMA pipe made the forward's kernel slower (16352 x 33278 x 256: 217 us
+// without, 227 and 237 with, at one clock): the instructions cost more clock than the unit does.
 __device__ __forceinline__ f32x2 exp2_pair(f32x2 x) {
   const float2 v = unpack(x);
   return pack(ex2(v.x), ex2(v.y));

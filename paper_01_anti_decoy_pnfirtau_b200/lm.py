@@ -49,7 +49,7 @@ class LMConfig:
     silence_gamma: float | None = 0.5
     tau_init: float = 0.0
     fir_k: int = 7
-    ffn: str = "gelu"  # "gelu" (the reference's), "swiglu" or "geglu"
+    ffn: str = "gelu"  # "gelu" (the reference's), "swiglu" or "geglu" (with fused_step_ops: bf16 only)
 
 
 _GATES = {"swiglu": "silu", "geglu": "gelu"}
@@ -57,7 +57,8 @@ _GATES = {"swiglu": "silu", "geglu": "gelu"}
 
 class GatedFFN(nn.Module):
     """``down(act(gate(x)) * up(x))`` with biases, as the reference's feed-forward has;
-    ``fused``: the product on this library's kernel (``gated_mlp``), else plain modules."""
+    ``fused``: the product on this library's kernel (``gated_mlp``; a 16-bit input or CUDA
+    autocast, float32 raises), else plain modules of any type."""
 
     def __init__(self, d_model: int, d_ff: int, kind: str, dropout: float = 0.0, fused: bool = True):
         super().__init__()
@@ -96,7 +97,8 @@ class Block(nn.Module):
 class PnFirLM(nn.Module):
     """exp4_wikitext2_lm.py:203-247 (``WikiLM``) with a pn_fir_tau variant.
     ``streamed_loss`` and ``checkpoint_8bit`` (module docstring) need ``fused_step_ops``
-    and a bf16 computation; ``checkpoint_8bit`` covers the attention's projections and,
+    and a bf16 computation, and so does a gated ``cfg.ffn`` with ``fused_step_ops``
+    (float32 raises); ``checkpoint_8bit`` covers the attention's projections and,
     where ``cfg.ffn`` is gated, the feed-forward (``mlp_gelu`` keeps its 16-bit
     activations)."""
 

@@ -1,20 +1,23 @@
-"""Operators of a decoder's training step that keep little for the backward pass,
+"""Operators of a decoder's training step that can keep little for the backward pass,
 on this library's tcgen05 kernels (csrc/gated.cu, csrc/xent_stream.cu, csrc/act8.cu
 over the GEMM core csrc/gemm_tc.cuh). They stand beside ``mlp_gelu``,
 ``head_cross_entropy`` and ``Linear`` (lm_ops) of the Pre-LN decoder of the
 reference's language-model experiments (experiments/exp4_wikitext2_lm.py:183-259).
 
 - ``gated_linear``: ``act(x Wg^T + bg) * (x Wu^T + bu)`` (SwiGLU / GEGLU), both
-  projections, the activation and the product in one kernel. The backward keeps x and
-  the two pre-activations, or with ``checkpoint_8bit`` only x in 8 bits, from which it
-  computes the pre-activations again. Calls of a few rows (single tokens) that need no
-  gradient take the same entry.
+  projections, the activation and the product in one kernel. Kept for the backward are x
+  and, from width 896 on, where computing them again costs more, the two pre-activations
+  with 24 bits each (as many bytes as a 16-bit composition keeps); with ``checkpoint_8bit``
+  x in 8 bits alone. Calls of a few rows (single tokens) that need no gradient take the
+  same entry.
 - ``gated_mlp``: the block ``down(gated_linear(x))`` of three ``nn.Linear`` layers.
-- ``streamed_cross_entropy``: the head's softmax cross entropy without its logits: the
-  forward keeps one number per row, the backward computes the logits again for one
-  piece of the vocabulary at a time.
+- ``streamed_cross_entropy``: the head's softmax cross entropy without its logits: kept
+  are a 16-bit copy of the rows that count and 16 bytes a row beside it (room for all
+  rows: ``2 M D + 16 M`` bytes), and the backward computes the logits again for one piece
+  of the vocabulary at a time.
 - ``act8_pack`` / ``act8_unpack`` / ``act8_weight_grad``: an activation in 8 bits (e4m3
-  with a power of two per row and 128 columns) and the weight gradient that reads it;
+  with a power of two per row and 128 columns) and the weight gradient that reads it (by
+  way of a 16-bit copy in its workspace);
   ``lm_ops.Linear`` uses them when its ``checkpoint_8bit`` is set.
 
 Operands are bfloat16 or float16: under CUDA autocast the inputs are cast to the
@@ -162,7 +165,9 @@ class Act8:
 def act8_pack(x: torch.Tensor) -> Act8:
     """``x`` (float32, bfloat16 or float16; ``[..., D]``) in 8 bits: per row and block of
     128 columns e4m3 values times the least power of two that brings the block's largest
-    magnitude to 448 or less, rounded to nearest even. NaN and infinities become NaN."""
+    magnitude to 448 or less, rounded to nearest even. NaN and infinities become NaN. The
+    powers reach from 2^-110 to 2^120 (float16: 2^-15 to 2^8), so blocks below 2^-110 keep
+    fewer bits, and in the largest one magnitudes end at 240 times it."""
     dev = _require_cuda("act8_pack", x)
     _plain_values("act8_pack", x)
     code = _DTYPES.get(x.dtype)
@@ -349,7 +354,11 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     ``checkpoint_8bit``: the backward keeps ``x`` in 8 bits (``act8_pack``) and nothing else,
     and is the gradient at that 8-bit ``x``: it computes the pre-activations again from it.
     The forward's result does not change. ``casts``: an ``lm_ops.Bf16Casts`` with current
-    bf16 copies of the weights, used when the dtype is bf16."""
+    bf16 copies of the weights, used when the dtype is bf16.
+
+    The gradients of the pre-activations are rounded to the 16-bit type before the products
+    with the weights and x. In float16 they overflow past 65504 as in a float16 composition:
+    scale the loss accordingly."""
     biases = () if b_gate is None and b_up is None else tuple(b for b in (b_gate, b_up) if b is not None)
     dev = _require_cuda("gated_linear", x, w_gate, w_up, *biases)
     _plain_values("gated_linear", x, w_gate, w_up, *biases)
@@ -461,7 +470,13 @@ def streamed_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch
     Ignored rows cost nothing, and what they hold (NaN included) reaches no result: their
     gradient is 0. A target outside ``[0, V)`` that is not ``ignore_index`` gives a NaN loss
     and is reported by ``check_device_status()`` or the next call. ``casts``: an
-    ``lm_ops.Bf16Casts`` with a current bf16 copy of ``weight``. Twice differentiating raises."""
+    ``lm_ops.Bf16Casts`` with a current bf16 copy of ``weight``. Twice differentiating raises.
+
+    Logits are fp32 and so are the exponents that come from them: a probability in the gradient
+    is off by about 2^-24 times the largest logit's magnitude, and logits past 2^30 have no
+    result. The logits' gradient is rounded to the 16-bit type, in float16 scaled by one factor
+    for all rows: with ``reduction="none"`` a row whose upstream gradient is far below the
+    largest keeps fewer bits of its small probabilities."""
     dev = _require_cuda("streamed_cross_entropy", h, weight, targets)
     _plain_values("streamed_cross_entropy", h, weight)
     if reduction not in ("mean", "sum", "none"):
