@@ -320,10 +320,10 @@ __global__ void __launch_bounds__(256) xent_join_kernel(JoinArgs p) {
   const int lane = threadIdx.x & 31, tiles_m = (p.counts[0] + PM - 1) / PM;
   const int64_t total = (int64_t)tiles_m * p.tiles_n;
   const int pairs = Walk::run_pairs(total, p.pairs);
-  const float a = *p.alpha;
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < p.M; r += (int64_t)gridDim.x * 8) {
     const int at = p.pos[r];
     if (at < 0 && !p.last) continue;
+    const float a = at >= 0 ? *p.alpha : 0.f;  // alpha may be infinite or NaN
     int k0 = 0, k1 = -1, mt = 0;
     if (at >= 0) {
       mt = at / PM;

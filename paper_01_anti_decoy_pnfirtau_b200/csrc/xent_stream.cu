@@ -559,10 +559,10 @@ __global__ void __launch_bounds__(256) xent_dh_kernel(const float* acc, int64_t 
                                                       void* dh, int64_t lddh, int dtype, int64_t M, int D, int vec) {
   launch_next();
   wait_previous();
-  const float a = *alpha;
   const int lane = threadIdx.x & 31;
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < M; r += (int64_t)gridDim.x * 8) {
     const int at = pos[r];
+    const float a = at >= 0 ? *alpha : 0.f;  // alpha may be infinite or NaN
     for (int c0 = 4 * lane; c0 < D; c0 += 512) {  // four loads in flight before the first store
       float4 v[4];
 #pragma unroll

@@ -168,6 +168,24 @@ def test_saved_tensors_that_were_moved_come_back(cuda, D):
     check_device_status(cuda)
 
 
+# ------------------------------------------------------------------ masked rows
+@pytest.mark.parametrize("D", [64, 320])
+@pytest.mark.parametrize("up", [float("inf"), float("nan")])
+def test_ignored_rows_have_no_gradient_whatever_the_loss_s_own(cuda, D, up):
+    """As F.cross_entropy: an upstream gradient that is not finite reaches the rows that count alone."""
+    h, w = rand(300, D).requires_grad_(True), rand(500, D, std=D ** -0.5, seed=1)
+    t = torch.arange(300, device=cuda)
+    t[::3] = -100
+    for reduction in ("mean", "sum"):
+        loss = streamed_cross_entropy(h, w, t, reduction=reduction)
+        dh, = torch.autograd.grad(loss, h, torch.tensor(up, device=cuda))
+        ref, = torch.autograd.grad(torch.nn.functional.cross_entropy(h.float() @ w.float().T, t, reduction=reduction), h,
+                                   torch.tensor(up, device=cuda))
+        assert torch.all(ref[::3] == 0) and torch.all(dh[::3] == 0)
+        counted = t != -100
+        assert not torch.isfinite(dh[counted]).any()
+
+
 # ------------------------------------------------------------------ precision of what is kept and summed in fp32
 @pytest.mark.parametrize("D", [520, 1000])
 @pytest.mark.parametrize("name", ["silu", "gelu"])
