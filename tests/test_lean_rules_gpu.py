@@ -321,3 +321,46 @@ def test_lean_lm_step_replayed_bit_for_bit(cuda):
     finally:
         torch.use_deterministic_algorithms(was, warn_only=warn)
     check_device_status(cuda)
+
+
+def test_calls_captured_behind_copies_and_other_streams(cuda):
+    """In a capture the first kernel of a call may follow a copy, a fill, or work of another stream."""
+    x, wg, wu, w = rand(600, 128), rand(256, 128, std=0.1, seed=1), rand(256, 128, std=0.1, seed=2), rand(2000, 128, std=0.1, seed=3)
+    t, source = torch.arange(600, device=cuda), rand(600, 128, seed=4)
+    xs = [torch.empty_like(x) for _ in range(3)]
+    side = torch.cuda.Stream()
+
+    def calls(v):
+        return gated_linear(v, wg, wu), streamed_cross_entropy(v, w, t, reduction="none"), act8_unpack(act8_pack(v))
+
+    def step():
+        out = []
+        xs[0].copy_(source)
+        out.append(calls(xs[0]))
+        xs[1].zero_()
+        out.append(calls(xs[1]))
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            xs[2].copy_(source)
+            a = calls(xs[2])
+        b = calls(x)
+        here.wait_stream(side)
+        out += [a, b, calls(xs[2])]
+        return out
+
+    with torch.no_grad():
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        for seed in (7, 8):
+            source.copy_(rand(600, 128, seed=seed))
+            x.copy_(rand(600, 128, seed=seed + 10))
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, v in zip(got, (source, torch.zeros_like(x), source, x, source)):
+                for p, q in zip(a, calls(v)):
+                    assert torch.equal(p, q)
+    check_device_status(cuda)
